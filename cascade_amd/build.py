@@ -1,6 +1,7 @@
 """Compiles the native libraries of this package in-tree.
 
   libcascade_hip.so        hand-written HIP for gfx950 behind the C ABI of include/cascade_hip.h
+  libcascade_lm.so         the language-model operators for the same token texts behind the C ABI of include/cascade_lm.h
   libcascade_workloads.so  host-only generator of the synthetic benchmark partitions
   cascade_sa               the reference's command-line builder (text file in, sa40 file out) over the C ABI
 
@@ -13,13 +14,16 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 HIP_LIB = os.path.join(HERE, "libcascade_hip.so")
+LM_LIB = os.path.join(HERE, "libcascade_lm.so")
 WORKLOADS_LIB = os.path.join(HERE, "libcascade_workloads.so")
 CLI = os.path.join(HERE, "cascade_sa")
 
-HIPCC_FLAGS = [
+COMMON_FLAGS = [
     "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-shared", "-Wall",
-    # packed FP32 instructions stay off (nothing here is floating point, the flag is policy for this target)
+    # packed FP32 instructions stay off (the flag is policy for this target)
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+]
+HIPCC_FLAGS = COMMON_FLAGS + [
     # machine-level loop-invariant code motion hoists values out of loops that then stay live through the whole body:
     # without it partition_ids_kernel fits 5 waves per SIMD instead of 4 (8.7 -> 7.7 ms per 1e9 suffixes); the other
     # kernels are unchanged by it
@@ -36,6 +40,12 @@ def build_hip(extra_flags=()):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     _run([hipcc, *HIPCC_FLAGS, *extra_flags, "-o", HIP_LIB, os.path.join(CSRC, "cascade_hip.hip")])
     return HIP_LIB
+
+
+def build_lm():
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    _run([hipcc, *COMMON_FLAGS, "-o", LM_LIB, os.path.join(CSRC, "cascade_lm.hip")])
+    return LM_LIB
 
 
 def build_workloads():
@@ -68,6 +78,7 @@ def build_cpp_tests():
 
 def build_all():
     build_hip()
+    build_lm()
     build_workloads()
     build_cli()
     build_cpp_tests()

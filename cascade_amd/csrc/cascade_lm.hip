@@ -1,0 +1,528 @@
+// Host side of the language-model operators: argument checks, launch shapes and the C ABI declared in include/cascade_lm.h. gfx950 only.
+#include "../../include/cascade_lm.h"
+
+#include "lm_attention.hpp"
+#include "lm_clip.hpp"
+#include "lm_cross_entropy.hpp"
+#include "lm_spans.hpp"
+
+#include <cstdarg>
+#include <cstdio>
+
+using namespace lm;
+
+namespace {
+
+thread_local char g_err[512] = "";
+
+int fail(int code, const char* fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+int launched(const char* who)
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? CSA_OK : fail(CSA_ERR_HIP, "%s: a launch failed: %s", who, hipGetErrorString(e));
+}
+
+uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+uint64_t parts_of(uint64_t x, uint64_t size) { return (x + size - 1) / size; }
+bool aligned(const void* p, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Hands out the pieces of a workspace, or only adds them up.
+struct Carver {
+    char* base;
+    uint64_t used = 0;
+    template <class T>
+    T* take(uint64_t count)
+    {
+        T* at = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used = up(used + count * sizeof(T), 256);
+        return at;
+    }
+};
+
+int check_work(const char* who, const void* work, uint64_t have, uint64_t need)
+{
+    if (need && (!work || !aligned(work, 256)))
+        return fail(CSA_ERR_ARG, "%s: the workspace is null or not aligned to 256 bytes", who);
+    if (have < need)
+        return fail(CSA_ERR_ARG, "%s: a workspace of %llu bytes where %llu are needed", who, (unsigned long long)have, (unsigned long long)need);
+    return CSA_OK;
+}
+
+// ---- spans ----
+
+uint64_t span_tile(uint64_t n)
+{
+    return up(parts_of(n, SPAN_TILES), SPAN_TURN);
+}
+
+// ---- attention ----
+
+int check_heads(const char* who, const char* what, const csa_lm_heads& h, const csa_lm_attention& a)
+{
+    if (!h.data || !aligned(h.data, 16))
+        return fail(CSA_ERR_ARG, "%s: %s is null or not aligned to 16 bytes", who, what);
+    if (h.token_stride % 8 || h.head_stride % 8 || h.token_stride < static_cast<int64_t>(a.head_dim) || h.token_stride >= 1 << 22 || h.head_stride < 0)
+        return fail(CSA_ERR_ARG, "%s: strides of %s (%lld between tokens, %lld between heads) have to be multiples of 8, the first at least head_dim and below 2^22",
+                    who, what, (long long)h.token_stride, (long long)h.head_stride);
+    return CSA_OK;
+}
+
+int check_attention(const char* who, const csa_lm_attention* a)
+{
+    if (!a)
+        return fail(CSA_ERR_ARG, "%s: null description", who);
+    if (a->type != CSA_LM_BF16 && a->type != CSA_LM_F16)
+        return fail(CSA_ERR_ARG, "%s: type %d is neither CSA_LM_BF16 nor CSA_LM_F16", who, a->type);
+    if (!a->kv_heads || !a->q_heads || a->q_heads % a->kv_heads || a->q_heads > 65535)
+        return fail(CSA_ERR_ARG, "%s: %u heads of q do not share %u heads of k and v", who, a->q_heads, a->kv_heads);
+    if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8)
+        return fail(CSA_ERR_ARG, "%s: head_dim = %u is no multiple of 8 in [8, 128]", who, a->head_dim);
+    if (a->tokens > 1u << 30)
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens", who, (unsigned long long)a->tokens);
+    if (!(a->scale > 0.f) || a->scale > 3e38f)
+        return fail(CSA_ERR_ARG, "%s: scale = %g is not positive and finite", who, a->scale);
+    if (!(a->cap >= 0.f) || a->cap > 3e38f)
+        return fail(CSA_ERR_ARG, "%s: cap = %g is neither 0 nor positive and finite", who, a->cap);
+    if (a->tokens) {
+        if (int rc = check_heads(who, "q", a->q, *a))
+            return rc;
+        if (int rc = check_heads(who, "k", a->k, *a))
+            return rc;
+        if (int rc = check_heads(who, "v", a->v, *a))
+            return rc;
+    }
+    const uint64_t groups = parts_of(a->tokens, ROWS_PER_GROUP) * a->q_heads;
+    if (groups > 0x7fffffffu)
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens of %u heads", who, (unsigned long long)a->tokens, a->q_heads);
+    return CSA_OK;
+}
+
+Heads heads(const csa_lm_heads& h) { return {h.data, h.token_stride, h.head_stride}; }
+
+Attention attention(const csa_lm_attention& a)
+{
+    return {heads(a.q), heads(a.k), heads(a.v), a.d_lo, a.d_hi, a.d_slope, static_cast<int64_t>(a.tokens), a.q_heads, a.q_heads / a.kv_heads,
+            static_cast<int>(a.head_dim), a.scale, a.cap};
+}
+
+struct AttentionWork {
+    uint32_t* norms;
+    int2* bounds;
+    RowBlock* blocks;
+    uint64_t bytes;
+    AttentionWork(void* base, uint64_t tokens, uint64_t q_heads)
+    {
+        Carver c{static_cast<char*>(base)};
+        const uint64_t tiles = parts_of(tokens, BLOCK_ROWS);
+        norms = c.take<uint32_t>(2);
+        bounds = c.take<int2>(tiles);
+        blocks = c.take<RowBlock>(tiles * q_heads);
+        bytes = c.used;
+    }
+};
+
+template <class Type, int DIM>
+void forward(const csa_lm_attention& a, const csa_lm_heads& out, float* lse, hipStream_t s)
+{
+    attention_forward_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
+        attention(a), static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
+}
+
+template <class Type, int DIM>
+void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* lse, const csa_lm_heads& d_out, const csa_lm_heads& d_q, const csa_lm_heads& d_k,
+              const csa_lm_heads& d_v, const AttentionWork& w, hipStream_t s)
+{
+    const Attention at = attention(a);
+    const uint32_t tiles = static_cast<uint32_t>(parts_of(a.tokens, BLOCK_ROWS));
+    span_bounds_kernel<<<tiles, 64, 0, s>>>(at, w.bounds, w.norms);
+    row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
+    attention_d_q_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
+        at, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
+    attention_d_kv_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads), 256, 0, s>>>(
+        at, heads(d_out), w.blocks, w.bounds, tiles, w.norms, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride,
+        static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
+}
+
+template <class F>
+void with_dim(uint32_t dim, F f)
+{
+    if (dim <= 64)
+        f(std::integral_constant<int, 64>());
+    else if (dim <= 96)
+        f(std::integral_constant<int, 96>());
+    else
+        f(std::integral_constant<int, 128>());
+}
+template <class F>
+void with_type(int type, F f)
+{
+    if (type == CSA_LM_F16)
+        f(F16());
+    else
+        f(Bf16());
+}
+
+// ---- cross entropy ----
+
+// Vocabulary by tokens. Up to 512 tokens the tiles of 256 tokens would leave compute units without work.
+template <class Type>
+using WideLogits = Product<Type, 256, 256, 2, 4, false, false>;
+template <class Type>
+using NarrowLogits = Product<Type, 256, 64, 4, 1, false, false>;
+template <class Type>
+using WeightGradients = Product<Type, 256, 256, 2, 4, false, true>;
+template <class Type>
+using WideHidden = Product<Type, 256, 256, 2, 4, true, true>;
+template <class Type>
+using NarrowHidden = Product<Type, 64, 256, 1, 4, true, true>;
+
+constexpr uint64_t NARROW_TOKENS = 512;
+constexpr uint64_t PIECE_BYTES = 256ull << 20; // of P
+constexpr uint64_t SHARE_BYTES = 64ull << 20;  // of d_hidden's shares beside the first
+
+struct EntropyPlan {
+    uint64_t padded_dim, padded_tokens, words, pieces, shares, share_words;
+    bool narrow;
+    EntropyPlan(uint64_t tokens, uint64_t dim, uint64_t vocab)
+    {
+        padded_dim = up(dim, 8);
+        padded_tokens = up(tokens, 8);
+        narrow = tokens <= NARROW_TOKENS;
+        const uint64_t fit = PIECE_BYTES / (512 * (padded_tokens ? padded_tokens : 8));
+        words = (fit ? fit : 1) * 256;
+        if (words > up(vocab, 256))
+            words = up(vocab, 256);
+        pieces = parts_of(vocab, words);
+        // d_hidden has few tiles where there are few tokens: its sum over the words of a piece is then shared out
+        const uint64_t tiles = parts_of(tokens, narrow ? 64 : 256) * parts_of(padded_dim, 256);
+        const uint64_t want = tiles ? (narrow ? 1024 : 512) / tiles : 1, room = SHARE_BYTES / (4 * (tokens * padded_dim ? tokens * padded_dim : 1)) + 1;
+        const uint64_t most = parts_of(words, 4 * SLICE);
+        shares = want < room ? want : room;
+        shares = shares < most ? shares : most;
+        shares = shares ? shares : 1;
+        share_words = up(parts_of(words, shares), 2 * SLICE);
+        shares = parts_of(words, share_words);
+    }
+};
+
+struct EntropyWork {
+    short *hidden, *weight, *kept, *p;
+    float2* part;
+    float *target_logit, *scale, *shares;
+    uint64_t bytes;
+    EntropyWork(void* base, const EntropyPlan& plan, uint64_t tokens, uint64_t vocab, bool backward, bool copies)
+    {
+        Carver c{static_cast<char*>(base)};
+        hidden = c.take<short>(copies ? tokens * plan.padded_dim : 0);
+        weight = c.take<short>(copies ? vocab * plan.padded_dim : 0);
+        if (backward) {
+            kept = c.take<short>(tokens * plan.padded_dim);
+            p = c.take<short>(plan.words * plan.padded_tokens);
+            shares = c.take<float>(plan.shares * tokens * plan.padded_dim);
+            scale = c.take<float>(2);
+        } else {
+            part = c.take<float2>(parts_of(vocab, 256) * 4 * tokens);
+            target_logit = c.take<float>(tokens);
+        }
+        bytes = c.used;
+    }
+};
+
+int check_entropy(const char* who, int type, const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, const void* target,
+                  uint64_t tokens, uint64_t dim, uint64_t vocab)
+{
+    if (type != CSA_LM_BF16 && type != CSA_LM_F16)
+        return fail(CSA_ERR_ARG, "%s: type %d is neither CSA_LM_BF16 nor CSA_LM_F16", who, type);
+    if (!dim || !vocab)
+        return fail(CSA_ERR_ARG, "%s: %llu values a row, %llu words", who, (unsigned long long)dim, (unsigned long long)vocab);
+    if (tokens > 1u << 30 || vocab > 1u << 30 || dim >= 1u << 22)
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens, %llu words, %llu values a row", who, (unsigned long long)tokens, (unsigned long long)vocab,
+                    (unsigned long long)dim);
+    if (parts_of(vocab, 256) * parts_of(tokens, 64) > 0x7fffffffu || (tokens > vocab ? tokens : vocab) * up(dim, 8) / 2048 > 0x7fffffffu)
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens by %llu words of %llu values in one call", who, (unsigned long long)tokens, (unsigned long long)vocab,
+                    (unsigned long long)dim);
+    if (!weight || !aligned(weight, 2) || (tokens && (!hidden || !aligned(hidden, 2) || !target)))
+        return fail(CSA_ERR_ARG, "%s: a null or odd address", who);
+    if (hidden_stride < static_cast<int64_t>(dim) || weight_stride < static_cast<int64_t>(dim) || hidden_stride >= 1 << 22 || weight_stride >= 1 << 22)
+        return fail(CSA_ERR_ARG, "%s: strides of %lld and %lld values for rows of %llu", who, (long long)hidden_stride, (long long)weight_stride,
+                    (unsigned long long)dim);
+    return CSA_OK;
+}
+
+bool walks(const void* p, int64_t stride, uint64_t dim) { return aligned(p, 16) && stride % 8 == 0 && dim % 8 == 0; }
+
+void lay_out(const void* in, int64_t in_stride, uint64_t rows, uint64_t dim, const int32_t* target, uint64_t vocab, short* out, uint64_t stride, hipStream_t s)
+{
+    if (const uint64_t threads = rows * (stride / 8))
+        lay_out_rows_kernel<<<static_cast<uint32_t>(parts_of(threads, 256)), 256, 0, s>>>(static_cast<const short*>(in), in_stride, rows, dim, target, vocab, out, stride,
+                                                                                          walks(in, in_stride, dim));
+}
+
+template <class Type>
+void entropy_forward(const EntropyPlan& plan, const EntropyWork& w, const Operand& hidden, const Operand& weight, const int32_t* target, float* loss, float* lse,
+                     hipStream_t s)
+{
+    typedef WideLogits<Type> W;
+    typedef NarrowLogits<Type> N;
+    const uint32_t mt = static_cast<uint32_t>(parts_of(weight.rows, 256)), nt = static_cast<uint32_t>(parts_of(hidden.rows, plan.narrow ? 64 : 256));
+    const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), mt, nt, target, 0};
+    if (plan.narrow)
+        logit_sums_kernel<N><<<mt * nt, N::THREADS, 0, s>>>(l, w.part, w.target_logit);
+    else
+        logit_sums_kernel<W><<<mt * nt, W::THREADS, 0, s>>>(l, w.part, w.target_logit);
+    join_sums_kernel<<<static_cast<uint32_t>(parts_of(hidden.rows, 16)), 256, 0, s>>>(w.part, mt * static_cast<int64_t>(plan.narrow ? N::WM : W::WM),
+                                                                                      w.target_logit, target, hidden.rows, weight.rows, loss, lse);
+}
+
+template <class Type>
+void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Operand& hidden, const Operand& weight, const int32_t* target, const float* lse,
+                      const float* d_loss, uint64_t dim, short* d_hidden, int64_t d_hidden_stride, short* d_weight, int64_t d_weight_stride, hipStream_t s)
+{
+    typedef WideLogits<Type> WL;
+    typedef NarrowLogits<Type> NL;
+    typedef WeightGradients<Type> G;
+    typedef WideHidden<Type> WH;
+    typedef NarrowHidden<Type> NH;
+    const int64_t tokens = hidden.rows, vocab = weight.rows, d = static_cast<int64_t>(dim), pd = static_cast<int64_t>(plan.padded_dim),
+                  pt = static_cast<int64_t>(plan.padded_tokens);
+    if (!Type::wide_range)
+        loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, w.scale);
+    const uint32_t dt = static_cast<uint32_t>(parts_of(dim, 256)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow ? 64 : 256));
+    for (uint64_t piece = 0; piece < plan.pieces; ++piece) {
+        const int64_t first = static_cast<int64_t>(piece * plan.words), words = vocab - first < static_cast<int64_t>(plan.words) ? vocab - first : plan.words;
+        const Operand part{static_cast<const short*>(weight.data) + first * weight.stride, weight.stride, words};
+        const uint32_t wt = static_cast<uint32_t>(parts_of(words, 256));
+        const Logits l{part, hidden, pd, wt, tt, target, first};
+        if (plan.narrow)
+            logit_gradients_kernel<NL, Type><<<wt * tt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, pt);
+        else
+            logit_gradients_kernel<WL, Type><<<wt * tt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, pt);
+        if (d_weight)
+            weight_gradients_kernel<G, Type><<<wt * dt, G::THREADS, 0, s>>>({w.p, pt, words}, {w.kept, pd, d}, tokens, wt, dt, w.scale,
+                                                                            d_weight + first * d_weight_stride, d_weight_stride);
+        if (d_hidden) {
+            const Operand p{w.p, pt, tokens}, across{part.data, part.stride, d};
+            const uint32_t shares = static_cast<uint32_t>(plan.shares), groups = tt * dt * shares;
+            if (plan.narrow)
+                hidden_gradients_kernel<NH><<<groups, NH::THREADS, 0, s>>>(p, across, words, plan.share_words, tt, dt, w.shares, pd, piece > 0);
+            else
+                hidden_gradients_kernel<WH><<<groups, WH::THREADS, 0, s>>>(p, across, words, plan.share_words, tt, dt, w.shares, pd, piece > 0);
+        }
+    }
+    if (d_hidden)
+        join_shares_kernel<Type><<<static_cast<uint32_t>(parts_of(tokens * pd / 4, 256)), 256, 0, s>>>(w.shares, static_cast<uint32_t>(plan.shares), tokens, d, pd, w.scale,
+                                                                                                      d_hidden, d_hidden_stride);
+}
+
+} // namespace
+
+extern "C" {
+
+const char* csa_lm_last_error(void) { return g_err; }
+
+uint64_t csa_lm_spans_workspace(uint64_t n) { return n > SPAN_TURN ? SPAN_TILES * sizeof(int32_t) : 0; }
+
+int csa_lm_spans_u16_dev(const uint16_t* d_text, uint64_t n, uint32_t separator, int32_t* d_lo, int32_t* d_hi, int32_t* d_target, void* d_work,
+                         uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_spans_u16_dev";
+    if (n > CSA_MAX_PART_SZ)
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu symbols", who, (unsigned long long)n);
+    if (separator > 0xFFFF)
+        return fail(CSA_ERR_ARG, "%s: separator %u is no uint16", who, separator);
+    if (n == 0)
+        return CSA_OK;
+    if (!d_text || !d_lo || !d_hi || !d_target || !aligned(d_text, 2) || !aligned(d_lo, 4) || !aligned(d_hi, 4) || !aligned(d_target, 4))
+        return fail(CSA_ERR_ARG, "%s: a null or unaligned buffer", who);
+    if (int rc = check_work(who, d_work, work_bytes, csa_lm_spans_workspace(n)))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const uint64_t tile = span_tile(n);
+    const uint32_t tiles = static_cast<uint32_t>(parts_of(n, tile));
+    const bool wide = aligned(d_text, 16) && aligned(d_lo, 16) && aligned(d_hi, 16) && aligned(d_target, 16);
+    if (tiles > 1)
+        last_separators_kernel<<<tiles, 256, 0, s>>>(d_text, n, static_cast<uint16_t>(separator), tile, wide, static_cast<int32_t*>(d_work));
+    spans_kernel<<<tiles, 256, 0, s>>>(d_text, n, static_cast<uint16_t>(separator), tile, wide, static_cast<int32_t*>(d_work), d_lo, d_hi, d_target);
+    return launched(who);
+}
+
+int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, float* d_lse, void* stream)
+{
+    const char* who = "csa_lm_attention_forward_dev";
+    if (int rc = check_attention(who, a))
+        return rc;
+    if (a->tokens == 0)
+        return CSA_OK;
+    if (int rc = check_heads(who, "out", out, *a))
+        return rc;
+    if (!d_lse || !aligned(d_lse, 4))
+        return fail(CSA_ERR_ARG, "%s: d_lse is null or unaligned", who);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    with_type(a->type, [&](auto type) { with_dim(a->head_dim, [&](auto dim) { forward<decltype(type), dim()>(*a, out, d_lse, s); }); });
+    return launched(who);
+}
+
+uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads) { return AttentionWork(nullptr, tokens, q_heads).bytes; }
+
+int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, const float* d_lse, csa_lm_heads d_out, csa_lm_heads d_q, csa_lm_heads d_k,
+                                  csa_lm_heads d_v, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_attention_backward_dev";
+    if (int rc = check_attention(who, a))
+        return rc;
+    if (a->tokens == 0)
+        return CSA_OK;
+    const struct {
+        const char* name;
+        const csa_lm_heads& h;
+    } arrays[] = {{"out", out}, {"d_out", d_out}, {"d_q", d_q}, {"d_k", d_k}, {"d_v", d_v}};
+    for (const auto& x : arrays)
+        if (int rc = check_heads(who, x.name, x.h, *a))
+            return rc;
+    if (!d_lse || !aligned(d_lse, 4))
+        return fail(CSA_ERR_ARG, "%s: d_lse is null or unaligned", who);
+    const AttentionWork w(d_work, a->tokens, a->q_heads);
+    if (int rc = check_work(who, d_work, work_bytes, w.bytes))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    with_type(a->type, [&](auto type) { with_dim(a->head_dim, [&](auto dim) { backward<decltype(type), dim()>(*a, out, d_lse, d_out, d_q, d_k, d_v, w, s); }); });
+    return launched(who);
+}
+
+uint64_t csa_lm_cross_entropy_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t flags)
+{
+    if (!dim || !vocab || tokens > 1u << 30 || vocab > 1u << 30 || dim >= 1u << 22)
+        return 0;
+    return EntropyWork(nullptr, EntropyPlan(tokens, dim, vocab), tokens, vocab, flags & CSA_LM_BACKWARD, flags & CSA_LM_COPY_ROWS || dim % 8).bytes;
+}
+
+int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_target,
+                                     uint64_t tokens, uint64_t dim, uint64_t vocab, float* d_loss, float* d_lse, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_cross_entropy_forward_dev";
+    if (int rc = check_entropy(who, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
+        return rc;
+    if (tokens == 0)
+        return CSA_OK;
+    if (!d_loss || !d_lse || !aligned(d_loss, 4) || !aligned(d_lse, 4))
+        return fail(CSA_ERR_ARG, "%s: d_loss or d_lse is null or unaligned", who);
+    const EntropyPlan plan(tokens, dim, vocab);
+    const bool copies = !walks(d_hidden, hidden_stride, dim) || !walks(d_weight, weight_stride, dim);
+    const EntropyWork w(d_work, plan, tokens, vocab, false, copies);
+    if (int rc = check_work(who, d_work, work_bytes, w.bytes))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    Operand hidden{d_hidden, hidden_stride, static_cast<int64_t>(tokens)}, weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
+    if (!walks(d_hidden, hidden_stride, dim)) {
+        lay_out(d_hidden, hidden_stride, tokens, dim, nullptr, vocab, w.hidden, plan.padded_dim, s);
+        hidden = {w.hidden, static_cast<int64_t>(plan.padded_dim), hidden.rows};
+    }
+    if (!walks(d_weight, weight_stride, dim)) {
+        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
+    }
+    with_type(type, [&](auto t) { entropy_forward<decltype(t)>(plan, w, hidden, weight, d_target, d_loss, d_lse, s); });
+    return launched(who);
+}
+
+int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_target,
+                                      const float* d_lse, const float* d_loss_grad, uint64_t tokens, uint64_t dim, uint64_t vocab, void* d_hidden_grad,
+                                      int64_t hidden_grad_stride, void* d_weight_grad, int64_t weight_grad_stride, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_cross_entropy_backward_dev";
+    if (int rc = check_entropy(who, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
+        return rc;
+    if (tokens && (!d_lse || !d_loss_grad))
+        return fail(CSA_ERR_ARG, "%s: d_lse or d_loss_grad is null", who);
+    if ((d_hidden_grad && (!aligned(d_hidden_grad, 2) || hidden_grad_stride < static_cast<int64_t>(dim))) ||
+        (d_weight_grad && (!aligned(d_weight_grad, 2) || weight_grad_stride < static_cast<int64_t>(dim))))
+        return fail(CSA_ERR_ARG, "%s: a gradient's address is odd or its stride below its rows' length", who);
+    const EntropyPlan plan(tokens, dim, vocab);
+    const EntropyWork w(d_work, plan, tokens, vocab, true, !walks(d_weight, weight_stride, dim));
+    if (int rc = check_work(who, d_work, work_bytes, w.bytes))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (tokens == 0) { // the sum over no tokens
+        if (d_weight_grad)
+            zero_rows_kernel<<<static_cast<uint32_t>(parts_of(vocab * dim, 1024)), 256, 0, s>>>(static_cast<short*>(d_weight_grad), weight_grad_stride, vocab, dim);
+        return launched(who);
+    }
+    Operand weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
+    lay_out(d_hidden, hidden_stride, tokens, dim, d_target, vocab, w.kept, plan.padded_dim, s);
+    const Operand hidden{w.kept, static_cast<int64_t>(plan.padded_dim), static_cast<int64_t>(tokens)};
+    if (!walks(d_weight, weight_stride, dim)) {
+        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
+    }
+    with_type(type, [&](auto t) {
+        entropy_backward<decltype(t)>(plan, w, hidden, weight, d_target, d_lse, d_loss_grad, dim, static_cast<short*>(d_hidden_grad), hidden_grad_stride,
+                                      static_cast<short*>(d_weight_grad), weight_grad_stride, s);
+    });
+    return launched(who);
+}
+
+uint64_t csa_lm_clip_workspace(uint32_t count) { return parts_of(count, CLIP_TENSORS) * CLIP_GROUPS * sizeof(double); }
+
+int csa_lm_clip_dev(const csa_lm_values* list, uint32_t count, float max_norm, float* d_norm, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_clip_dev";
+    if (!list && count)
+        return fail(CSA_ERR_ARG, "%s: null list", who);
+    if (!(max_norm >= 0.f))
+        return fail(CSA_ERR_ARG, "%s: max_norm = %g", who, max_norm);
+    if (d_norm && !aligned(d_norm, 4))
+        return fail(CSA_ERR_ARG, "%s: d_norm is unaligned", who);
+    for (uint32_t i = 0; i < count; ++i) {
+        const csa_lm_values& v = list[i];
+        if (v.type != CSA_LM_BF16 && v.type != CSA_LM_F16 && v.type != CSA_LM_F32)
+            return fail(CSA_ERR_ARG, "%s: array %u has type %d", who, i, v.type);
+        const uint64_t size = v.type == CSA_LM_F32 ? 4 : 2;
+        if (v.n && (!v.in || !v.out || !aligned(v.in, size) || !aligned(v.out, size)))
+            return fail(CSA_ERR_ARG, "%s: array %u is null or not aligned to its type", who, i);
+        if (v.n > 1ull << 40)
+            return fail(CSA_ERR_TOO_LARGE, "%s: array %u has %llu values", who, i, (unsigned long long)v.n);
+    }
+    if (int rc = check_work(who, d_work, work_bytes, csa_lm_clip_workspace(count)))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    double* partial = static_cast<double*>(d_work);
+    uint32_t partials = 0;
+    // Twice the list, as many arrays a launch as its arguments hold: all sums first, then all products.
+    for (int way = 0; way < 2; ++way)
+        for (uint32_t begin = 0; begin < count || (way == 1 && begin == 0); begin += CLIP_TENSORS) {
+            ClipList c;
+            c.count = 0;
+            uint64_t chunks = 0;
+            for (uint32_t i = begin; i < count && i < begin + CLIP_TENSORS; ++i)
+                if (list[i].n) {
+                    c.in[c.count] = list[i].in;
+                    c.out[c.count] = list[i].out;
+                    c.n[c.count] = list[i].n;
+                    c.type[c.count] = static_cast<uint8_t>(list[i].type);
+                    c.wide[c.count] = aligned(list[i].in, 16) && aligned(list[i].out, 16);
+                    c.first[c.count++] = static_cast<uint32_t>(chunks);
+                    chunks += parts_of(list[i].n, CLIP_CHUNK);
+                }
+            c.first[c.count] = static_cast<uint32_t>(chunks);
+            if (chunks > 0x7fffffffu)
+                return fail(CSA_ERR_TOO_LARGE, "%s: too many values", who);
+            const uint32_t groups = static_cast<uint32_t>(chunks < CLIP_GROUPS ? chunks : CLIP_GROUPS);
+            if (way == 0 && groups) {
+                squares_kernel<<<groups, 256, 0, s>>>(c, partial + partials);
+                partials += groups;
+            } else if (way == 1 && (groups || begin == 0)) { // the norm is written even of nothing
+                clip_kernel<<<groups ? groups : 1, 256, 0, s>>>(c, partial, partials, max_norm, begin == 0 ? d_norm : nullptr);
+            }
+        }
+    return launched(who);
+}
+
+} // extern "C"

@@ -1,0 +1,701 @@
+// Attention of every position over a span of keys, and its gradients:
+//   z[i][j] = scale q_i . k_j, bent to cap tanh(z / cap) where cap > 0, less slope |i - j|;   p = softmax of z over j in [lo_i, hi_i);
+//   out_i = sum_j p v_j, lse_i = ln sum_j exp z;
+//   D_i = d_out_i . out_i, ds = p (d_out_i . v_j - D_i) (1 - tanh^2), d_q = scale ds k, d_k = scale ds^T q, d_v = p^T d_out.
+// A span is two numbers a row: causal, documents, prefixes seen both ways and windows are all spans, and so is no key at all.
+//
+// All three kernels keep the scores on the side where they are needed next. The matrix unit leaves column lane % 32 and rows
+// 8 (r / 4) + 4 (lane / 32) + r % 4 in a lane's sixteen registers; taken as the second operand of the next product, whose sum runs
+// over those rows, they are two fragments as they stand, if the first operand's values come in the same order: its LDS reads are transposed
+// ones of four rows each, so the order costs nothing. Scores therefore never pass through LDS.
+//   forward and d_q: a lane holds one row i; its keys run along the registers (scores transposed: K Q^T), so the softmax's maximum, sum,
+//                    mask and distance are a lane's own, with one exchange between the halves of the wave.
+//   d_k and d_v:     a lane holds one key and rows run along the registers; a workgroup owns its keys and walks the rows of all heads that share
+//                    them, so nothing is added by atomics and the results do not depend on the order of workgroups. The scores are
+//                    computed twice for that, once here and once for d_q (seven products instead of five).
+// Tiles of keys or rows come straight from memory into LDS, one tile ahead. The 16-byte pieces of a tile's row stand at
+// places that keep both kinds of reads, eight rows' same piece and four rows' neighbouring pieces, in different banks.
+#pragma once
+#include "lm_common.hpp"
+
+namespace lm {
+
+struct Heads {
+    const void* data;
+    int64_t token, head; // values between tokens and between heads
+};
+
+struct Attention {
+    Heads q, k, v;
+    const int32_t *lo, *hi;
+    const float* slope; // of each head of q, or null
+    int64_t tokens;
+    uint32_t q_heads, group; // group: heads of q that share one of k and v
+    int dim;
+    float scale, cap;
+};
+
+template <int DIM>
+struct HeadTile {
+    static constexpr int PIECES = DIM / 8;
+    // Place of a row's 16-byte piece: rows 0 to 7 put the same piece at eight places of 128 bytes, and the pairs of pieces of rows 4 a ... 4 a + 3
+    // at four. Rows of 12 pieces alternate between two of the eight places already.
+    static __device__ int place(int row, int piece)
+    {
+        return PIECES % 8 == 0 ? piece ^ ((row & 3) * 2 | (row >> 2 & 1)) : piece ^ ((row >> 1 & 1) * 2 | (row >> 2 & 1));
+    }
+    // Operand with the head's values along k: 32 rows, values 16 step ... of them
+    static __device__ s16x8 along(const short* tile, int row0, int step, int lane)
+    {
+        const int row = row0 + lane % 32;
+        return read16(tile + row * DIM + place(row, step * 2 + lane / 32) * 8);
+    }
+    // Operand with the rows along k in the order of the registers above: values 32 e ... 32 e + 31 of the head, rows row0 ... row0 + 15
+    static __device__ s16x8 across(const short* tile, int row0, int e, int lane)
+    {
+        const int g = lane / 16, j = lane % 16, col = 32 * e + (g % 2) * 16 + 4 * (j % 4);
+        const int row = row0 + 4 * (g / 2) + j / 4;
+        return join(read_turned(tile + row * DIM + place(row, col / 8) * 8 + col % 8),
+                    read_turned(tile + (row + 8) * DIM + place(row + 8, col / 8) * 8 + col % 8));
+    }
+};
+
+// ROWS rows of one head, padded to DIM values with zeros, by WAVES waves.
+template <int ROWS, int DIM, int WAVES>
+struct HeadLoader {
+    static constexpr int LOADS = ROWS * DIM / 8 / 64 / WAVES;
+    static_assert(ROWS * DIM / 8 % (64 * WAVES) == 0, "every wave loads as much");
+    int64_t line; // bytes
+    uint32_t offset[LOADS];
+    __device__ void begin(const Heads& h, int dim, int wave, int lane)
+    {
+        line = h.token * 2;
+        for (int j = 0; j < LOADS; ++j) {
+            const int at = (wave * LOADS + j) * 64 + lane, row = at / (DIM / 8), piece = HeadTile<DIM>::place(row, at % (DIM / 8));
+            offset[j] = piece * 8 < dim ? static_cast<uint32_t>(row * line + piece * 16) : OUTSIDE;
+        }
+    }
+    // rows row0 ... of the head that `base` points at, of `rows`; those past the end are zeros
+    __device__ void load(const char* base, int64_t row0, int64_t rows, short* tile, int wave) const
+    {
+        const int64_t left = rows - row0;
+        const buffer_t w = window(base + row0 * line, left > 0 ? static_cast<uint32_t>((left < ROWS ? left : ROWS) * line) : 0);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            load_to_lds(w, tile + (wave * LOADS + j) * 512, offset[j]);
+    }
+};
+
+// A row's fragments of 16 values a step, from memory: zeros past `dim` and for rows past the end.
+template <int DIM>
+__device__ inline void read_rows(const Heads& h, uint32_t head, int64_t row, int64_t rows, int dim, int lane, s16x8 (&f)[DIM / 16])
+{
+    const short* p = static_cast<const short*>(h.data) + head * h.head + row * h.token;
+#pragma unroll
+    for (int s = 0; s < DIM / 16; ++s) {
+        const int at = s * 16 + lane / 32 * 8;
+        f[s] = row < rows && at < dim ? *reinterpret_cast<const s16x8*>(p + at) : s16x8{};
+    }
+}
+
+__device__ inline int wave_min(int x)
+{
+    for (int d = 32; d; d /= 2)
+        x = min(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ inline int wave_most(int x)
+{
+    for (int d = 32; d; d /= 2)
+        x = max(x, __shfl_xor(x, d));
+    return x;
+}
+
+constexpr int NONE = 0x7fffffff; // lo of a row that sees nothing, whose hi is 0: it lowers no minimum and raises no maximum
+
+__device__ inline void span_of(const Attention& a, int64_t i, int& lo, int& hi)
+{
+    lo = NONE;
+    hi = 0;
+    if (i < a.tokens) {
+        const int l = a.lo ? max(a.lo[i], 0) : 0;
+        const int h = a.hi ? min(static_cast<int64_t>(a.hi[i]), a.tokens) : i + 1;
+        if (l < h) {
+            lo = l;
+            hi = h;
+        }
+    }
+}
+
+template <class Type>
+__device__ inline s16x8 round8(const f32x16& x, int u)
+{
+    s16x8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        y[i] = to16<Type>(x[8 * u + i]);
+    return y;
+}
+
+// Workgroup's tile of rows and head. Neighbouring workgroup ids run on different XCDs: where there are eight heads or a multiple, an XCD gets
+// neighbouring heads, which share keys and values in its L2. Tiles come last first: those of long causal spans, the longest, are the last ones.
+__device__ inline void place_of(uint32_t id, uint32_t heads, uint32_t tiles, uint32_t& head, uint32_t& tile)
+{
+    const uint32_t in = id % heads;
+    head = heads % 8 == 0 ? in % 8 * (heads / 8) + in / 8 : in;
+    tile = tiles - 1 - id / heads;
+}
+
+constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
+
+// Scores of a tile, still raw products: to exponents of 2 less nothing, with `unit` left to multiply. Returns with z = s * unit.
+template <int TILES>
+__device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit, float slope2, int row, int key0, int half)
+{
+    unit = a.scale * LOG2E;
+    if (a.cap > 0.f) {
+        const float in = 2.f * LOG2E * a.scale / a.cap, cap2 = a.cap * LOG2E;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) // tanh y = 1 - 2 / (1 + e^2y)
+                s[t][r] = cap2 - 2.f * cap2 * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[t][r] * in));
+        unit = 1.f;
+    }
+    if (a.slope) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int key = key0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+                s[t][r] = s[t][r] * unit - slope2 * fabsf(static_cast<float>(row - key));
+            }
+        unit = 1.f;
+    }
+}
+
+template <class Type, int DIM>
+__global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, short* out, int64_t out_token, int64_t out_head, float* lse)
+{
+    typedef HeadTile<DIM> Tile;
+    constexpr int KT = KEYS_PER_TILE;
+    __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
+    const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    uint32_t head, tile;
+    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, head, tile);
+    const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
+
+    // The keys that this workgroup's rows see, this wave's rows see, and all of this wave's rows see.
+    int lo, hi, l2, h2;
+    span_of(a, first + lane, lo, hi);
+    span_of(a, first + 64 + lane, l2, h2);
+    const int group_lo = __builtin_amdgcn_readfirstlane(wave_min(min(lo, l2))), group_hi = __builtin_amdgcn_readfirstlane(wave_most(max(hi, h2)));
+    span_of(a, row, lo, hi);
+    const int wave_lo = __builtin_amdgcn_readfirstlane(wave_min(lo)), wave_hi = __builtin_amdgcn_readfirstlane(wave_most(hi));
+    const int all_lo = __builtin_amdgcn_readfirstlane(wave_most(lo)), all_hi = __builtin_amdgcn_readfirstlane(wave_min(hi));
+
+    s16x8 q[DIM / 16];
+    read_rows<DIM>(a.q, head, row, a.tokens, a.dim, lane, q);
+    const uint32_t kv = head / a.group;
+    const char* kb = reinterpret_cast<const char*>(static_cast<const short*>(a.k.data) + kv * a.k.head);
+    const char* vb = reinterpret_cast<const char*>(static_cast<const short*>(a.v.data) + kv * a.v.head);
+    HeadLoader<KT, DIM, 4> kl, vl;
+    kl.begin(a.k, a.dim, wave, lane);
+    vl.begin(a.v, a.dim, wave, lane);
+    const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
+
+    f32x16 o[DIM / 32];
+#pragma unroll
+    for (int e = 0; e < DIM / 32; ++e)
+        o[e] = f32x16{};
+    float top = -3.0e38f, sum = 0.f; // the running maximum may lag behind by 2^8, which spares most rescalings
+
+    auto turn = [&](const short* ks, const short* vs, int key0) {
+        if (key0 + KT <= wave_lo || key0 >= wave_hi)
+            return;
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = f32x16{};
+#pragma unroll
+            for (int d = 0; d < DIM / 16; ++d)
+                s[t] = Type::mfma32(Tile::along(ks, 32 * t, d, lane), q[d], s[t]);
+        }
+        float unit;
+        bend(a, s, unit, slope2, static_cast<int>(row), key0, half);
+        if (key0 < all_lo || key0 + KT > all_hi) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = key0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+                    s[t][r] = key >= lo && key < hi ? s[t][r] : -INFINITY;
+                }
+        }
+        float most = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r)
+            most = fmaxf(most, s[0][r]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            most = fmaxf(most, s[1][r]);
+        most = fmaxf(most, other_half(most)) * unit;
+        if (__any(most > top + 8.f)) {
+            const float high = fmaxf(top, most), down = __builtin_amdgcn_exp2f(top - high);
+            top = high;
+            sum *= down;
+#pragma unroll
+            for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    o[e][r] *= down;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[t][r] = __builtin_amdgcn_exp2f(s[t][r] * unit - top);
+                sum += s[t][r];
+            }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const s16x8 p = round8<Type>(s[t], u);
+#pragma unroll
+                for (int e = 0; e < DIM / 32; ++e)
+                    o[e] = Type::mfma32(Tile::across(vs, 32 * t + 16 * u, e, lane), p, o[e]);
+            }
+    };
+
+    if (group_lo < group_hi) {
+        const int begin = group_lo / KT * KT;
+        kl.load(kb, begin, a.tokens, k0s, wave);
+        vl.load(vb, begin, a.tokens, v0s, wave);
+        for (int key0 = begin; key0 < group_hi; key0 += 2 * KT) {
+            wait_for_all();
+            meet();
+            kl.load(kb, key0 + KT, a.tokens, k1s, wave);
+            vl.load(vb, key0 + KT, a.tokens, v1s, wave);
+            turn(k0s, v0s, key0);
+            wait_for_all();
+            meet();
+            kl.load(kb, key0 + 2 * KT, a.tokens, k0s, wave);
+            vl.load(vb, key0 + 2 * KT, a.tokens, v0s, wave);
+            turn(k1s, v1s, key0 + KT);
+        }
+        wait_for_all();
+    }
+    sum += other_half(sum);
+    if (row < a.tokens) {
+        const float share = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        short* to = out + head * out_head + row * out_token;
+#pragma unroll
+        for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * e + 8 * g + 4 * half;
+                if (d < a.dim) {
+                    s16x4 y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        y[i] = to16<Type>(o[e][4 * g + i] * share);
+                    *reinterpret_cast<s16x4*>(to + d) = y;
+                }
+            }
+        if (half == 0)
+            lse[head * a.tokens + row] = sum > 0.f || sum != sum ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
+    }
+}
+
+// ---- backward ----
+
+// What the backward kernels read of 64 rows of a head: 64 values each of lse in base 2 (infinite for rows that see nothing: their
+// probabilities are zeros), D, lo and hi. The block of (head, tile) is 1 KB, one load of a wave.
+constexpr int BLOCK_ROWS = 64;
+struct RowBlock {
+    float lse2[BLOCK_ROWS], delta[BLOCK_ROWS];
+    int lo[BLOCK_ROWS], hi[BLOCK_ROWS];
+};
+
+// The least lo and the largest hi of every 64 rows, and zeros where the largest norms of d_out and v will be.
+__global__ __launch_bounds__(64) void span_bounds_kernel(Attention a, int2* bounds, uint32_t* norms)
+{
+    int lo, hi;
+    span_of(a, static_cast<int64_t>(blockIdx.x) * BLOCK_ROWS + threadIdx.x, lo, hi);
+    lo = wave_min(lo);
+    hi = wave_most(hi);
+    if (threadIdx.x == 0) {
+        bounds[blockIdx.x] = make_int2(lo, hi);
+        if (blockIdx.x == 0)
+            norms[0] = norms[1] = 0;
+    }
+}
+
+template <class Type>
+__device__ inline float dot16(const short* x, const short* y, int dim, int lane16)
+{
+    float sum = 0.f;
+    const int d = lane16 * 8;
+    if (d < dim) {
+        const s16x8 a = *reinterpret_cast<const s16x8*>(x + d), b = *reinterpret_cast<const s16x8*>(y + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            sum += to32<Type>(a[i]) * to32<Type>(b[i]);
+    }
+    for (int k = 8; k; k /= 2)
+        sum += __shfl_xor(sum, k);
+    return sum;
+}
+
+// Row blocks of every head: sixteen lanes a row, sixteen rows a workgroup at a time. Half precision also asks for the largest norms of rows of d_out and v.
+template <class Type>
+__global__ __launch_bounds__(256) void row_blocks_kernel(Attention a, Heads out, Heads d_out, const float* lse, RowBlock* blocks, uint32_t* norms)
+{
+    const uint32_t head = blockIdx.y, tile = blockIdx.x;
+    RowBlock& to = blocks[static_cast<int64_t>(head) * gridDim.x + tile];
+    const int lane16 = threadIdx.x % 16;
+    float most = 0.f, most_v = 0.f;
+    for (int r = threadIdx.x / 16; r < BLOCK_ROWS; r += 16) {
+        const int64_t row = static_cast<int64_t>(tile) * BLOCK_ROWS + r;
+        float delta = 0.f;
+        if (row < a.tokens) {
+            const short* g = static_cast<const short*>(d_out.data) + head * d_out.head + row * d_out.token;
+            delta = dot16<Type>(static_cast<const short*>(out.data) + head * out.head + row * out.token, g, a.dim, lane16);
+            if (!Type::wide_range) {
+                most = fmaxf(most, dot16<Type>(g, g, a.dim, lane16));
+                if (head % a.group == 0) {
+                    const short* v = static_cast<const short*>(a.v.data) + head / a.group * a.v.head + row * a.v.token;
+                    most_v = fmaxf(most_v, dot16<Type>(v, v, a.dim, lane16));
+                }
+            }
+        }
+        if (lane16 == 0) {
+            int lo, hi;
+            span_of(a, row, lo, hi);
+            to.lse2[r] = lo < hi ? lse[head * a.tokens + row] * LOG2E : INFINITY;
+            to.delta[r] = lo < hi ? delta : 0.f;
+            to.lo[r] = lo;
+            to.hi[r] = hi;
+        }
+    }
+    if (!Type::wide_range) { // a maximum does not depend on the order in which it is taken; squares are positive, so their bits compare as they do
+        for (int k = 32; k >= 16; k /= 2) {
+            most = fmaxf(most, __shfl_xor(most, k));
+            most_v = fmaxf(most_v, __shfl_xor(most_v, k));
+        }
+        if (threadIdx.x % 64 == 0) {
+            const uint32_t bits = __builtin_bit_cast(uint32_t, most), bits_v = __builtin_bit_cast(uint32_t, most_v);
+            if (bits > __hip_atomic_load(norms, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) // most waves find a larger one there
+                atomicMax(norms, bits);
+            if (bits_v > __hip_atomic_load(norms + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+                atomicMax(norms + 1, bits_v);
+        }
+    }
+}
+
+// In half precision ds is rounded to 16 bits times the power of two that brings the bound 2 |d_out| |v| of |d_out . v - D| under 2^15, and p
+// times 2^15 in the sums for d_v: small probabilities and gradients would otherwise vanish. The inverse is applied in 32 bits.
+template <class Type>
+__device__ inline float gradient_scale(const uint32_t* norms)
+{
+    if (Type::wide_range)
+        return 1.f;
+    const float bound = 2.f * sqrtf(__builtin_bit_cast(float, norms[0])) * sqrtf(__builtin_bit_cast(float, norms[1]));
+    if (!(bound > 0.f && bound < INFINITY))
+        return 1.f;
+    int e = 14 - ilogbf(bound);
+    e = e > 60 ? 60 : e < -60 ? -60 : e;
+    return ldexpf(1.f, e);
+}
+template <class Type>
+constexpr float P_SHIFT = Type::wide_range ? 0.f : 15.f;
+
+// p and ds of 32 x 32 scores: s and dp in, p (times 2^shift) and ds (times `grow`) out. `lse2(r)`, `delta(r)`, `distance(r)`, `seen(r)` of register r.
+template <class L, class D, class X, class S>
+__device__ inline void score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, float grow, bool masked, L lse2, D delta, X distance,
+                                       S seen)
+{
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        dp[r] = (dp[r] - delta(r)) * grow;
+    float unit = a.scale * LOG2E;
+    if (a.cap > 0.f) {
+        const float in = 2.f * LOG2E * a.scale / a.cap, cap2 = a.cap * LOG2E;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * in));
+            s[r] = cap2 * t;
+            dp[r] *= 1.f - t * t;
+        }
+        unit = 1.f;
+    }
+    if (a.slope) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            s[r] = s[r] * unit - slope2 * fabsf(distance(r));
+        unit = 1.f;
+    }
+    if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const bool there = seen(r);
+            s[r] = there ? s[r] : -INFINITY;
+            dp[r] = there ? dp[r] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(s[r] * unit - (lse2(r) - shift));
+        dp[r] *= s[r];
+    }
+}
+
+template <class Type, int DIM>
+__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Heads d_out, const RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
+                                                               short* d_q, int64_t out_token, int64_t out_head)
+{
+    typedef HeadTile<DIM> Tile;
+    constexpr int KT = KEYS_PER_TILE;
+    __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
+    const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    uint32_t head, tile;
+    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, head, tile);
+    const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
+    int lo, hi, l2, h2;
+    span_of(a, first + lane, lo, hi);
+    span_of(a, first + 64 + lane, l2, h2);
+    const int group_lo = __builtin_amdgcn_readfirstlane(wave_min(min(lo, l2))), group_hi = __builtin_amdgcn_readfirstlane(wave_most(max(hi, h2)));
+    span_of(a, row, lo, hi);
+    const int wave_lo = __builtin_amdgcn_readfirstlane(wave_min(lo)), wave_hi = __builtin_amdgcn_readfirstlane(wave_most(hi));
+    const int all_lo = __builtin_amdgcn_readfirstlane(wave_most(lo)), all_hi = __builtin_amdgcn_readfirstlane(wave_min(hi));
+
+    s16x8 q[DIM / 16], g[DIM / 16];
+    read_rows<DIM>(a.q, head, row, a.tokens, a.dim, lane, q);
+    read_rows<DIM>(d_out, head, row, a.tokens, a.dim, lane, g);
+    float lse2 = INFINITY, delta = 0.f;
+    if (row < a.tokens) {
+        const RowBlock& b = blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS];
+        lse2 = b.lse2[row % BLOCK_ROWS];
+        delta = b.delta[row % BLOCK_ROWS];
+    }
+    const float grow = gradient_scale<Type>(norms);
+    const uint32_t kv = head / a.group;
+    const char* kb = reinterpret_cast<const char*>(static_cast<const short*>(a.k.data) + kv * a.k.head);
+    const char* vb = reinterpret_cast<const char*>(static_cast<const short*>(a.v.data) + kv * a.v.head);
+    HeadLoader<KT, DIM, 4> kl, vl;
+    kl.begin(a.k, a.dim, wave, lane);
+    vl.begin(a.v, a.dim, wave, lane);
+    const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
+    f32x16 o[DIM / 32];
+#pragma unroll
+    for (int e = 0; e < DIM / 32; ++e)
+        o[e] = f32x16{};
+
+    auto turn = [&](const short* ks, const short* vs, int key0) {
+        if (key0 + KT <= wave_lo || key0 >= wave_hi)
+            return;
+        const bool masked = key0 < all_lo || key0 + KT > all_hi;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int d = 0; d < DIM / 16; ++d) {
+                s = Type::mfma32(Tile::along(ks, 32 * t, d, lane), q[d], s);
+                dp = Type::mfma32(Tile::along(vs, 32 * t, d, lane), g[d], dp);
+            }
+            const int key = key0 + 32 * t + 4 * half, i = static_cast<int>(row);
+            score_gradients(
+                a, s, dp, slope2, 0.f, grow, masked, [&](int) { return lse2; }, [&](int) { return delta; },
+                [&](int r) { return static_cast<float>(i - (key + 8 * (r / 4) + r % 4)); },
+                [&](int r) { const int k = key + 8 * (r / 4) + r % 4; return k >= lo && k < hi; });
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const s16x8 ds = round8<Type>(dp, u);
+#pragma unroll
+                for (int e = 0; e < DIM / 32; ++e)
+                    o[e] = Type::mfma32(Tile::across(ks, 32 * t + 16 * u, e, lane), ds, o[e]);
+            }
+        }
+    };
+
+    if (group_lo < group_hi) {
+        const int begin = group_lo / KT * KT;
+        kl.load(kb, begin, a.tokens, k0s, wave);
+        vl.load(vb, begin, a.tokens, v0s, wave);
+        for (int key0 = begin; key0 < group_hi; key0 += 2 * KT) {
+            wait_for_all();
+            meet();
+            kl.load(kb, key0 + KT, a.tokens, k1s, wave);
+            vl.load(vb, key0 + KT, a.tokens, v1s, wave);
+            turn(k0s, v0s, key0);
+            wait_for_all();
+            meet();
+            kl.load(kb, key0 + 2 * KT, a.tokens, k0s, wave);
+            vl.load(vb, key0 + 2 * KT, a.tokens, v0s, wave);
+            turn(k1s, v1s, key0 + KT);
+        }
+        wait_for_all();
+    }
+    if (row < a.tokens) {
+        const float back = a.scale / grow;
+        short* to = d_q + head * out_head + row * out_token;
+#pragma unroll
+        for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int d = 32 * e + 8 * k + 4 * half;
+                if (d < a.dim) {
+                    s16x4 y;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        y[i] = to16<Type>(o[e][4 * k + i] * back);
+                    *reinterpret_cast<s16x4*>(to + d) = y;
+                }
+            }
+    }
+}
+
+constexpr int KEYS_PER_GROUP = 128;
+
+template <class Type, int DIM>
+__global__ __launch_bounds__(256, 1) void attention_d_kv_kernel(Attention a, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
+                                                                const uint32_t* norms, short* d_k, int64_t dk_token, int64_t dk_head, short* d_v,
+                                                                int64_t dv_token, int64_t dv_head)
+{
+    typedef HeadTile<DIM> Tile;
+    constexpr int RT = BLOCK_ROWS;
+    __shared__ __attribute__((aligned(16))) short q0s[RT * DIM], g0s[RT * DIM], q1s[RT * DIM], g1s[RT * DIM];
+    __shared__ __attribute__((aligned(16))) RowBlock b0s, b1s;
+    __shared__ int ends[8];
+    const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t kv_heads = a.q_heads / a.group, kv = blockIdx.x % kv_heads, which = blockIdx.x / kv_heads;
+    const int first = static_cast<int>(which) * KEYS_PER_GROUP, last = min(first + KEYS_PER_GROUP, static_cast<int>(a.tokens)); // keys [first, last)
+    const int key = first + wave * 32 + lane % 32, wave_key = first + wave * 32;
+
+    // The first and the last tile of 64 rows that sees any of these keys.
+    int from = NONE, to = -1;
+    for (uint32_t t = threadIdx.x; t < tiles; t += 256) {
+        const int2 b = bounds[t];
+        if (b.x < last && b.y > first) {
+            from = min(from, static_cast<int>(t));
+            to = max(to, static_cast<int>(t));
+        }
+    }
+    from = wave_min(from);
+    to = wave_most(to);
+    if (lane == 0) {
+        ends[wave] = from;
+        ends[4 + wave] = to;
+    }
+    __syncthreads();
+    from = __builtin_amdgcn_readfirstlane(min(min(ends[0], ends[1]), min(ends[2], ends[3])));
+    to = __builtin_amdgcn_readfirstlane(max(max(ends[4], ends[5]), max(ends[6], ends[7])));
+
+    s16x8 k[DIM / 16], v[DIM / 16];
+    read_rows<DIM>(a.k, kv, key, a.tokens, a.dim, lane, k);
+    read_rows<DIM>(a.v, kv, key, a.tokens, a.dim, lane, v);
+    HeadLoader<RT, DIM, 4> ql, gl;
+    ql.begin(a.q, a.dim, wave, lane);
+    gl.begin(d_out, a.dim, wave, lane);
+    const float grow = gradient_scale<Type>(norms);
+    f32x16 ok[DIM / 32], ov[DIM / 32];
+#pragma unroll
+    for (int e = 0; e < DIM / 32; ++e)
+        ok[e] = ov[e] = f32x16{};
+
+    // Turns: all heads of the group, and of each the tiles from `from` to `to`.
+    const int count = to - from + 1, turns = count > 0 ? count * static_cast<int>(a.group) : 0;
+    auto load = [&](int n, short* qs, short* gs, RowBlock& bs) {
+        const bool there = n < turns;
+        const uint32_t head = kv * a.group + (there ? n / count : 0);
+        const int64_t t = there ? from + n % count : tiles;
+        ql.load(reinterpret_cast<const char*>(static_cast<const short*>(a.q.data) + head * a.q.head), t * RT, a.tokens, qs, wave);
+        gl.load(reinterpret_cast<const char*>(static_cast<const short*>(d_out.data) + head * d_out.head), t * RT, a.tokens, gs, wave);
+        if (wave == 0)
+            load_to_lds(window(blocks + static_cast<int64_t>(head) * tiles + t, there ? sizeof(RowBlock) : 0), &bs, lane * 16);
+    };
+    auto turn = [&](int n, const short* qs, const short* gs, const RowBlock& bs) {
+        if (n >= turns)
+            return;
+        const uint32_t head = kv * a.group + n / count;
+        const int t = from + n % count;
+        const int2 b = bounds[t];
+        if (b.x >= wave_key + 32 || b.y <= wave_key)
+            return;
+        const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) { // 32 rows
+            // do all rows see all of the wave's keys?
+            const int mine = 32 * w + lane % 32;
+            const bool masked = __any(bs.lo[mine] > wave_key || bs.hi[mine] < wave_key + 32);
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int d = 0; d < DIM / 16; ++d) {
+                s = Type::mfma32(Tile::along(qs, 32 * w, d, lane), k[d], s);
+                dp = Type::mfma32(Tile::along(gs, 32 * w, d, lane), v[d], dp);
+            }
+            f32x4 lse2[4], delta[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                lse2[x] = *reinterpret_cast<const f32x4*>(bs.lse2 + 32 * w + 8 * x + 4 * half);
+                delta[x] = *reinterpret_cast<const f32x4*>(bs.delta + 32 * w + 8 * x + 4 * half);
+            }
+            const int row = t * RT + 32 * w + 4 * half;
+            score_gradients(
+                a, s, dp, slope2, P_SHIFT<Type>, grow * (Type::wide_range ? 1.f : 0x1p-15f), masked, [&](int r) { return lse2[r / 4][r % 4]; },
+                [&](int r) { return delta[r / 4][r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
+                [&](int r) {
+                    const int at = 32 * w + 4 * half + 8 * (r / 4) + r % 4;
+                    return key >= bs.lo[at] && key < bs.hi[at];
+                });
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const s16x8 p = round8<Type>(s, u), ds = round8<Type>(dp, u);
+#pragma unroll
+                for (int e = 0; e < DIM / 32; ++e) {
+                    ov[e] = Type::mfma32(Tile::across(gs, 32 * w + 16 * u, e, lane), p, ov[e]);
+                    ok[e] = Type::mfma32(Tile::across(qs, 32 * w + 16 * u, e, lane), ds, ok[e]);
+                }
+            }
+        }
+    };
+
+    if (turns > 0) {
+        load(0, q0s, g0s, b0s);
+        for (int n = 0; n < turns; n += 2) {
+            wait_for_all();
+            meet();
+            load(n + 1, q1s, g1s, b1s);
+            turn(n, q0s, g0s, b0s);
+            wait_for_all();
+            meet();
+            load(n + 2, q0s, g0s, b0s);
+            turn(n + 1, q1s, g1s, b1s);
+        }
+        wait_for_all();
+    }
+    if (key < a.tokens) {
+        const float back_k = a.scale / grow, back_v = Type::wide_range ? 1.f : 0x1p-15f;
+        short* kt = d_k + kv * dk_head + static_cast<int64_t>(key) * dk_token;
+        short* vt = d_v + kv * dv_head + static_cast<int64_t>(key) * dv_token;
+#pragma unroll
+        for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * e + 8 * x + 4 * half;
+                if (d < a.dim) {
+                    s16x4 y, z;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[i] = to16<Type>(ok[e][4 * x + i] * back_k);
+                        z[i] = to16<Type>(ov[e][4 * x + i] * back_v);
+                    }
+                    *reinterpret_cast<s16x4*>(kt + d) = y;
+                    *reinterpret_cast<s16x4*>(vt + d) = z;
+                }
+            }
+    }
+}
+
+} // namespace lm

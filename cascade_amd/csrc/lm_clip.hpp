@@ -1,0 +1,153 @@
+// The global norm of a list of gradients and their clipping: norm = sqrt(sum of all squares), every value times min(1, max_norm / norm).
+//
+// Bound by memory: all values are read once for the norm and once more, and written, for the product. Squares are summed in 64
+// bits (no overflow, and nothing lost over 1e9 values), in a fixed order without atomics: a workgroup's chunks, then the
+// workgroups' sums, which every workgroup of the second kernel adds up again by itself instead of waiting for a third launch.
+// The second kernel walks the chunks from the last to the first, so that it meets what the first has left in the
+// 256 MB of the last-level cache.
+#pragma once
+#include "lm_common.hpp"
+
+namespace lm {
+
+constexpr int CLIP_TENSORS = 112;        // a launch's list travels in its arguments, 4 KB at most
+constexpr int CLIP_CHUNK = 16384;        // values
+constexpr uint32_t CLIP_GROUPS = 2048;   // workgroups and partial sums
+
+struct ClipList {
+    const void* in[CLIP_TENSORS];
+    void* out[CLIP_TENSORS];
+    uint64_t n[CLIP_TENSORS];
+    uint32_t first[CLIP_TENSORS + 1]; // chunk
+    uint8_t type[CLIP_TENSORS];       // 0 bf16, 1 f16, 2 f32
+    uint8_t wide[CLIP_TENSORS];       // 16-byte accesses
+    uint32_t count;
+};
+static_assert(sizeof(ClipList) <= 3900, "kernel arguments");
+
+__device__ inline uint32_t tensor_of(const ClipList& list, uint32_t chunk)
+{
+    uint32_t lo = 0, hi = list.count - 1; // the last tensor that begins at or before the chunk
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (list.first[mid] <= chunk)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+template <class T>
+__device__ inline double chunk_squares(const T* p, uint64_t n, bool wide)
+{
+    constexpr int V = 16 / sizeof(T);
+    double sum = 0, sum2 = 0;
+    uint64_t i = threadIdx.x * V;
+    if (wide) {
+        for (; i + V <= n; i += 256 * V) {
+            const u32x4 raw = *reinterpret_cast<const u32x4*>(p + i);
+            T x[V];
+            __builtin_memcpy(x, &raw, 16);
+#pragma unroll
+            for (int k = 0; k < V; k += 2) {
+                const double a = static_cast<double>(static_cast<float>(x[k])), b = static_cast<double>(static_cast<float>(x[k + 1]));
+                sum += a * a;
+                sum2 += b * b;
+            }
+        }
+        for (uint64_t k = i; k < n && k < i + V; ++k) {
+            const double a = static_cast<double>(static_cast<float>(p[k]));
+            sum += a * a;
+        }
+    } else {
+        for (uint64_t k = threadIdx.x; k < n; k += 256) {
+            const double a = static_cast<double>(static_cast<float>(p[k]));
+            sum += a * a;
+        }
+    }
+    return sum + sum2;
+}
+
+__device__ inline double workgroup_sum(double x, double* lds)
+{
+    for (int d = 32; d; d /= 2)
+        x += __shfl_xor(x, d);
+    if (threadIdx.x % 64 == 0)
+        lds[threadIdx.x / 64] = x;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+__global__ __launch_bounds__(256) void squares_kernel(ClipList list, double* partial)
+{
+    __shared__ double lds[4];
+    double sum = 0;
+    const uint32_t chunks = list.first[list.count];
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const uint32_t t = tensor_of(list, c);
+        const uint64_t at = static_cast<uint64_t>(c - list.first[t]) * CLIP_CHUNK, left = list.n[t] - at, n = left < CLIP_CHUNK ? left : CLIP_CHUNK;
+        if (list.type[t] == 2)
+            sum += chunk_squares(static_cast<const float*>(list.in[t]) + at, n, list.wide[t]);
+        else if (list.type[t] == 1)
+            sum += chunk_squares(static_cast<const f16_t*>(list.in[t]) + at, n, list.wide[t]);
+        else
+            sum += chunk_squares(static_cast<const bf16_t*>(list.in[t]) + at, n, list.wide[t]);
+    }
+    sum = workgroup_sum(sum, lds);
+    if (threadIdx.x == 0)
+        partial[blockIdx.x] = sum;
+}
+
+template <class T>
+__device__ inline void scale_chunk(const T* in, T* out, uint64_t n, bool wide, float factor)
+{
+    constexpr int V = 16 / sizeof(T);
+    if (wide) {
+        uint64_t i = threadIdx.x * V;
+        for (; i + V <= n; i += 256 * V) {
+            u32x4 raw = *reinterpret_cast<const u32x4*>(in + i);
+            T x[V];
+            __builtin_memcpy(x, &raw, 16);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                x[k] = static_cast<T>(static_cast<float>(x[k]) * factor);
+            __builtin_memcpy(&raw, x, 16);
+            *reinterpret_cast<u32x4*>(out + i) = raw;
+        }
+        for (uint64_t k = i; k < n && k < i + V; ++k)
+            out[k] = static_cast<T>(static_cast<float>(in[k]) * factor);
+    } else {
+        for (uint64_t k = threadIdx.x; k < n; k += 256)
+            out[k] = static_cast<T>(static_cast<float>(in[k]) * factor);
+    }
+}
+
+__global__ __launch_bounds__(256) void clip_kernel(ClipList list, const double* partial, uint32_t partials, float max_norm, float* norm_out)
+{
+    __shared__ double lds[4];
+    double sum = 0;
+    for (uint32_t p = threadIdx.x; p < partials; p += 256)
+        sum += partial[p];
+    sum = workgroup_sum(sum, lds);
+    const double norm = sqrt(sum);
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0)
+        *norm_out = static_cast<float>(norm);
+    // no finite norm, no direction to keep: the values stay, and the norm says so
+    const float factor = norm > max_norm && norm < static_cast<double>(INFINITY) ? static_cast<float>(max_norm / norm) : 1.f;
+    const uint32_t chunks = list.first[list.count];
+    for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
+        const uint32_t c = chunks - 1 - k, t = tensor_of(list, c);
+        if (factor == 1.f && list.in[t] == list.out[t])
+            continue;
+        const uint64_t at = static_cast<uint64_t>(c - list.first[t]) * CLIP_CHUNK, left = list.n[t] - at, n = left < CLIP_CHUNK ? left : CLIP_CHUNK;
+        if (list.type[t] == 2)
+            scale_chunk(static_cast<const float*>(list.in[t]) + at, static_cast<float*>(list.out[t]) + at, n, list.wide[t], factor);
+        else if (list.type[t] == 1)
+            scale_chunk(static_cast<const f16_t*>(list.in[t]) + at, static_cast<f16_t*>(list.out[t]) + at, n, list.wide[t], factor);
+        else
+            scale_chunk(static_cast<const bf16_t*>(list.in[t]) + at, static_cast<bf16_t*>(list.out[t]) + at, n, list.wide[t], factor);
+    }
+}
+
+} // namespace lm
