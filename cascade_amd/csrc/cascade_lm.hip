@@ -113,15 +113,27 @@ Attention attention(const csa_lm_attention& a)
             static_cast<int>(a.head_dim), a.scale, a.cap};
 }
 
+// Heads of q that share one of k and v are shared out over workgroups, each with sums of its own that are joined at the end, until there are
+// KV_GROUPS workgroups: a workgroup fills a compute unit, and those of a causal text differ in work by as much as their keys.
+constexpr uint64_t KV_GROUPS = 2048;
+
+int head_width(uint64_t dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+
 struct AttentionWork {
     uint32_t* norms;
     int2* bounds;
     RowBlock* blocks;
+    float* parts;
+    uint32_t shares, share_heads;
     uint64_t bytes;
-    AttentionWork(void* base, uint64_t tokens, uint64_t q_heads)
+    AttentionWork(void* base, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim)
     {
         Carver c{static_cast<char*>(base)};
-        const uint64_t tiles = parts_of(tokens, BLOCK_ROWS);
+        const uint64_t tiles = parts_of(tokens, BLOCK_ROWS), group = q_heads / kv_heads, groups = parts_of(tokens, KEYS_PER_GROUP) * kv_heads;
+        const uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1;
+        share_heads = static_cast<uint32_t>(want < group ? group / want : 1);
+        shares = static_cast<uint32_t>(parts_of(group, share_heads));
+        parts = c.take<float>(shares > 1 ? 2 * shares * kv_heads * tokens * head_width(dim) : 0);
         norms = c.take<uint32_t>(2);
         bounds = c.take<int2>(tiles);
         blocks = c.take<RowBlock>(tiles * q_heads);
@@ -146,17 +158,21 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
     attention_d_q_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
         at, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
-    attention_d_kv_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads), 256, 0, s>>>(
-        at, heads(d_out), w.blocks, w.bounds, tiles, w.norms, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride,
-        static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
+    attention_d_kv_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
+        at, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.share_heads, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
+        d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
+    if (w.shares > 1)
+        join_heads_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.kv_heads, 2), 256, 0, s>>>(
+            w.parts, w.shares, at.tokens, at.dim, DIM, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride, static_cast<short*>(d_v.data),
+            d_v.token_stride, d_v.head_stride);
 }
 
 template <class F>
 void with_dim(uint32_t dim, F f)
 {
-    if (dim <= 64)
+    if (head_width(dim) == 64)
         f(std::integral_constant<int, 64>());
-    else if (dim <= 96)
+    else if (head_width(dim) == 96)
         f(std::integral_constant<int, 96>());
     else
         f(std::integral_constant<int, 128>());
@@ -370,7 +386,10 @@ int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, fl
     return launched(who);
 }
 
-uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads) { return AttentionWork(nullptr, tokens, q_heads).bytes; }
+uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim)
+{
+    return kv_heads ? AttentionWork(nullptr, tokens, q_heads, kv_heads, head_dim).bytes : 0;
+}
 
 int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, const float* d_lse, csa_lm_heads d_out, csa_lm_heads d_q, csa_lm_heads d_k,
                                   csa_lm_heads d_v, void* d_work, uint64_t work_bytes, void* stream)
@@ -389,7 +408,7 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
             return rc;
     if (!d_lse || !aligned(d_lse, 4))
         return fail(CSA_ERR_ARG, "%s: d_lse is null or unaligned", who);
-    const AttentionWork w(d_work, a->tokens, a->q_heads);
+    const AttentionWork w(d_work, a->tokens, a->q_heads, a->kv_heads, a->head_dim);
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -44,19 +44,26 @@ struct HeadTile {
     {
         return PIECES % 8 == 0 ? piece ^ ((row & 3) * 2 | (row >> 2 & 1)) : piece ^ ((row >> 1 & 1) * 2 | (row >> 2 & 1));
     }
-    // Operand with the head's values along k: 32 rows, values 16 step ... of them
-    static __device__ s16x8 along(const short* tile, int row0, int step, int lane)
+    // A lane's reads start at two places of a tile. `place` changes bits of the piece within a run of `TURN + 1` values only, and a row is a whole
+    // number of runs, so the pieces of a row are reached by flipping bits of the place and by offsets that instructions hold.
+    static constexpr int TURN = PIECES % 8 == 0 ? 63 : 31;
+    int along_, across_;
+    __device__ explicit HeadTile(int lane)
     {
-        const int row = row0 + lane % 32;
-        return read16(tile + row * DIM + place(row, step * 2 + lane / 32) * 8);
+        const int row = lane % 32, g = lane / 16, j = lane % 16, line = 4 * (g / 2) + j / 4, col = (g % 2) * 16 + 4 * (j % 4);
+        along_ = row * DIM + place(row, lane / 32) * 8;
+        across_ = line * DIM + place(line, col / 8) * 8 + col % 8;
+    }
+    // Operand with the head's values along k: rows row0 ... row0 + 31, values 16 step ... of them
+    __device__ s16x8 along(const short* tile, int row0, int step) const
+    {
+        return read16(tile + (along_ ^ (step * 16 & TURN)) + (step * 16 & ~TURN) + row0 * DIM);
     }
     // Operand with the rows along k in the order of the registers above: values 32 e ... 32 e + 31 of the head, rows row0 ... row0 + 15
-    static __device__ s16x8 across(const short* tile, int row0, int e, int lane)
+    __device__ s16x8 across(const short* tile, int row0, int e) const
     {
-        const int g = lane / 16, j = lane % 16, col = 32 * e + (g % 2) * 16 + 4 * (j % 4);
-        const int row = row0 + 4 * (g / 2) + j / 4;
-        return join(read_turned(tile + row * DIM + place(row, col / 8) * 8 + col % 8),
-                    read_turned(tile + (row + 8) * DIM + place(row + 8, col / 8) * 8 + col % 8));
+        const short* p = tile + (across_ ^ (e * 32 & TURN)) + (e * 32 & ~TURN) + row0 * DIM;
+        return join(read_turned(p), read_turned(p + 8 * DIM));
     }
 };
 
@@ -146,6 +153,17 @@ __device__ inline void place_of(uint32_t id, uint32_t heads, uint32_t tiles, uin
     tile = tiles - 1 - id / heads;
 }
 
+// What round8 left of registers 8 u ... 8 u + 7 (zeros elsewhere)
+template <class Type>
+__device__ inline f32x16 widen(const s16x8& x, int u)
+{
+    f32x16 y = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        y[8 * u + i] = to32<Type>(x[i]);
+    return y;
+}
+
 constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
 
 // Scores of a tile, still raw products: to exponents of 2 less nothing, with `unit` left to multiply. Returns with z = s * unit.
@@ -177,7 +195,7 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
 template <class Type, int DIM>
 __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, short* out, int64_t out_token, int64_t out_head, float* lse)
 {
-    typedef HeadTile<DIM> Tile;
+    const HeadTile<DIM> tiles_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -219,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
             s[t] = f32x16{};
 #pragma unroll
             for (int d = 0; d < DIM / 16; ++d)
-                s[t] = Type::mfma32(Tile::along(ks, 32 * t, d, lane), q[d], s[t]);
+                s[t] = Type::mfma32(tiles_at.along(ks, 32 * t, d), q[d], s[t]);
         }
         float unit;
         bend(a, s, unit, slope2, static_cast<int>(row), key0, half);
@@ -264,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
                 const s16x8 p = round8<Type>(s[t], u);
 #pragma unroll
                 for (int e = 0; e < DIM / 32; ++e)
-                    o[e] = Type::mfma32(Tile::across(vs, 32 * t + 16 * u, e, lane), p, o[e]);
+                    o[e] = Type::mfma32(tiles_at.across(vs, 32 * t + 16 * u, e), p, o[e]);
             }
     };
 
@@ -412,10 +430,12 @@ template <class Type>
 constexpr float P_SHIFT = Type::wide_range ? 0.f : 15.f;
 
 // p and ds of 32 x 32 scores: s and dp in, p (times 2^shift) and ds (times `grow`) out. `lse2(r)`, `delta(r)`, `distance(r)`, `seen(r)` of register r.
-template <class L, class D, class X, class S>
-__device__ inline void score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, float grow, bool masked, L lse2, D delta, X distance,
-                                       S seen)
+// With REST, returns the sum of p (dp - delta) over the lane's registers, times both factors.
+template <bool REST, class L, class D, class X, class S>
+__device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, float grow, bool masked, L lse2, D delta, X distance,
+                                        S seen)
 {
+    f32x16 bent;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
         dp[r] = (dp[r] - delta(r)) * grow;
@@ -426,7 +446,10 @@ __device__ inline void score_gradients(const Attention& a, f32x16& s, f32x16& dp
         for (int r = 0; r < 16; ++r) {
             const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * in));
             s[r] = cap2 * t;
-            dp[r] *= 1.f - t * t;
+            if (REST)
+                bent[r] = 1.f - t * t;
+            else
+                dp[r] *= 1.f - t * t;
         }
         unit = 1.f;
     }
@@ -449,13 +472,25 @@ __device__ inline void score_gradients(const Attention& a, f32x16& s, f32x16& dp
         s[r] = __builtin_amdgcn_exp2f(s[r] * unit - (lse2(r) - shift));
         dp[r] *= s[r];
     }
+    float sum = 0.f;
+    if (!REST)
+        return sum;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        sum += dp[r];
+    if (a.cap > 0.f) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            dp[r] *= bent[r];
+    }
+    return sum;
 }
 
 template <class Type, int DIM>
-__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Heads d_out, const RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
+__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Heads d_out, RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
                                                                short* d_q, int64_t out_token, int64_t out_head)
 {
-    typedef HeadTile<DIM> Tile;
+    const HeadTile<DIM> tiles_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -491,6 +526,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
 #pragma unroll
     for (int e = 0; e < DIM / 32; ++e)
         o[e] = f32x16{};
+    float rest = 0.f; // sum of p (dp - D), which would be 0 if D were exact
 
     auto turn = [&](const short* ks, const short* vs, int key0) {
         if (key0 + KT <= wave_lo || key0 >= wave_hi)
@@ -501,20 +537,23 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
             f32x16 s = {}, dp = {};
 #pragma unroll
             for (int d = 0; d < DIM / 16; ++d) {
-                s = Type::mfma32(Tile::along(ks, 32 * t, d, lane), q[d], s);
-                dp = Type::mfma32(Tile::along(vs, 32 * t, d, lane), g[d], dp);
+                s = Type::mfma32(tiles_at.along(ks, 32 * t, d), q[d], s);
+                dp = Type::mfma32(tiles_at.along(vs, 32 * t, d), g[d], dp);
             }
             const int key = key0 + 32 * t + 4 * half, i = static_cast<int>(row);
-            score_gradients(
+            rest += score_gradients<true>(
                 a, s, dp, slope2, 0.f, grow, masked, [&](int) { return lse2; }, [&](int) { return delta; },
                 [&](int r) { return static_cast<float>(i - (key + 8 * (r / 4) + r % 4)); },
                 [&](int r) { const int k = key + 8 * (r / 4) + r % 4; return k >= lo && k < hi; });
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const s16x8 ds = round8<Type>(dp, u);
+                const s16x8 ds = round8<Type>(dp, u), low = round8<Type>(dp - widen<Type>(ds, u), u);
 #pragma unroll
-                for (int e = 0; e < DIM / 32; ++e)
-                    o[e] = Type::mfma32(Tile::across(ks, 32 * t + 16 * u, e, lane), ds, o[e]);
+                for (int e = 0; e < DIM / 32; ++e) {
+                    const s16x8 f = tiles_at.across(ks, 32 * t + 16 * u, e);
+                    o[e] = Type::mfma32(f, ds, o[e]);
+                    o[e] = Type::mfma32(f, low, o[e]);
+                }
             }
         }
     };
@@ -537,7 +576,10 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
         }
         wait_for_all();
     }
+    rest += other_half(rest);
     if (row < a.tokens) {
+        if (half == 0)
+            blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = delta + rest / grow;
         const float back = a.scale / grow;
         short* to = d_q + head * out_head + row * out_token;
 #pragma unroll
@@ -558,18 +600,30 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
 
 constexpr int KEYS_PER_GROUP = 128;
 
-template <class Type, int DIM>
-__global__ __launch_bounds__(256, 1) void attention_d_kv_kernel(Attention a, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
-                                                                const uint32_t* norms, short* d_k, int64_t dk_token, int64_t dk_head, short* d_v,
-                                                                int64_t dv_token, int64_t dv_head)
+// x, as something that the compiler cannot tell from a new value: what is made of it is made again where it is used instead of being kept
+// in registers throughout a loop.
+__device__ inline int again(int x)
 {
-    typedef HeadTile<DIM> Tile;
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+template <class Type, int DIM>
+__global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
+                                                                const uint32_t* norms, uint32_t shares, uint32_t share_heads, float* parts, short* d_k,
+                                                                int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
+{
+    const HeadTile<DIM> tiles_at(threadIdx.x % 64);
     constexpr int RT = BLOCK_ROWS;
     __shared__ __attribute__((aligned(16))) short q0s[RT * DIM], g0s[RT * DIM], q1s[RT * DIM], g1s[RT * DIM];
     __shared__ __attribute__((aligned(16))) RowBlock b0s, b1s;
     __shared__ int ends[8];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t kv_heads = a.q_heads / a.group, kv = blockIdx.x % kv_heads, which = blockIdx.x / kv_heads;
+    const uint32_t kv_heads = a.q_heads / a.group, units = kv_heads * shares;
+    uint32_t unit, which;
+    place_of(blockIdx.x, units, gridDim.x / units, unit, which);
+    which = gridDim.x / units - 1 - which; // the first keys, which causal rows see most of, first
+    const uint32_t kv = unit / shares, head0 = kv * a.group + unit % shares * share_heads, heads = min(share_heads, kv * a.group + a.group - head0);
     const int first = static_cast<int>(which) * KEYS_PER_GROUP, last = min(first + KEYS_PER_GROUP, static_cast<int>(a.tokens)); // keys [first, last)
     const int key = first + wave * 32 + lane % 32, wave_key = first + wave * 32;
 
@@ -595,69 +649,71 @@ __global__ __launch_bounds__(256, 1) void attention_d_kv_kernel(Attention a, Hea
     s16x8 k[DIM / 16], v[DIM / 16];
     read_rows<DIM>(a.k, kv, key, a.tokens, a.dim, lane, k);
     read_rows<DIM>(a.v, kv, key, a.tokens, a.dim, lane, v);
-    HeadLoader<RT, DIM, 4> ql, gl;
-    ql.begin(a.q, a.dim, wave, lane);
-    gl.begin(d_out, a.dim, wave, lane);
     const float grow = gradient_scale<Type>(norms);
     f32x16 ok[DIM / 32], ov[DIM / 32];
 #pragma unroll
     for (int e = 0; e < DIM / 32; ++e)
         ok[e] = ov[e] = f32x16{};
 
-    // Turns: all heads of the group, and of each the tiles from `from` to `to`.
-    const int count = to - from + 1, turns = count > 0 ? count * static_cast<int>(a.group) : 0;
+    // Turns: the heads of this share, and of each the tiles from `from` to `to`.
+    const int count = to - from + 1, turns = count > 0 ? count * static_cast<int>(heads) : 0;
     auto load = [&](int n, short* qs, short* gs, RowBlock& bs) {
         const bool there = n < turns;
-        const uint32_t head = kv * a.group + (there ? n / count : 0);
+        const uint32_t head = head0 + (there ? n / count : 0);
         const int64_t t = there ? from + n % count : tiles;
+        HeadLoader<RT, DIM, 4> ql, gl;
+        ql.begin(a.q, a.dim, wave, again(lane));
+        gl.begin(d_out, a.dim, wave, again(lane));
         ql.load(reinterpret_cast<const char*>(static_cast<const short*>(a.q.data) + head * a.q.head), t * RT, a.tokens, qs, wave);
         gl.load(reinterpret_cast<const char*>(static_cast<const short*>(d_out.data) + head * d_out.head), t * RT, a.tokens, gs, wave);
         if (wave == 0)
             load_to_lds(window(blocks + static_cast<int64_t>(head) * tiles + t, there ? sizeof(RowBlock) : 0), &bs, lane * 16);
     };
+    auto scores = [&](const short* qs, const short* gs, int w, f32x16& s, f32x16& dp) {
+#pragma unroll
+        for (int d = 0; d < DIM / 16; ++d) {
+            s = Type::mfma32(tiles_at.along(qs, 32 * w, d), k[d], s);
+            dp = Type::mfma32(tiles_at.along(gs, 32 * w, d), v[d], dp);
+        }
+    };
+    auto sums = [&](const short* qs, const short* gs, int w, const s16x8 (&p)[2], const s16x8 (&ds)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < DIM / 32; ++e) {
+                ov[e] = Type::mfma32(tiles_at.across(gs, 32 * w + 16 * u, e), p[u], ov[e]);
+                ok[e] = Type::mfma32(tiles_at.across(qs, 32 * w + 16 * u, e), ds[u], ok[e]);
+            }
+    };
+    const float grow_k = grow * (Type::wide_range ? 1.f : 0x1p-15f);
     auto turn = [&](int n, const short* qs, const short* gs, const RowBlock& bs) {
         if (n >= turns)
             return;
-        const uint32_t head = kv * a.group + n / count;
-        const int t = from + n % count;
-        const int2 b = bounds[t];
-        if (b.x >= wave_key + 32 || b.y <= wave_key)
+        // which of the 64 rows see any of the wave's 32 keys, and which do not see all of them
+        const int lo = bs.lo[lane], hi = bs.hi[lane];
+        const uint64_t some = __ballot(lo < wave_key + 32 && hi > wave_key), less = __ballot(lo > wave_key || hi < wave_key + 32);
+        if (!some)
             return;
+        const uint32_t head = head0 + n / count;
+        const int t = from + n % count;
         const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < 2; ++w) { // 32 rows
-            // do all rows see all of the wave's keys?
-            const int mine = 32 * w + lane % 32;
-            const bool masked = __any(bs.lo[mine] > wave_key || bs.hi[mine] < wave_key + 32);
+            if (!static_cast<uint32_t>(some >> 32 * w))
+                continue;
+            const bool masked = static_cast<uint32_t>(less >> 32 * w);
             f32x16 s = {}, dp = {};
-#pragma unroll
-            for (int d = 0; d < DIM / 16; ++d) {
-                s = Type::mfma32(Tile::along(qs, 32 * w, d, lane), k[d], s);
-                dp = Type::mfma32(Tile::along(gs, 32 * w, d, lane), v[d], dp);
-            }
-            f32x4 lse2[4], delta[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                lse2[x] = *reinterpret_cast<const f32x4*>(bs.lse2 + 32 * w + 8 * x + 4 * half);
-                delta[x] = *reinterpret_cast<const f32x4*>(bs.delta + 32 * w + 8 * x + 4 * half);
-            }
+            scores(qs, gs, w, s, dp);
             const int row = t * RT + 32 * w + 4 * half;
-            score_gradients(
-                a, s, dp, slope2, P_SHIFT<Type>, grow * (Type::wide_range ? 1.f : 0x1p-15f), masked, [&](int r) { return lse2[r / 4][r % 4]; },
-                [&](int r) { return delta[r / 4][r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
+            score_gradients<false>(
+                a, s, dp, slope2, P_SHIFT<Type>, grow_k, masked, [&](int r) { return bs.lse2[32 * w + 4 * half + 8 * (r / 4) + r % 4]; },
+                [&](int r) { return bs.delta[32 * w + 4 * half + 8 * (r / 4) + r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
                 [&](int r) {
                     const int at = 32 * w + 4 * half + 8 * (r / 4) + r % 4;
                     return key >= bs.lo[at] && key < bs.hi[at];
                 });
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const s16x8 p = round8<Type>(s, u), ds = round8<Type>(dp, u);
-#pragma unroll
-                for (int e = 0; e < DIM / 32; ++e) {
-                    ov[e] = Type::mfma32(Tile::across(gs, 32 * w + 16 * u, e, lane), p, ov[e]);
-                    ok[e] = Type::mfma32(Tile::across(qs, 32 * w + 16 * u, e, lane), ds, ok[e]);
-                }
-            }
+            const s16x8 p[2] = {round8<Type>(s, 0), round8<Type>(s, 1)}, ds[2] = {round8<Type>(dp, 0), round8<Type>(dp, 1)};
+            sums(qs, gs, w, p, ds);
         }
     };
 
@@ -677,6 +733,24 @@ __global__ __launch_bounds__(256, 1) void attention_d_kv_kernel(Attention a, Hea
     }
     if (key < a.tokens) {
         const float back_k = a.scale / grow, back_v = Type::wide_range ? 1.f : 0x1p-15f;
+        if (shares > 1) {
+            float* to = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
+#pragma unroll
+            for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    f32x4 y, z;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[i] = ok[e][4 * x + i] * back_k;
+                        z[i] = ov[e][4 * x + i] * back_v;
+                    }
+                    const int d = 32 * e + 8 * x + 4 * half;
+                    *reinterpret_cast<f32x4*>(to + d) = y;
+                    *reinterpret_cast<f32x4*>(to + a.tokens * DIM + d) = z;
+                }
+            return;
+        }
         short* kt = d_k + kv * dk_head + static_cast<int64_t>(key) * dk_token;
         short* vt = d_v + kv * dv_head + static_cast<int64_t>(key) * dv_token;
 #pragma unroll
@@ -696,6 +770,29 @@ __global__ __launch_bounds__(256, 1) void attention_d_kv_kernel(Attention a, Hea
                 }
             }
     }
+}
+
+// d_k (blockIdx.z 0) and d_v (1) of a head from its shares, four values a thread.
+template <class Type>
+__global__ __launch_bounds__(256) void join_heads_kernel(const float* parts, uint32_t shares, int64_t tokens, int dim, int width, short* d_k, int64_t dk_token,
+                                                         int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
+{
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int quads = dim / 4;
+    if (at >= tokens * quads)
+        return;
+    const int64_t token = at / quads;
+    const int d = static_cast<int>(at % quads) * 4;
+    const uint32_t kv = blockIdx.y, which = blockIdx.z;
+    f32x4 sum = {};
+    for (uint32_t i = 0; i < shares; ++i)
+        sum += *reinterpret_cast<const f32x4*>(parts + ((static_cast<int64_t>(kv * shares + i) * 2 + which) * tokens + token) * width + d);
+    s16x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y[i] = to16<Type>(sum[i]);
+    short* to = which ? d_v + kv * dv_head + token * dv_token : d_k + kv * dk_head + token * dk_token;
+    *reinterpret_cast<s16x4*>(to + d) = y;
 }
 
 } // namespace lm

@@ -159,7 +159,7 @@ def span_attention_backward(d_out, q, k, v, out, lse, lo=None, hi=None, scale=No
     d_q, d_k, d_v = (torch.empty(x.shape, dtype=q.dtype, device=device) for x in (q, k, v))
     if q.shape[0]:
         lib = native.load()
-        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1])
+        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1], k.shape[1], q.shape[2])
         work = _work(size, device)
         with _Call(device) as stream:
             native.check(lib.csa_lm_attention_backward_dev(C.byref(a), _heads(out), lse.data_ptr(), _heads(d_out), _heads(d_q), _heads(d_k), _heads(d_v),

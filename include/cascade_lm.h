@@ -66,7 +66,7 @@ int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, fl
 
 /* Gradients of q, k and v for the gradient d_out of out; out and d_lse as the forward call left them. Gradients of a head of k and v are summed
  * over the heads of q that share it. A key that no row sees gets zeros. */
-uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads);
+uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim);
 int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, const float* d_lse, csa_lm_heads d_out, csa_lm_heads d_q,
                                   csa_lm_heads d_k, csa_lm_heads d_v, void* d_work, uint64_t work_bytes, void* stream);
 

@@ -500,6 +500,6 @@ def test_the_library_refuses_what_the_kernels_cannot_read():
     assert call(tokens=(1 << 30) + 1) == -2
     work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
     a = native.CsaLmAttention(0, 2, 2, 64, 64, None, None, None, 1.0, 0.0, heads, heads, heads)
-    need = lib.csa_lm_attention_workspace(64, 2)
+    need = lib.csa_lm_attention_workspace(64, 2, 2, 64)
     assert lib.csa_lm_attention_backward_dev(C.byref(a), heads, lse.data_ptr(), heads, heads, heads, heads, work.data_ptr(), need - 1, None) == -1
     assert b"workspace" in lib.csa_lm_last_error()
