@@ -154,7 +154,7 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
 {
     const Attention at = attention(a);
     const uint32_t tiles = static_cast<uint32_t>(parts_of(a.tokens, BLOCK_ROWS));
-    span_bounds_kernel<<<tiles, 64, 0, s>>>(at, w.bounds, w.norms);
+    span_bounds_kernel<<<static_cast<uint32_t>(parts_of(a.tokens, 64)), 64, 0, s>>>(at, w.bounds, w.norms);
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
     attention_d_q_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
         at, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);

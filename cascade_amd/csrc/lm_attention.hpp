@@ -14,7 +14,7 @@
 //                    them, so nothing is added by atomics and the results do not depend on the order of workgroups. The scores are
 //                    computed twice for that, once here and once for d_q (seven products instead of five).
 // Tiles of keys or rows come straight from memory into LDS, one tile ahead. The 16-byte pieces of a tile's row stand at
-// places that keep both kinds of reads, eight rows' same piece and four rows' neighbouring pieces, in different banks.
+// places that keep both kinds of reads, sixteen rows' same piece and four rows' neighbouring pieces, in different banks.
 #pragma once
 #include "lm_common.hpp"
 
@@ -35,18 +35,27 @@ struct Attention {
     float scale, cap;
 };
 
+// x, as something that the compiler cannot tell from a new value: what is made of it is made again where it is used instead of being kept in
+// registers throughout a loop.
+__device__ inline int again(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 template <int DIM>
 struct HeadTile {
     static constexpr int PIECES = DIM / 8;
-    // Place of a row's 16-byte piece: rows 0 to 7 put the same piece at eight places of 128 bytes, and the pairs of pieces of rows 4 a ... 4 a + 3
-    // at four. Rows of 12 pieces alternate between two of the eight places already.
+    // Place of a row's 16-byte piece. LDS serves 256 bytes at a time: sixteen lanes that read the same piece of sixteen rows meet sixteen places
+    // of it, and so do 32 lanes that read half pieces, two by two pieces of four rows.
     static __device__ int place(int row, int piece)
     {
-        return PIECES % 8 == 0 ? piece ^ ((row & 3) * 2 | (row >> 2 & 1)) : piece ^ ((row >> 1 & 1) * 2 | (row >> 2 & 1));
+        const int turn = row >> 2 & 3;
+        return piece ^ (PIECES == 16 ? (row & 3) * 4 | turn : PIECES == 8 ? (row >> 1 & 1) * 4 | turn : turn);
     }
     // A lane's reads start at two places of a tile. `place` changes bits of the piece within a run of `TURN + 1` values only, and a row is a whole
     // number of runs, so the pieces of a row are reached by flipping bits of the place and by offsets that instructions hold.
-    static constexpr int TURN = PIECES % 8 == 0 ? 63 : 31;
+    static constexpr int TURN = PIECES == 16 ? 127 : PIECES == 8 ? 63 : 31;
     int along_, across_;
     __device__ explicit HeadTile(int lane)
     {
@@ -54,6 +63,8 @@ struct HeadTile {
         along_ = row * DIM + place(row, lane / 32) * 8;
         across_ = line * DIM + place(line, col / 8) * 8 + col % 8;
     }
+    __device__ HeadTile(int along, int across) : along_(along), across_(across) {}
+    __device__ HeadTile afresh() const { return {again(along_), again(across_)}; }
     // Operand with the head's values along k: rows row0 ... row0 + 31, values 16 step ... of them
     __device__ s16x8 along(const short* tile, int row0, int step) const
     {
@@ -62,23 +73,24 @@ struct HeadTile {
     // Operand with the rows along k in the order of the registers above: values 32 e ... 32 e + 31 of the head, rows row0 ... row0 + 15
     __device__ s16x8 across(const short* tile, int row0, int e) const
     {
-        const short* p = tile + (across_ ^ (e * 32 & TURN)) + (e * 32 & ~TURN) + row0 * DIM;
-        return join(read_turned(p), read_turned(p + 8 * DIM));
+        const short* p = tile + (e * 32 & ~TURN) + row0 * DIM;
+        const int at = across_ ^ (e * 32 & TURN); // eight rows on, `turn` differs by 2
+        return join(read_turned(p + at), read_turned(p + (at ^ 16) + 8 * DIM));
     }
 };
 
 // ROWS rows of one head, padded to DIM values with zeros, by WAVES waves.
 template <int ROWS, int DIM, int WAVES>
 struct HeadLoader {
-    static constexpr int LOADS = ROWS * DIM / 8 / 64 / WAVES;
-    static_assert(ROWS * DIM / 8 % (64 * WAVES) == 0, "every wave loads as much");
+    static constexpr int TOTAL = ROWS * DIM / 8 / 64, LOADS = (TOTAL + WAVES - 1) / WAVES; // instructions, of all waves and of one
+    static_assert(ROWS * DIM / 8 % 64 == 0, "whole waves");
     int64_t line; // bytes
     uint32_t offset[LOADS];
     __device__ void begin(const Heads& h, int dim, int wave, int lane)
     {
         line = h.token * 2;
         for (int j = 0; j < LOADS; ++j) {
-            const int at = (wave * LOADS + j) * 64 + lane, row = at / (DIM / 8), piece = HeadTile<DIM>::place(row, at % (DIM / 8));
+            const int at = (j * WAVES + wave) * 64 + lane, row = at / (DIM / 8), piece = HeadTile<DIM>::place(row, at % (DIM / 8));
             offset[j] = piece * 8 < dim ? static_cast<uint32_t>(row * line + piece * 16) : OUTSIDE;
         }
     }
@@ -89,7 +101,8 @@ struct HeadLoader {
         const buffer_t w = window(base + row0 * line, left > 0 ? static_cast<uint32_t>((left < ROWS ? left : ROWS) * line) : 0);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j)
-            load_to_lds(w, tile + (wave * LOADS + j) * 512, offset[j]);
+            if (TOTAL % WAVES == 0 || j * WAVES + wave < TOTAL)
+                load_to_lds(w, tile + (j * WAVES + wave) * 512, offset[j]);
     }
 };
 
@@ -195,7 +208,7 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
 template <class Type, int DIM>
 __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, short* out, int64_t out_token, int64_t out_head, float* lse)
 {
-    const HeadTile<DIM> tiles_at(threadIdx.x % 64);
+    const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -231,6 +244,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
     auto turn = [&](const short* ks, const short* vs, int key0) {
         if (key0 + KT <= wave_lo || key0 >= wave_hi)
             return;
+        const HeadTile<DIM> tiles_at = lane_at.afresh();
         f32x16 s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -328,24 +342,28 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
 
 // ---- backward ----
 
-// What the backward kernels read of 64 rows of a head: 64 values each of lse in base 2 (infinite for rows that see nothing: their
-// probabilities are zeros), D, lo and hi. The block of (head, tile) is 1 KB, one load of a wave.
-constexpr int BLOCK_ROWS = 64;
+// What the backward kernels read of 32 rows of a head: 32 values each of lse in base 2 (infinite for rows that see nothing: their
+// probabilities are zeros), D, lo and hi. The block of (head, tile) is 512 bytes, one load of half a wave.
+constexpr int BLOCK_ROWS = 32;
 struct RowBlock {
     float lse2[BLOCK_ROWS], delta[BLOCK_ROWS];
     int lo[BLOCK_ROWS], hi[BLOCK_ROWS];
 };
 
-// The least lo and the largest hi of every 64 rows, and zeros where the largest norms of d_out and v will be.
+// The least lo and the largest hi of every 32 rows, and zeros where the largest norms of d_out and v will be.
 __global__ __launch_bounds__(64) void span_bounds_kernel(Attention a, int2* bounds, uint32_t* norms)
 {
     int lo, hi;
-    span_of(a, static_cast<int64_t>(blockIdx.x) * BLOCK_ROWS + threadIdx.x, lo, hi);
-    lo = wave_min(lo);
-    hi = wave_most(hi);
-    if (threadIdx.x == 0) {
-        bounds[blockIdx.x] = make_int2(lo, hi);
-        if (blockIdx.x == 0)
+    span_of(a, static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x, lo, hi);
+    for (int d = 16; d; d /= 2) {
+        lo = min(lo, __shfl_xor(lo, d));
+        hi = max(hi, __shfl_xor(hi, d));
+    }
+    if (threadIdx.x % 32 == 0) {
+        const int64_t tile = blockIdx.x * 2 + threadIdx.x / 32;
+        if (tile * BLOCK_ROWS < a.tokens)
+            bounds[tile] = make_int2(lo, hi);
+        if (blockIdx.x == 0 && threadIdx.x == 0)
             norms[0] = norms[1] = 0;
     }
 }
@@ -490,7 +508,7 @@ template <class Type, int DIM>
 __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Heads d_out, RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
                                                                short* d_q, int64_t out_token, int64_t out_head)
 {
-    const HeadTile<DIM> tiles_at(threadIdx.x % 64);
+    const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -532,6 +550,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
         if (key0 + KT <= wave_lo || key0 >= wave_hi)
             return;
         const bool masked = key0 < all_lo || key0 + KT > all_hi;
+        const HeadTile<DIM> tiles_at = lane_at.afresh();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 s = {}, dp = {};
@@ -600,23 +619,17 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
 
 constexpr int KEYS_PER_GROUP = 128;
 
-// x, as something that the compiler cannot tell from a new value: what is made of it is made again where it is used instead of being kept
-// in registers throughout a loop.
-__device__ inline int again(int x)
-{
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
+// The workgroup's 128 keys by 32 rows a turn, 32 keys a wave. Two waves of a SIMD have 256 registers each: at 128 values a head the sums of d_k and
+// d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
 template <class Type, int DIM>
 __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
                                                                 const uint32_t* norms, uint32_t shares, uint32_t share_heads, float* parts, short* d_k,
                                                                 int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
 {
-    const HeadTile<DIM> tiles_at(threadIdx.x % 64);
+    const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int RT = BLOCK_ROWS;
-    __shared__ __attribute__((aligned(16))) short q0s[RT * DIM], g0s[RT * DIM], q1s[RT * DIM], g1s[RT * DIM];
-    __shared__ __attribute__((aligned(16))) RowBlock b0s, b1s;
+    __shared__ __attribute__((aligned(16))) short q0s[RT * DIM], g0s[RT * DIM], q1s[RT * DIM], g1s[RT * DIM], vs[KEYS_PER_GROUP * DIM];
+    __shared__ __attribute__((aligned(16))) RowBlock b0s[2], b1s[2]; // the second of each is where the load's other half wave puts zeros
     __shared__ int ends[8];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t kv_heads = a.q_heads / a.group, units = kv_heads * shares;
@@ -625,9 +638,9 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Hea
     which = gridDim.x / units - 1 - which; // the first keys, which causal rows see most of, first
     const uint32_t kv = unit / shares, head0 = kv * a.group + unit % shares * share_heads, heads = min(share_heads, kv * a.group + a.group - head0);
     const int first = static_cast<int>(which) * KEYS_PER_GROUP, last = min(first + KEYS_PER_GROUP, static_cast<int>(a.tokens)); // keys [first, last)
-    const int key = first + wave * 32 + lane % 32, wave_key = first + wave * 32;
+    const int wave_key = first + wave * 32, key = wave_key + lane % 32;
 
-    // The first and the last tile of 64 rows that sees any of these keys.
+    // The first and the last tile of rows that sees any of these keys.
     int from = NONE, to = -1;
     for (uint32_t t = threadIdx.x; t < tiles; t += 256) {
         const int2 b = bounds[t];
@@ -646,95 +659,98 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Hea
     from = __builtin_amdgcn_readfirstlane(min(min(ends[0], ends[1]), min(ends[2], ends[3])));
     to = __builtin_amdgcn_readfirstlane(max(max(ends[4], ends[5]), max(ends[6], ends[7])));
 
-    s16x8 k[DIM / 16], v[DIM / 16];
+    s16x8 k[DIM / 16];
     read_rows<DIM>(a.k, kv, key, a.tokens, a.dim, lane, k);
-    read_rows<DIM>(a.v, kv, key, a.tokens, a.dim, lane, v);
-    const float grow = gradient_scale<Type>(norms);
+    {
+        HeadLoader<KEYS_PER_GROUP, DIM, 4> vl;
+        vl.begin(a.v, a.dim, wave, lane);
+        vl.load(reinterpret_cast<const char*>(static_cast<const short*>(a.v.data) + kv * a.v.head), first, a.tokens, vs, wave);
+    }
+    HeadLoader<RT, DIM, 4> ql, gl;
+    ql.begin(a.q, a.dim, wave, lane);
+    gl.begin(d_out, a.dim, wave, lane);
+    const float grow = gradient_scale<Type>(norms), grow_k = grow * (Type::wide_range ? 1.f : 0x1p-15f);
     f32x16 ok[DIM / 32], ov[DIM / 32];
 #pragma unroll
     for (int e = 0; e < DIM / 32; ++e)
         ok[e] = ov[e] = f32x16{};
 
-    // Turns: the heads of this share, and of each the tiles from `from` to `to`.
-    const int count = to - from + 1, turns = count > 0 ? count * static_cast<int>(heads) : 0;
-    auto load = [&](int n, short* qs, short* gs, RowBlock& bs) {
-        const bool there = n < turns;
-        const uint32_t head = head0 + (there ? n / count : 0);
-        const int64_t t = there ? from + n % count : tiles;
-        HeadLoader<RT, DIM, 4> ql, gl;
-        ql.begin(a.q, a.dim, wave, again(lane));
-        gl.begin(d_out, a.dim, wave, again(lane));
-        ql.load(reinterpret_cast<const char*>(static_cast<const short*>(a.q.data) + head * a.q.head), t * RT, a.tokens, qs, wave);
-        gl.load(reinterpret_cast<const char*>(static_cast<const short*>(d_out.data) + head * d_out.head), t * RT, a.tokens, gs, wave);
+    // Turns: the heads of this share, and of each the tiles from `from` to `to`. The next tile to load:
+    uint32_t load_head = head0;
+    int load_tile = from;
+    auto load = [&](short* qs, short* gs, RowBlock* bs) {
+        const bool there = load_head < head0 + heads;
+        const int64_t row0 = there ? static_cast<int64_t>(load_tile) * RT : a.tokens; // past the last one: an empty window
+        const uint32_t head = there ? load_head : head0;
+        ql.load(reinterpret_cast<const char*>(static_cast<const short*>(a.q.data) + head * a.q.head), row0, a.tokens, qs, wave);
+        gl.load(reinterpret_cast<const char*>(static_cast<const short*>(d_out.data) + head * d_out.head), row0, a.tokens, gs, wave);
         if (wave == 0)
-            load_to_lds(window(blocks + static_cast<int64_t>(head) * tiles + t, there ? sizeof(RowBlock) : 0), &bs, lane * 16);
+            load_to_lds(window(blocks + static_cast<int64_t>(head) * tiles + load_tile, there ? sizeof(RowBlock) : 0), bs, lane * 16);
+        load_tile = load_tile < to ? load_tile + 1 : from;
+        load_head += load_tile == from;
     };
-    auto scores = [&](const short* qs, const short* gs, int w, f32x16& s, f32x16& dp) {
+    uint32_t head = head0;
+    int tile = from;
+    auto turn = [&](const short* qs, const short* gs, const RowBlock& bs) {
+        // which of the rows see any of the wave's 32 keys, and which do not see all of them
+        const int lo = bs.lo[lane % 32], hi = bs.hi[lane % 32];
+        if (!__any(lo < wave_key + 32 && hi > wave_key))
+            return;
+        const bool masked = __any(lo > wave_key || hi < wave_key + 32);
+        const HeadTile<DIM> tiles_at = lane_at.afresh();
+        f32x16 s = {}, dp = {};
 #pragma unroll
         for (int d = 0; d < DIM / 16; ++d) {
-            s = Type::mfma32(tiles_at.along(qs, 32 * w, d), k[d], s);
-            dp = Type::mfma32(tiles_at.along(gs, 32 * w, d), v[d], dp);
+            s = Type::mfma32(tiles_at.along(qs, 0, d), k[d], s);
+            dp = Type::mfma32(tiles_at.along(gs, 0, d), tiles_at.along(vs, 32 * wave, d), dp);
         }
-    };
-    auto sums = [&](const short* qs, const short* gs, int w, const s16x8 (&p)[2], const s16x8 (&ds)[2]) {
+        const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
+        const int row = tile * RT + 4 * half;
+        score_gradients<false>(
+            a, s, dp, slope2, P_SHIFT<Type>, grow_k, masked, [&](int r) { return bs.lse2[4 * half + 8 * (r / 4) + r % 4]; },
+            [&](int r) { return bs.delta[4 * half + 8 * (r / 4) + r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
+            [&](int r) {
+                const int at = 4 * half + 8 * (r / 4) + r % 4;
+                return key >= bs.lo[at] && key < bs.hi[at];
+            });
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u) {
+            const s16x8 p = round8<Type>(s, u), ds = round8<Type>(dp, u);
 #pragma unroll
             for (int e = 0; e < DIM / 32; ++e) {
-                ov[e] = Type::mfma32(tiles_at.across(gs, 32 * w + 16 * u, e), p[u], ov[e]);
-                ok[e] = Type::mfma32(tiles_at.across(qs, 32 * w + 16 * u, e), ds[u], ok[e]);
+                ov[e] = Type::mfma32(tiles_at.across(gs, 16 * u, e), p, ov[e]);
+                ok[e] = Type::mfma32(tiles_at.across(qs, 16 * u, e), ds, ok[e]);
             }
-    };
-    const float grow_k = grow * (Type::wide_range ? 1.f : 0x1p-15f);
-    auto turn = [&](int n, const short* qs, const short* gs, const RowBlock& bs) {
-        if (n >= turns)
-            return;
-        // which of the 64 rows see any of the wave's 32 keys, and which do not see all of them
-        const int lo = bs.lo[lane], hi = bs.hi[lane];
-        const uint64_t some = __ballot(lo < wave_key + 32 && hi > wave_key), less = __ballot(lo > wave_key || hi < wave_key + 32);
-        if (!some)
-            return;
-        const uint32_t head = head0 + n / count;
-        const int t = from + n % count;
-        const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
-#pragma unroll 1
-        for (int w = 0; w < 2; ++w) { // 32 rows
-            if (!static_cast<uint32_t>(some >> 32 * w))
-                continue;
-            const bool masked = static_cast<uint32_t>(less >> 32 * w);
-            f32x16 s = {}, dp = {};
-            scores(qs, gs, w, s, dp);
-            const int row = t * RT + 32 * w + 4 * half;
-            score_gradients<false>(
-                a, s, dp, slope2, P_SHIFT<Type>, grow_k, masked, [&](int r) { return bs.lse2[32 * w + 4 * half + 8 * (r / 4) + r % 4]; },
-                [&](int r) { return bs.delta[32 * w + 4 * half + 8 * (r / 4) + r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
-                [&](int r) {
-                    const int at = 32 * w + 4 * half + 8 * (r / 4) + r % 4;
-                    return key >= bs.lo[at] && key < bs.hi[at];
-                });
-            const s16x8 p[2] = {round8<Type>(s, 0), round8<Type>(s, 1)}, ds[2] = {round8<Type>(dp, 0), round8<Type>(dp, 1)};
-            sums(qs, gs, w, p, ds);
         }
     };
+    auto next = [&] {
+        tile = tile < to ? tile + 1 : from;
+        head += tile == from;
+        return head < head0 + heads;
+    };
 
-    if (turns > 0) {
-        load(0, q0s, g0s, b0s);
-        for (int n = 0; n < turns; n += 2) {
+    if (from <= to) {
+        load(q0s, g0s, b0s);
+        for (;;) {
             wait_for_all();
             meet();
-            load(n + 1, q1s, g1s, b1s);
-            turn(n, q0s, g0s, b0s);
+            load(q1s, g1s, b1s);
+            turn(q0s, g0s, b0s[0]);
+            const bool more = next();
             wait_for_all();
             meet();
-            load(n + 2, q0s, g0s, b0s);
-            turn(n + 1, q1s, g1s, b1s);
+            load(q0s, g0s, b0s);
+            if (more)
+                turn(q1s, g1s, b1s[0]);
+            if (!more || !next())
+                break;
         }
         wait_for_all();
     }
     if (key < a.tokens) {
         const float back_k = a.scale / grow, back_v = Type::wide_range ? 1.f : 0x1p-15f;
         if (shares > 1) {
-            float* to = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
+            float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
 #pragma unroll
             for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
@@ -746,8 +762,8 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Hea
                         z[i] = ov[e][4 * x + i] * back_v;
                     }
                     const int d = 32 * e + 8 * x + 4 * half;
-                    *reinterpret_cast<f32x4*>(to + d) = y;
-                    *reinterpret_cast<f32x4*>(to + a.tokens * DIM + d) = z;
+                    *reinterpret_cast<f32x4*>(part + d) = y;
+                    *reinterpret_cast<f32x4*>(part + a.tokens * DIM + d) = z;
                 }
             return;
         }

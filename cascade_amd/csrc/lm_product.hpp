@@ -26,7 +26,7 @@ struct Loader {
     static constexpr int LOADS = ROWS / 8 / WAVES; // instructions of a wave per slice
     static_assert(ROWS % (8 * WAVES) == 0, "every wave loads as much");
     static constexpr int PIECES = ACROSS ? ROWS / 8 : 8; // 16-byte pieces of a row or line
-    static constexpr int TURN = PIECES >= 16 ? 7 : 3;
+    static __device__ int turn(int row) { return !ACROSS ? row >> 1 & 7 : PIECES >= 16 ? (row & 3) * 4 : (row >> 1 & 1) * 4; }
 
     const char* base;
     int64_t line; // bytes between rows or lines
@@ -44,7 +44,7 @@ struct Loader {
         for (int j = 0; j < LOADS; ++j) {
             const int at = (wave * LOADS + j) * 64 + lane; // which 16-byte place of the buffer
             const int row = at / PIECES, place = at % PIECES;
-            piece[j] = place ^ (ACROSS ? (row & TURN) * 2 : row & 7);
+            piece[j] = place ^ turn(row);
             offset[j] = static_cast<uint32_t>(row * line + piece[j] * 16);
         }
     }
@@ -69,7 +69,7 @@ struct Loader {
 // Fragments of 32 rows x 16 k from a buffer.
 template <int ROWS, bool ACROSS, int TILES>
 struct Reader {
-    static constexpr int TURN = ROWS / 8 >= 16 ? 7 : 3;
+    typedef Loader<ROWS, ACROSS, 1> Places;
     int at[ACROSS ? 2 * TILES : 4];
 
     __device__ void begin(int first_row, int lane)
@@ -80,13 +80,13 @@ struct Reader {
                 const int line = (g / 2) * 8 + u * 4 + j / 4;
                 for (int t = 0; t < TILES; ++t) {
                     const int col = first_row + t * 32 + (g % 2) * 16 + 4 * (j % 4);
-                    at[u * TILES + t] = line * ROWS + ((col / 8) ^ ((line & TURN) * 2)) * 8 + col % 8;
+                    at[u * TILES + t] = line * ROWS + ((col / 8) ^ Places::turn(line)) * 8 + col % 8;
                 }
             }
         } else {
             const int row = first_row + lane % 32;
             for (int s = 0; s < 4; ++s)
-                at[s] = row * SLICE + (((s * 2 + lane / 32) ^ (row & 7)) * 8);
+                at[s] = row * SLICE + (((s * 2 + lane / 32) ^ Places::turn(row)) * 8);
         }
     }
     __device__ s16x8 read(const short* buffer, int tile, int step) const
