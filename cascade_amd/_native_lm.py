@@ -54,9 +54,9 @@ def load():
     lib.csa_lm_spans_u16_dev.restype = i32
     lib.csa_lm_spans_u16_dev.argtypes = [vp, u64, u32, vp, vp, vp, vp, u64, vp]
     lib.csa_lm_attention_forward_dev.restype = i32
-    lib.csa_lm_attention_forward_dev.argtypes = [C.POINTER(CsaLmAttention), CsaLmHeads, vp, vp]
+    lib.csa_lm_attention_forward_dev.argtypes = [C.POINTER(CsaLmAttention), CsaLmHeads, vp, vp, u64, vp]
     lib.csa_lm_attention_workspace.restype = u64
-    lib.csa_lm_attention_workspace.argtypes = [u64, u32, u32, u32]
+    lib.csa_lm_attention_workspace.argtypes = [u64, u32, u32, u32, u32]
     lib.csa_lm_attention_backward_dev.restype = i32
     lib.csa_lm_attention_backward_dev.argtypes = [C.POINTER(CsaLmAttention), CsaLmHeads, vp, CsaLmHeads, CsaLmHeads, CsaLmHeads, CsaLmHeads, vp, u64, vp]
     lib.csa_lm_cross_entropy_workspace.restype = u64

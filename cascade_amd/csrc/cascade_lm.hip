@@ -124,11 +124,18 @@ struct AttentionWork {
     int2* bounds;
     RowBlock* blocks;
     float* parts;
+    uint32_t *row_order, *key_order; // null where there is none
     uint32_t shares, share_heads;
     uint64_t bytes;
-    AttentionWork(void* base, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim)
+    AttentionWork(void* base, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim, bool backward)
     {
         Carver c{static_cast<char*>(base)};
+        row_order = c.take<uint32_t>(ORDER_TILES);
+        if (!backward) {
+            bytes = c.used;
+            return;
+        }
+        key_order = c.take<uint32_t>(ORDER_TILES);
         const uint64_t tiles = parts_of(tokens, BLOCK_ROWS), group = q_heads / kv_heads, groups = parts_of(tokens, KEYS_PER_GROUP) * kv_heads;
         const uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1;
         share_heads = static_cast<uint32_t>(want < group ? group / want : 1);
@@ -141,11 +148,22 @@ struct AttentionWork {
     }
 };
 
-template <class Type, int DIM>
-void forward(const csa_lm_attention& a, const csa_lm_heads& out, float* lse, hipStream_t s)
+// Tiles are put in order where spans are given (a causal text is in order the other way round), where not all workgroups run at once anyway
+// (two fit a compute unit), and where a workgroup can rank them.
+bool in_order(const csa_lm_attention& a)
 {
+    const uint64_t tiles = parts_of(a.tokens, ROWS_PER_GROUP);
+    return (a.d_lo || a.d_hi) && tiles <= ORDER_TILES && tiles * a.q_heads > 512;
+}
+
+template <class Type, int DIM>
+void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_heads& out, float* lse, hipStream_t s)
+{
+    const bool order = in_order(a);
+    if (order)
+        tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), w.row_order, nullptr);
     attention_forward_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
-        attention(a), static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
+        attention(a), order ? w.row_order : nullptr, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
 }
 
 template <class Type, int DIM>
@@ -155,11 +173,14 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     const Attention at = attention(a);
     const uint32_t tiles = static_cast<uint32_t>(parts_of(a.tokens, BLOCK_ROWS));
     span_bounds_kernel<<<static_cast<uint32_t>(parts_of(a.tokens, 64)), 64, 0, s>>>(at, w.bounds, w.norms);
+    const bool order = in_order(a);
+    if (order)
+        tile_order_kernel<<<1, 1024, 0, s>>>(at, w.row_order, w.key_order);
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
     attention_d_q_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
-        at, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
+        at, order ? w.row_order : nullptr, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
     attention_d_kv_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
-        at, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.share_heads, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
+        at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.share_heads, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
         d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
     if (w.shares > 1)
         join_heads_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.kv_heads, 2), 256, 0, s>>>(
@@ -370,7 +391,7 @@ int csa_lm_spans_u16_dev(const uint16_t* d_text, uint64_t n, uint32_t separator,
     return launched(who);
 }
 
-int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, float* d_lse, void* stream)
+int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream)
 {
     const char* who = "csa_lm_attention_forward_dev";
     if (int rc = check_attention(who, a))
@@ -381,14 +402,17 @@ int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, fl
         return rc;
     if (!d_lse || !aligned(d_lse, 4))
         return fail(CSA_ERR_ARG, "%s: d_lse is null or unaligned", who);
+    const AttentionWork w(d_work, a->tokens, a->q_heads, a->kv_heads, a->head_dim, false);
+    if (int rc = check_work(who, d_work, work_bytes, w.bytes))
+        return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    with_type(a->type, [&](auto type) { with_dim(a->head_dim, [&](auto dim) { forward<decltype(type), dim()>(*a, out, d_lse, s); }); });
+    with_type(a->type, [&](auto type) { with_dim(a->head_dim, [&](auto dim) { forward<decltype(type), dim()>(*a, w, out, d_lse, s); }); });
     return launched(who);
 }
 
-uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim)
+uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t flags)
 {
-    return kv_heads ? AttentionWork(nullptr, tokens, q_heads, kv_heads, head_dim).bytes : 0;
+    return kv_heads && q_heads >= kv_heads ? AttentionWork(nullptr, tokens, q_heads, kv_heads, head_dim, flags & CSA_LM_BACKWARD).bytes : 0;
 }
 
 int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, const float* d_lse, csa_lm_heads d_out, csa_lm_heads d_q, csa_lm_heads d_k,
@@ -408,7 +432,7 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
             return rc;
     if (!d_lse || !aligned(d_lse, 4))
         return fail(CSA_ERR_ARG, "%s: d_lse is null or unaligned", who);
-    const AttentionWork w(d_work, a->tokens, a->q_heads, a->kv_heads, a->head_dim);
+    const AttentionWork w(d_work, a->tokens, a->q_heads, a->kv_heads, a->head_dim, true);
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);

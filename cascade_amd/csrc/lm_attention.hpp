@@ -158,12 +158,13 @@ __device__ inline s16x8 round8(const f32x16& x, int u)
 }
 
 // Workgroup's tile of rows and head. Neighbouring workgroup ids run on different XCDs: where there are eight heads or a multiple, an XCD gets
-// neighbouring heads, which share keys and values in its L2. Tiles come last first: those of long causal spans, the longest, are the last ones.
-__device__ inline void place_of(uint32_t id, uint32_t heads, uint32_t tiles, uint32_t& head, uint32_t& tile)
+// neighbouring heads, which share keys and values in its L2. Tiles come in `order`, the most work first; without one the last tile comes
+// first: in a causal text it sees most.
+__device__ inline void place_of(uint32_t id, uint32_t heads, uint32_t tiles, const uint32_t* order, uint32_t& head, uint32_t& tile)
 {
-    const uint32_t in = id % heads;
+    const uint32_t in = id % heads, at = id / heads;
     head = heads % 8 == 0 ? in % 8 * (heads / 8) + in / 8 : in;
-    tile = tiles - 1 - id / heads;
+    tile = order ? order[at] : tiles - 1 - at;
 }
 
 // What round8 left of registers 8 u ... 8 u + 7 (zeros elsewhere)
@@ -175,6 +176,22 @@ __device__ inline f32x16 widen(const s16x8& x, int u)
     for (int i = 0; i < 8; ++i)
         y[8 * u + i] = to32<Type>(x[i]);
     return y;
+}
+
+// Order for the stretch of code before it: AHEAD LDS reads first, then EACH of them behind every matrix instruction as long as there are any, so that
+// an operand is on its way while the ones before it are multiplied.
+template <int READS, int PRODUCTS, int AHEAD, int EACH>
+__device__ inline void read_ahead()
+{
+    constexpr int TURNS = (READS - AHEAD) / EACH;
+    static_assert(TURNS <= PRODUCTS && (READS - AHEAD) % EACH == 0, "reads are shared out");
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, PRODUCTS - TURNS, 0);
 }
 
 constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
@@ -206,14 +223,14 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
 }
 
 template <class Type, int DIM>
-__global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, short* out, int64_t out_token, int64_t out_head, float* lse)
+__global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, const uint32_t* order, short* out, int64_t out_token, int64_t out_head, float* lse)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     uint32_t head, tile;
-    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, head, tile);
+    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, order, head, tile);
     const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
 
     // The keys that this workgroup's rows see, this wave's rows see, and all of this wave's rows see.
@@ -298,6 +315,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
                 for (int e = 0; e < DIM / 32; ++e)
                     o[e] = Type::mfma32(tiles_at.across(vs, 32 * t + 16 * u, e), p, o[e]);
             }
+        read_ahead<DIM / 4, DIM / 8, 6, 2>();
     };
 
     if (group_lo < group_hi) {
@@ -505,7 +523,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
 }
 
 template <class Type, int DIM>
-__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Heads d_out, RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
+__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, Heads d_out, RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
                                                                short* d_q, int64_t out_token, int64_t out_head)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
@@ -513,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, Head
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     uint32_t head, tile;
-    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, head, tile);
+    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, order, head, tile);
     const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
     int lo, hi, l2, h2;
     span_of(a, first + lane, lo, hi);
@@ -622,7 +640,7 @@ constexpr int KEYS_PER_GROUP = 128;
 // The workgroup's 128 keys by 32 rows a turn, 32 keys a wave. Two waves of a SIMD have 256 registers each: at 128 values a head the sums of d_k and
 // d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
 template <class Type, int DIM>
-__global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
+__global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, const uint32_t* order, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
                                                                 const uint32_t* norms, uint32_t shares, uint32_t share_heads, float* parts, short* d_k,
                                                                 int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
 {
@@ -634,8 +652,9 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Hea
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t kv_heads = a.q_heads / a.group, units = kv_heads * shares;
     uint32_t unit, which;
-    place_of(blockIdx.x, units, gridDim.x / units, unit, which);
-    which = gridDim.x / units - 1 - which; // the first keys, which causal rows see most of, first
+    place_of(blockIdx.x, units, gridDim.x / units, order, unit, which);
+    if (!order)
+        which = gridDim.x / units - 1 - which; // the first keys, which most rows of a causal text see, first
     const uint32_t kv = unit / shares, head0 = kv * a.group + unit % shares * share_heads, heads = min(share_heads, kv * a.group + a.group - head0);
     const int first = static_cast<int>(which) * KEYS_PER_GROUP, last = min(first + KEYS_PER_GROUP, static_cast<int>(a.tokens)); // keys [first, last)
     const int wave_key = first + wave * 32, key = wave_key + lane % 32;
@@ -722,6 +741,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Hea
                 ok[e] = Type::mfma32(tiles_at.across(qs, 16 * u, e), ds, ok[e]);
             }
         }
+        read_ahead<DIM / 4, DIM / 8, 6, 2>();
     };
     auto next = [&] {
         tile = tile < to ? tile + 1 : from;
@@ -785,6 +805,72 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, Hea
                     *reinterpret_cast<s16x4*>(vt + d) = z;
                 }
             }
+    }
+}
+
+// The order of tiles by work, most first, for texts whose spans are given: documents differ in length by more than workgroups can make up for by
+// their number (six texts of 16384 tokens and documents of lognormal lengths: the last workgroup ends 10 to 25 % earlier). One workgroup
+// reads all spans once, and ranks tiles by the 64-key tiles that their rows see, and by the 32-row tiles that see their keys.
+constexpr int ORDER_TILES = 1024; // of 128 rows or keys
+
+__global__ __launch_bounds__(1024) void tile_order_kernel(Attention a, uint32_t* row_order, uint32_t* key_order)
+{
+    __shared__ int los[ORDER_TILES], his[ORDER_TILES]; // of the rows of a tile
+    __shared__ int change[ORDER_TILES + 1];            // of the number of 32-row tiles that see a tile of keys, from the tile before it
+    __shared__ int work[ORDER_TILES], sums[16];
+    const int t = threadIdx.x, lane = t % 64, tiles = static_cast<int>((a.tokens + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP);
+    los[t] = NONE;
+    his[t] = change[t] = 0;
+    __syncthreads();
+    constexpr int MINE = 4; // neighbouring rows of a lane: eight lanes see 32
+    for (int64_t first = t * MINE; first < tiles * ROWS_PER_GROUP; first += 1024 * MINE) {
+        int lo = NONE, hi = 0;
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            int l, h;
+            span_of(a, first + k, l, h);
+            lo = min(lo, l);
+            hi = max(hi, h);
+        }
+        for (int d = 1; d < BLOCK_ROWS / MINE; d *= 2) {
+            lo = min(lo, __shfl_xor(lo, d));
+            hi = max(hi, __shfl_xor(hi, d));
+        }
+        if (t % (BLOCK_ROWS / MINE) == 0 && lo < hi) {
+            const int64_t tile = first / ROWS_PER_GROUP;
+            atomicMin(los + tile, lo);
+            atomicMax(his + tile, hi);
+            atomicAdd(change + lo / KEYS_PER_GROUP, 1);
+            atomicAdd(change + (hi - 1) / KEYS_PER_GROUP + 1, -1);
+        }
+    }
+    __syncthreads();
+    for (int keys = 0; keys < (key_order ? 2 : 1); ++keys) {
+        int mine = 0;
+        if (keys) { // the running sum of the changes
+            mine = change[t];
+            for (int d = 1; d < 64; d *= 2) {
+                const int below = __shfl_up(mine, d);
+                mine += lane >= d ? below : 0;
+            }
+            if (lane == 63)
+                sums[t / 64] = mine;
+            __syncthreads();
+            for (int w = 0; w < t / 64; ++w)
+                mine += sums[w];
+        } else if (los[t] < his[t]) {
+            mine = (his[t] - los[t] / KEYS_PER_TILE * KEYS_PER_TILE + KEYS_PER_TILE - 1) / KEYS_PER_TILE;
+        }
+        work[t] = mine;
+        __syncthreads();
+        if (t < tiles) {
+            int rank = 0;
+#pragma unroll 8
+            for (int other = 0; other < tiles; ++other)
+                rank += work[other] > mine || (work[other] == mine && other < t);
+            (keys ? key_order : row_order)[rank] = t;
+        }
+        __syncthreads();
     }
 }
 

@@ -142,8 +142,11 @@ def span_attention(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
     if q.shape[0]:
+        lib = native.load()
+        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1], k.shape[1], q.shape[2], 0)
+        work = _work(size, device)
         with _Call(device) as stream:
-            native.check(native.load().csa_lm_attention_forward_dev(C.byref(a), _heads(out), lse.data_ptr(), stream))
+            native.check(lib.csa_lm_attention_forward_dev(C.byref(a), _heads(out), lse.data_ptr(), work.data_ptr(), size, stream))
     return out, lse
 
 
@@ -159,7 +162,7 @@ def span_attention_backward(d_out, q, k, v, out, lse, lo=None, hi=None, scale=No
     d_q, d_k, d_v = (torch.empty(x.shape, dtype=q.dtype, device=device) for x in (q, k, v))
     if q.shape[0]:
         lib = native.load()
-        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1], k.shape[1], q.shape[2])
+        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1], k.shape[1], q.shape[2], native.CSA_LM_BACKWARD)
         work = _work(size, device)
         with _Call(device) as stream:
             native.check(lib.csa_lm_attention_backward_dev(C.byref(a), _heads(out), lse.data_ptr(), _heads(d_out), _heads(d_q), _heads(d_k), _heads(d_v),

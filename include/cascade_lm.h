@@ -26,6 +26,12 @@ typedef enum csa_lm_type {
     CSA_LM_F32 = 2 /* gradients to clip only: the matrix units multiply 16-bit values */
 } csa_lm_type;
 
+/* Flags of the *_workspace functions. */
+enum {
+    CSA_LM_BACKWARD = 1,  /* for the backward call; else for the forward one */
+    CSA_LM_COPY_ROWS = 2, /* cross entropy: hidden or weight has rows that 16-byte loads cannot walk (below) */
+};
+
 /* ---- spans of documents ---- */
 
 /* For position i of d_text[0, n): d_lo[i] = the last position j <= i with text[j] == separator, 0 if there is none;
@@ -62,11 +68,11 @@ typedef struct csa_lm_attention {
 
 /* out = the softmax over each row's span times v (zeros for rows that see nothing), d_lse[h * tokens + i] = the
  * logarithm of the sum of exponentials of row i's scores (-infinity for rows that see nothing). */
-int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, float* d_lse, void* stream);
+uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t flags);
+int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream);
 
 /* Gradients of q, k and v for the gradient d_out of out; out and d_lse as the forward call left them. Gradients of a head of k and v are summed
  * over the heads of q that share it. A key that no row sees gets zeros. */
-uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim);
 int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, const float* d_lse, csa_lm_heads d_out, csa_lm_heads d_q,
                                   csa_lm_heads d_k, csa_lm_heads d_v, void* d_work, uint64_t work_bytes, void* stream);
 
@@ -78,10 +84,6 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
  * apart (>= dim, below 2^22). Rows that 16-byte loads cannot walk (an address, a stride or dim that is no multiple of 8 values)
  * are copied to the workspace first, for which it has to be sized with CSA_LM_COPY_ROWS; the rest is read where it lies.
  * tokens, vocab <= 2^30. */
-enum {
-    CSA_LM_BACKWARD = 1,  /* the backward call; 0: the forward one */
-    CSA_LM_COPY_ROWS = 2, /* hidden or weight has such rows */
-};
 uint64_t csa_lm_cross_entropy_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t flags);
 int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride,
                                      const int32_t* d_target, uint64_t tokens, uint64_t dim, uint64_t vocab, float* d_loss, float* d_lse,

@@ -217,6 +217,8 @@ def test_attention_caps_and_distances(cap, slopes, mask, dtype):
 def test_attention_of_a_long_text():
     check_attention(3001, 2, 1, 128, torch.bfloat16, "causal", seed=5)
     check_attention(2800, 2, 2, 96, torch.float16, "documents", seed=6)
+    check_attention(4200, 16, 16, 8, torch.bfloat16, "random", seed=9)  # tiles in the order of their work
+    check_attention(2111, 32, 2, 16, torch.float16, "documents", seed=10)  # shared heads in that order, too
 
 
 def test_attention_of_large_scores():
@@ -485,12 +487,13 @@ def test_the_library_refuses_what_the_kernels_cannot_read():
     lib = native.load()
     x = torch.zeros(64, 2, 64, dtype=torch.bfloat16, device="cuda")
     lse = torch.zeros(2, 64, device="cuda")
+    work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
     heads = native.CsaLmHeads(x.data_ptr(), 128, 64)
 
     def call(**change):
         a = dict(type=0, q_heads=2, kv_heads=2, head_dim=64, tokens=64, d_lo=None, d_hi=None, d_slope=None, scale=1.0, cap=0.0, q=heads, k=heads, v=heads)
         a.update(change)
-        return lib.csa_lm_attention_forward_dev(C.byref(native.CsaLmAttention(**a)), heads, lse.data_ptr(), None)
+        return lib.csa_lm_attention_forward_dev(C.byref(native.CsaLmAttention(**a)), heads, lse.data_ptr(), work.data_ptr(), work.numel(), None)
     odd = native.CsaLmHeads(x.data_ptr() + 2, 128, 64)
     for change in (dict(type=2), dict(q_heads=3), dict(kv_heads=0), dict(head_dim=60), dict(head_dim=136), dict(scale=0.0), dict(scale=math.nan), dict(cap=-1.0),
                    dict(q=odd), dict(k=native.CsaLmHeads(None, 128, 64)), dict(v=native.CsaLmHeads(x.data_ptr(), 100, 64)),
@@ -498,8 +501,7 @@ def test_the_library_refuses_what_the_kernels_cannot_read():
         with pytest.raises(CascadeError):
             native.check(call(**change))
     assert call(tokens=(1 << 30) + 1) == -2
-    work = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
     a = native.CsaLmAttention(0, 2, 2, 64, 64, None, None, None, 1.0, 0.0, heads, heads, heads)
-    need = lib.csa_lm_attention_workspace(64, 2, 2, 64)
+    need = lib.csa_lm_attention_workspace(64, 2, 2, 64, native.CSA_LM_BACKWARD)
     assert lib.csa_lm_attention_backward_dev(C.byref(a), heads, lse.data_ptr(), heads, heads, heads, heads, work.data_ptr(), need - 1, None) == -1
     assert b"workspace" in lib.csa_lm_last_error()

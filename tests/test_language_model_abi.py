@@ -55,7 +55,7 @@ def test_argument_errors_need_no_gpu():
     assert lib.csa_lm_spans_u16_dev(None, 5, 0x10000, None, None, None, None, 0, None) == bad
     assert lib.csa_lm_spans_u16_dev(None, 1 << 31, 0xFFFF, None, None, None, None, 0, None) == large
     assert lib.csa_lm_spans_u16_dev(None, 0, 0xFFFF, None, None, None, None, 0, None) == 0
-    assert lib.csa_lm_attention_forward_dev(None, native.CsaLmHeads(), None, None) == bad
+    assert lib.csa_lm_attention_forward_dev(None, native.CsaLmHeads(), None, None, 0, None) == bad
     assert b"null" in lib.csa_lm_last_error()
     assert lib.csa_lm_cross_entropy_forward_dev(0, None, 8, None, 8, None, 4, 8, 10, None, None, None, 0, None) == bad
     assert lib.csa_lm_cross_entropy_forward_dev(7, None, 8, None, 8, None, 4, 8, 10, None, None, None, 0, None) == bad
