@@ -119,6 +119,15 @@ constexpr uint64_t KV_GROUPS = 2048;
 
 int head_width(uint64_t dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
+// Tiles are put in order where spans are given (a causal text is in order the other way round), where not all workgroups run at once anyway
+// (two fit a compute unit), and where one workgroup can rank them.
+bool may_be_ordered(uint64_t tokens, uint64_t q_heads)
+{
+    const uint64_t tiles = parts_of(tokens, ROWS_PER_GROUP);
+    return tiles <= ORDER_TILES && tiles * q_heads > 512;
+}
+bool in_order(const csa_lm_attention& a) { return (a.d_lo || a.d_hi) && may_be_ordered(a.tokens, a.q_heads); }
+
 struct AttentionWork {
     uint32_t* norms;
     int2* bounds;
@@ -130,12 +139,12 @@ struct AttentionWork {
     AttentionWork(void* base, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim, bool backward)
     {
         Carver c{static_cast<char*>(base)};
-        row_order = c.take<uint32_t>(ORDER_TILES);
+        row_order = c.take<uint32_t>(may_be_ordered(tokens, q_heads) ? ORDER_TILES : 0);
         if (!backward) {
             bytes = c.used;
             return;
         }
-        key_order = c.take<uint32_t>(ORDER_TILES);
+        key_order = c.take<uint32_t>(may_be_ordered(tokens, q_heads) ? ORDER_TILES : 0);
         const uint64_t tiles = parts_of(tokens, BLOCK_ROWS), group = q_heads / kv_heads, groups = parts_of(tokens, KEYS_PER_GROUP) * kv_heads;
         const uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1;
         share_heads = static_cast<uint32_t>(want < group ? group / want : 1);
@@ -147,14 +156,6 @@ struct AttentionWork {
         bytes = c.used;
     }
 };
-
-// Tiles are put in order where spans are given (a causal text is in order the other way round), where not all workgroups run at once anyway
-// (two fit a compute unit), and where a workgroup can rank them.
-bool in_order(const csa_lm_attention& a)
-{
-    const uint64_t tiles = parts_of(a.tokens, ROWS_PER_GROUP);
-    return (a.d_lo || a.d_hi) && tiles <= ORDER_TILES && tiles * a.q_heads > 512;
-}
 
 template <class Type, int DIM>
 void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_heads& out, float* lse, hipStream_t s)
@@ -315,8 +316,12 @@ void entropy_forward(const EntropyPlan& plan, const EntropyWork& w, const Operan
         logit_sums_kernel<N><<<mt * nt, N::THREADS, 0, s>>>(l, w.part, w.target_logit);
     else
         logit_sums_kernel<W><<<mt * nt, W::THREADS, 0, s>>>(l, w.part, w.target_logit);
-    join_sums_kernel<<<static_cast<uint32_t>(parts_of(hidden.rows, 16)), 256, 0, s>>>(w.part, mt * static_cast<int64_t>(plan.narrow ? N::WM : W::WM),
-                                                                                      w.target_logit, target, hidden.rows, weight.rows, loss, lse);
+    // few tokens: more runs for each, the sums would otherwise be one lane's work after the other
+    const int64_t parts = mt * static_cast<int64_t>(plan.narrow ? N::WM : W::WM);
+    if (plan.narrow)
+        join_sums_kernel<4><<<static_cast<uint32_t>(parts_of(hidden.rows, 4)), 256, 0, s>>>(w.part, parts, w.target_logit, target, hidden.rows, weight.rows, loss, lse);
+    else
+        join_sums_kernel<16><<<static_cast<uint32_t>(parts_of(hidden.rows, 16)), 256, 0, s>>>(w.part, parts, w.target_logit, target, hidden.rows, weight.rows, loss, lse);
 }
 
 template <class Type>

@@ -82,31 +82,42 @@ __global__ __launch_bounds__(P::THREADS) void logit_sums_kernel(Logits l, float2
     }
 }
 
-// lse and loss from the waves' maxima and sums: 16 tokens by 16 runs of them a workgroup.
+// lse and loss from the waves' maxima and sums: TOKENS tokens by 256 / TOKENS runs of them a workgroup.
+template <int TOKENS>
 __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int64_t parts, const float* target_logit, const int32_t* target,
                                                         int64_t tokens, int64_t vocab, float* loss, float* lse)
 {
-    __shared__ float2 got[16][17];
-    const int x = threadIdx.x % 16, y = threadIdx.x / 16;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 16 + x;
-    float top = -3.0e38f, sum = 0.f;
+    constexpr int RUNS = 256 / TOKENS;
+    __shared__ float2 got[RUNS][TOKENS + 1];
+    const int x = threadIdx.x % TOKENS, y = threadIdx.x / TOKENS;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * TOKENS + x;
+    auto add = [](float2& sum, float2 v) { // (maximum, sum of exponentials over it)
+        const float high = fmaxf(sum.x, v.x);
+        sum.y = sum.y * __builtin_amdgcn_exp2f((sum.x - high) * LOG2E) + v.y * __builtin_amdgcn_exp2f((v.x - high) * LOG2E);
+        sum.x = high;
+    };
+    const float2 none = make_float2(-3.0e38f, 0.f);
+    float2 sum = none;
     if (n < tokens)
-        for (int64_t p = y; p < parts; p += 16) {
-            const float2 v = part[p * tokens + n];
-            const float high = fmaxf(top, v.x);
-            sum = sum * __builtin_amdgcn_exp2f((top - high) * LOG2E) + v.y * __builtin_amdgcn_exp2f((v.x - high) * LOG2E);
-            top = high;
+        for (int64_t p = y; p < parts; p += 8 * RUNS) {
+            float2 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                v[k] = p + k * RUNS < parts ? part[(p + k * RUNS) * tokens + n] : none;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                add(sum, v[k]);
         }
-    got[y][x] = make_float2(top, sum);
-    __syncthreads();
+    got[y][x] = sum;
+    for (int far = RUNS / 2; far; far /= 2) {
+        __syncthreads();
+        if (y < far) {
+            add(sum, got[y + far][x]);
+            got[y][x] = sum;
+        }
+    }
     if (y == 0 && n < tokens) {
-        for (int k = 1; k < 16; ++k) {
-            const float2 v = got[k][x];
-            const float high = fmaxf(top, v.x);
-            sum = sum * __builtin_amdgcn_exp2f((top - high) * LOG2E) + v.y * __builtin_amdgcn_exp2f((v.x - high) * LOG2E);
-            top = high;
-        }
-        const float all = top + logf(sum);
+        const float all = sum.x + logf(sum.y);
         const int32_t t = target[n];
         lse[n] = all;
         loss[n] = t >= 0 && t < vocab ? all - target_logit[n] : 0.f;

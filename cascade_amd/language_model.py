@@ -17,12 +17,18 @@ from . import _native_lm as native
 SEPARATOR = 0xFFFF
 
 
+_kinds = None  # the library's number of every dtype; made when first asked for: this package imports torch only where it is used
+
+
 def _type(dtype):
-    import torch
-    kinds = {torch.bfloat16: native.CSA_LM_BF16, torch.float16: native.CSA_LM_F16, torch.float32: native.CSA_LM_F32}
-    if dtype not in kinds:
+    global _kinds
+    if _kinds is None:
+        import torch
+        _kinds = {torch.bfloat16: native.CSA_LM_BF16, torch.float16: native.CSA_LM_F16, torch.float32: native.CSA_LM_F32}
+    kind = _kinds.get(dtype)
+    if kind is None:
         raise TypeError(f"{dtype} is none of bfloat16, float16 and float32")
-    return kinds[dtype]
+    return kind
 
 
 def _matrix_type(dtype):
@@ -37,34 +43,38 @@ def _check(condition, message):
         raise ValueError(message)
 
 
-def _on_gpu(tensors):
-    """The device that all of them lie on, which has to be a GPU."""
-    device = tensors[0].device
+def _on_gpu(*tensors):
+    """The number of the device that all of them (None aside) lie on, which has to be a GPU."""
+    device = tensors[0].get_device()
     for t in tensors:
-        _check(t.is_cuda and t.device == device, "all tensors have to lie on one GPU")
+        if t is not None and t.get_device() != device:
+            device = -1
+    _check(device >= 0, "all tensors have to lie on one GPU")
     return device
 
 
-class _Call:
-    """The device's current stream, with the device made current for the launches."""
-
-    def __init__(self, device):
-        import torch
-        self._guard = torch.cuda.device(device)
-        self._device = device
-
-    def __enter__(self):
-        import torch
-        self._guard.__enter__()
-        return torch.cuda.current_stream(self._device).cuda_stream or None
-
-    def __exit__(self, *exc):
-        return self._guard.__exit__(*exc)
-
-
-def _work(size, device):
+def _enqueue(device, call, *args):
+    """call(*args, stream) with the device's current stream, and the device made current for the launches."""
     import torch
-    return torch.empty(max(int(size), 1), dtype=torch.uint8, device=device)
+    stream = torch.cuda.current_stream(device).cuda_stream or None
+    if device == torch.cuda.current_device():
+        native.check(call(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            native.check(call(*args, stream))
+
+
+def _work(size, like):
+    """`size` bytes of scratch memory beside the tensor `like`, and their address; none where size is 0."""
+    if not size:
+        return None, None
+    import torch
+    work = like.new_empty(size, dtype=torch.uint8)
+    return work, work.data_ptr()
+
+
+def _address(x):
+    return (x.data_ptr() or None) if x is not None else None
 
 
 def token_spans(text, separator=SEPARATOR):
@@ -72,16 +82,14 @@ def token_spans(text, separator=SEPARATOR):
     position i may see the keys [lo[i], hi[i]), which begin at the last separator at or before i and end with i itself, and has to
     predict target[i], the token behind it, or nothing (-1) at the end and in front of a separator (csa_lm_spans_u16_dev)."""
     import torch
-    device = _on_gpu([text])
+    device = _on_gpu(text)
     _check(text.dim() == 1 and text.element_size() == 2 and not text.is_floating_point() and text.is_contiguous(), "text: a dense vector of 16-bit tokens")
     _check(0 <= separator <= 0xFFFF, "separator: a 16-bit token")
     lib, n = native.load(), text.numel()
-    lo, hi, target = (torch.empty(n, dtype=torch.int32, device=device) for _ in range(3))
+    lo, hi, target = (text.new_empty(n, dtype=torch.int32) for _ in range(3))
     size = lib.csa_lm_spans_workspace(n)
-    work = _work(size, device) if size else None
-    with _Call(device) as stream:
-        native.check(lib.csa_lm_spans_u16_dev(text.data_ptr() or None, n, int(separator), lo.data_ptr() or None, hi.data_ptr() or None,
-                                              target.data_ptr() or None, work.data_ptr() if size else None, size, stream))
+    keep, work = _work(size, text)
+    _enqueue(device, lib.csa_lm_spans_u16_dev, _address(text), n, int(separator), _address(lo), _address(hi), _address(target), work, size)
     return lo, hi, target
 
 
@@ -89,42 +97,40 @@ def token_spans(text, separator=SEPARATOR):
 
 
 def _walkable(x):
-    """x (tokens, heads, dim) as the kernels can read it: itself, or a copy where its strides or its address do not allow 16-byte loads."""
-    fine = (x.stride(2) == 1 or x.shape[2] == 1) and x.data_ptr() % 16 == 0
-    for size, stride in ((x.shape[0], x.stride(0)), (x.shape[1], x.stride(1))):
-        fine = fine and (size <= 1 or stride % 8 == 0)
-    if x.shape[0] > 1:
-        fine = fine and x.shape[2] <= x.stride(0) < 1 << 22
-    import torch
-    return x if fine else x.clone(memory_format=torch.contiguous_format)
-
-
-def _heads(x):
-    """Strides of axes of length one mean nothing, and are named as a dense array's."""
-    token = x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
-    head = x.stride(1) if x.shape[1] > 1 else x.shape[2]
-    return native.CsaLmHeads(x.data_ptr() or None, max(token, x.shape[2]), head)
+    """x (tokens, heads, dim) as the kernels can read it, and its address and strides: itself, or a copy where its strides or its address do not
+    allow 16-byte loads. Strides of axes of length one mean nothing, and are named as a dense array's."""
+    tokens, heads, dim = x.shape
+    token, head, one = x.stride()
+    token, head = token if tokens > 1 else heads * dim, head if heads > 1 else dim
+    if one != 1 or token % 8 or head % 8 or not dim <= token < 1 << 22 or head < 0 or x.data_ptr() % 16:
+        import torch
+        x = x.clone(memory_format=torch.contiguous_format)
+        token, head = heads * dim, dim
+    return x, native.CsaLmHeads(x.data_ptr() or None, token, head)
 
 
 def _describe(q, k, v, lo, hi, scale, cap, slopes):
+    """The call's description, the device, and what has to live until it is enqueued."""
     import torch
     _check(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v: (tokens, heads, head_dim)")
     _check(q.dtype == k.dtype == v.dtype, "q, k and v have to be of one type")
-    _check(k.shape == v.shape, "k and v have to be of one shape")
     tokens, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    _check(k.shape == v.shape, "k and v have to be of one shape")
     _check(k.shape[0] == tokens and k.shape[2] == dim, "q and k have to agree in tokens and head_dim")
-    _check(k.shape[1] > 0 and heads > 0 and heads % k.shape[1] == 0, "the heads of q have to be a multiple of those of k and v")
+    _check(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "the heads of q have to be a multiple of those of k and v")
     _check(8 <= dim <= 128 and dim % 8 == 0, "head_dim has to be a multiple of 8 from 8 to 128")
-    for name, span in (("lo", lo), ("hi", hi)):
-        _check(span is None or (span.dtype == torch.int32 and span.shape == (tokens,) and span.is_contiguous()), f"{name}: one int32 a token")
-    _check(slopes is None or (slopes.dtype == torch.float32 and slopes.shape == (heads,) and slopes.is_contiguous()), "slopes: one float32 a head of q")
+    for span in (lo, hi):
+        if span is not None:
+            _check(span.dtype == torch.int32 and span.dim() == 1 and span.numel() == tokens and span.is_contiguous(), "lo, hi: one int32 a token")
+    if slopes is not None:
+        _check(slopes.dtype == torch.float32 and slopes.dim() == 1 and slopes.numel() == heads and slopes.is_contiguous(), "slopes: one float32 a head of q")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     _check(0 < scale < 3e38 and 0 <= cap < 3e38, "scale has to be positive and finite, cap positive or 0")
-    q, k, v = _walkable(q), _walkable(k), _walkable(v)
-    pointer = lambda t: t.data_ptr() or None if t is not None else None  # noqa: E731
-    a = native.CsaLmAttention(_matrix_type(q.dtype), heads, k.shape[1], dim, tokens, pointer(lo), pointer(hi), pointer(slopes), scale, float(cap),
-                              _heads(q), _heads(k), _heads(v))
-    device = _on_gpu([t for t in (q, k, v, lo, hi, slopes) if t is not None])
+    kind = _matrix_type(q.dtype)
+    device = _on_gpu(q, k, v, lo, hi, slopes)
+    (q, qh), (k, kh), (v, vh) = _walkable(q), _walkable(k), _walkable(v)
+    a = native.CsaLmAttention(kind, heads, kv_heads, dim, tokens, _address(lo), _address(hi), _address(slopes), scale, float(cap), qh, kh, vh)
     return a, device, (q, k, v)
 
 
@@ -139,14 +145,13 @@ def span_attention(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
     Returns (out of q's shape, lse float32 (heads, tokens)); rows that see nothing are zeros with lse -inf (csa_lm_attention_forward_dev)."""
     import torch
     a, device, keep = _describe(q, k, v, lo, hi, scale, cap, slopes)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device)
-    if q.shape[0]:
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((a.q_heads, a.tokens), dtype=torch.float32)
+    if a.tokens:
         lib = native.load()
-        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1], k.shape[1], q.shape[2], 0)
-        work = _work(size, device)
-        with _Call(device) as stream:
-            native.check(lib.csa_lm_attention_forward_dev(C.byref(a), _heads(out), lse.data_ptr(), work.data_ptr(), size, stream))
+        size = lib.csa_lm_attention_workspace(a.tokens, a.q_heads, a.kv_heads, a.head_dim, 0)
+        scratch, work = _work(size, q)
+        _enqueue(device, lib.csa_lm_attention_forward_dev, C.byref(a), _walkable(out)[1], lse.data_ptr(), work, size)
     return out, lse
 
 
@@ -156,17 +161,15 @@ def span_attention_backward(d_out, q, k, v, out, lse, lo=None, hi=None, scale=No
     import torch
     a, device, keep = _describe(q, k, v, lo, hi, scale, cap, slopes)
     _check(out.shape == q.shape and d_out.shape == q.shape and out.dtype == q.dtype and d_out.dtype == q.dtype, "out and d_out have to be like q")
-    _check(lse.shape == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse: float32 (heads, tokens)")
-    _on_gpu([q, out, d_out, lse])
-    out, d_out = _walkable(out), _walkable(d_out)
-    d_q, d_k, d_v = (torch.empty(x.shape, dtype=q.dtype, device=device) for x in (q, k, v))
-    if q.shape[0]:
+    _check(lse.shape == (a.q_heads, a.tokens) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse: float32 (heads, tokens)")
+    _on_gpu(q, out, d_out, lse)
+    (out, oh), (d_out, gh) = _walkable(out), _walkable(d_out)
+    d_q, d_k, d_v = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    if a.tokens:
         lib = native.load()
-        size = lib.csa_lm_attention_workspace(q.shape[0], q.shape[1], k.shape[1], q.shape[2], native.CSA_LM_BACKWARD)
-        work = _work(size, device)
-        with _Call(device) as stream:
-            native.check(lib.csa_lm_attention_backward_dev(C.byref(a), _heads(out), lse.data_ptr(), _heads(d_out), _heads(d_q), _heads(d_k), _heads(d_v),
-                                                           work.data_ptr(), size, stream))
+        size = lib.csa_lm_attention_workspace(a.tokens, a.q_heads, a.kv_heads, a.head_dim, native.CSA_LM_BACKWARD)
+        scratch, work = _work(size, q)
+        _enqueue(device, lib.csa_lm_attention_backward_dev, C.byref(a), oh, lse.data_ptr(), gh, _walkable(d_q)[1], _walkable(d_k)[1], _walkable(d_v)[1], work, size)
     return d_q, d_k, d_v
 
 
@@ -180,19 +183,19 @@ def _rows(x):
     return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _entropy_work(lib, device, hidden, hs, weight, ws, flags):
+def _entropy_work(lib, hidden, hs, weight, ws, flags):
     if hidden.data_ptr() % 16 or weight.data_ptr() % 16 or hs % 8 or ws % 8:
         flags |= native.CSA_LM_COPY_ROWS
     size = lib.csa_lm_cross_entropy_workspace(hidden.shape[0], hidden.shape[1], weight.shape[0], flags)
-    return _work(size, device), size
+    return (size, *_work(size, hidden))
 
 
 def _check_entropy(hidden, weight, target):
     import torch
     _check(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1], "hidden: (tokens, dim), weight: (vocabulary, dim)")
     _check(hidden.dtype == weight.dtype, "hidden and weight have to be of one type")
-    _check(weight.shape[0] > 0 and weight.shape[1] > 0, "weight has to hold something")
-    _check(target.shape == (hidden.shape[0],) and target.dtype == torch.int32 and target.is_contiguous(), "target: one int32 a token")
+    _check(weight.numel() > 0, "weight has to hold something")
+    _check(target.dim() == 1 and target.numel() == hidden.shape[0] and target.dtype == torch.int32 and target.is_contiguous(), "target: one int32 a token")
     return _matrix_type(hidden.dtype)
 
 
@@ -204,16 +207,15 @@ def linear_cross_entropy(hidden, weight, target):
     (csa_lm_cross_entropy_forward_dev)."""
     import torch
     kind = _check_entropy(hidden, weight, target)
-    device = _on_gpu([hidden, weight, target])
+    device = _on_gpu(hidden, weight, target)
     n, dim = hidden.shape
-    loss, lse = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(2))
+    loss, lse = hidden.new_empty(n, dtype=torch.float32), hidden.new_empty(n, dtype=torch.float32)
     if n:
         lib = native.load()
         (hidden, hs), (weight, ws) = _rows(hidden), _rows(weight)
-        work, size = _entropy_work(lib, device, hidden, hs, weight, ws, 0)
-        with _Call(device) as stream:
-            native.check(lib.csa_lm_cross_entropy_forward_dev(kind, hidden.data_ptr(), hs, weight.data_ptr(), ws, target.data_ptr(), n, dim, weight.shape[0],
-                                                              loss.data_ptr(), lse.data_ptr(), work.data_ptr(), size, stream))
+        size, scratch, work = _entropy_work(lib, hidden, hs, weight, ws, 0)
+        _enqueue(device, lib.csa_lm_cross_entropy_forward_dev, kind, hidden.data_ptr(), hs, weight.data_ptr(), ws, target.data_ptr(), n, dim, weight.shape[0],
+                 loss.data_ptr(), lse.data_ptr(), work, size)
     return loss, lse
 
 
@@ -222,20 +224,17 @@ def linear_cross_entropy_backward(d_loss, hidden, weight, target, lse, want_hidd
     linear_cross_entropy returned it (csa_lm_cross_entropy_backward_dev). A gradient that is not wanted is None."""
     import torch
     kind = _check_entropy(hidden, weight, target)
-    device = _on_gpu([hidden, weight, target, d_loss, lse])
+    device = _on_gpu(hidden, weight, target, d_loss, lse)
     n, dim = hidden.shape
-    for name, x in (("d_loss", d_loss), ("lse", lse)):
-        _check(x.shape == (n,) and x.dtype == torch.float32 and x.is_contiguous(), f"{name}: one float32 a token")
-    d_hidden = torch.empty((n, dim), dtype=hidden.dtype, device=device) if want_hidden else None
-    d_weight = torch.empty(weight.shape, dtype=weight.dtype, device=device) if want_weight else None
+    for x in (d_loss, lse):
+        _check(x.dim() == 1 and x.numel() == n and x.dtype == torch.float32 and x.is_contiguous(), "d_loss, lse: one float32 a token")
+    d_hidden = hidden.new_empty((n, dim)) if want_hidden else None
+    d_weight = weight.new_empty(weight.shape) if want_weight else None
     lib = native.load()
     (hidden, hs), (weight, ws) = _rows(hidden), _rows(weight)
-    work, size = _entropy_work(lib, device, hidden, hs, weight, ws, native.CSA_LM_BACKWARD)
-    with _Call(device) as stream:
-        native.check(lib.csa_lm_cross_entropy_backward_dev(kind, hidden.data_ptr() or None, hs, weight.data_ptr(), ws, target.data_ptr() or None,
-                                                           lse.data_ptr() or None, d_loss.data_ptr() or None, n, dim, weight.shape[0],
-                                                           (d_hidden.data_ptr() or None) if want_hidden else None, dim,
-                                                           d_weight.data_ptr() if want_weight else None, dim, work.data_ptr(), size, stream))
+    size, scratch, work = _entropy_work(lib, hidden, hs, weight, ws, native.CSA_LM_BACKWARD)
+    _enqueue(device, lib.csa_lm_cross_entropy_backward_dev, kind, _address(hidden), hs, weight.data_ptr(), ws, _address(target), _address(lse), _address(d_loss), n,
+             dim, weight.shape[0], _address(d_hidden), dim, _address(d_weight), dim, work, size)
     return d_hidden, d_weight
 
 
@@ -252,18 +251,21 @@ def clip_gradients(grads, max_norm, out=None):
     _check(len(grads) > 0, "no gradients")
     _check(len(out) == len(grads), "out: a tensor for each gradient")
     _check(max_norm >= 0, "max_norm is negative or no number")
-    for g, o in zip(grads, out):
-        _check(g.is_contiguous() and o.is_contiguous() and g.shape == o.shape and g.dtype == o.dtype, "gradients and out: dense tensors, alike one by one")
-    device = _on_gpu(grads + (out if out is not grads else []))
-    lib = native.load()
+    device = grads[0].get_device()
+    _check(device >= 0, "the gradients have to lie on a GPU")
     items = (native.CsaLmValues * len(grads))()
     for item, g, o in zip(items, grads, out):
-        item.inp, item.out, item.n, item.type = g.data_ptr() or None, o.data_ptr() or None, g.numel(), _type(g.dtype)
-    norm = torch.empty((), dtype=torch.float32, device=device)
+        kind = _type(g.dtype)
+        _check(g.is_contiguous() and g.get_device() == device, "gradients: dense tensors on one GPU")
+        item.inp, item.n, item.type = g.data_ptr() or None, g.numel(), kind
+        if o is not g:
+            _check(o.is_contiguous() and o.shape == g.shape and o.dtype == g.dtype and o.get_device() == device, "out: tensors like the gradients, one by one")
+        item.out = o.data_ptr() or None
+    lib = native.load()
+    norm = grads[0].new_empty((), dtype=torch.float32)
     size = lib.csa_lm_clip_workspace(len(grads))
-    work = _work(size, device)
-    with _Call(device) as stream:
-        native.check(lib.csa_lm_clip_dev(items, len(grads), float(max_norm), norm.data_ptr(), work.data_ptr(), size, stream))
+    scratch, work = _work(size, norm)
+    _enqueue(device, lib.csa_lm_clip_dev, items, len(grads), float(max_norm), norm.data_ptr(), work, size)
     return norm
 
 
