@@ -79,17 +79,20 @@ struct HeadTile {
     }
 };
 
-// ROWS rows of one head, padded to DIM values with zeros, by WAVES waves.
+// ROWS rows of one head, padded to DIM values with zeros, by WAVES waves. Where the waves' loads together cover whole rows, sixteen or a multiple, a
+// lane's place within them is the same every time, and one register holds it; heads of 12 pieces need one a load.
 template <int ROWS, int DIM, int WAVES>
 struct HeadLoader {
     static constexpr int TOTAL = ROWS * DIM / 8 / 64, LOADS = (TOTAL + WAVES - 1) / WAVES; // instructions, of all waves and of one
+    static constexpr int STEP = WAVES * 64 * 8 / DIM;                                      // rows of an instruction of all waves
+    static constexpr bool SAME = WAVES * 64 * 8 % DIM == 0 && STEP % 16 == 0;
     static_assert(ROWS * DIM / 8 % 64 == 0, "whole waves");
     int64_t line; // bytes
-    uint32_t offset[LOADS];
+    uint32_t offset[SAME ? 1 : LOADS];
     __device__ void begin(const Heads& h, int dim, int wave, int lane)
     {
         line = h.token * 2;
-        for (int j = 0; j < LOADS; ++j) {
+        for (int j = 0; j < (SAME ? 1 : LOADS); ++j) {
             const int at = (j * WAVES + wave) * 64 + lane, row = at / (DIM / 8), piece = HeadTile<DIM>::place(row, at % (DIM / 8));
             offset[j] = piece * 8 < dim ? static_cast<uint32_t>(row * line + piece * 16) : OUTSIDE;
         }
@@ -97,12 +100,18 @@ struct HeadLoader {
     // rows row0 ... of the head that `base` points at, of `rows`; those past the end are zeros
     __device__ void load(const char* base, int64_t row0, int64_t rows, short* tile, int wave) const
     {
-        const int64_t left = rows - row0;
-        const buffer_t w = window(base + row0 * line, left > 0 ? static_cast<uint32_t>((left < ROWS ? left : ROWS) * line) : 0);
+        int left = static_cast<int>(rows - row0 < ROWS ? rows - row0 : ROWS);
+        const char* from = base + row0 * line;
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j)
+        for (int j = 0; j < LOADS; ++j) {
+            const buffer_t w = window(from, left > 0 ? static_cast<uint32_t>(left) * static_cast<uint32_t>(line) : 0);
             if (TOTAL % WAVES == 0 || j * WAVES + wave < TOTAL)
-                load_to_lds(w, tile + (j * WAVES + wave) * 512, offset[j]);
+                load_to_lds(w, tile + (j * WAVES + wave) * 512, offset[SAME ? 0 : j]);
+            if (SAME) {
+                left -= STEP;
+                from += STEP * line;
+            }
+        }
     }
 };
 
@@ -193,6 +202,57 @@ __device__ inline void read_ahead()
     }
     __builtin_amdgcn_sched_group_barrier(0x8, PRODUCTS - TURNS, 0);
 }
+
+// ---- what a row may not see ----
+//
+// A score that a row may not see becomes a probability of 0, but 0 times an infinity or NaN that stands there is none. What no row of a workgroup sees is
+// not loaded at all (padding behind a text may hold anything); where a sum has become infinite or NaN all the same, it is done again one by one, over what
+// counts and nothing else: documents next to one that has gone wrong stay as they are.
+
+template <int N>
+__device__ inline bool all_finite(const f32x16 (&x)[N])
+{
+    float worst = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            worst = fmaxf(worst, x[e][r] - x[e][r] == 0.f ? 0.f : 1.f);
+    return worst == 0.f;
+}
+
+template <class Type>
+__device__ inline float dot_rows(const short* x, const short* y, int dim)
+{
+    float sum = 0.f;
+    for (int d = 0; d < dim; d += 8) {
+        const s16x8 a = *reinterpret_cast<const s16x8*>(x + d), b = *reinterpret_cast<const s16x8*>(y + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            sum += to32<Type>(a[i]) * to32<Type>(b[i]);
+    }
+    return sum;
+}
+
+// The exponent of 2 of one score, and what its gradient is multiplied by.
+__device__ inline float one_score(const Attention& a, float product, float slope2, float distance, float& bent)
+{
+    float z = product * a.scale * LOG2E;
+    bent = 1.f;
+    if (a.cap > 0.f) {
+        const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * (2.f * LOG2E * a.scale / a.cap)));
+        z = a.cap * LOG2E * t;
+        bent = 1.f - t * t;
+    }
+    return z - slope2 * fabsf(distance);
+}
+
+__device__ inline const short* row_of(const Heads& h, uint32_t head, int64_t row)
+{
+    return static_cast<const short*>(h.data) + head * h.head + row * h.token;
+}
+
+__device__ inline float lane_of(float x, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane)); }
 
 constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
 
@@ -319,33 +379,61 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
     };
 
     if (group_lo < group_hi) {
-        const int begin = group_lo / KT * KT;
-        kl.load(kb, begin, a.tokens, k0s, wave);
-        vl.load(vb, begin, a.tokens, v0s, wave);
+        const int begin = group_lo;
+        kl.load(kb, begin, group_hi, k0s, wave);
+        vl.load(vb, begin, group_hi, v0s, wave);
         for (int key0 = begin; key0 < group_hi; key0 += 2 * KT) {
             wait_for_all();
             meet();
-            kl.load(kb, key0 + KT, a.tokens, k1s, wave);
-            vl.load(vb, key0 + KT, a.tokens, v1s, wave);
+            kl.load(kb, key0 + KT, group_hi, k1s, wave);
+            vl.load(vb, key0 + KT, group_hi, v1s, wave);
             turn(k0s, v0s, key0);
             wait_for_all();
             meet();
-            kl.load(kb, key0 + 2 * KT, a.tokens, k0s, wave);
-            vl.load(vb, key0 + 2 * KT, a.tokens, v0s, wave);
+            kl.load(kb, key0 + 2 * KT, group_hi, k0s, wave);
+            vl.load(vb, key0 + 2 * KT, group_hi, v0s, wave);
             turn(k1s, v1s, key0 + KT);
         }
         wait_for_all();
     }
     sum += other_half(sum);
+    const float share = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const uint64_t lost = __ballot(!all_finite(o));
+    const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
+    for (uint32_t left = redo; left; left &= left - 1) {
+        const int r = __builtin_ctz(left);
+        const int64_t i = first + wave * 32 + r;
+        if (i >= a.tokens)
+            continue;
+        const int from = __builtin_amdgcn_readlane(lo, r), to = __builtin_amdgcn_readlane(hi, r);
+        const float high = lane_of(top, r), part = lane_of(share, r);
+        float x = 0.f, y = 0.f;
+        for (int j0 = from; j0 < to; j0 += 64) {
+            const int j = j0 + lane, count = min(64, to - j0);
+            float bent, p = 0.f;
+            if (j < to)
+                p = __builtin_amdgcn_exp2f(one_score(a, dot_rows<Type>(row_of(a.q, head, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent) - high) * part;
+            for (int c = 0; c < count; ++c) {
+                const short* v = row_of(a.v, kv, j0 + c);
+                const float pc = lane_of(p, c);
+                x += lane < a.dim ? pc * to32<Type>(v[lane]) : 0.f;
+                y += lane + 64 < a.dim ? pc * to32<Type>(v[lane + 64]) : 0.f;
+            }
+        }
+        short* to_row = out + head * out_head + i * out_token;
+        if (lane < a.dim)
+            to_row[lane] = to16<Type>(x);
+        if (lane + 64 < a.dim)
+            to_row[lane + 64] = to16<Type>(y);
+    }
     if (row < a.tokens) {
-        const float share = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         short* to = out + head * out_head + row * out_token;
 #pragma unroll
         for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * e + 8 * g + 4 * half;
-                if (d < a.dim) {
+                if (d < a.dim && !(redo >> lane % 32 & 1)) {
                     s16x4 y;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -416,11 +504,13 @@ __global__ __launch_bounds__(256) void row_blocks_kernel(Attention a, Heads out,
         if (row < a.tokens) {
             const short* g = static_cast<const short*>(d_out.data) + head * d_out.head + row * d_out.token;
             delta = dot16<Type>(static_cast<const short*>(out.data) + head * out.head + row * out.token, g, a.dim, lane16);
-            if (!Type::wide_range) {
-                most = fmaxf(most, dot16<Type>(g, g, a.dim, lane16));
+            if (!Type::wide_range) { // finite ones: the others belong to rows that nobody sees, or to ones that are lost anyway
+                const float square = dot16<Type>(g, g, a.dim, lane16);
+                most = square < INFINITY ? fmaxf(most, square) : most;
                 if (head % a.group == 0) {
                     const short* v = static_cast<const short*>(a.v.data) + head / a.group * a.v.head + row * a.v.token;
-                    most_v = fmaxf(most_v, dot16<Type>(v, v, a.dim, lane16));
+                    const float square_v = dot16<Type>(v, v, a.dim, lane16);
+                    most_v = square_v < INFINITY ? fmaxf(most_v, square_v) : most_v;
                 }
             }
         }
@@ -596,27 +686,58 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
     };
 
     if (group_lo < group_hi) {
-        const int begin = group_lo / KT * KT;
-        kl.load(kb, begin, a.tokens, k0s, wave);
-        vl.load(vb, begin, a.tokens, v0s, wave);
+        const int begin = group_lo;
+        kl.load(kb, begin, group_hi, k0s, wave);
+        vl.load(vb, begin, group_hi, v0s, wave);
         for (int key0 = begin; key0 < group_hi; key0 += 2 * KT) {
             wait_for_all();
             meet();
-            kl.load(kb, key0 + KT, a.tokens, k1s, wave);
-            vl.load(vb, key0 + KT, a.tokens, v1s, wave);
+            kl.load(kb, key0 + KT, group_hi, k1s, wave);
+            vl.load(vb, key0 + KT, group_hi, v1s, wave);
             turn(k0s, v0s, key0);
             wait_for_all();
             meet();
-            kl.load(kb, key0 + 2 * KT, a.tokens, k0s, wave);
-            vl.load(vb, key0 + 2 * KT, a.tokens, v0s, wave);
+            kl.load(kb, key0 + 2 * KT, group_hi, k0s, wave);
+            vl.load(vb, key0 + 2 * KT, group_hi, v0s, wave);
             turn(k1s, v1s, key0 + KT);
         }
         wait_for_all();
     }
     rest += other_half(rest);
+    const float exact = delta + rest / grow;
+    const uint64_t lost = __ballot(!all_finite(o));
+    const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
+    for (uint32_t left = redo; left; left &= left - 1) {
+        const int r = __builtin_ctz(left);
+        const int64_t i = first + wave * 32 + r;
+        if (i >= a.tokens)
+            continue;
+        const int from = __builtin_amdgcn_readlane(lo, r), to = __builtin_amdgcn_readlane(hi, r);
+        const float base = lane_of(lse2, r), mean = lane_of(exact, r);
+        float x = 0.f, y = 0.f;
+        for (int j0 = from; j0 < to; j0 += 64) {
+            const int j = j0 + lane, count = min(64, to - j0);
+            float bent, ds = 0.f;
+            if (j < to) {
+                const float z = one_score(a, dot_rows<Type>(row_of(a.q, head, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent);
+                ds = __builtin_amdgcn_exp2f(z - base) * (dot_rows<Type>(row_of(d_out, head, i), row_of(a.v, kv, j), a.dim) - mean) * bent * a.scale;
+            }
+            for (int c = 0; c < count; ++c) {
+                const short* k = row_of(a.k, kv, j0 + c);
+                const float dc = lane_of(ds, c);
+                x += lane < a.dim ? dc * to32<Type>(k[lane]) : 0.f;
+                y += lane + 64 < a.dim ? dc * to32<Type>(k[lane + 64]) : 0.f;
+            }
+        }
+        short* to_row = d_q + head * out_head + i * out_token;
+        if (lane < a.dim)
+            to_row[lane] = to16<Type>(x);
+        if (lane + 64 < a.dim)
+            to_row[lane + 64] = to16<Type>(y);
+    }
     if (row < a.tokens) {
         if (half == 0)
-            blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = delta + rest / grow;
+            blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = exact;
         const float back = a.scale / grow;
         short* to = d_q + head * out_head + row * out_token;
 #pragma unroll
@@ -624,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int d = 32 * e + 8 * k + 4 * half;
-                if (d < a.dim) {
+                if (d < a.dim && !(redo >> lane % 32 & 1)) {
                     s16x4 y;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -743,6 +864,20 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         }
         read_ahead<DIM / 4, DIM / 8, 6, 2>();
     };
+    // Rows that see nothing may hold anything: they become zeros, by all waves, before the tile is used.
+    auto clear = [&](short* qs, short* gs, const RowBlock& bs) {
+        const int r = lane % 32;
+        uint32_t empty = static_cast<uint32_t>(__ballot(bs.lo[r] == NONE && static_cast<int64_t>(tile) * RT + r < a.tokens));
+        if (!empty)
+            return;
+        for (; empty; empty &= empty - 1) {
+            const int at = __builtin_ctz(empty) * DIM + static_cast<int>(threadIdx.x % (DIM / 8)) * 8;
+            if (threadIdx.x < DIM / 4)
+                *reinterpret_cast<s16x8*>((threadIdx.x < DIM / 8 ? qs : gs) + at) = s16x8{};
+        }
+        wait_for_lds();
+        meet();
+    };
     auto next = [&] {
         tile = tile < to ? tile + 1 : from;
         head += tile == from;
@@ -755,19 +890,71 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
             wait_for_all();
             meet();
             load(q1s, g1s, b1s);
+            clear(q0s, g0s, b0s[0]);
             turn(q0s, g0s, b0s[0]);
             const bool more = next();
             wait_for_all();
             meet();
             load(q0s, g0s, b0s);
-            if (more)
+            if (more) {
+                clear(q1s, g1s, b1s[0]);
                 turn(q1s, g1s, b1s[0]);
+            }
             if (!more || !next())
                 break;
         }
         wait_for_all();
     }
-    if (key < a.tokens) {
+    const uint64_t lost = __ballot(!all_finite(ok) || !all_finite(ov));
+    const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
+    for (uint32_t left = redo; left; left &= left - 1) {
+        const int j = wave_key + __builtin_ctz(left);
+        if (j >= a.tokens)
+            continue;
+        float kx = 0.f, ky = 0.f, vx = 0.f, vy = 0.f;
+        for (uint32_t h = head0; h < head0 + heads; ++h) {
+            const float slope2 = a.slope ? a.slope[h] * LOG2E : 0.f;
+            for (int t = from; t <= to; ++t) {
+                const RowBlock& b = blocks[static_cast<int64_t>(h) * tiles + t];
+                const int r = lane % 32, i = t * RT + r;
+                const bool sees = lane < 32 && b.lo[r] <= j && j < b.hi[r];
+                float bent, p = 0.f, ds = 0.f;
+                if (sees) {
+                    const float z = one_score(a, dot_rows<Type>(row_of(a.q, h, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent);
+                    p = __builtin_amdgcn_exp2f(z - b.lse2[r]);
+                    ds = p * (dot_rows<Type>(row_of(d_out, h, i), row_of(a.v, kv, j), a.dim) - b.delta[r]) * bent * a.scale;
+                }
+                for (uint32_t rows = static_cast<uint32_t>(__ballot(sees)); rows; rows &= rows - 1) {
+                    const int c = __builtin_ctz(rows);
+                    const short *q = row_of(a.q, h, t * RT + c), *g = row_of(d_out, h, t * RT + c);
+                    const float pc = lane_of(p, c), dc = lane_of(ds, c);
+                    if (lane < a.dim) {
+                        kx += dc * to32<Type>(q[lane]);
+                        vx += pc * to32<Type>(g[lane]);
+                    }
+                    if (lane + 64 < a.dim) {
+                        ky += dc * to32<Type>(q[lane + 64]);
+                        vy += pc * to32<Type>(g[lane + 64]);
+                    }
+                }
+            }
+        }
+        for (int half64 = 0; half64 < 2; ++half64) {
+            const int d = lane + 64 * half64;
+            const float gk = half64 ? ky : kx, gv = half64 ? vy : vx;
+            if (d >= a.dim)
+                continue;
+            if (shares > 1) {
+                float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + j) * DIM + d;
+                part[0] = gk;
+                part[a.tokens * DIM] = gv;
+            } else {
+                d_k[kv * dk_head + static_cast<int64_t>(j) * dk_token + d] = to16<Type>(gk);
+                d_v[kv * dv_head + static_cast<int64_t>(j) * dv_token + d] = to16<Type>(gv);
+            }
+        }
+    }
+    if (key < a.tokens && !(redo >> lane % 32 & 1)) {
         const float back_k = a.scale / grow, back_v = Type::wide_range ? 1.f : 0x1p-15f;
         if (shares > 1) {
             float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
@@ -859,7 +1046,7 @@ __global__ __launch_bounds__(1024) void tile_order_kernel(Attention a, uint32_t*
             for (int w = 0; w < t / 64; ++w)
                 mine += sums[w];
         } else if (los[t] < his[t]) {
-            mine = (his[t] - los[t] / KEYS_PER_TILE * KEYS_PER_TILE + KEYS_PER_TILE - 1) / KEYS_PER_TILE;
+            mine = (his[t] - los[t] + KEYS_PER_TILE - 1) / KEYS_PER_TILE;
         }
         work[t] = mine;
         __syncthreads();

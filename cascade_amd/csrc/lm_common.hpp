@@ -82,11 +82,9 @@ __device__ inline float other_half(float x)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-template <int N>
-__device__ inline void wait_for_loads_but() { __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14); } // all but the last N
-__device__ inline void wait_for_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); } // vmcnt(0), the other counters free
 
-__device__ inline void wait_for_all() { __builtin_amdgcn_s_waitcnt(0x0070); }   // LDS reads too
+__device__ inline void wait_for_all() { __builtin_amdgcn_s_waitcnt(0x0070); } // loads and LDS accesses: vmcnt(0), lgkmcnt(0)
+__device__ inline void wait_for_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); } // LDS accesses alone: lgkmcnt(0)
 // All waves of the workgroup, without a wait for loads in flight; the compiler moves no memory access across it.
 __device__ inline void meet()
 {

@@ -238,6 +238,43 @@ def test_half_precision_keeps_small_gradients():
         within(x, want[name], 1.1 * (sums[name] + U[torch.float16] * want[name].abs()) + 2.0 ** -24, name)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 1, 128), (3, 3, 88)])
+def test_what_a_row_may_not_see_may_hold_anything(dtype, heads, kv_heads, dim):
+    """Infinities and NaN in padding, and in one document of three, change nothing elsewhere, forwards and backwards."""
+    g = gen(13)
+    n, text = 500, 470  # padding behind 470 positions
+    at = torch.arange(n, device="cuda")
+    ends = torch.tensor([0, 150, 301, text], device="cuda")
+    lo = ends[torch.searchsorted(ends, at, right=True) - 1].int()
+    hi = (at + 1).int()
+    lo[text:], hi[text:] = 0, 0
+    q, d_out = (randn(g, n, heads, dim, dtype=dtype) for _ in range(2))
+    k, v = (randn(g, n, kv_heads, dim, dtype=dtype) for _ in range(2))
+
+    def once(q, k, v, d_out, **how):
+        out, lse = cascade_amd.span_attention(q, k, v, lo, hi, **how)
+        return out, lse.T, *cascade_amd.span_attention_backward(d_out, q, k, v, out, lse, lo, hi, **how)
+    for how in ({}, {"cap": 10.0, "slopes": torch.linspace(0.01, 0.1, heads, device="cuda")}):
+        clean = once(q, k, v, d_out, **how)
+        for where in (slice(text, n), slice(150, 301)):
+            spoilt = [x.clone() for x in (q, k, v, d_out)]
+            for i, x in enumerate(spoilt):
+                x[where][i % 2::2] = math.nan
+                x[where][(i + 1) % 2::3] = math.inf
+            got = once(*spoilt, **how)
+            rest = torch.ones(n, dtype=torch.bool, device="cuda")
+            rest[where] = False
+            for a, b, name in zip(got, clean, ("out", "lse", "d_q", "d_k", "d_v")):
+                # sums that were done again one by one are rounded elsewhere: by two roundings of the type at most, of the largest terms
+                a, b = a[rest].double(), b[rest].double()
+                fine = torch.isfinite(b)
+                assert torch.equal(torch.isfinite(a), fine) and torch.equal(a[~fine], b[~fine]), name
+                assert ((a - b)[fine].abs() <= 4 * U[dtype] * b[fine].abs().max()).all(), name
+            if where.start == text:
+                assert all((x[text:] == 0).all() for x in (got[0], got[2], got[3], got[4]))
+
+
 def test_attention_gradients_agree_with_differences():
     g = gen(10)
     n, h, d = 70, 2, 64
