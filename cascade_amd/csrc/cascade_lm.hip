@@ -157,17 +157,17 @@ struct AttentionWork {
     }
 };
 
-template <class Type, int DIM>
+template <class Type, int DIM, bool BENT>
 void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_heads& out, float* lse, hipStream_t s)
 {
     const bool order = in_order(a);
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), w.row_order, nullptr);
-    attention_forward_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
+    attention_forward_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
         attention(a), order ? w.row_order : nullptr, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
 }
 
-template <class Type, int DIM>
+template <class Type, int DIM, bool BENT>
 void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* lse, const csa_lm_heads& d_out, const csa_lm_heads& d_q, const csa_lm_heads& d_k,
               const csa_lm_heads& d_v, const AttentionWork& w, hipStream_t s)
 {
@@ -178,9 +178,9 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(at, w.row_order, w.key_order);
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
-    attention_d_q_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
+    attention_d_q_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
         at, order ? w.row_order : nullptr, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
-    attention_d_kv_kernel<Type, DIM><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
+    attention_d_kv_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
         at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.share_heads, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
         d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
     if (w.shares > 1)
@@ -190,22 +190,32 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
 }
 
 template <class F>
-void with_dim(uint32_t dim, F f)
-{
-    if (head_width(dim) == 64)
-        f(std::integral_constant<int, 64>());
-    else if (head_width(dim) == 96)
-        f(std::integral_constant<int, 96>());
-    else
-        f(std::integral_constant<int, 128>());
-}
-template <class F>
 void with_type(int type, F f)
 {
     if (type == CSA_LM_F16)
         f(F16());
     else
         f(Bf16());
+}
+
+// f(type, head width, whether scores are bent) as types
+template <class F>
+void with_kind(const csa_lm_attention& a, F f)
+{
+    with_type(a.type, [&](auto type) {
+        auto with_width = [&](auto width) {
+            if (a.cap > 0.f || a.d_slope)
+                f(type, width, std::true_type());
+            else
+                f(type, width, std::false_type());
+        };
+        if (head_width(a.head_dim) == 64)
+            with_width(std::integral_constant<int, 64>());
+        else if (head_width(a.head_dim) == 96)
+            with_width(std::integral_constant<int, 96>());
+        else
+            with_width(std::integral_constant<int, 128>());
+    });
 }
 
 // ---- cross entropy ----
@@ -411,7 +421,7 @@ int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, fl
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    with_type(a->type, [&](auto type) { with_dim(a->head_dim, [&](auto dim) { forward<decltype(type), dim()>(*a, w, out, d_lse, s); }); });
+    with_kind(*a, [&](auto type, auto width, auto bent) { forward<decltype(type), width(), bent()>(*a, w, out, d_lse, s); });
     return launched(who);
 }
 
@@ -441,7 +451,7 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    with_type(a->type, [&](auto type) { with_dim(a->head_dim, [&](auto dim) { backward<decltype(type), dim()>(*a, out, d_lse, d_out, d_q, d_k, d_v, w, s); }); });
+    with_kind(*a, [&](auto type, auto width, auto bent) { backward<decltype(type), width(), bent()>(*a, out, d_lse, d_out, d_q, d_k, d_v, w, s); });
     return launched(who);
 }
 

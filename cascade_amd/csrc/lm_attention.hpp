@@ -256,11 +256,16 @@ __device__ inline float lane_of(float x, int lane) { return __builtin_bit_cast(f
 
 constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
 
+// BENT: there is a cap or a slope. Kernels without them are compiled without the code for them, which costs the others registers even where it
+// does not run.
+//
 // Scores of a tile, still raw products: to exponents of 2 less nothing, with `unit` left to multiply. Returns with z = s * unit.
-template <int TILES>
+template <bool BENT, int TILES>
 __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit, float slope2, int row, int key0, int half)
 {
     unit = a.scale * LOG2E;
+    if (!BENT)
+        return;
     if (a.cap > 0.f) {
         const float in = 2.f * LOG2E * a.scale / a.cap, cap2 = a.cap * LOG2E;
 #pragma unroll
@@ -282,7 +287,7 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
     }
 }
 
-template <class Type, int DIM>
+template <class Type, int DIM, bool BENT>
 __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, const uint32_t* order, short* out, int64_t out_token, int64_t out_head, float* lse)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
@@ -324,14 +329,16 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
         const HeadTile<DIM> tiles_at = lane_at.afresh();
         f32x16 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < 2; ++t)
             s[t] = f32x16{};
 #pragma unroll
-            for (int d = 0; d < DIM / 16; ++d)
+        for (int d = 0; d < DIM / 16; ++d)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
                 s[t] = Type::mfma32(tiles_at.along(ks, 32 * t, d), q[d], s[t]);
-        }
+        read_ahead<DIM / 8, DIM / 8, 4, 1>();
         float unit;
-        bend(a, s, unit, slope2, static_cast<int>(row), key0, half);
+        bend<BENT>(a, s, unit, slope2, static_cast<int>(row), key0, half);
         if (key0 < all_lo || key0 + KT > all_hi) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -557,7 +564,7 @@ constexpr float P_SHIFT = Type::wide_range ? 0.f : 15.f;
 
 // p and ds of 32 x 32 scores: s and dp in, p (times 2^shift) and ds (times `grow`) out. `lse2(r)`, `delta(r)`, `distance(r)`, `seen(r)` of register r.
 // With REST, returns the sum of p (dp - delta) over the lane's registers, times both factors.
-template <bool REST, class L, class D, class X, class S>
+template <bool BENT, bool REST, class L, class D, class X, class S>
 __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, float grow, bool masked, L lse2, D delta, X distance,
                                         S seen)
 {
@@ -566,7 +573,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
     for (int r = 0; r < 16; ++r)
         dp[r] = (dp[r] - delta(r)) * grow;
     float unit = a.scale * LOG2E;
-    if (a.cap > 0.f) {
+    if (BENT && a.cap > 0.f) {
         const float in = 2.f * LOG2E * a.scale / a.cap, cap2 = a.cap * LOG2E;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -579,7 +586,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
         }
         unit = 1.f;
     }
-    if (a.slope) {
+    if (BENT && a.slope) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             s[r] = s[r] * unit - slope2 * fabsf(distance(r));
@@ -604,7 +611,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
 #pragma unroll
     for (int r = 0; r < 16; ++r)
         sum += dp[r];
-    if (a.cap > 0.f) {
+    if (BENT && a.cap > 0.f) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             dp[r] *= bent[r];
@@ -612,7 +619,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
     return sum;
 }
 
-template <class Type, int DIM>
+template <class Type, int DIM, bool BENT>
 __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, Heads d_out, RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
                                                                short* d_q, int64_t out_token, int64_t out_head)
 {
@@ -668,7 +675,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
                 dp = Type::mfma32(tiles_at.along(vs, 32 * t, d), g[d], dp);
             }
             const int key = key0 + 32 * t + 4 * half, i = static_cast<int>(row);
-            rest += score_gradients<true>(
+            rest += score_gradients<BENT, true>(
                 a, s, dp, slope2, 0.f, grow, masked, [&](int) { return lse2; }, [&](int) { return delta; },
                 [&](int r) { return static_cast<float>(i - (key + 8 * (r / 4) + r % 4)); },
                 [&](int r) { const int k = key + 8 * (r / 4) + r % 4; return k >= lo && k < hi; });
@@ -760,7 +767,7 @@ constexpr int KEYS_PER_GROUP = 128;
 
 // The workgroup's 128 keys by 32 rows a turn, 32 keys a wave. Two waves of a SIMD have 256 registers each: at 128 values a head the sums of d_k and
 // d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
-template <class Type, int DIM>
+template <class Type, int DIM, bool BENT>
 __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, const uint32_t* order, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
                                                                 const uint32_t* norms, uint32_t shares, uint32_t share_heads, float* parts, short* d_k,
                                                                 int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
@@ -831,9 +838,19 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
     };
     uint32_t head = head0;
     int tile = from;
-    auto turn = [&](const short* qs, const short* gs, const RowBlock& bs) {
+    auto turn = [&](short* qs, short* gs, const RowBlock& bs) {
         // which of the rows see any of the wave's 32 keys, and which do not see all of them
         const int lo = bs.lo[lane % 32], hi = bs.hi[lane % 32];
+        // Rows that see nothing may hold anything: they become zeros, by all waves, before the tile is used.
+        if (uint32_t empty = static_cast<uint32_t>(__ballot(lo == NONE && tile * RT + lane % 32 < static_cast<int>(a.tokens)))) {
+            for (; empty; empty &= empty - 1) {
+                const int at = __builtin_ctz(empty) * DIM + static_cast<int>(threadIdx.x % (DIM / 8)) * 8;
+                if (threadIdx.x < DIM / 4)
+                    *reinterpret_cast<s16x8*>((threadIdx.x < DIM / 8 ? qs : gs) + at) = s16x8{};
+            }
+            wait_for_lds();
+            meet();
+        }
         if (!__any(lo < wave_key + 32 && hi > wave_key))
             return;
         const bool masked = __any(lo > wave_key || hi < wave_key + 32);
@@ -846,7 +863,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         }
         const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
         const int row = tile * RT + 4 * half;
-        score_gradients<false>(
+        score_gradients<BENT, false>(
             a, s, dp, slope2, P_SHIFT<Type>, grow_k, masked, [&](int r) { return bs.lse2[4 * half + 8 * (r / 4) + r % 4]; },
             [&](int r) { return bs.delta[4 * half + 8 * (r / 4) + r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
             [&](int r) {
@@ -864,20 +881,6 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         }
         read_ahead<DIM / 4, DIM / 8, 6, 2>();
     };
-    // Rows that see nothing may hold anything: they become zeros, by all waves, before the tile is used.
-    auto clear = [&](short* qs, short* gs, const RowBlock& bs) {
-        const int r = lane % 32;
-        uint32_t empty = static_cast<uint32_t>(__ballot(bs.lo[r] == NONE && static_cast<int64_t>(tile) * RT + r < a.tokens));
-        if (!empty)
-            return;
-        for (; empty; empty &= empty - 1) {
-            const int at = __builtin_ctz(empty) * DIM + static_cast<int>(threadIdx.x % (DIM / 8)) * 8;
-            if (threadIdx.x < DIM / 4)
-                *reinterpret_cast<s16x8*>((threadIdx.x < DIM / 8 ? qs : gs) + at) = s16x8{};
-        }
-        wait_for_lds();
-        meet();
-    };
     auto next = [&] {
         tile = tile < to ? tile + 1 : from;
         head += tile == from;
@@ -890,16 +893,13 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
             wait_for_all();
             meet();
             load(q1s, g1s, b1s);
-            clear(q0s, g0s, b0s[0]);
             turn(q0s, g0s, b0s[0]);
             const bool more = next();
             wait_for_all();
             meet();
             load(q0s, g0s, b0s);
-            if (more) {
-                clear(q1s, g1s, b1s[0]);
+            if (more)
                 turn(q1s, g1s, b1s[0]);
-            }
             if (!more || !next())
                 break;
         }
