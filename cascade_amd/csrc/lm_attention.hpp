@@ -674,6 +674,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
                 s = Type::mfma32(tiles_at.along(ks, 32 * t, d), q[d], s);
                 dp = Type::mfma32(tiles_at.along(vs, 32 * t, d), g[d], dp);
             }
+            read_ahead<DIM / 8, DIM / 8, 4, 1>();
             const int key = key0 + 32 * t + 4 * half, i = static_cast<int>(row);
             rest += score_gradients<BENT, true>(
                 a, s, dp, slope2, 0.f, grow, masked, [&](int) { return lse2; }, [&](int) { return delta; },
@@ -689,6 +690,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
                     o[e] = Type::mfma32(f, low, o[e]);
                 }
             }
+            read_ahead<DIM / 4, DIM / 4, 6, 1>();
         }
     };
 
