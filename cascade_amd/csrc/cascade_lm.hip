@@ -226,25 +226,24 @@ using WideLogits = Product<Type, 256, 256, 2, 4, false, false>;
 template <class Type>
 using NarrowLogits = Product<Type, 256, 64, 4, 1, false, false>;
 template <class Type>
-using WeightGradients = Product<Type, 256, 256, 2, 4, false, true>;
+using WeightGradients = Product<Type, 256, 256, 2, 4, true, true>;
 template <class Type>
-using WideHidden = Product<Type, 256, 256, 2, 4, true, true>;
+using WideHidden = Product<Type, 256, 256, 2, 4, false, true>;
 template <class Type>
-using NarrowHidden = Product<Type, 64, 256, 1, 4, true, true>;
+using NarrowHidden = Product<Type, 64, 256, 1, 4, false, true>;
 
 constexpr uint64_t NARROW_TOKENS = 512;
 constexpr uint64_t PIECE_BYTES = 256ull << 20; // of P
 constexpr uint64_t SHARE_BYTES = 64ull << 20;  // of d_hidden's shares beside the first
 
 struct EntropyPlan {
-    uint64_t padded_dim, padded_tokens, words, pieces, shares, share_words;
+    uint64_t padded_dim, words, pieces, shares, share_words;
     bool narrow;
     EntropyPlan(uint64_t tokens, uint64_t dim, uint64_t vocab)
     {
         padded_dim = up(dim, 8);
-        padded_tokens = up(tokens, 8);
         narrow = tokens <= NARROW_TOKENS;
-        const uint64_t fit = PIECE_BYTES / (512 * (padded_tokens ? padded_tokens : 8));
+        const uint64_t fit = PIECE_BYTES / (512 * (tokens ? tokens : 1));
         words = (fit ? fit : 1) * 256;
         if (words > up(vocab, 256))
             words = up(vocab, 256);
@@ -273,7 +272,7 @@ struct EntropyWork {
         weight = c.take<short>(copies ? vocab * plan.padded_dim : 0);
         if (backward) {
             kept = c.take<short>(tokens * plan.padded_dim);
-            p = c.take<short>(plan.words * plan.padded_tokens);
+            p = c.take<short>(tokens * plan.words);
             shares = c.take<float>(plan.shares * tokens * plan.padded_dim);
             scale = c.take<float>(2);
         } else {
@@ -343,8 +342,8 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
     typedef WeightGradients<Type> G;
     typedef WideHidden<Type> WH;
     typedef NarrowHidden<Type> NH;
-    const int64_t tokens = hidden.rows, vocab = weight.rows, d = static_cast<int64_t>(dim), pd = static_cast<int64_t>(plan.padded_dim),
-                  pt = static_cast<int64_t>(plan.padded_tokens);
+    const int64_t tokens = hidden.rows, vocab = weight.rows, d = static_cast<int64_t>(dim), pd = static_cast<int64_t>(plan.padded_dim);
+    const bool wide = d_weight && aligned(d_weight, 16) && d_weight_stride % 8 == 0;
     if (!Type::wide_range)
         loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, w.scale);
     const uint32_t dt = static_cast<uint32_t>(parts_of(dim, 256)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow ? 64 : 256));
@@ -352,16 +351,17 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
         const int64_t first = static_cast<int64_t>(piece * plan.words), words = vocab - first < static_cast<int64_t>(plan.words) ? vocab - first : plan.words;
         const Operand part{static_cast<const short*>(weight.data) + first * weight.stride, weight.stride, words};
         const uint32_t wt = static_cast<uint32_t>(parts_of(words, 256));
+        const int64_t ps = static_cast<int64_t>(up(words, 8)); // rows of P
         const Logits l{part, hidden, pd, wt, tt, target, first};
         if (plan.narrow)
-            logit_gradients_kernel<NL, Type><<<wt * tt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, pt);
+            logit_gradients_kernel<NL, Type><<<wt * tt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
         else
-            logit_gradients_kernel<WL, Type><<<wt * tt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, pt);
+            logit_gradients_kernel<WL, Type><<<wt * tt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
         if (d_weight)
-            weight_gradients_kernel<G, Type><<<wt * dt, G::THREADS, 0, s>>>({w.p, pt, words}, {w.kept, pd, d}, tokens, wt, dt, w.scale,
-                                                                            d_weight + first * d_weight_stride, d_weight_stride);
+            weight_gradients_kernel<G, Type><<<dt * wt, G::THREADS, 0, s>>>({w.kept, pd, d}, {w.p, ps, words}, tokens, dt, wt, w.scale,
+                                                                            d_weight + first * d_weight_stride, d_weight_stride, wide);
         if (d_hidden) {
-            const Operand p{w.p, pt, tokens}, across{part.data, part.stride, d};
+            const Operand p{w.p, ps, tokens}, across{part.data, part.stride, d};
             const uint32_t shares = static_cast<uint32_t>(plan.shares), groups = tt * dt * shares;
             if (plan.narrow)
                 hidden_gradients_kernel<NH><<<groups, NH::THREADS, 0, s>>>(p, across, words, plan.share_words, tt, dt, w.shares, pd, piece > 0);

@@ -4,8 +4,8 @@
 // of every token over the 128 (or 64) words of a wave, 8 bytes where the logits would have been 512; a second kernel joins
 // them. Vocabulary runs along a lane's registers, so that a token's maximum and sum are taken without leaving the lane but once.
 // Backward: the vocabulary in pieces, each piece's logits computed again and turned into
-//   P[v][n] = d_loss[n] (exp(logit - lse[n]) - (v == target[n])),
-// rounded to 16 bits as the operand of the two products that follow, d_weight = P H and d_hidden = P^T W. The rounding is the
+//   P[n][v] = d_loss[n] (exp(logit - lse[n]) - (v == target[n])),
+// rounded to 16 bits as the operand of the two products that follow, d_weight = P^T H and d_hidden = P W. The rounding is the
 // matrix unit's price, of the size of the gradients' own last rounding. P of a piece is all that is kept.
 // In half precision P is scaled by a power of two that brings the largest |d_loss| near 2^15, and the products are scaled back in
 // 32 bits: probabilities of 1e-9 would otherwise vanish.
@@ -159,69 +159,51 @@ __global__ __launch_bounds__(P::THREADS) void logit_gradients_kernel(Logits l, c
     typename P::Sums sums;
     const int64_t m0 = static_cast<int64_t>(mi) * P::BM, n0 = static_cast<int64_t>(ni) * P::BN;
     P::run(l.weight, l.hidden, m0, n0, 0, l.dim, a0, a1, b0, b1, sums);
-    const int lane = threadIdx.x % 64, half = lane / 32;
+    const int lane = threadIdx.x % 64;
     const int64_t tokens = l.hidden.rows, mw = m0 + P::wave_m();
-    const int64_t rows = l.weight.rows - mw;
-    const int left = static_cast<int>(rows < P::BM / P::WM ? rows : P::BM / P::WM) - 4 * half;
+    float factor[P::TN], shift[P::TN];
+    int word[P::TN]; // the target's row of the wave's part, if it is one
 #pragma unroll
     for (int j = 0; j < P::TN; ++j) {
-        const int64_t n = n0 + P::wave_n() + 32 * j + lane % 32;
-        const bool there = n < tokens;
-        const int64_t goal = there ? l.target[n] : -1;
+        const int64_t n = n0 + P::wave_n() + 32 * j + lane % 32, goal = n < tokens ? l.target[n] : -1;
         const bool counts = goal >= 0 && goal < vocab;
-        float factor = counts ? d_loss[n] : 0.f;
-        if (!Type::wide_range)
-            factor *= scale[0];
-        const float shift = counts ? lse[n] : 0.f;
-        const int64_t t = goal - (l.first_word + mw) - 4 * half;
-        const int word = t >= 0 && t < left ? static_cast<int>(t) : -1;
-        short* to = out + (mw + 4 * half) * stride + n;
-        if (n < stride) { // columns between the last token and the padded width hold zeros
-#pragma unroll
-            for (int i = 0; i < P::TM; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = 32 * i + 8 * (r / 4) + r % 4;
-                    const float p = __builtin_amdgcn_exp2f((sums[i][j][r] - shift) * LOG2E) - (word == row ? 1.f : 0.f);
-                    if (row < left) // tokens left out: exactly zero, whatever their logits are
-                        to[static_cast<int64_t>(row) * stride] = to16<Type>(counts ? p * factor : 0.f);
-                }
-        }
+        factor[j] = counts ? d_loss[n] * (Type::wide_range ? 1.f : scale[0]) : 0.f;
+        shift[j] = counts ? lse[n] : INFINITY; // tokens left out: zeros, whatever their logits are
+        const int64_t t = goal - (l.first_word + mw);
+        word[j] = counts && t >= 0 && t < P::BM ? static_cast<int>(t) : -1;
     }
+    meet(); // everybody has read the last slice
+    P::template store_turned<Type>(
+        sums, P::wave_region(a0, a1, b0, b1), m0, n0, l.weight.rows, tokens, out, stride, true,
+        [&](int j, int row, float x) {
+            const float p = __builtin_amdgcn_exp2f((x - shift[j]) * LOG2E) - (word[j] == row ? 1.f : 0.f);
+            return shift[j] == INFINITY ? 0.f : p * factor[j];
+        });
+    // k of the products to come runs along these rows, to a multiple of 8
+    const int64_t tail = l.weight.rows + threadIdx.x % 8;
+    if (mi == l.mt - 1 && tail < stride)
+        for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8)
+            out[n * stride + tail] = 0;
 }
 
-// d_weight rows of a piece: sum over tokens of P[v][n] h[n].
+// d_weight rows of a piece, turned: sum over tokens of h[n] P[n][v].
 template <class P, class Type>
-__global__ __launch_bounds__(P::THREADS) void weight_gradients_kernel(Operand p, Operand hidden, int64_t tokens, uint32_t mt, uint32_t nt, const float* scale,
-                                                                      short* out, int64_t stride)
+__global__ __launch_bounds__(P::THREADS) void weight_gradients_kernel(Operand hidden, Operand p, int64_t tokens, uint32_t mt, uint32_t nt, const float* scale,
+                                                                      short* out, int64_t stride, bool wide)
 {
     LM_TILE_BUFFERS(P);
     uint32_t mi, ni;
     tile_of(blockIdx.x, mt, nt, mi, ni);
     typename P::Sums sums;
     const int64_t m0 = static_cast<int64_t>(mi) * P::BM, n0 = static_cast<int64_t>(ni) * P::BN;
-    P::run(p, hidden, m0, n0, 0, tokens, a0, a1, b0, b1, sums);
-    const int lane = threadIdx.x % 64, half = lane / 32;
+    P::run(hidden, p, m0, n0, 0, tokens, a0, a1, b0, b1, sums);
     const float back = Type::wide_range ? 1.f : scale[1];
-    const int64_t mw = m0 + P::wave_m(), rows = p.rows - mw;
-    const int left = static_cast<int>(rows < P::BM / P::WM ? rows : P::BM / P::WM) - 4 * half;
-#pragma unroll
-    for (int j = 0; j < P::TN; ++j) {
-        const int64_t n = n0 + P::wave_n() + 32 * j + lane % 32;
-        short* to = out + (mw + 4 * half) * stride + n;
-        if (n < hidden.rows)
-#pragma unroll
-            for (int i = 0; i < P::TM; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = 32 * i + 8 * (r / 4) + r % 4;
-                    if (row < left)
-                        to[static_cast<int64_t>(row) * stride] = to16<Type>(sums[i][j][r] * back);
-                }
-    }
+    meet();
+    P::template store_turned<Type>(sums, P::wave_region(a0, a1, b0, b1), m0, n0, hidden.rows, p.rows, out, stride, wide,
+                                   [&](int, int, float x) { return x * back; });
 }
 
-// One share of d_hidden: the sum over words [k, k + share) of P[v][n] w[v], in 32 bits, added to what earlier pieces left.
+// One share of d_hidden: the sum over words [k, k + share) of P[n][v] w[v], in 32 bits, added to what earlier pieces left.
 template <class P>
 __global__ __launch_bounds__(P::THREADS) void hidden_gradients_kernel(Operand p, Operand weight, int64_t words, int64_t share, uint32_t mt, uint32_t nt,
                                                                       float* out, int64_t stride, bool add)

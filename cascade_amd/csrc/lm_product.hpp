@@ -217,6 +217,61 @@ struct Product {
         }
         wait_for_all(); // the last loads have written their zeros
     }
+
+    // LDS for a wave's part of C in 16 bits, from the buffers of the operands.
+    static __device__ short* wave_region(short* a0, short* a1, short* b0, short* b1)
+    {
+        constexpr int SIZE = (BM / WM) * (BN / WN), IN_A = BM * SLICE / SIZE, IN_B = BN * SLICE / SIZE;
+        static_assert(2 * IN_A + 2 * IN_B >= WAVES, "the parts fit the buffers");
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        return w < IN_A ? a0 + w * SIZE : w < 2 * IN_A ? a1 + (w - IN_A) * SIZE : w < 2 * IN_A + IN_B ? b0 + (w - 2 * IN_A) * SIZE : b1 + (w - 2 * IN_A - IN_B) * SIZE;
+    }
+
+    // out[n * stride + m] = round(value(j, m', x)) for x = C[m][n], where the lane's column is n0 + wave_n() + 32 j + lane % 32 and m' counts from the wave's
+    // first row; rows m < rows, columns n < columns. Four neighbouring rows are a lane's own, so the wave turns its part in LDS, 8 bytes in
+    // and 16 out a lane, and stores whole lines. `mine`: the wave_region, once all waves are done with what was there.
+    // wide: 16-byte stores are allowed (out, stride).
+    template <class Type16, class F>
+    static __device__ void store_turned(Sums& sums, short* mine, int64_t m0, int64_t n0, int64_t rows, int64_t columns, short* out, int64_t stride, bool wide,
+                                        F value)
+    {
+        constexpr int LINE = BM / WM, PIECES = LINE / 8, COLUMNS = BN / WN; // a line holds a column's rows; its pieces stand at places piece ^ column
+        static_assert((PIECES & (PIECES - 1)) == 0 && 64 % PIECES == 0, "whole lines");
+        const int lane = threadIdx.x % 64, half = lane / 32;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int column = 32 * j + lane % 32;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    s16x4 y;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        y[r] = to16<Type16>(value(j, 32 * i + 8 * g + 4 * half + r, sums[i][j][4 * g + r]));
+                    *reinterpret_cast<s16x4*>(mine + column * LINE + ((4 * i + g) ^ column % PIECES) * 8 + 4 * half) = y;
+                }
+        }
+        wait_for_lds();
+        const int64_t mw = m0 + wave_m(), nw = n0 + wave_n();
+        const int piece = lane % PIECES;
+        const int64_t m = mw + piece * 8;
+#pragma unroll
+        for (int c = 0; c < COLUMNS; c += 64 / PIECES) {
+            const int column = c + lane / PIECES;
+            const s16x8 y = read16(mine + column * LINE + (piece ^ column % PIECES) * 8);
+            if (nw + column >= columns || m >= rows)
+                continue;
+            short* to = out + (nw + column) * stride + m;
+            if (wide && m + 8 <= rows) {
+                *reinterpret_cast<s16x8*>(to) = y;
+            } else {
+                for (int r = 0; r < 8; ++r)
+                    if (m + r < rows)
+                        to[r] = y[r];
+            }
+        }
+    }
 };
 
 } // namespace lm
