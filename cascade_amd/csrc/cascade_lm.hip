@@ -224,7 +224,7 @@ void with_kind(const csa_lm_attention& a, F f)
 template <class Type>
 using WideLogits = Product<Type, 256, 256, 2, 4, false, false>;
 template <class Type>
-using NarrowLogits = Product<Type, 256, 64, 4, 1, false, false>;
+using NarrowLogits = Product<Type, 128, 64, 2, 2, false, false>;
 template <class Type>
 using WeightGradients = Product<Type, 256, 256, 2, 4, true, true>;
 template <class Type>
@@ -237,17 +237,20 @@ constexpr uint64_t PIECE_BYTES = 256ull << 20; // of P
 constexpr uint64_t SHARE_BYTES = 64ull << 20;  // of d_hidden's shares beside the first
 
 struct EntropyPlan {
-    uint64_t padded_dim, words, pieces, shares, share_words;
+    uint64_t padded_dim, words, piece_words, pieces, // words: of the largest piece
+        shares, share_words;
     bool narrow;
     EntropyPlan(uint64_t tokens, uint64_t dim, uint64_t vocab)
     {
         padded_dim = up(dim, 8);
         narrow = tokens <= NARROW_TOKENS;
         const uint64_t fit = PIECE_BYTES / (512 * (tokens ? tokens : 1));
-        words = (fit ? fit : 1) * 256;
-        if (words > up(vocab, 256))
-            words = up(vocab, 256);
-        pieces = parts_of(vocab, words);
+        const uint64_t tiles256 = parts_of(vocab, 256), per = fit && fit < tiles256 ? fit : fit ? tiles256 : 1;
+        pieces = tiles256 / per;
+        if (tiles256 % per * 2 >= per) // a rest of less than half a piece goes with the last one
+            ++pieces;
+        piece_words = per * 256;
+        words = pieces * per >= tiles256 ? piece_words : (tiles256 - (pieces - 1) * per) * 256;
         // d_hidden has few tiles where there are few tokens: its sum over the words of a piece is then shared out
         const uint64_t tiles = parts_of(tokens, narrow ? 64 : 256) * parts_of(padded_dim, 256);
         const uint64_t want = tiles ? (narrow ? 1024 : 512) / tiles : 1, room = SHARE_BYTES / (4 * (tokens * padded_dim ? tokens * padded_dim : 1)) + 1;
@@ -319,7 +322,7 @@ void entropy_forward(const EntropyPlan& plan, const EntropyWork& w, const Operan
 {
     typedef WideLogits<Type> W;
     typedef NarrowLogits<Type> N;
-    const uint32_t mt = static_cast<uint32_t>(parts_of(weight.rows, 256)), nt = static_cast<uint32_t>(parts_of(hidden.rows, plan.narrow ? 64 : 256));
+    const uint32_t mt = static_cast<uint32_t>(parts_of(weight.rows, plan.narrow ? N::BM : W::BM)), nt = static_cast<uint32_t>(parts_of(hidden.rows, plan.narrow ? 64 : 256));
     const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), mt, nt, target, 0};
     if (plan.narrow)
         logit_sums_kernel<N><<<mt * nt, N::THREADS, 0, s>>>(l, w.part, w.target_logit);
@@ -348,15 +351,16 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
         loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, w.scale);
     const uint32_t dt = static_cast<uint32_t>(parts_of(dim, 256)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow ? 64 : 256));
     for (uint64_t piece = 0; piece < plan.pieces; ++piece) {
-        const int64_t first = static_cast<int64_t>(piece * plan.words), words = vocab - first < static_cast<int64_t>(plan.words) ? vocab - first : plan.words;
+        const int64_t first = static_cast<int64_t>(piece * plan.piece_words), words = piece + 1 < plan.pieces ? static_cast<int64_t>(plan.piece_words) : vocab - first;
         const Operand part{static_cast<const short*>(weight.data) + first * weight.stride, weight.stride, words};
         const uint32_t wt = static_cast<uint32_t>(parts_of(words, 256));
         const int64_t ps = static_cast<int64_t>(up(words, 8)); // rows of P
-        const Logits l{part, hidden, pd, wt, tt, target, first};
+        const uint32_t lt = static_cast<uint32_t>(parts_of(words, plan.narrow ? NL::BM : WL::BM));
+        const Logits l{part, hidden, pd, lt, tt, target, first};
         if (plan.narrow)
-            logit_gradients_kernel<NL, Type><<<wt * tt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
+            logit_gradients_kernel<NL, Type><<<lt * tt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
         else
-            logit_gradients_kernel<WL, Type><<<wt * tt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
+            logit_gradients_kernel<WL, Type><<<lt * tt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
         if (d_weight)
             weight_gradients_kernel<G, Type><<<dt * wt, G::THREADS, 0, s>>>({w.kept, pd, d}, {w.p, ps, words}, tokens, dt, wt, w.scale,
                                                                             d_weight + first * d_weight_stride, d_weight_stride, wide);
