@@ -68,7 +68,7 @@ def load():
     lib.csa_lm_clip_workspace.restype = u64
     lib.csa_lm_clip_workspace.argtypes = [u32]
     lib.csa_lm_clip_dev.restype = i32
-    lib.csa_lm_clip_dev.argtypes = [C.POINTER(CsaLmValues), u32, f32, vp, vp, u64, vp]
+    lib.csa_lm_clip_dev.argtypes = [vp, u32, f32, vp, vp, u64, vp]
     lib.csa_lm_last_error.restype = C.c_char_p
     lib.csa_lm_last_error.argtypes = []
     _lib = lib

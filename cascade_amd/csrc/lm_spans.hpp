@@ -3,31 +3,43 @@
 //
 // 2 bytes in and 12 out a position: bound by memory. A running maximum of separator positions: up to 4096 tiles, each of a whole
 // number of 4096-token turns; the first kernel leaves every tile's last separator (skipped where there is one tile), the second looks back over
-// those of the tiles before its own, at most 16 loads a lane, and walks its tile with a scan of the workgroup a turn.
+// those of the tiles before its own, at most 16 loads a lane, and walks its tile with a scan of the workgroup a turn. Lanes hold four neighbouring
+// tokens of every 1024, so that a wave's stores are whole lines.
 #pragma once
 #include "lm_common.hpp"
 
 namespace lm {
 
-constexpr int SPAN_ITEMS = 16, SPAN_TURN = 256 * SPAN_ITEMS, SPAN_TILES = 4096;
+constexpr int SPAN_GROUPS = 4, SPAN_TURN = 256 * 4 * SPAN_GROUPS, SPAN_TILES = 4096; // a lane has four tokens of every 1024
 
-__device__ inline void load_tokens(const uint16_t* text, int64_t n, int64_t at, bool wide, uint16_t (&t)[SPAN_ITEMS])
+__device__ inline void load_tokens(const uint16_t* text, int64_t n, int64_t at, bool wide, uint16_t (&t)[4])
 {
-    if (wide && at + SPAN_ITEMS <= n) {
-        *reinterpret_cast<u32x4*>(t) = *reinterpret_cast<const u32x4*>(text + at);
-        *reinterpret_cast<u32x4*>(t + 8) = *reinterpret_cast<const u32x4*>(text + at + 8);
+    if (wide && at + 4 <= n) {
+        const uint64_t x = *reinterpret_cast<const uint64_t*>(text + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            t[i] = static_cast<uint16_t>(x >> 16 * i);
     } else {
-        for (int i = 0; i < SPAN_ITEMS; ++i)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
             t[i] = at + i < n ? text[at + i] : 0;
     }
 }
 
-__device__ inline int wave_max(int x)
+// The last separator among a lane's four tokens, -1 if there is none.
+__device__ inline int last_of(const uint16_t (&t)[4], int64_t at, int64_t n, uint16_t separator)
 {
-    for (int d = 32; d; d /= 2) {
-        const int y = __shfl_xor(x, d);
-        x = y > x ? y : x;
-    }
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        last = t[i] == separator && at + i < n ? static_cast<int>(at + i) : last;
+    return last;
+}
+
+__device__ inline int largest(int x)
+{
+    for (int d = 32; d; d /= 2)
+        x = max(x, __shfl_xor(x, d));
     return x;
 }
 
@@ -36,14 +48,16 @@ __global__ __launch_bounds__(256) void last_separators_kernel(const uint16_t* te
     __shared__ int tops[4];
     int top = -1;
     const int64_t begin = blockIdx.x * tile, end = begin + tile < n ? begin + tile : n;
-    for (int64_t at = begin + threadIdx.x * SPAN_ITEMS; at < end; at += SPAN_TURN) {
-        alignas(16) uint16_t t[SPAN_ITEMS];
-        load_tokens(text, n, at, wide, t);
-        for (int i = 0; i < SPAN_ITEMS; ++i)
-            if (t[i] == separator && at + i < n)
-                top = static_cast<int>(at + i);
+    for (int64_t first = begin; first < end; first += SPAN_TURN) {
+        uint16_t t[SPAN_GROUPS][4];
+#pragma unroll
+        for (int g = 0; g < SPAN_GROUPS; ++g)
+            load_tokens(text, n, first + g * 1024 + threadIdx.x * 4, wide, t[g]);
+#pragma unroll
+        for (int g = 0; g < SPAN_GROUPS; ++g)
+            top = max(top, last_of(t[g], first + g * 1024 + threadIdx.x * 4, n, separator));
     }
-    top = wave_max(top);
+    top = largest(top);
     if (threadIdx.x % 64 == 0)
         tops[threadIdx.x / 64] = top;
     __syncthreads();
@@ -54,66 +68,79 @@ __global__ __launch_bounds__(256) void last_separators_kernel(const uint16_t* te
 __global__ __launch_bounds__(256) void spans_kernel(const uint16_t* text, int64_t n, uint16_t separator, int64_t tile, bool wide, const int32_t* last, int32_t* lo,
                                                     int32_t* hi, int32_t* target)
 {
-    __shared__ int tops[2][4];
+    __shared__ int tops[2][SPAN_GROUPS][4];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     int before = -1; // the last separator in front of the turn
     for (uint32_t t = threadIdx.x; t < blockIdx.x; t += 256)
         before = max(before, last[t]);
-    before = wave_max(before);
+    before = largest(before);
     if (lane == 0)
-        tops[1][wave] = before;
+        tops[1][0][wave] = before;
     __syncthreads();
-    before = max(max(tops[1][0], tops[1][1]), max(tops[1][2], tops[1][3]));
+    before = max(max(tops[1][0][0], tops[1][0][1]), max(tops[1][0][2], tops[1][0][3]));
 
     const int64_t begin = blockIdx.x * tile, end = begin + tile < n ? begin + tile : n;
     int turn = 0;
     for (int64_t first = begin; first < end; first += SPAN_TURN, turn ^= 1) {
-        const int64_t at = first + threadIdx.x * SPAN_ITEMS;
-        alignas(16) uint16_t t[SPAN_ITEMS + 1];
-        uint16_t(&mine)[SPAN_ITEMS] = *reinterpret_cast<uint16_t(*)[SPAN_ITEMS]>(t);
-        load_tokens(text, n, at, wide, mine);
-        t[SPAN_ITEMS] = at + SPAN_ITEMS < n ? text[at + SPAN_ITEMS] : separator;
-        int top = -1;
-        for (int i = 0; i < SPAN_ITEMS; ++i)
-            if (t[i] == separator && at + i < n)
-                top = static_cast<int>(at + i);
-        for (int d = 1; d < 64; d *= 2) {
-            const int y = __shfl_up(top, d);
-            if (lane >= d)
-                top = max(top, y);
+        uint16_t t[SPAN_GROUPS][4];
+        uint16_t next[SPAN_GROUPS]; // the token behind a lane's four
+        int top[SPAN_GROUPS], own[SPAN_GROUPS];
+#pragma unroll
+        for (int g = 0; g < SPAN_GROUPS; ++g) {
+            const int64_t at = first + g * 1024 + threadIdx.x * 4;
+            load_tokens(text, n, at, wide, t[g]);
+            next[g] = at + 4 < n ? text[at + 4] : separator;
         }
-        __syncthreads(); // the turn before last has been read
-        if (lane == 63)
-            tops[turn][wave] = top;
-        __syncthreads();
-        int own = __shfl_up(top, 1);
-        own = lane ? max(own, before) : before;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave)
-                own = max(own, tops[turn][w]);
-            before = max(before, tops[turn][w]);
-        }
-        int32_t los[SPAN_ITEMS], his[SPAN_ITEMS], targets[SPAN_ITEMS];
-        for (int i = 0; i < SPAN_ITEMS; ++i) {
-            if (t[i] == separator)
-                own = static_cast<int>(at + i);
-            los[i] = max(own, 0);
-            his[i] = static_cast<int32_t>(at + i + 1);
-            targets[i] = at + i + 1 < n && t[i + 1] != separator ? t[i + 1] : -1;
-        }
-        if (wide && at + SPAN_ITEMS <= n) {
-            for (int i = 0; i < SPAN_ITEMS; i += 4) {
-                *reinterpret_cast<int4*>(lo + at + i) = *reinterpret_cast<int4*>(los + i);
-                *reinterpret_cast<int4*>(hi + at + i) = *reinterpret_cast<int4*>(his + i);
-                *reinterpret_cast<int4*>(target + at + i) = *reinterpret_cast<int4*>(targets + i);
+#pragma unroll
+        for (int g = 0; g < SPAN_GROUPS; ++g) {
+            top[g] = last_of(t[g], first + g * 1024 + threadIdx.x * 4, n, separator);
+            for (int d = 1; d < 64; d *= 2) {
+                const int y = __shfl_up(top[g], d);
+                top[g] = lane >= d ? max(top[g], y) : top[g];
             }
-        } else {
-            for (int i = 0; i < SPAN_ITEMS; ++i)
-                if (at + i < n) {
-                    lo[at + i] = los[i];
-                    hi[at + i] = his[i];
-                    target[at + i] = targets[i];
-                }
+        }
+        __syncthreads(); // what the turn before last left has been read
+        if (lane == 63)
+#pragma unroll
+            for (int g = 0; g < SPAN_GROUPS; ++g)
+                tops[turn][g][wave] = top[g];
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < SPAN_GROUPS; ++g) {
+            own[g] = __shfl_up(top[g], 1);
+            own[g] = lane ? max(own[g], before) : before;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int x = tops[turn][g][w];
+                own[g] = w < wave ? max(own[g], x) : own[g];
+                before = max(before, x);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < SPAN_GROUPS; ++g) {
+            const int64_t at = first + g * 1024 + threadIdx.x * 4;
+            int los[4], his[4], targets[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                own[g] = t[g][i] == separator ? static_cast<int>(at + i) : own[g];
+                const uint16_t follows = i < 3 ? t[g][i + 1] : next[g];
+                los[i] = max(own[g], 0);
+                his[i] = static_cast<int>(at + i + 1);
+                targets[i] = at + i + 1 < n && follows != separator ? follows : -1;
+            }
+            if (wide && at + 4 <= n) {
+                *reinterpret_cast<int4*>(lo + at) = make_int4(los[0], los[1], los[2], los[3]);
+                *reinterpret_cast<int4*>(hi + at) = make_int4(his[0], his[1], his[2], his[3]);
+                *reinterpret_cast<int4*>(target + at) = make_int4(targets[0], targets[1], targets[2], targets[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at + i < n) {
+                        lo[at + i] = los[i];
+                        hi[at + i] = his[i];
+                        target[at + i] = targets[i];
+                    }
+            }
         }
     }
 }

@@ -9,6 +9,7 @@
 All take torch tensors on the GPU, enqueue kernels on the current stream of the tensors' device and return without waiting
 (include/cascade_lm.h; there is no CPU form). Scratch memory comes from torch's allocator and belongs to the stream.
 """
+import array
 import ctypes as C
 import math
 
@@ -253,19 +254,19 @@ def clip_gradients(grads, max_norm, out=None):
     _check(max_norm >= 0, "max_norm is negative or no number")
     device = grads[0].get_device()
     _check(device >= 0, "the gradients have to lie on a GPU")
-    items = (native.CsaLmValues * len(grads))()
-    for item, g, o in zip(items, grads, out):
-        kind = _type(g.dtype)
-        _check(g.is_contiguous() and g.get_device() == device, "gradients: dense tensors on one GPU")
-        item.inp, item.n, item.type = g.data_ptr() or None, g.numel(), kind
-        if o is not g:
-            _check(o.is_contiguous() and o.shape == g.shape and o.dtype == g.dtype and o.get_device() == device, "out: tensors like the gradients, one by one")
-        item.out = o.data_ptr() or None
+    items = []  # csa_lm_values as four 64-bit words each
+    for g, o in zip(grads, out):
+        if not g.is_contiguous() or g.get_device() != device:
+            raise ValueError("gradients: dense tensors on one GPU")
+        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or not o.is_contiguous() or o.get_device() != device):
+            raise ValueError("out: tensors like the gradients, one by one")
+        items += (g.data_ptr(), o.data_ptr(), g.numel(), _type(g.dtype))
+    items = array.array("Q", items)
     lib = native.load()
     norm = grads[0].new_empty((), dtype=torch.float32)
     size = lib.csa_lm_clip_workspace(len(grads))
     scratch, work = _work(size, norm)
-    _enqueue(device, lib.csa_lm_clip_dev, items, len(grads), float(max_norm), norm.data_ptr(), work, size)
+    _enqueue(device, lib.csa_lm_clip_dev, items.buffer_info()[0], len(grads), float(max_norm), norm.data_ptr(), work, size)
     return norm
 
 
