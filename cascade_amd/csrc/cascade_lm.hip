@@ -100,7 +100,7 @@ int check_attention(const char* who, const csa_lm_attention* a)
             return rc;
     }
     const uint64_t groups = parts_of(a->tokens, ROWS_PER_GROUP) * a->q_heads;
-    if (groups > 0x7fffffffu)
+    if (groups > 0x7fffffffu || parts_of(a->tokens, BLOCK_ROWS) * a->q_heads > 0x7fffffffu)
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens of %u heads", who, (unsigned long long)a->tokens, a->q_heads);
     return CSA_OK;
 }
@@ -113,9 +113,10 @@ Attention attention(const csa_lm_attention& a)
             static_cast<int>(a.head_dim), a.scale, a.cap};
 }
 
-// Heads of q that share one of k and v are shared out over workgroups, each with sums of its own that are joined at the end, until there are
-// KV_GROUPS workgroups: a workgroup fills a compute unit, and those of a causal text differ in work by as much as their keys.
-constexpr uint64_t KV_GROUPS = 2048;
+// The rows that a tile of keys meets are shared out over workgroups, each with sums of its own that are joined at the end, until there are
+// KV_GROUPS workgroups: a workgroup takes half a compute unit, and those of a causal text differ in work by as much as their keys. A share has
+// KV_TURNS tiles of rows at least.
+constexpr uint64_t KV_GROUPS = 2048, KV_TURNS = 16;
 
 int head_width(uint64_t dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
@@ -134,7 +135,7 @@ struct AttentionWork {
     RowBlock* blocks;
     float* parts;
     uint32_t *row_order, *key_order; // null where there is none
-    uint32_t shares, share_heads;
+    uint32_t shares;
     uint64_t bytes;
     AttentionWork(void* base, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim, bool backward)
     {
@@ -146,9 +147,8 @@ struct AttentionWork {
         }
         key_order = c.take<uint32_t>(may_be_ordered(tokens, q_heads) ? ORDER_TILES : 0);
         const uint64_t tiles = parts_of(tokens, BLOCK_ROWS), group = q_heads / kv_heads, groups = parts_of(tokens, KEYS_PER_GROUP) * kv_heads;
-        const uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1;
-        share_heads = static_cast<uint32_t>(want < group ? group / want : 1);
-        shares = static_cast<uint32_t>(parts_of(group, share_heads));
+        const uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1, most = group * tiles / KV_TURNS;
+        shares = static_cast<uint32_t>(want < most ? want : most > 1 ? most : 1);
         parts = c.take<float>(shares > 1 ? 2 * shares * kv_heads * tokens * head_width(dim) : 0);
         norms = c.take<uint32_t>(2);
         bounds = c.take<int2>(tiles);
@@ -181,10 +181,10 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     attention_d_q_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
         at, order ? w.row_order : nullptr, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
     attention_d_kv_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
-        at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.share_heads, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
+        at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
         d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
     if (w.shares > 1)
-        join_heads_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.kv_heads, 2), 256, 0, s>>>(
+        join_parts_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.kv_heads, 2), 256, 0, s>>>(
             w.parts, w.shares, at.tokens, at.dim, DIM, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride, static_cast<short*>(d_v.data),
             d_v.token_stride, d_v.head_stride);
 }

@@ -11,7 +11,7 @@
 //   forward and d_q: a lane holds one row i; its keys run along the registers (scores transposed: K Q^T), so the softmax's maximum, sum,
 //                    mask and distance are a lane's own, with one exchange between the halves of the wave.
 //   d_k and d_v:     a lane holds one key and rows run along the registers; a workgroup owns its keys and walks the rows of all heads that share
-//                    them, so nothing is added by atomics and the results do not depend on the order of workgroups. The scores are
+//                    them, or a part of those that is joined with the others' in a fixed order, so nothing is added by atomics and the results do not depend on the order of workgroups. The scores are
 //                    computed twice for that, once here and once for d_q (seven products instead of five).
 // Tiles of keys or rows come straight from memory into LDS, one tile ahead. The 16-byte pieces of a tile's row stand at
 // places that keep both kinds of reads, sixteen rows' same piece and four rows' neighbouring pieces, in different banks.
@@ -771,7 +771,7 @@ constexpr int KEYS_PER_GROUP = 128;
 // d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
 template <class Type, int DIM, bool BENT>
 __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, const uint32_t* order, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
-                                                                const uint32_t* norms, uint32_t shares, uint32_t share_heads, float* parts, short* d_k,
+                                                                const uint32_t* norms, uint32_t shares, float* parts, short* d_k,
                                                                 int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
@@ -785,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
     place_of(blockIdx.x, units, gridDim.x / units, order, unit, which);
     if (!order)
         which = gridDim.x / units - 1 - which; // the first keys, which most rows of a causal text see, first
-    const uint32_t kv = unit / shares, head0 = kv * a.group + unit % shares * share_heads, heads = min(share_heads, kv * a.group + a.group - head0);
+    const uint32_t kv = unit / shares;
     const int first = static_cast<int>(which) * KEYS_PER_GROUP, last = min(first + KEYS_PER_GROUP, static_cast<int>(a.tokens)); // keys [first, last)
     const int wave_key = first + wave * 32, key = wave_key + lane % 32;
 
@@ -824,22 +824,29 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
     for (int e = 0; e < DIM / 32; ++e)
         ok[e] = ov[e] = f32x16{};
 
-    // Turns: the heads of this share, and of each the tiles from `from` to `to`. The next tile to load:
-    uint32_t load_head = head0;
-    int load_tile = from;
+    // Turns: the heads that share these keys, and of each the tiles from `from` to `to`; this workgroup's are `mine` of them, `begin` the first.
+    const int count = from <= to ? to - from + 1 : 0;
+    const int64_t turns = static_cast<int64_t>(count) * a.group, share = unit % shares;
+    const int begin = static_cast<int>(turns * share / shares), mine = static_cast<int>(turns * (share + 1) / shares) - begin;
+    const uint32_t first_head = kv * a.group + (count ? begin / count : 0);
+    const int first_tile = from + (count ? begin % count : 0);
+    int to_load = mine;
+    uint32_t load_head = first_head;
+    int load_tile = first_tile;
     auto load = [&](short* qs, short* gs, RowBlock* bs) {
-        const bool there = load_head < head0 + heads;
+        const bool there = to_load > 0;
         const int64_t row0 = there ? static_cast<int64_t>(load_tile) * RT : a.tokens; // past the last one: an empty window
-        const uint32_t head = there ? load_head : head0;
+        const uint32_t head = there ? load_head : first_head;
         ql.load(reinterpret_cast<const char*>(static_cast<const short*>(a.q.data) + head * a.q.head), row0, a.tokens, qs, wave);
         gl.load(reinterpret_cast<const char*>(static_cast<const short*>(d_out.data) + head * d_out.head), row0, a.tokens, gs, wave);
         if (wave == 0)
             load_to_lds(window(blocks + static_cast<int64_t>(head) * tiles + load_tile, there ? sizeof(RowBlock) : 0), bs, lane * 16);
+        --to_load;
+        load_head += load_tile == to;
         load_tile = load_tile < to ? load_tile + 1 : from;
-        load_head += load_tile == from;
     };
-    uint32_t head = head0;
-    int tile = from;
+    uint32_t head = first_head;
+    int tile = first_tile;
     auto turn = [&](short* qs, short* gs, const RowBlock& bs) {
         // which of the rows see any of the wave's 32 keys, and which do not see all of them
         const int lo = bs.lo[lane % 32], hi = bs.hi[lane % 32];
@@ -863,6 +870,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
             s = Type::mfma32(tiles_at.along(qs, 0, d), k[d], s);
             dp = Type::mfma32(tiles_at.along(gs, 0, d), tiles_at.along(vs, 32 * wave, d), dp);
         }
+        read_ahead<3 * DIM / 16, DIM / 8, 4, 2>();
         const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
         const int row = tile * RT + 4 * half;
         score_gradients<BENT, false>(
@@ -884,29 +892,28 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         read_ahead<DIM / 4, DIM / 8, 6, 2>();
     };
     auto next = [&] {
+        head += tile == to;
         tile = tile < to ? tile + 1 : from;
-        head += tile == from;
-        return head < head0 + heads;
     };
 
-    if (from <= to) {
+    if (mine > 0) {
         load(q0s, g0s, b0s);
-        for (;;) {
+        for (int n = 0; n < mine; n += 2) {
             wait_for_all();
             meet();
             load(q1s, g1s, b1s);
             turn(q0s, g0s, b0s[0]);
-            const bool more = next();
+            next();
             wait_for_all();
             meet();
             load(q0s, g0s, b0s);
-            if (more)
+            if (n + 1 < mine) {
                 turn(q1s, g1s, b1s[0]);
-            if (!more || !next())
-                break;
+                next();
+            }
         }
-        wait_for_all();
     }
+    wait_for_all();
     const uint64_t lost = __ballot(!all_finite(ok) || !all_finite(ov));
     const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
     for (uint32_t left = redo; left; left &= left - 1) {
@@ -914,32 +921,34 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         if (j >= a.tokens)
             continue;
         float kx = 0.f, ky = 0.f, vx = 0.f, vy = 0.f;
-        for (uint32_t h = head0; h < head0 + heads; ++h) {
+        uint32_t h = first_head;
+        int t = first_tile;
+        for (int n = 0; n < mine; ++n) {
             const float slope2 = a.slope ? a.slope[h] * LOG2E : 0.f;
-            for (int t = from; t <= to; ++t) {
-                const RowBlock& b = blocks[static_cast<int64_t>(h) * tiles + t];
-                const int r = lane % 32, i = t * RT + r;
-                const bool sees = lane < 32 && b.lo[r] <= j && j < b.hi[r];
-                float bent, p = 0.f, ds = 0.f;
-                if (sees) {
-                    const float z = one_score(a, dot_rows<Type>(row_of(a.q, h, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent);
-                    p = __builtin_amdgcn_exp2f(z - b.lse2[r]);
-                    ds = p * (dot_rows<Type>(row_of(d_out, h, i), row_of(a.v, kv, j), a.dim) - b.delta[r]) * bent * a.scale;
+            const RowBlock& b = blocks[static_cast<int64_t>(h) * tiles + t];
+            const int r = lane % 32, i = t * RT + r;
+            const bool sees = lane < 32 && b.lo[r] <= j && j < b.hi[r];
+            float bent, p = 0.f, ds = 0.f;
+            if (sees) {
+                const float z = one_score(a, dot_rows<Type>(row_of(a.q, h, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent);
+                p = __builtin_amdgcn_exp2f(z - b.lse2[r]);
+                ds = p * (dot_rows<Type>(row_of(d_out, h, i), row_of(a.v, kv, j), a.dim) - b.delta[r]) * bent * a.scale;
+            }
+            for (uint32_t rows = static_cast<uint32_t>(__ballot(sees)); rows; rows &= rows - 1) {
+                const int c = __builtin_ctz(rows);
+                const short *q = row_of(a.q, h, t * RT + c), *g = row_of(d_out, h, t * RT + c);
+                const float pc = lane_of(p, c), dc = lane_of(ds, c);
+                if (lane < a.dim) {
+                    kx += dc * to32<Type>(q[lane]);
+                    vx += pc * to32<Type>(g[lane]);
                 }
-                for (uint32_t rows = static_cast<uint32_t>(__ballot(sees)); rows; rows &= rows - 1) {
-                    const int c = __builtin_ctz(rows);
-                    const short *q = row_of(a.q, h, t * RT + c), *g = row_of(d_out, h, t * RT + c);
-                    const float pc = lane_of(p, c), dc = lane_of(ds, c);
-                    if (lane < a.dim) {
-                        kx += dc * to32<Type>(q[lane]);
-                        vx += pc * to32<Type>(g[lane]);
-                    }
-                    if (lane + 64 < a.dim) {
-                        ky += dc * to32<Type>(q[lane + 64]);
-                        vy += pc * to32<Type>(g[lane + 64]);
-                    }
+                if (lane + 64 < a.dim) {
+                    ky += dc * to32<Type>(q[lane + 64]);
+                    vy += pc * to32<Type>(g[lane + 64]);
                 }
             }
+            h += t == to;
+            t = t < to ? t + 1 : from;
         }
         for (int half64 = 0; half64 < 2; ++half64) {
             const int d = lane + 64 * half64;
@@ -1065,7 +1074,7 @@ __global__ __launch_bounds__(1024) void tile_order_kernel(Attention a, uint32_t*
 
 // d_k (blockIdx.z 0) and d_v (1) of a head from its shares, four values a thread.
 template <class Type>
-__global__ __launch_bounds__(256) void join_heads_kernel(const float* parts, uint32_t shares, int64_t tokens, int dim, int width, short* d_k, int64_t dk_token,
+__global__ __launch_bounds__(256) void join_parts_kernel(const float* parts, uint32_t shares, int64_t tokens, int dim, int width, short* d_k, int64_t dk_token,
                                                          int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
 {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
