@@ -118,7 +118,20 @@ Attention attention(const csa_lm_attention& a)
 // KV_TURNS tiles of rows at least, and where there are as many shares as heads, whole heads: workgroups next to each other then read the same rows
 // (12289 tokens, 16 heads of 2: 8 shares 2.91 ms, 11 shares 3.03 ms; 16384 tokens of documents, 16 heads of 4: 4 shares 1.05 ms, 3 shares 1.15 ms,
 // 2 shares 1.36 ms; 3001 tokens, 12 heads of 12: 8 shares 0.26 ms, none 0.34 ms).
-constexpr uint64_t KV_GROUPS = 2048, KV_TURNS = 16;
+constexpr uint64_t KV_GROUPS = 1024, KV_LONG = 512, KV_TURNS = 16;
+
+// The keys that a tile of rows sees are shared out in the same way where there are too few tiles for two workgroups a compute unit; a share has eight tiles of
+// keys at least if its rows see the whole text.
+constexpr uint64_t ROW_GROUPS = 768, ROW_KEYS = 8 * KEYS_PER_TILE;
+
+uint64_t shares_of_rows(uint64_t tokens, uint64_t q_heads)
+{
+    const uint64_t groups = parts_of(tokens, ROWS_PER_GROUP) * q_heads;
+    if (!groups || groups > 512)
+        return 1;
+    const uint64_t want = ROW_GROUPS / groups, most = tokens / ROW_KEYS;
+    return want < most ? want : most > 1 ? most : 1;
+}
 
 int head_width(uint64_t dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
@@ -137,12 +150,17 @@ struct AttentionWork {
     RowBlock* blocks;
     float* parts;
     uint32_t *row_order, *key_order; // null where there is none
-    uint32_t shares;
+    uint32_t shares, row_shares;
+    float* row_parts;
+    float2* row_stats;
     uint64_t bytes;
     AttentionWork(void* base, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim, bool backward)
     {
         Carver c{static_cast<char*>(base)};
         row_order = c.take<uint32_t>(may_be_ordered(tokens, q_heads) ? ORDER_TILES : 0);
+        row_shares = static_cast<uint32_t>(shares_of_rows(tokens, q_heads));
+        row_parts = c.take<float>(row_shares > 1 ? row_shares * q_heads * tokens * head_width(dim) : 0);
+        row_stats = c.take<float2>(row_shares > 1 ? row_shares * q_heads * tokens : 0);
         if (!backward) {
             bytes = c.used;
             return;
@@ -150,8 +168,12 @@ struct AttentionWork {
         key_order = c.take<uint32_t>(may_be_ordered(tokens, q_heads) ? ORDER_TILES : 0);
         const uint64_t tiles = parts_of(tokens, BLOCK_ROWS), group = q_heads / kv_heads, groups = parts_of(tokens, KEYS_PER_GROUP) * kv_heads;
         uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1;
-        want = want > group ? want / group * group : want;
-        const uint64_t most = group * tiles / KV_TURNS;
+        const uint64_t long_ones = parts_of(group * tiles, KV_LONG), most = group * tiles / KV_TURNS;
+        want = want > long_ones ? want : long_ones;
+        if (want > group)
+            want = want / group * group;
+        while (want < group && group % want)
+            ++want;
         shares = static_cast<uint32_t>(want < most ? want : most > 1 ? most : 1);
         parts = c.take<float>(shares > 1 ? 2 * shares * kv_heads * tokens * head_width(dim) : 0);
         norms = c.take<uint32_t>(2);
@@ -167,8 +189,12 @@ void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_hea
     const bool order = in_order(a);
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), w.row_order, nullptr);
-    attention_forward_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
-        attention(a), order ? w.row_order : nullptr, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
+    attention_forward_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
+        attention(a), order ? w.row_order : nullptr, w.row_shares, w.row_parts, w.row_stats, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
+    if (w.row_shares > 1)
+        join_rows_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
+            w.row_parts, w.row_stats, w.row_shares, static_cast<int64_t>(a.tokens), static_cast<int>(a.head_dim), DIM, static_cast<short*>(out.data),
+            out.token_stride, out.head_stride, lse);
 }
 
 template <class Type, int DIM, bool BENT>
@@ -182,8 +208,13 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(at, w.row_order, w.key_order);
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
-    attention_d_q_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads), 256, 0, s>>>(
-        at, order ? w.row_order : nullptr, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
+    float* rests = reinterpret_cast<float*>(w.row_stats);
+    attention_d_q_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
+        at, order ? w.row_order : nullptr, w.row_shares, w.row_parts, rests, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data),
+        d_q.token_stride, d_q.head_stride);
+    if (w.row_shares > 1)
+        join_d_q_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
+            w.row_parts, rests, w.row_shares, at.tokens, at.dim, DIM, w.blocks, tiles, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
     attention_d_kv_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
         at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
         d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);

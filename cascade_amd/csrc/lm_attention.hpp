@@ -256,6 +256,16 @@ __device__ inline float lane_of(float x, int lane) { return __builtin_bit_cast(f
 
 constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
 
+// The part [start, stop) of the keys [lo, hi) that one of `shares` workgroups walks, whole tiles but for the last.
+__device__ inline void share_of(int lo, int hi, uint32_t share, uint32_t shares, int& start, int& stop)
+{
+    const int64_t tiles = lo < hi ? (hi - lo + KEYS_PER_TILE - 1) / KEYS_PER_TILE : 0;
+    start = lo + static_cast<int>(tiles * share / shares) * KEYS_PER_TILE;
+    stop = min(hi, lo + static_cast<int>(tiles * (share + 1) / shares) * KEYS_PER_TILE);
+    if (!tiles)
+        start = stop = 0;
+}
+
 // BENT: there is a cap or a slope. Kernels without them are compiled without the code for them, which costs the others registers even where it
 // does not run.
 //
@@ -288,14 +298,16 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
 }
 
 template <class Type, int DIM, bool BENT>
-__global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, const uint32_t* order, short* out, int64_t out_token, int64_t out_head, float* lse)
+__global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float2* stats, short* out,
+                                                                   int64_t out_token, int64_t out_head, float* lse)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    uint32_t head, tile;
-    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, order, head, tile);
+    uint32_t unit, tile;
+    place_of(blockIdx.x, a.q_heads * shares, gridDim.x / (a.q_heads * shares), order, unit, tile);
+    const uint32_t head = unit / shares;
     const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
 
     // The keys that this workgroup's rows see, this wave's rows see, and all of this wave's rows see.
@@ -303,6 +315,8 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
     span_of(a, first + lane, lo, hi);
     span_of(a, first + 64 + lane, l2, h2);
     const int group_lo = __builtin_amdgcn_readfirstlane(wave_min(min(lo, l2))), group_hi = __builtin_amdgcn_readfirstlane(wave_most(max(hi, h2)));
+    int start, stop;
+    share_of(group_lo, group_hi, unit % shares, shares, start, stop);
     span_of(a, row, lo, hi);
     const int wave_lo = __builtin_amdgcn_readfirstlane(wave_min(lo)), wave_hi = __builtin_amdgcn_readfirstlane(wave_most(hi));
     const int all_lo = __builtin_amdgcn_readfirstlane(wave_most(lo)), all_hi = __builtin_amdgcn_readfirstlane(wave_min(hi));
@@ -385,26 +399,28 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
         read_ahead<DIM / 4, DIM / 8, 6, 2>();
     };
 
-    if (group_lo < group_hi) {
-        const int begin = group_lo;
-        kl.load(kb, begin, group_hi, k0s, wave);
-        vl.load(vb, begin, group_hi, v0s, wave);
-        for (int key0 = begin; key0 < group_hi; key0 += 2 * KT) {
+    if (start < stop) {
+        kl.load(kb, start, stop, k0s, wave);
+        vl.load(vb, start, stop, v0s, wave);
+        for (int key0 = start; key0 < stop; key0 += 2 * KT) {
             wait_for_all();
             meet();
-            kl.load(kb, key0 + KT, group_hi, k1s, wave);
-            vl.load(vb, key0 + KT, group_hi, v1s, wave);
+            kl.load(kb, key0 + KT, stop, k1s, wave);
+            vl.load(vb, key0 + KT, stop, v1s, wave);
             turn(k0s, v0s, key0);
             wait_for_all();
             meet();
-            kl.load(kb, key0 + 2 * KT, group_hi, k0s, wave);
-            vl.load(vb, key0 + 2 * KT, group_hi, v0s, wave);
-            turn(k1s, v1s, key0 + KT);
+            kl.load(kb, key0 + 2 * KT, stop, k0s, wave);
+            vl.load(vb, key0 + 2 * KT, stop, v0s, wave);
+            if (key0 + KT < stop)
+                turn(k1s, v1s, key0 + KT);
         }
         wait_for_all();
     }
     sum += other_half(sum);
-    const float share = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    // shares leave their sums as they are, for the kernel that joins them
+    const float share = shares > 1 ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    float* part = parts + (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens * DIM;
     const uint64_t lost = __ballot(!all_finite(o));
     const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
     for (uint32_t left = redo; left; left &= left - 1) {
@@ -412,14 +428,14 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
         const int64_t i = first + wave * 32 + r;
         if (i >= a.tokens)
             continue;
-        const int from = __builtin_amdgcn_readlane(lo, r), to = __builtin_amdgcn_readlane(hi, r);
-        const float high = lane_of(top, r), part = lane_of(share, r);
+        const int from = max(start, __builtin_amdgcn_readlane(lo, r)), to = min(stop, __builtin_amdgcn_readlane(hi, r));
+        const float high = lane_of(top, r), factor = lane_of(share, r);
         float x = 0.f, y = 0.f;
         for (int j0 = from; j0 < to; j0 += 64) {
             const int j = j0 + lane, count = min(64, to - j0);
             float bent, p = 0.f;
             if (j < to)
-                p = __builtin_amdgcn_exp2f(one_score(a, dot_rows<Type>(row_of(a.q, head, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent) - high) * part;
+                p = __builtin_amdgcn_exp2f(one_score(a, dot_rows<Type>(row_of(a.q, head, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent) - high) * factor;
             for (int c = 0; c < count; ++c) {
                 const short* v = row_of(a.v, kv, j0 + c);
                 const float pc = lane_of(p, c);
@@ -427,13 +443,26 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
                 y += lane + 64 < a.dim ? pc * to32<Type>(v[lane + 64]) : 0.f;
             }
         }
-        short* to_row = out + head * out_head + i * out_token;
-        if (lane < a.dim)
-            to_row[lane] = to16<Type>(x);
-        if (lane + 64 < a.dim)
-            to_row[lane + 64] = to16<Type>(y);
+        for (int upper = 0; upper < 2; ++upper) {
+            const int d = lane + 64 * upper;
+            if (d >= a.dim)
+                continue;
+            if (shares > 1)
+                part[i * DIM + d] = upper ? y : x;
+            else
+                out[head * out_head + i * out_token + d] = to16<Type>(upper ? y : x);
+        }
     }
-    if (row < a.tokens) {
+    if (row < a.tokens && shares > 1) {
+        if (!(redo >> lane % 32 & 1))
+#pragma unroll
+            for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4*>(part + row * DIM + 32 * e + 8 * g + 4 * half) = f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]};
+        if (half == 0)
+            stats[(static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row] = make_float2(top, sum);
+    } else if (row < a.tokens) {
         short* to = out + head * out_head + row * out_token;
 #pragma unroll
         for (int e = 0; e < DIM / 32; ++e)
@@ -453,7 +482,43 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
     }
 }
 
+// out and lse of a row from its shares, four values a thread: sums of exponentials of different maxima.
+template <class Type>
+__global__ __launch_bounds__(256) void join_rows_kernel(const float* parts, const float2* stats, uint32_t shares, int64_t tokens, int dim, int width, short* out,
+                                                        int64_t out_token, int64_t out_head, float* lse)
+{
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int quads = dim / 4;
+    if (at >= tokens * quads)
+        return;
+    const int64_t row = at / quads;
+    const int d = static_cast<int>(at % quads) * 4;
+    const uint32_t head = blockIdx.y, heads = gridDim.y;
+    float high = -3.0e38f;
+    for (uint32_t i = 0; i < shares; ++i)
+        high = fmaxf(high, stats[(static_cast<int64_t>(i) * heads + head) * tokens + row].x);
+    float sum = 0.f;
+    f32x4 x = {};
+    for (uint32_t i = 0; i < shares; ++i) {
+        const int64_t place = (static_cast<int64_t>(i) * heads + head) * tokens + row;
+        const float2 v = stats[place];
+        const float factor = __builtin_amdgcn_exp2f(v.x - high);
+        sum += v.y * factor;
+        x += *reinterpret_cast<const f32x4*>(parts + place * width + d) * factor;
+    }
+    const bool any = sum > 0.f || sum != sum;
+    const float share = any ? 1.f / sum : 0.f;
+    s16x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y[i] = to16<Type>(any ? x[i] * share : 0.f);
+    *reinterpret_cast<s16x4*>(out + head * out_head + row * out_token + d) = y;
+    if (d == 0)
+        lse[head * tokens + row] = any ? (high + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
+}
+
 // ---- backward ----
+
 
 // What the backward kernels read of 32 rows of a head: 32 values each of lse in base 2 (infinite for rows that see nothing: their
 // probabilities are zeros), D, lo and hi. The block of (head, tile) is 512 bytes, one load of half a wave.
@@ -620,20 +685,24 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
 }
 
 template <class Type, int DIM, bool BENT>
-__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, Heads d_out, RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
+__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float* rests, Heads d_out,
+                                                               RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
                                                                short* d_q, int64_t out_token, int64_t out_head)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    uint32_t head, tile;
-    place_of(blockIdx.x, a.q_heads, gridDim.x / a.q_heads, order, head, tile);
+    uint32_t unit, tile;
+    place_of(blockIdx.x, a.q_heads * shares, gridDim.x / (a.q_heads * shares), order, unit, tile);
+    const uint32_t head = unit / shares;
     const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
     int lo, hi, l2, h2;
     span_of(a, first + lane, lo, hi);
     span_of(a, first + 64 + lane, l2, h2);
     const int group_lo = __builtin_amdgcn_readfirstlane(wave_min(min(lo, l2))), group_hi = __builtin_amdgcn_readfirstlane(wave_most(max(hi, h2)));
+    int start, stop;
+    share_of(group_lo, group_hi, unit % shares, shares, start, stop);
     span_of(a, row, lo, hi);
     const int wave_lo = __builtin_amdgcn_readfirstlane(wave_min(lo)), wave_hi = __builtin_amdgcn_readfirstlane(wave_most(hi));
     const int all_lo = __builtin_amdgcn_readfirstlane(wave_most(lo)), all_hi = __builtin_amdgcn_readfirstlane(wave_min(hi));
@@ -694,26 +763,29 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
         }
     };
 
-    if (group_lo < group_hi) {
-        const int begin = group_lo;
-        kl.load(kb, begin, group_hi, k0s, wave);
-        vl.load(vb, begin, group_hi, v0s, wave);
-        for (int key0 = begin; key0 < group_hi; key0 += 2 * KT) {
+    if (start < stop) {
+        kl.load(kb, start, stop, k0s, wave);
+        vl.load(vb, start, stop, v0s, wave);
+        for (int key0 = start; key0 < stop; key0 += 2 * KT) {
             wait_for_all();
             meet();
-            kl.load(kb, key0 + KT, group_hi, k1s, wave);
-            vl.load(vb, key0 + KT, group_hi, v1s, wave);
+            kl.load(kb, key0 + KT, stop, k1s, wave);
+            vl.load(vb, key0 + KT, stop, v1s, wave);
             turn(k0s, v0s, key0);
             wait_for_all();
             meet();
-            kl.load(kb, key0 + 2 * KT, group_hi, k0s, wave);
-            vl.load(vb, key0 + 2 * KT, group_hi, v0s, wave);
-            turn(k1s, v1s, key0 + KT);
+            kl.load(kb, key0 + 2 * KT, stop, k0s, wave);
+            vl.load(vb, key0 + 2 * KT, stop, v0s, wave);
+            if (key0 + KT < stop)
+                turn(k1s, v1s, key0 + KT);
         }
         wait_for_all();
     }
     rest += other_half(rest);
-    const float exact = delta + rest / grow;
+    // A share knows only its own part of what D is off by: its d_q is the one of the rounded D, and the kernel that joins them corrects D for the
+    // kernel of d_k alone.
+    const float exact = shares > 1 ? delta : delta + rest / grow;
+    float* part = parts + (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens * DIM;
     const uint64_t lost = __ballot(!all_finite(o));
     const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
     for (uint32_t left = redo; left; left &= left - 1) {
@@ -721,7 +793,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
         const int64_t i = first + wave * 32 + r;
         if (i >= a.tokens)
             continue;
-        const int from = __builtin_amdgcn_readlane(lo, r), to = __builtin_amdgcn_readlane(hi, r);
+        const int from = max(start, __builtin_amdgcn_readlane(lo, r)), to = min(stop, __builtin_amdgcn_readlane(hi, r));
         const float base = lane_of(lse2, r), mean = lane_of(exact, r);
         float x = 0.f, y = 0.f;
         for (int j0 = from; j0 < to; j0 += 64) {
@@ -738,13 +810,27 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
                 y += lane + 64 < a.dim ? dc * to32<Type>(k[lane + 64]) : 0.f;
             }
         }
-        short* to_row = d_q + head * out_head + i * out_token;
-        if (lane < a.dim)
-            to_row[lane] = to16<Type>(x);
-        if (lane + 64 < a.dim)
-            to_row[lane + 64] = to16<Type>(y);
+        for (int upper = 0; upper < 2; ++upper) {
+            const int d = lane + 64 * upper;
+            if (d >= a.dim)
+                continue;
+            if (shares > 1)
+                part[i * DIM + d] = upper ? y : x;
+            else
+                d_q[head * out_head + i * out_token + d] = to16<Type>(upper ? y : x);
+        }
     }
-    if (row < a.tokens) {
+    if (row < a.tokens && shares > 1) {
+        if (!(redo >> lane % 32 & 1))
+#pragma unroll
+            for (int e = 0; e < DIM / 32; ++e)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4*>(part + row * DIM + 32 * e + 8 * g + 4 * half) =
+                        f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]} * (a.scale / grow);
+        if (half == 0)
+            rests[(static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row] = rest / grow;
+    } else if (row < a.tokens) {
         if (half == 0)
             blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = exact;
         const float back = a.scale / grow;
@@ -763,6 +849,34 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
                 }
             }
     }
+}
+
+// d_q of a row from its shares, four values a thread, and D of the row corrected.
+template <class Type>
+__global__ __launch_bounds__(256) void join_d_q_kernel(const float* parts, const float* rests, uint32_t shares, int64_t tokens, int dim, int width, RowBlock* blocks,
+                                                       uint32_t blocks_per_head, short* d_q, int64_t out_token, int64_t out_head)
+{
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int quads = dim / 4;
+    if (at >= tokens * quads)
+        return;
+    const int64_t row = at / quads;
+    const int d = static_cast<int>(at % quads) * 4;
+    const uint32_t head = blockIdx.y, heads = gridDim.y;
+    f32x4 x = {};
+    float rest = 0.f;
+    for (uint32_t i = 0; i < shares; ++i) {
+        const int64_t place = (static_cast<int64_t>(i) * heads + head) * tokens + row;
+        x += *reinterpret_cast<const f32x4*>(parts + place * width + d);
+        rest += rests[place];
+    }
+    s16x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y[i] = to16<Type>(x[i]);
+    *reinterpret_cast<s16x4*>(d_q + head * out_head + row * out_token + d) = y;
+    if (d == 0)
+        blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] += rest;
 }
 
 constexpr int KEYS_PER_GROUP = 128;

@@ -221,6 +221,12 @@ def test_attention_of_a_long_text():
     check_attention(2111, 32, 2, 16, torch.float16, "documents", seed=10)  # shared heads in that order, too
 
 
+@pytest.mark.parametrize("mask", ["causal", "all", "window", "random", "none"])
+def test_attention_of_few_heads_shares_out_keys(mask):
+    check_attention(1301, 2, 1, 64, torch.bfloat16, mask, seed=21)
+    check_attention(1100, 1, 1, 96, torch.float16, mask, cap=5.0, slopes=True, seed=22)
+
+
 def test_attention_of_large_scores():
     check_attention(300, 2, 2, 64, torch.bfloat16, "causal", scale=4.0, seed=8)  # a softmax of one or two keys a row
 
@@ -239,13 +245,13 @@ def test_half_precision_keeps_small_gradients():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 1, 128), (3, 3, 88)])
-def test_what_a_row_may_not_see_may_hold_anything(dtype, heads, kv_heads, dim):
+@pytest.mark.parametrize("heads,kv_heads,dim,n", [(2, 2, 64, 500), (4, 1, 128, 500), (3, 3, 88, 500), (2, 1, 64, 1700), (2, 2, 80, 1700)])
+def test_what_a_row_may_not_see_may_hold_anything(dtype, heads, kv_heads, dim, n):
     """Infinities and NaN in padding, and in one document of three, change nothing elsewhere, forwards and backwards."""
     g = gen(13)
-    n, text = 500, 470  # padding behind 470 positions
+    text = n - 30  # padding behind it
     at = torch.arange(n, device="cuda")
-    ends = torch.tensor([0, 150, 301, text], device="cuda")
+    ends = torch.tensor([0, n - 350, n - 199, text], device="cuda")
     lo = ends[torch.searchsorted(ends, at, right=True) - 1].int()
     hi = (at + 1).int()
     lo[text:], hi[text:] = 0, 0
@@ -257,7 +263,7 @@ def test_what_a_row_may_not_see_may_hold_anything(dtype, heads, kv_heads, dim):
         return out, lse.T, *cascade_amd.span_attention_backward(d_out, q, k, v, out, lse, lo, hi, **how)
     for how in ({}, {"cap": 10.0, "slopes": torch.linspace(0.01, 0.1, heads, device="cuda")}):
         clean = once(q, k, v, d_out, **how)
-        for where in (slice(text, n), slice(150, 301)):
+        for where in (slice(text, n), slice(n - 350, n - 199)):
             spoilt = [x.clone() for x in (q, k, v, d_out)]
             for i, x in enumerate(spoilt):
                 x[where][i % 2::2] = math.nan
