@@ -120,16 +120,17 @@ Attention attention(const csa_lm_attention& a)
 // 2 shares 1.36 ms; 3001 tokens, 12 heads of 12: 8 shares 0.26 ms, none 0.34 ms).
 constexpr uint64_t KV_GROUPS = 1024, KV_LONG = 512, KV_TURNS = 16;
 
-// The keys that a tile of rows sees are shared out in the same way where there are too few tiles for two workgroups a compute unit; a share has eight tiles of
-// keys at least if its rows see the whole text.
-constexpr uint64_t ROW_GROUPS = 768, ROW_KEYS = 8 * KEYS_PER_TILE;
+// The keys that a tile of rows sees are shared out in the same way where there are too few tiles for two workgroups a compute unit; a share has five tiles of
+// keys at least if its rows see the whole text (4000 tokens of 4 heads trained 186 -> 113 us, 3001 of 12 heads 264 -> 215, 1000 of 8 heads 98 -> 81;
+// a share of four tiles and 768 workgroups: 2000 tokens of documents of 8 heads 136 where these take 120).
+constexpr uint64_t ROW_GROUPS = 512, ROW_KEYS = 5 * KEYS_PER_TILE;
 
 uint64_t shares_of_rows(uint64_t tokens, uint64_t q_heads)
 {
     const uint64_t groups = parts_of(tokens, ROWS_PER_GROUP) * q_heads;
-    if (!groups || groups > 512)
+    if (!groups || groups >= ROW_GROUPS)
         return 1;
-    const uint64_t want = ROW_GROUPS / groups, most = tokens / ROW_KEYS;
+    const uint64_t want = parts_of(ROW_GROUPS, groups), most = tokens / ROW_KEYS;
     return want < most ? want : most > 1 ? most : 1;
 }
 
