@@ -256,44 +256,57 @@ void with_kind(const csa_lm_attention& a, F f)
 
 // ---- cross entropy ----
 
-// Vocabulary by tokens. Up to 512 tokens the tiles of 256 tokens would leave compute units without work.
+// Tiles of 256 x 256 use the matrix units best, one workgroup a compute unit. Where fewer than half of the places that they would take in whole
+// rounds over the compute units hold words and tokens, smaller ones take less time (1024 values a row, 50257 words, forward: 200 tokens, 60 % of the
+// places, 36 us and 44 in small tiles; 300 tokens, 45 %, 64 us and 49).
 template <class Type>
 using WideLogits = Product<Type, 256, 256, 2, 4, false, false>;
 template <class Type>
 using NarrowLogits = Product<Type, 128, 64, 2, 2, false, false>;
 template <class Type>
-using WeightGradients = Product<Type, 256, 256, 2, 4, true, true>;
+using WideWeights = Product<Type, 256, 256, 2, 4, true, true>;
+template <class Type>
+using NarrowWeights = Product<Type, 128, 64, 2, 2, true, true>;
 template <class Type>
 using WideHidden = Product<Type, 256, 256, 2, 4, false, true>;
 template <class Type>
 using NarrowHidden = Product<Type, 64, 256, 1, 4, false, true>;
 
-constexpr uint64_t NARROW_TOKENS = 512;
+constexpr uint64_t UNITS = 256;               // compute units
 constexpr uint64_t PIECE_BYTES = 256ull << 20; // of P
-constexpr uint64_t SHARE_BYTES = 64ull << 20;  // of d_hidden's shares beside the first
+constexpr uint64_t SHARE_BYTES = 128ull << 20; // of d_hidden's shares beside the first
 
 struct EntropyPlan {
-    uint64_t padded_dim, words, piece_words, pieces, // words: of the largest piece
-        shares, share_words;
-    bool narrow;
+    uint64_t padded_dim, words, piece_words, pieces; // words: of the largest piece
+    uint64_t shares, share_words;
+    bool narrow_logits, narrow_hidden;
     EntropyPlan(uint64_t tokens, uint64_t dim, uint64_t vocab)
     {
         padded_dim = up(dim, 8);
-        narrow = tokens <= NARROW_TOKENS;
-        const uint64_t fit = PIECE_BYTES / (512 * (tokens ? tokens : 1));
-        const uint64_t tiles256 = parts_of(vocab, 256), per = fit && fit < tiles256 ? fit : fit ? tiles256 : 1;
+        const uint64_t tiles256 = parts_of(vocab, 256);
+        narrow_logits = tokens * vocab * 2 < up(tiles256 * parts_of(tokens, 256), UNITS) * 65536;
+        const uint64_t fit = PIECE_BYTES / (512 * (tokens ? tokens : 1)), per = fit && fit < tiles256 ? fit : fit ? tiles256 : 1;
         pieces = tiles256 / per;
         if (tiles256 % per * 2 >= per) // a rest of less than half a piece goes with the last one
             ++pieces;
         piece_words = per * 256;
         words = pieces * per >= tiles256 ? piece_words : (tiles256 - (pieces - 1) * per) * 256;
-        // d_hidden has few tiles where there are few tokens: its sum over the words of a piece is then shared out
-        const uint64_t tiles = parts_of(tokens, narrow ? 64 : 256) * parts_of(padded_dim, 256);
-        const uint64_t want = tiles ? (narrow ? 1024 : 512) / tiles : 1, room = SHARE_BYTES / (4 * (tokens * padded_dim ? tokens * padded_dim : 1)) + 1;
-        const uint64_t most = parts_of(words, 4 * SLICE);
-        shares = want < room ? want : room;
-        shares = shares < most ? shares : most;
-        shares = shares ? shares : 1;
+
+        // d_hidden has few tiles where there are few tokens: its sum over the words of a piece is then shared out, so that workgroups fill the
+        // compute units (two small ones fit one) in whole rounds as well as shares can.
+        narrow_hidden = tokens <= 128;
+        const uint64_t tiles = parts_of(tokens, narrow_hidden ? 64 : 256) * parts_of(padded_dim, 256), slots = narrow_hidden ? 2 * UNITS : UNITS;
+        const uint64_t room = SHARE_BYTES / (4 * (tokens * padded_dim ? tokens * padded_dim : 1)) + 1, longest = parts_of(words, 4 * SLICE);
+        const uint64_t most = room < longest ? room : longest;
+        shares = 1;
+        double best = 0;
+        for (uint64_t n = 1; n <= most && tiles && n * tiles <= 2 * slots; ++n) {
+            const double used = static_cast<double>(n * tiles) / up(n * tiles, slots);
+            if (used > best + 0.05) {
+                best = used;
+                shares = n;
+            }
+        }
         share_words = up(parts_of(words, shares), 2 * SLICE);
         shares = parts_of(words, share_words);
     }
@@ -358,15 +371,15 @@ void entropy_forward(const EntropyPlan& plan, const EntropyWork& w, const Operan
 {
     typedef WideLogits<Type> W;
     typedef NarrowLogits<Type> N;
-    const uint32_t mt = static_cast<uint32_t>(parts_of(weight.rows, plan.narrow ? N::BM : W::BM)), nt = static_cast<uint32_t>(parts_of(hidden.rows, plan.narrow ? 64 : 256));
+    const uint32_t mt = static_cast<uint32_t>(parts_of(weight.rows, plan.narrow_logits ? N::BM : W::BM)), nt = static_cast<uint32_t>(parts_of(hidden.rows, plan.narrow_logits ? N::BN : W::BN));
     const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), mt, nt, target, 0};
-    if (plan.narrow)
+    if (plan.narrow_logits)
         logit_sums_kernel<N><<<mt * nt, N::THREADS, 0, s>>>(l, w.part, w.target_logit);
     else
         logit_sums_kernel<W><<<mt * nt, W::THREADS, 0, s>>>(l, w.part, w.target_logit);
     // few tokens: more runs for each, the sums would otherwise be one lane's work after the other
-    const int64_t parts = mt * static_cast<int64_t>(plan.narrow ? N::WM : W::WM);
-    if (plan.narrow)
+    const int64_t parts = mt * static_cast<int64_t>(plan.narrow_logits ? N::WM : W::WM);
+    if (hidden.rows <= 512)
         join_sums_kernel<4><<<static_cast<uint32_t>(parts_of(hidden.rows, 4)), 256, 0, s>>>(w.part, parts, w.target_logit, target, hidden.rows, weight.rows, loss, lse);
     else
         join_sums_kernel<16><<<static_cast<uint32_t>(parts_of(hidden.rows, 16)), 256, 0, s>>>(w.part, parts, w.target_logit, target, hidden.rows, weight.rows, loss, lse);
@@ -378,40 +391,53 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
 {
     typedef WideLogits<Type> WL;
     typedef NarrowLogits<Type> NL;
-    typedef WeightGradients<Type> G;
+    typedef WideWeights<Type> WW;
+    typedef NarrowWeights<Type> NW;
     typedef WideHidden<Type> WH;
     typedef NarrowHidden<Type> NH;
     const int64_t tokens = hidden.rows, vocab = weight.rows, d = static_cast<int64_t>(dim), pd = static_cast<int64_t>(plan.padded_dim);
     const bool wide = d_weight && aligned(d_weight, 16) && d_weight_stride % 8 == 0;
     if (!Type::wide_range)
         loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, w.scale);
-    const uint32_t dt = static_cast<uint32_t>(parts_of(dim, 256)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow ? 64 : 256));
+    const uint32_t dt = static_cast<uint32_t>(parts_of(dim, WH::BN)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow_hidden ? NH::BM : WH::BM));
     for (uint64_t piece = 0; piece < plan.pieces; ++piece) {
         const int64_t first = static_cast<int64_t>(piece * plan.piece_words), words = piece + 1 < plan.pieces ? static_cast<int64_t>(plan.piece_words) : vocab - first;
         const Operand part{static_cast<const short*>(weight.data) + first * weight.stride, weight.stride, words};
-        const uint32_t wt = static_cast<uint32_t>(parts_of(words, 256));
         const int64_t ps = static_cast<int64_t>(up(words, 8)); // rows of P
-        const uint32_t lt = static_cast<uint32_t>(parts_of(words, plan.narrow ? NL::BM : WL::BM));
-        const Logits l{part, hidden, pd, lt, tt, target, first};
-        if (plan.narrow)
-            logit_gradients_kernel<NL, Type><<<lt * tt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
+        const uint32_t lt = static_cast<uint32_t>(parts_of(words, plan.narrow_logits ? NL::BM : WL::BM)), nt = static_cast<uint32_t>(parts_of(tokens, plan.narrow_logits ? NL::BN : WL::BN));
+        const Logits l{part, hidden, pd, lt, nt, target, first};
+        if (plan.narrow_logits)
+            logit_gradients_kernel<NL, Type><<<lt * nt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
         else
-            logit_gradients_kernel<WL, Type><<<lt * tt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
-        if (d_weight)
-            weight_gradients_kernel<G, Type><<<dt * wt, G::THREADS, 0, s>>>({w.kept, pd, d}, {w.p, ps, words}, tokens, dt, wt, w.scale,
-                                                                            d_weight + first * d_weight_stride, d_weight_stride, wide);
+            logit_gradients_kernel<WL, Type><<<lt * nt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
+        if (d_weight) {
+            const Operand p{w.p, ps, words}, kept{w.kept, pd, d};
+            short* to = d_weight + first * d_weight_stride;
+            // small tiles where large ones would leave half of the compute units without work
+            const uint32_t dw = static_cast<uint32_t>(parts_of(dim, WW::BM)), ww = static_cast<uint32_t>(parts_of(words, WW::BN));
+            const uint32_t dn = static_cast<uint32_t>(parts_of(dim, NW::BM)), wn = static_cast<uint32_t>(parts_of(words, NW::BN));
+            if (static_cast<uint64_t>(dw) * ww * 2 > UNITS)
+                weight_gradients_kernel<WW, Type><<<dw * ww, WW::THREADS, 0, s>>>(kept, p, tokens, dw, ww, w.scale, to, d_weight_stride, wide);
+            else
+                weight_gradients_kernel<NW, Type><<<dn * wn, NW::THREADS, 0, s>>>(kept, p, tokens, dn, wn, w.scale, to, d_weight_stride, wide);
+        }
         if (d_hidden) {
             const Operand p{w.p, ps, tokens}, across{part.data, part.stride, d};
             const uint32_t shares = static_cast<uint32_t>(plan.shares), groups = tt * dt * shares;
-            if (plan.narrow)
+            if (plan.narrow_hidden)
                 hidden_gradients_kernel<NH><<<groups, NH::THREADS, 0, s>>>(p, across, words, plan.share_words, tt, dt, w.shares, pd, piece > 0);
             else
                 hidden_gradients_kernel<WH><<<groups, WH::THREADS, 0, s>>>(p, across, words, plan.share_words, tt, dt, w.shares, pd, piece > 0);
         }
     }
-    if (d_hidden)
-        join_shares_kernel<Type><<<static_cast<uint32_t>(parts_of(tokens * pd / 4, 256)), 256, 0, s>>>(w.shares, static_cast<uint32_t>(plan.shares), tokens, d, pd, w.scale,
-                                                                                                      d_hidden, d_hidden_stride);
+    if (d_hidden) {
+        const uint64_t quads = static_cast<uint64_t>(tokens * pd / 4);
+        const uint32_t shares = static_cast<uint32_t>(plan.shares);
+        if (shares > 16) // many shares of few values: sixteen lanes add up those of four
+            join_shares_kernel<Type, 16><<<static_cast<uint32_t>(parts_of(quads, 16)), 256, 0, s>>>(w.shares, shares, tokens, d, pd, w.scale, d_hidden, d_hidden_stride);
+        else
+            join_shares_kernel<Type, 1><<<static_cast<uint32_t>(parts_of(quads, 256)), 256, 0, s>>>(w.shares, shares, tokens, d, pd, w.scale, d_hidden, d_hidden_stride);
+    }
 }
 
 } // namespace

@@ -237,18 +237,31 @@ __global__ __launch_bounds__(P::THREADS) void hidden_gradients_kernel(Operand p,
     }
 }
 
-// d_hidden from its shares.
-template <class Type>
+// d_hidden from its shares: LANES lanes for four values, each with every LANES-th share.
+template <class Type, int LANES>
 __global__ __launch_bounds__(256) void join_shares_kernel(const float* shares, uint32_t count, int64_t tokens, int64_t dim, int64_t stride, const float* scale,
                                                           short* out, int64_t out_stride)
 {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, quads = stride / 4;
-    if (at >= tokens * quads)
-        return;
-    const int64_t n = at / quads, d = at % quads * 4;
+    constexpr int HERE = 256 / LANES; // fours of values a workgroup: neighbouring lanes hold neighbouring ones
+    __shared__ f32x4 got[LANES][HERE];
+    const int x = threadIdx.x % HERE, y = threadIdx.x / HERE;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * HERE + x, quads = stride / 4;
+    const bool there = at < tokens * quads;
+    const int64_t n = there ? at / quads : 0, d = there ? at % quads * 4 : 0;
     f32x4 sum = {};
-    for (uint32_t c = 0; c < count; ++c)
-        sum += *reinterpret_cast<const f32x4*>(shares + (c * tokens + n) * stride + d);
+    if (there)
+#pragma unroll 4
+        for (uint32_t c = y; c < count; c += LANES)
+            sum += *reinterpret_cast<const f32x4*>(shares + (c * tokens + n) * stride + d);
+    if (LANES > 1) {
+        got[y][x] = sum;
+        __syncthreads();
+        if (y == 0)
+            for (int k = 1; k < LANES; ++k)
+                sum += got[k][x];
+    }
+    if (!there || y)
+        return;
     const float back = Type::wide_range ? 1.f : scale[1];
     for (int i = 0; i < 4; ++i)
         if (d + i < dim)
