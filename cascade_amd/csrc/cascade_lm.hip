@@ -397,8 +397,7 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
     typedef NarrowHidden<Type> NH;
     const int64_t tokens = hidden.rows, vocab = weight.rows, d = static_cast<int64_t>(dim), pd = static_cast<int64_t>(plan.padded_dim);
     const bool wide = d_weight && aligned(d_weight, 16) && d_weight_stride % 8 == 0;
-    if (!Type::wide_range)
-        loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, w.scale);
+    loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, Type::wide_range ? 1.f : 16384.f, w.scale);
     const uint32_t dt = static_cast<uint32_t>(parts_of(dim, WH::BN)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow_hidden ? NH::BM : WH::BM));
     for (uint64_t piece = 0; piece < plan.pieces; ++piece) {
         const int64_t first = static_cast<int64_t>(piece * plan.piece_words), words = piece + 1 < plan.pieces ? static_cast<int64_t>(plan.piece_words) : vocab - first;

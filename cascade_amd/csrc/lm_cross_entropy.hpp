@@ -7,8 +7,10 @@
 //   P[n][v] = d_loss[n] (exp(logit - lse[n]) - (v == target[n])),
 // rounded to 16 bits as the operand of the two products that follow, d_weight = P^T H and d_hidden = P W. The rounding is the
 // matrix unit's price, of the size of the gradients' own last rounding. P of a piece is all that is kept.
-// In half precision P is scaled by a power of two that brings the largest |d_loss| near 2^15, and the products are scaled back in
-// 32 bits: probabilities of 1e-9 would otherwise vanish.
+// P is held relative to the largest |d_loss|, and the products are scaled back in 32 bits. The entries that weigh most are those of the targets, nearly
+// -d_loss[n] each, and a mean over tokens gives all tokens one d_loss: rounded as it is, its error (up to 2^-9) would be the same in all of
+// them and stay in every sum; relative to itself it is 1, which rounds to itself. In half precision that 1 is 2^14, since probabilities of 1e-9 would
+// otherwise vanish.
 #pragma once
 #include "lm_product.hpp"
 
@@ -124,8 +126,8 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int6
     }
 }
 
-// The power of two that P is scaled by, and its inverse: 1 where the type has 32-bit exponents.
-__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, const int32_t* target, int64_t tokens, int64_t vocab, float* scale)
+// The factor of P, range / max |d_loss|, and its inverse.
+__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, const int32_t* target, int64_t tokens, int64_t vocab, float range, float* scale)
 {
     __shared__ float tops[16];
     float top = 0.f;
@@ -140,12 +142,9 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, c
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w)
             top = fmaxf(top, tops[w]);
-        int e = 0;
-        if (top > 0.f && top < INFINITY)
-            e = 15 - ilogbf(top) - 1; // |P| < 2 top <= 2^15
-        e = e > 100 ? 100 : e < -100 ? -100 : e;
-        scale[0] = ldexpf(1.f, e);
-        scale[1] = ldexpf(1.f, -e);
+        const bool fine = top > 1e-30f && top < 1e30f; // both factors are ordinary numbers
+        scale[0] = fine ? range / top : 1.f;
+        scale[1] = fine ? top / range : 1.f;
     }
 }
 
@@ -167,7 +166,7 @@ __global__ __launch_bounds__(P::THREADS) void logit_gradients_kernel(Logits l, c
     for (int j = 0; j < P::TN; ++j) {
         const int64_t n = n0 + P::wave_n() + 32 * j + lane % 32, goal = n < tokens ? l.target[n] : -1;
         const bool counts = goal >= 0 && goal < vocab;
-        factor[j] = counts ? d_loss[n] * (Type::wide_range ? 1.f : scale[0]) : 0.f;
+        factor[j] = counts ? d_loss[n] * scale[0] : 0.f;
         shift[j] = counts ? lse[n] : INFINITY; // tokens left out: zeros, whatever their logits are
         const int64_t t = goal - (l.first_word + mw);
         word[j] = counts && t >= 0 && t < P::BM ? static_cast<int>(t) : -1;
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(P::THREADS) void weight_gradients_kernel(Operand hi
     typename P::Sums sums;
     const int64_t m0 = static_cast<int64_t>(mi) * P::BM, n0 = static_cast<int64_t>(ni) * P::BN;
     P::run(hidden, p, m0, n0, 0, tokens, a0, a1, b0, b1, sums);
-    const float back = Type::wide_range ? 1.f : scale[1];
+    const float back = scale[1];
     meet();
     P::template store_turned<Type>(sums, P::wave_region(a0, a1, b0, b1), m0, n0, hidden.rows, p.rows, out, stride, wide,
                                    [&](int, int, float x) { return x * back; });
@@ -262,7 +261,7 @@ __global__ __launch_bounds__(256) void join_shares_kernel(const float* shares, u
     }
     if (!there || y)
         return;
-    const float back = Type::wide_range ? 1.f : scale[1];
+    const float back = scale[1];
     for (int i = 0; i < 4; ++i)
         if (d + i < dim)
             out[n * out_stride + d + i] = to16<Type>(sum[i] * back);

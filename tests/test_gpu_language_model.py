@@ -387,6 +387,25 @@ def test_cross_entropy_small_and_uneven_weights():
     check_entropy(300, 128, 1000, torch.bfloat16, weights=w, seed=6)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_equal_weights_of_tokens_leave_no_common_error(dtype):
+    """A mean's weight of 1 / n is no number of 16 bits; its rounding, the same for every token, would stay in every sum. The 2-norm of the error is held to
+    that of two independent roundings, of the result and of the terms: each is u / sqrt(3) of a value at most, and u / 2 on average over a binade."""
+    g = gen(14)
+    n, dim, vocab = 700, 256, 3000
+    hidden, weight = randn(g, n, dim, dtype=dtype), randn(g, vocab, dim, dtype=dtype, scale=2 * dim ** -0.5)
+    target = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    lse = cascade_amd.linear_cross_entropy(hidden, weight, target)[1]
+    h, w = hidden.double(), weight.double()
+    p = torch.softmax(h @ w.T, 1)
+    p[torch.arange(n, device="cuda"), target.long()] -= 1
+    for x in (1.00390625 - 2.0 ** -10, 1.001953, 1.2539, 1.9941):  # far from 8-bit and from 11-bit numbers
+        d_loss = torch.full((n,), x, device="cuda")
+        d_hidden, d_weight = cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse)
+        for got, want in ((d_hidden, x * (p @ w)), (d_weight, x * (p.T @ h))):
+            assert (got.double() - want).norm() <= math.sqrt(2) * 0.5 * U[dtype] * want.norm()
+
+
 def test_tokens_without_a_target_may_hold_anything():
     g = gen(7)
     for n in (50, 600):
