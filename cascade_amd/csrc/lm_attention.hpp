@@ -596,16 +596,21 @@ __global__ __launch_bounds__(256) void row_blocks_kernel(Attention a, Heads out,
         }
     }
     if (!Type::wide_range) { // a maximum does not depend on the order in which it is taken; squares are positive, so their bits compare as they do
+        __shared__ float tops[2][4];
         for (int k = 32; k >= 16; k /= 2) {
             most = fmaxf(most, __shfl_xor(most, k));
             most_v = fmaxf(most_v, __shfl_xor(most_v, k));
         }
         if (threadIdx.x % 64 == 0) {
-            const uint32_t bits = __builtin_bit_cast(uint32_t, most), bits_v = __builtin_bit_cast(uint32_t, most_v);
-            if (bits > __hip_atomic_load(norms, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) // most waves find a larger one there
-                atomicMax(norms, bits);
-            if (bits_v > __hip_atomic_load(norms + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-                atomicMax(norms + 1, bits_v);
+            tops[0][threadIdx.x / 64] = most;
+            tops[1][threadIdx.x / 64] = most_v;
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) { // most workgroups find a larger one there
+            const float x = fmaxf(fmaxf(tops[threadIdx.x][0], tops[threadIdx.x][1]), fmaxf(tops[threadIdx.x][2], tops[threadIdx.x][3]));
+            const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+            if (bits > __hip_atomic_load(norms + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+                atomicMax(norms + threadIdx.x, bits);
         }
     }
 }
