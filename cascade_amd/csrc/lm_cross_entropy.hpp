@@ -11,13 +11,16 @@
 // -d_loss[n] each, and a mean over tokens gives all tokens one d_loss: rounded as it is, its error (up to 2^-9) would be the same in all of
 // them and stay in every sum; relative to itself it is 1, which rounds to itself. In half precision that 1 is 2^14, since probabilities of 1e-9 would
 // otherwise vanish.
+//
+// Measured on 8192 tokens of 4096 values and 50257 words (bfloat16): forward 2.7 ms, 1250 TFLOP/s; backward 8.2 ms for three products of that size, 1230.
+// Bound by the product (lm_product.hpp); the gradients' stores as whole lines took 0.7 ms off. 61 tokens of 512 values, forward: 11.6 us for 51 MB of weights, 4.4 TB/s.
 #pragma once
 #include "lm_product.hpp"
 
 namespace lm {
 
 // The order in which workgroups take tiles: each of the 8 XCDs (workgroup id % 8) a run of its own, in bands of 8 row tiles that are
-// walked column by column, so that the 32 workgroups of an XCD that run together share operands in its L2.
+// walked column by column, so that the 32 workgroups of an XCD that run together share operands in its L2 (bands of 4 take the same time, of 16 5 % more, of 32 13 % more).
 __device__ inline void tile_of(uint32_t id, uint32_t mt, uint32_t nt, uint32_t& m, uint32_t& n)
 {
     const uint32_t total = mt * nt, xcd = id % 8, per = total / 8, more = total % 8;

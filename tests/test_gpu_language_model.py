@@ -502,6 +502,46 @@ def test_clip_does_not_overflow_and_leaves_what_has_no_norm():
     assert cascade_amd.clip_gradients([zero], 1.0).item() == 0 and (zero == 0).all()
 
 
+# ---- graphs ----
+
+
+def test_calls_recorded_into_a_graph_give_the_same_in_every_replay():
+    g = gen(15)
+    n, heads, dim, vocab = 1100, 4, 64, 2000
+    text = torch.randint(0, vocab, (n,), generator=g, device="cuda").to(torch.int16)
+    text[torch.randint(0, n, (9,), generator=g, device="cuda")] = -1
+    q, d_out = (randn(g, n, heads, dim, dtype=torch.float16) for _ in range(2))
+    k, v = (randn(g, n, 2, dim, dtype=torch.float16) for _ in range(2))
+    words, d_loss = randn(g, vocab, heads * dim, dtype=torch.float16, scale=0.1), torch.rand(n, generator=g, device="cuda")
+
+    def step():
+        lo, hi, target = cascade_amd.token_spans(text)
+        out, lse = cascade_amd.span_attention(q, k, v, lo, hi, cap=20.0)
+        grads = cascade_amd.span_attention_backward(d_out, q, k, v, out, lse, lo, hi, cap=20.0)
+        hidden = out.view(n, -1)
+        loss, sums = cascade_amd.linear_cross_entropy(hidden, words, target)
+        grads = [*grads, *cascade_amd.linear_cross_entropy_backward(d_loss, hidden, words, target, sums)]
+        norm = cascade_amd.clip_gradients(grads, 0.5)
+        return [lo, hi, target, out, lse, loss, sums, norm, *grads]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = step()
+    for turn in range(4):
+        for x in (q, k, v, d_out):
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        text.copy_(torch.where(text == -1, text, (text + turn) % vocab))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(recorded, want)):
+            assert torch.equal(a, b), f"value {i} of replay {turn}"
+
+
 # ---- refusals ----
 
 
