@@ -114,10 +114,11 @@ Attention attention(const csa_lm_attention& a)
 }
 
 // The rows that a tile of keys meets are shared out over workgroups, each with sums of its own that are joined at the end, until there are
-// KV_GROUPS workgroups: a workgroup takes half a compute unit, and those of a causal text differ in work by as much as their keys. A share has
-// KV_TURNS tiles of rows at least, and where there are as many shares as heads, whole heads: workgroups next to each other then read the same rows
-// (12289 tokens, 16 heads of 2: 8 shares 2.91 ms, 11 shares 3.03 ms; 16384 tokens of documents, 16 heads of 4: 4 shares 1.05 ms, 3 shares 1.15 ms,
-// 2 shares 1.36 ms; 3001 tokens, 12 heads of 12: 8 shares 0.26 ms, none 0.34 ms).
+// KV_GROUPS workgroups (a workgroup takes half a compute unit), or up to twice as many where a share would otherwise hold more than KV_LONG tiles of rows: the
+// workgroups of a long document are the last ones to end. A share has KV_TURNS tiles of rows at least, and where it can be, whole heads: workgroups next to
+// each other then read the same rows (12289 tokens, 16 heads of 2: 8 shares 2.91 ms, 11 shares 3.03 ms; 16384 tokens of documents, 16 heads of 4: 4 shares 1.05 ms,
+// 3 shares 1.15 ms, 2 shares 1.36 ms; 3001 tokens, 12 heads of 12: 8 shares 0.26 ms, none 0.34 ms).
+// The sums take 270 MB at most, but for the rounding to whole heads.
 constexpr uint64_t KV_GROUPS = 1024, KV_LONG = 512, KV_TURNS = 16;
 
 // The keys that a tile of rows sees are shared out in the same way where there are too few tiles for two workgroups a compute unit; a share has five tiles of
@@ -169,12 +170,12 @@ struct AttentionWork {
         key_order = c.take<uint32_t>(may_be_ordered(tokens, q_heads) ? ORDER_TILES : 0);
         const uint64_t tiles = parts_of(tokens, BLOCK_ROWS), group = q_heads / kv_heads, groups = parts_of(tokens, KEYS_PER_GROUP) * kv_heads;
         uint64_t want = groups ? parts_of(KV_GROUPS, groups) : 1;
-        const uint64_t long_ones = parts_of(group * tiles, KV_LONG), most = group * tiles / KV_TURNS;
-        want = want > long_ones ? want : long_ones;
-        if (want > group)
-            want = want / group * group;
-        while (want < group && group % want)
-            ++want;
+        const uint64_t long_ones = parts_of(group * tiles, KV_LONG), twice = groups ? parts_of(2 * KV_GROUPS, groups) : 1, most = group * tiles / KV_TURNS;
+        if (want < long_ones)
+            want = long_ones < twice ? long_ones : twice;
+        const uint64_t whole = want > group ? want / group * group : parts_of(group, group / want); // as many shares as heads, or as groups of heads
+        if (whole <= 2 * want)
+            want = whole;
         shares = static_cast<uint32_t>(want < most ? want : most > 1 ? most : 1);
         parts = c.take<float>(shares > 1 ? 2 * shares * kv_heads * tokens * head_width(dim) : 0);
         norms = c.take<uint32_t>(2);

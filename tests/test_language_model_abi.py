@@ -74,6 +74,11 @@ def test_workspace_sizes():
     lib = native.load()
     assert lib.csa_lm_spans_workspace(4096) == 0 and lib.csa_lm_spans_workspace(4097) == 16384
     assert lib.csa_lm_cross_entropy_workspace(8, 0, 10, 0) == 0
+    # attention: 16 bytes a row and head, and bounded sums, whatever the length and the heads
+    for tokens in (1, 129, 4000, 16384, 131072, 1 << 20, 1 << 24):
+        for heads, kv_heads in ((1, 1), (16, 16), (16, 2), (64, 8), (71, 1), (128, 1)):
+            for flags, most in ((0, 80 << 20), (native.CSA_LM_BACKWARD, (700 << 20) + (tokens + 32) * heads * 16 + tokens // 4)):
+                assert lib.csa_lm_attention_workspace(tokens, heads, kv_heads, 128, flags) <= most, (tokens, heads, kv_heads, flags)
     small, copies = (lib.csa_lm_cross_entropy_workspace(64, 512, 50257, f) for f in (0, native.CSA_LM_COPY_ROWS))
     assert copies - small >= 50257 * 512 * 2
     # the logits of a batch, or their gradients, are never all there: 8192 x 50257 values of 16 bits are 823 MB
