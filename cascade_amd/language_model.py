@@ -55,9 +55,10 @@ def _on_gpu(*tensors):
 
 
 def _enqueue(device, call, *args):
-    """call(*args, stream) with the device's current stream, and the device made current for the launches."""
+    """call(*args, stream) with the device's current stream, and the device made current for the launches. (The stream's address without
+    the object that torch.cuda.current_stream makes around it: 0.1 us instead of 1.2, of the 11 that a small call takes.)"""
     import torch
-    stream = torch.cuda.current_stream(device).cuda_stream or None
+    stream = torch._C._cuda_getCurrentRawStream(device) or None
     if device == torch.cuda.current_device():
         native.check(call(*args, stream))
     else:
@@ -274,7 +275,8 @@ def clip_gradients(grads, max_norm, out=None):
 
 
 def attend(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
-    """span_attention's out, differentiable in q, k and v."""
+    """span_attention's out, differentiable in q, k and v (slopes are constants: ones that want a gradient are refused)."""
+    _check(slopes is None or not slopes.requires_grad, "slopes have no gradient here: detach them")
     return _functions()[0].apply(q, k, v, lo, hi, scale, cap, slopes)
 
 

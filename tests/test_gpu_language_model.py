@@ -583,6 +583,14 @@ def test_refusals():
         cascade_amd.token_spans(torch.zeros(4, device="cuda"))
 
 
+def test_slopes_that_want_a_gradient_are_refused():
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    slopes = torch.ones(2, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="slopes"):
+        cascade_amd.attend(q, q, q, slopes=slopes)
+    assert cascade_amd.attend(q, q, q, slopes=slopes.detach()).shape == q.shape
+
+
 def test_the_library_refuses_what_the_kernels_cannot_read():
     import ctypes as C
     native = lm.native
