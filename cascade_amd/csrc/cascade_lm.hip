@@ -190,7 +190,7 @@ void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_hea
 {
     const bool order = in_order(a);
     if (order)
-        tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), w.row_order, nullptr);
+        tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), nullptr, w.row_order, nullptr);
     attention_forward_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
         attention(a), order ? w.row_order : nullptr, w.row_shares, w.row_parts, w.row_stats, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
     if (w.row_shares > 1)
@@ -208,7 +208,7 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     span_bounds_kernel<<<static_cast<uint32_t>(parts_of(a.tokens, 64)), 64, 0, s>>>(at, w.bounds, w.norms);
     const bool order = in_order(a);
     if (order)
-        tile_order_kernel<<<1, 1024, 0, s>>>(at, w.row_order, w.key_order);
+        tile_order_kernel<<<1, 1024, 0, s>>>(at, w.bounds, w.row_order, w.key_order);
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
     float* rests = reinterpret_cast<float*>(w.row_stats);
     attention_d_q_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(

@@ -146,17 +146,25 @@ __device__ inline int wave_most(int x)
 
 constexpr int NONE = 0x7fffffff; // lo of a row that sees nothing, whose hi is 0: it lowers no minimum and raises no maximum
 
+// lo and hi as given, to what of them there is
+__device__ inline void narrow(const Attention& a, int& lo, int& hi)
+{
+    lo = max(lo, 0);
+    hi = static_cast<int>(min(static_cast<int64_t>(hi), a.tokens));
+    if (lo >= hi) {
+        lo = NONE;
+        hi = 0;
+    }
+}
+
 __device__ inline void span_of(const Attention& a, int64_t i, int& lo, int& hi)
 {
     lo = NONE;
     hi = 0;
     if (i < a.tokens) {
-        const int l = a.lo ? max(a.lo[i], 0) : 0;
-        const int h = a.hi ? min(static_cast<int64_t>(a.hi[i]), a.tokens) : i + 1;
-        if (l < h) {
-            lo = l;
-            hi = h;
-        }
+        lo = a.lo ? a.lo[i] : 0;
+        hi = a.hi ? a.hi[i] : static_cast<int>(i) + 1;
+        narrow(a, lo, hi);
     }
 }
 
@@ -1131,41 +1139,78 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
 
 // The order of tiles by work, most first, for texts whose spans are given: documents differ in length by more than workgroups can make up for by
 // their number (six texts of 16384 tokens and documents of lognormal lengths: the last workgroup ends 10 to 25 % earlier). One workgroup
-// reads all spans once, and ranks tiles by the 64-key tiles that their rows see, and by the 32-row tiles that see their keys.
+// reads all spans once, or what span_bounds_kernel has left of them if `bounds` is there, and ranks tiles by the 64-key tiles that their rows see, and by
+// the 32-row tiles that see their keys. What it waits for is memory, so loads are as wide as they can be, two on their way
+// together (8192 tokens: 5.4 us, four single values a load 8.6; 16384 tokens with their keys: 8.8 us from spans, 6.2 from bounds, as single values 18).
 constexpr int ORDER_TILES = 1024; // of 128 rows or keys
 
-__global__ __launch_bounds__(1024) void tile_order_kernel(Attention a, uint32_t* row_order, uint32_t* key_order)
+__global__ __launch_bounds__(1024) void tile_order_kernel(Attention a, const int2* bounds, uint32_t* row_order, uint32_t* key_order)
 {
     __shared__ int los[ORDER_TILES], his[ORDER_TILES]; // of the rows of a tile
     __shared__ int change[ORDER_TILES + 1];            // of the number of 32-row tiles that see a tile of keys, from the tile before it
-    __shared__ int work[ORDER_TILES], sums[16];
+    __shared__ __attribute__((aligned(16))) int work[ORDER_TILES];
+    __shared__ int sums[16];
     const int t = threadIdx.x, lane = t % 64, tiles = static_cast<int>((a.tokens + ROWS_PER_GROUP - 1) / ROWS_PER_GROUP);
     los[t] = NONE;
     his[t] = change[t] = 0;
     __syncthreads();
-    constexpr int MINE = 4; // neighbouring rows of a lane: eight lanes see 32
-    for (int64_t first = t * MINE; first < tiles * ROWS_PER_GROUP; first += 1024 * MINE) {
-        int lo = NONE, hi = 0;
-#pragma unroll
-        for (int k = 0; k < MINE; ++k) {
-            int l, h;
-            span_of(a, first + k, l, h);
-            lo = min(lo, l);
-            hi = max(hi, h);
-        }
-        for (int d = 1; d < BLOCK_ROWS / MINE; d *= 2) {
-            lo = min(lo, __shfl_xor(lo, d));
-            hi = max(hi, __shfl_xor(hi, d));
-        }
-        if (t % (BLOCK_ROWS / MINE) == 0 && lo < hi) {
-            const int64_t tile = first / ROWS_PER_GROUP;
-            atomicMin(los + tile, lo);
-            atomicMax(his + tile, hi);
+    auto count = [&](int tile, int lo, int hi) { // of the rows of a 32-row tile
+        if (lo < hi) {
+            atomicMin(los + tile / (ROWS_PER_GROUP / BLOCK_ROWS), lo);
+            atomicMax(his + tile / (ROWS_PER_GROUP / BLOCK_ROWS), hi);
             atomicAdd(change + lo / KEYS_PER_GROUP, 1);
             atomicAdd(change + (hi - 1) / KEYS_PER_GROUP + 1, -1);
         }
+    };
+    if (bounds) {
+        const int blocks = static_cast<int>((a.tokens + BLOCK_ROWS - 1) / BLOCK_ROWS);
+        for (int tile = t; tile < blocks; tile += 1024)
+            count(tile, bounds[tile].x, bounds[tile].y);
+    } else {
+        constexpr int MINE = 4, TURNS = 2; // neighbouring rows of a lane, eight lanes to a 32-row tile, and loads of them at a time
+        const bool wide = (reinterpret_cast<uintptr_t>(a.lo) | reinterpret_cast<uintptr_t>(a.hi)) % 16 == 0;
+        for (int64_t first = t * MINE; first < tiles * ROWS_PER_GROUP; first += 1024 * MINE * TURNS) {
+            int lo[TURNS], hi[TURNS];
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u) {
+                lo[u] = NONE;
+                hi[u] = 0;
+                const int64_t row = first + u * 1024 * MINE;
+                int l[MINE] = {}, h[MINE];
+#pragma unroll
+                for (int k = 0; k < MINE; ++k)
+                    h[k] = static_cast<int>(row) + k + 1;
+                if (wide && row + MINE <= a.tokens) {
+                    if (a.lo)
+                        __builtin_memcpy(l, __builtin_assume_aligned(a.lo + row, 16), 16);
+                    if (a.hi)
+                        __builtin_memcpy(h, __builtin_assume_aligned(a.hi + row, 16), 16);
+                }
+#pragma unroll
+                for (int k = 0; k < MINE; ++k) {
+                    if (wide && row + MINE <= a.tokens)
+                        narrow(a, l[k], h[k]);
+                    else
+                        span_of(a, row + k, l[k], h[k]);
+                    lo[u] = min(lo[u], l[k]);
+                    hi[u] = max(hi[u], h[k]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u) {
+                for (int d = 1; d < BLOCK_ROWS / MINE; d *= 2) {
+                    lo[u] = min(lo[u], __shfl_xor(lo[u], d));
+                    hi[u] = max(hi[u], __shfl_xor(hi[u], d));
+                }
+                if (t % (BLOCK_ROWS / MINE) == 0)
+                    count(static_cast<int>((first + u * 1024 * MINE) / BLOCK_ROWS), lo[u], hi[u]);
+            }
+        }
     }
     __syncthreads();
+    int lanes = 1;
+    while (lanes < 64 && lanes * 2 * tiles <= 1024)
+        lanes *= 2;
     for (int keys = 0; keys < (key_order ? 2 : 1); ++keys) {
         int mine = 0;
         if (keys) { // the running sum of the changes
@@ -1184,12 +1229,20 @@ __global__ __launch_bounds__(1024) void tile_order_kernel(Attention a, uint32_t*
         }
         work[t] = mine;
         __syncthreads();
-        if (t < tiles) {
+        if (t / lanes < tiles) { // `lanes` of them for a tile
+            const int tile = t / lanes;
+            const uint32_t own = work[tile];
             int rank = 0;
-#pragma unroll 8
-            for (int other = 0; other < tiles; ++other)
-                rank += work[other] > mine || (work[other] == mine && other < t);
-            (keys ? key_order : row_order)[rank] = t;
+            for (int other = t % lanes * 4; other < tiles; other += lanes * 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(work + other); // tiles that are not there have no work and come later
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    rank += w[k] > own || (w[k] == own && other + k < tile);
+            }
+            for (int d = 1; d < lanes; d *= 2)
+                rank += __shfl_xor(rank, d);
+            if (t % lanes == 0)
+                (keys ? key_order : row_order)[rank] = tile;
         }
         __syncthreads();
     }

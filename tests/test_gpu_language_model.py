@@ -221,6 +221,24 @@ def test_attention_of_a_long_text():
     check_attention(2111, 32, 2, 16, torch.float16, "documents", seed=10)  # shared heads in that order, too
 
 
+@pytest.mark.parametrize("n", [8193, 9001])
+@pytest.mark.parametrize("mask", ["whole", "random"])
+def test_the_order_of_tiles_changes_no_result(n, mask):
+    g = gen(n)
+    q, k, v, d_out = (randn(g, n, h, 64, dtype=torch.bfloat16) for h in (8, 2, 2, 8))
+    lo, hi = spans_for("random", n, g)
+    if mask == "whole":  # as without spans, where no order is made
+        lo, hi = torch.zeros_like(lo), torch.arange(1, n + 1, device="cuda", dtype=torch.int32)
+    aside = [torch.cat([x[:1], x])[1:] for x in (lo, hi)]  # four bytes off the alignment of wide loads
+    assert aside[0].data_ptr() % 16 == 4
+    found = []
+    for spans in [(lo, hi), aside] + [(None, None)] * (mask == "whole"):
+        out, lse = cascade_amd.span_attention(q, k, v, *spans)
+        found.append((out, lse, *cascade_amd.span_attention_backward(d_out, q, k, v, out, lse, *spans)))
+    for other in found[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(found[0], other))
+
+
 @pytest.mark.parametrize("mask", ["causal", "all", "window", "random", "none"])
 def test_attention_of_few_heads_shares_out_keys(mask):
     check_attention(1301, 2, 1, 64, torch.bfloat16, mask, seed=21)
