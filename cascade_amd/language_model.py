@@ -147,7 +147,7 @@ def span_attention(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
     Returns (out of q's shape, lse float32 (heads, tokens)); rows that see nothing are zeros with lse -inf (csa_lm_attention_forward_dev)."""
     import torch
     a, device, keep = _describe(q, k, v, lo, hi, scale, cap, slopes)
-    out = q.new_empty(q.shape)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((a.q_heads, a.tokens), dtype=torch.float32)
     if a.tokens:
         lib = native.load()
@@ -166,7 +166,7 @@ def span_attention_backward(d_out, q, k, v, out, lse, lo=None, hi=None, scale=No
     _check(lse.shape == (a.q_heads, a.tokens) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse: float32 (heads, tokens)")
     _on_gpu(q, out, d_out, lse)
     (out, oh), (d_out, gh) = _walkable(out), _walkable(d_out)
-    d_q, d_k, d_v = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    d_q, d_k, d_v = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
     if a.tokens:
         lib = native.load()
         size = lib.csa_lm_attention_workspace(a.tokens, a.q_heads, a.kv_heads, a.head_dim, native.CSA_LM_BACKWARD)
