@@ -185,13 +185,13 @@ struct AttentionWork {
     }
 };
 
-template <class Type, int DIM, bool BENT>
+template <class Type, int DIM, int BEND>
 void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_heads& out, float* lse, hipStream_t s)
 {
     const bool order = in_order(a);
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), nullptr, w.row_order, nullptr);
-    attention_forward_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
+    attention_forward_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
         attention(a), order ? w.row_order : nullptr, w.row_shares, w.row_parts, w.row_stats, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
     if (w.row_shares > 1)
         join_rows_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
@@ -199,7 +199,7 @@ void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_hea
             out.token_stride, out.head_stride, lse);
 }
 
-template <class Type, int DIM, bool BENT>
+template <class Type, int DIM, int BEND>
 void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* lse, const csa_lm_heads& d_out, const csa_lm_heads& d_q, const csa_lm_heads& d_k,
               const csa_lm_heads& d_v, const AttentionWork& w, hipStream_t s)
 {
@@ -211,13 +211,13 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
         tile_order_kernel<<<1, 1024, 0, s>>>(at, w.bounds, w.row_order, w.key_order);
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
     float* rests = reinterpret_cast<float*>(w.row_stats);
-    attention_d_q_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
+    attention_d_q_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
         at, order ? w.row_order : nullptr, w.row_shares, w.row_parts, rests, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data),
         d_q.token_stride, d_q.head_stride);
     if (w.row_shares > 1)
         join_d_q_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
             w.row_parts, rests, w.row_shares, at.tokens, at.dim, DIM, w.blocks, tiles, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
-    attention_d_kv_kernel<Type, DIM, BENT><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
+    attention_d_kv_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
         at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
         d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
     if (w.shares > 1)
@@ -235,16 +235,18 @@ void with_type(int type, F f)
         f(Bf16());
 }
 
-// f(type, head width, whether scores are bent) as types
+// f(type, head width, how scores are bent) as types
 template <class F>
 void with_kind(const csa_lm_attention& a, F f)
 {
     with_type(a.type, [&](auto type) {
         auto with_width = [&](auto width) {
-            if (a.cap > 0.f || a.d_slope)
-                f(type, width, std::true_type());
+            if (a.cap > CAP_PLAIN)
+                f(type, width, std::integral_constant<int, FAR_CAP>());
+            else if (a.cap > 0.f || a.d_slope)
+                f(type, width, std::integral_constant<int, PLAIN>());
             else
-                f(type, width, std::false_type());
+                f(type, width, std::integral_constant<int, STRAIGHT>());
         };
         if (head_width(a.head_dim) == 64)
             with_width(std::integral_constant<int, 64>());
@@ -487,7 +489,7 @@ int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, fl
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    with_kind(*a, [&](auto type, auto width, auto bent) { forward<decltype(type), width(), bent()>(*a, w, out, d_lse, s); });
+    with_kind(*a, [&](auto type, auto width, auto bend) { forward<decltype(type), width(), bend()>(*a, w, out, d_lse, s); });
     return launched(who);
 }
 
@@ -517,7 +519,7 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    with_kind(*a, [&](auto type, auto width, auto bent) { backward<decltype(type), width(), bent()>(*a, out, d_lse, d_out, d_q, d_k, d_v, w, s); });
+    with_kind(*a, [&](auto type, auto width, auto bend) { backward<decltype(type), width(), bend()>(*a, out, d_lse, d_out, d_q, d_k, d_v, w, s); });
     return launched(who);
 }
 

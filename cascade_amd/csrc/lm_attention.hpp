@@ -215,6 +215,28 @@ __device__ inline void read_ahead()
     __builtin_amdgcn_sched_group_barrier(0x8, PRODUCTS - TURNS, 0);
 }
 
+// How scores are bent. Kernels of each kind are compiled without the code of the others, which costs them registers even where it does not run.
+enum Bend : int {
+    STRAIGHT, // neither a cap nor a slope
+    PLAIN,    // a cap of CAP_PLAIN at most, a slope, or both
+    FAR_CAP   // a larger cap, perhaps with a slope
+};
+
+// cap tanh(y), y = score / cap. As 1 - 2 / (1 + e^2y) a tanh is off by 1.5e-7 whatever y is, and the score by that part of the cap: 1e-5 at CAP_PLAIN, far below what 16-bit
+// operands leave of a score, but 0.1 at a cap of 1e6. With larger caps |y| < 1/2 takes y times tanh(y) / y, a polynomial in y^2 (interpolated at Chebyshev's points, off by 6e-8), so that a score is
+// off by 5e-7 of itself. Caps of CAP_PLAIN and less do not, which would cost them: 6000 tokens, 16 heads of 128 values trained 0.98 ms, with the polynomial 1.19 ms.
+constexpr float CAP_PLAIN = 64.f;
+
+// A product s bent, still to be multiplied by scale: s tanh(y) / y, y = s in. in: scale / cap, out: its inverse, finite.
+__device__ inline float bend_far(float s, float in, float out)
+{
+    const float y = s * in, y2 = y * y;
+    const float ratio = 1.f + y2 * (-0.333330679f + y2 * (0.133247505f + y2 * (-0.0529842388f + y2 * 0.0171313444f)));
+    return fabsf(y) < 0.5f ? s * ratio : out - 2.f * out * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * (2.f * LOG2E)));
+}
+__device__ inline float near_in(const Attention& a) { return fminf(2.f * LOG2E * a.scale / a.cap, 3e38f); } // finite, so that a product of 0 stays 0
+__device__ inline float far_out(const Attention& a) { return fminf(a.cap / a.scale, 1e38f); }
+
 // ---- what a row may not see ----
 //
 // A score that a row may not see becomes a probability of 0, but 0 times an infinity or NaN that stands there is none. What no row of a workgroup sees is
@@ -251,8 +273,12 @@ __device__ inline float one_score(const Attention& a, float product, float slope
 {
     float z = product * a.scale * LOG2E;
     bent = 1.f;
-    if (a.cap > 0.f) {
-        const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * (2.f * LOG2E * a.scale / a.cap)));
+    if (a.cap > CAP_PLAIN) {
+        product = bend_far(product, a.scale / a.cap, far_out(a));
+        z = product * a.scale * LOG2E;
+        bent = 1.f - product * (a.scale / a.cap) * (product * (a.scale / a.cap));
+    } else if (a.cap > 0.f) {
+        const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * near_in(a)));
         z = a.cap * LOG2E * t;
         bent = 1.f - t * t;
     }
@@ -278,18 +304,22 @@ __device__ inline void share_of(int lo, int hi, uint32_t share, uint32_t shares,
         start = stop = 0;
 }
 
-// BENT: there is a cap or a slope. Kernels without them are compiled without the code for them, which costs the others registers even where it
-// does not run.
-//
 // Scores of a tile, still raw products: to exponents of 2 less nothing, with `unit` left to multiply. Returns with z = s * unit.
-template <bool BENT, int TILES>
+template <int BEND, int TILES>
 __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit, float slope2, int row, int key0, int half)
 {
     unit = a.scale * LOG2E;
-    if (!BENT)
+    if (BEND == STRAIGHT)
         return;
-    if (a.cap > 0.f) {
-        const float in = 2.f * LOG2E * a.scale / a.cap, cap2 = a.cap * LOG2E;
+    if (BEND == FAR_CAP) {
+        const float in = a.scale / a.cap, back = far_out(a);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[t][r] = bend_far(s[t][r], in, back);
+    } else if (a.cap > 0.f) {
+        const float in = near_in(a), cap2 = a.cap * LOG2E;
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
@@ -309,7 +339,7 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
     }
 }
 
-template <class Type, int DIM, bool BENT>
+template <class Type, int DIM, int BEND>
 __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float2* stats, short* out,
                                                                    int64_t out_token, int64_t out_head, float* lse)
 {
@@ -364,7 +394,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
                 s[t] = Type::mfma32(tiles_at.along(ks, 32 * t, d), q[d], s[t]);
         read_ahead<DIM / 8, DIM / 8, 4, 1>();
         float unit;
-        bend<BENT>(a, s, unit, slope2, static_cast<int>(row), key0, half);
+        bend<BEND>(a, s, unit, slope2, static_cast<int>(row), key0, half);
         if (key0 < all_lo || key0 + KT > all_hi) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -646,7 +676,7 @@ constexpr float P_SHIFT = Type::wide_range ? 0.f : 15.f;
 
 // p and ds of 32 x 32 scores: s and dp in, p (times 2^shift) and ds (times `grow`) out. `lse2(r)`, `delta(r)`, `distance(r)`, `seen(r)` of register r.
 // With REST, returns the sum of p (dp - delta) over the lane's registers, times both factors.
-template <bool BENT, bool REST, class L, class D, class X, class S>
+template <int BEND, bool REST, class L, class D, class X, class S>
 __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, float grow, bool masked, L lse2, D delta, X distance,
                                         S seen)
 {
@@ -655,8 +685,19 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
     for (int r = 0; r < 16; ++r)
         dp[r] = (dp[r] - delta(r)) * grow;
     float unit = a.scale * LOG2E;
-    if (BENT && a.cap > 0.f) {
-        const float in = 2.f * LOG2E * a.scale / a.cap, cap2 = a.cap * LOG2E;
+    if (BEND == FAR_CAP) {
+        const float in = a.scale / a.cap, back = far_out(a);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = bend_far(s[r], in, back);
+            const float t = s[r] * in;
+            if (REST)
+                bent[r] = 1.f - t * t;
+            else
+                dp[r] *= 1.f - t * t;
+        }
+    } else if (BEND == PLAIN && a.cap > 0.f) {
+        const float in = near_in(a), cap2 = a.cap * LOG2E;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[r] * in));
@@ -668,7 +709,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
         }
         unit = 1.f;
     }
-    if (BENT && a.slope) {
+    if (BEND != STRAIGHT && a.slope) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             s[r] = s[r] * unit - slope2 * fabsf(distance(r));
@@ -693,7 +734,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
 #pragma unroll
     for (int r = 0; r < 16; ++r)
         sum += dp[r];
-    if (BENT && a.cap > 0.f) {
+    if (BEND != STRAIGHT && a.cap > 0.f) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             dp[r] *= bent[r];
@@ -701,7 +742,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
     return sum;
 }
 
-template <class Type, int DIM, bool BENT>
+template <class Type, int DIM, int BEND>
 __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float* rests, Heads d_out,
                                                                RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
                                                                short* d_q, int64_t out_token, int64_t out_head)
@@ -762,7 +803,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
             }
             read_ahead<DIM / 8, DIM / 8, 4, 1>();
             const int key = key0 + 32 * t + 4 * half, i = static_cast<int>(row);
-            rest += score_gradients<BENT, true>(
+            rest += score_gradients<BEND, true>(
                 a, s, dp, slope2, 0.f, grow, masked, [&](int) { return lse2; }, [&](int) { return delta; },
                 [&](int r) { return static_cast<float>(i - (key + 8 * (r / 4) + r % 4)); },
                 [&](int r) { const int k = key + 8 * (r / 4) + r % 4; return k >= lo && k < hi; });
@@ -900,7 +941,7 @@ constexpr int KEYS_PER_GROUP = 128;
 
 // The workgroup's 128 keys by 32 rows a turn, 32 keys a wave. Two waves of a SIMD have 256 registers each: at 128 values a head the sums of d_k and
 // d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
-template <class Type, int DIM, bool BENT>
+template <class Type, int DIM, int BEND>
 __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, const uint32_t* order, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
                                                                 const uint32_t* norms, uint32_t shares, float* parts, short* d_k,
                                                                 int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
@@ -1011,7 +1052,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
             __builtin_amdgcn_s_setprio(0);
         const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
         const int row = tile * RT + 4 * half;
-        score_gradients<BENT, false>(
+        score_gradients<BEND, false>(
             a, s, dp, slope2, P_SHIFT<Type>, grow_k, masked, [&](int r) { return bs.lse2[4 * half + 8 * (r / 4) + r % 4]; },
             [&](int r) { return bs.delta[4 * half + 8 * (r / 4) + r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
             [&](int r) {
