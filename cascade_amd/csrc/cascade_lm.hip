@@ -147,7 +147,6 @@ bool may_be_ordered(uint64_t tokens, uint64_t q_heads)
 bool in_order(const csa_lm_attention& a) { return (a.d_lo || a.d_hi) && may_be_ordered(a.tokens, a.q_heads); }
 
 struct AttentionWork {
-    uint32_t* norms;
     int2* bounds;
     RowBlock* blocks;
     float* parts;
@@ -178,7 +177,6 @@ struct AttentionWork {
             want = whole;
         shares = static_cast<uint32_t>(want < most ? want : most > 1 ? most : 1);
         parts = c.take<float>(shares > 1 ? 2 * shares * kv_heads * tokens * head_width(dim) : 0);
-        norms = c.take<uint32_t>(2);
         bounds = c.take<int2>(tiles);
         blocks = c.take<RowBlock>(tiles * q_heads);
         bytes = c.used;
@@ -205,21 +203,21 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
 {
     const Attention at = attention(a);
     const uint32_t tiles = static_cast<uint32_t>(parts_of(a.tokens, BLOCK_ROWS));
-    span_bounds_kernel<<<static_cast<uint32_t>(parts_of(a.tokens, 64)), 64, 0, s>>>(at, w.bounds, w.norms);
+    span_bounds_kernel<<<static_cast<uint32_t>(parts_of(a.tokens, 64)), 64, 0, s>>>(at, w.bounds);
     const bool order = in_order(a);
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(at, w.bounds, w.row_order, w.key_order);
-    row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks, w.norms);
+    row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks);
     float* rests = reinterpret_cast<float*>(w.row_stats);
     attention_d_q_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
-        at, order ? w.row_order : nullptr, w.row_shares, w.row_parts, rests, heads(d_out), w.blocks, tiles, w.norms, static_cast<short*>(d_q.data),
-        d_q.token_stride, d_q.head_stride);
+        at, order ? w.row_order : nullptr, w.row_shares, w.row_parts, rests, heads(d_out), w.blocks, tiles, static_cast<short*>(d_q.data), d_q.token_stride,
+        d_q.head_stride);
     if (w.row_shares > 1)
         join_d_q_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
             w.row_parts, rests, w.row_shares, at.tokens, at.dim, DIM, w.blocks, tiles, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
     attention_d_kv_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
-        at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.norms, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
-        d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
+        at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride,
+        static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
     if (w.shares > 1)
         join_parts_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.kv_heads, 2), 256, 0, s>>>(
             w.parts, w.shares, at.tokens, at.dim, DIM, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride, static_cast<short*>(d_v.data),

@@ -570,8 +570,8 @@ struct RowBlock {
     int lo[BLOCK_ROWS], hi[BLOCK_ROWS];
 };
 
-// The least lo and the largest hi of every 32 rows, and zeros where the largest norms of d_out and v will be.
-__global__ __launch_bounds__(64) void span_bounds_kernel(Attention a, int2* bounds, uint32_t* norms)
+// The least lo and the largest hi of every 32 rows.
+__global__ __launch_bounds__(64) void span_bounds_kernel(Attention a, int2* bounds)
 {
     int lo, hi;
     span_of(a, static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x, lo, hi);
@@ -583,8 +583,6 @@ __global__ __launch_bounds__(64) void span_bounds_kernel(Attention a, int2* boun
         const int64_t tile = blockIdx.x * 2 + threadIdx.x / 32;
         if (tile * BLOCK_ROWS < a.tokens)
             bounds[tile] = make_int2(lo, hi);
-        if (blockIdx.x == 0 && threadIdx.x == 0)
-            norms[0] = norms[1] = 0;
     }
 }
 
@@ -604,30 +602,19 @@ __device__ inline float dot16(const short* x, const short* y, int dim, int lane1
     return sum;
 }
 
-// Row blocks of every head: sixteen lanes a row, sixteen rows a workgroup at a time. Half precision also asks for the largest norms of rows of d_out and v.
+// Row blocks of every head: sixteen lanes a row, sixteen rows a workgroup at a time.
 template <class Type>
-__global__ __launch_bounds__(256) void row_blocks_kernel(Attention a, Heads out, Heads d_out, const float* lse, RowBlock* blocks, uint32_t* norms)
+__global__ __launch_bounds__(256) void row_blocks_kernel(Attention a, Heads out, Heads d_out, const float* lse, RowBlock* blocks)
 {
     const uint32_t head = blockIdx.y, tile = blockIdx.x;
     RowBlock& to = blocks[static_cast<int64_t>(head) * gridDim.x + tile];
     const int lane16 = threadIdx.x % 16;
-    float most = 0.f, most_v = 0.f;
     for (int r = threadIdx.x / 16; r < BLOCK_ROWS; r += 16) {
         const int64_t row = static_cast<int64_t>(tile) * BLOCK_ROWS + r;
         float delta = 0.f;
-        if (row < a.tokens) {
-            const short* g = static_cast<const short*>(d_out.data) + head * d_out.head + row * d_out.token;
-            delta = dot16<Type>(static_cast<const short*>(out.data) + head * out.head + row * out.token, g, a.dim, lane16);
-            if (!Type::wide_range) { // finite ones: the others belong to rows that nobody sees, or to ones that are lost anyway
-                const float square = dot16<Type>(g, g, a.dim, lane16);
-                most = square < INFINITY ? fmaxf(most, square) : most;
-                if (head % a.group == 0) {
-                    const short* v = static_cast<const short*>(a.v.data) + head / a.group * a.v.head + row * a.v.token;
-                    const float square_v = dot16<Type>(v, v, a.dim, lane16);
-                    most_v = square_v < INFINITY ? fmaxf(most_v, square_v) : most_v;
-                }
-            }
-        }
+        if (row < a.tokens)
+            delta = dot16<Type>(static_cast<const short*>(out.data) + head * out.head + row * out.token,
+                                static_cast<const short*>(d_out.data) + head * d_out.head + row * d_out.token, a.dim, lane16);
         if (lane16 == 0) {
             int lo, hi;
             span_of(a, row, lo, hi);
@@ -637,53 +624,56 @@ __global__ __launch_bounds__(256) void row_blocks_kernel(Attention a, Heads out,
             to.hi[r] = hi;
         }
     }
-    if (!Type::wide_range) { // a maximum does not depend on the order in which it is taken; squares are positive, so their bits compare as they do
-        __shared__ float tops[2][4];
-        for (int k = 32; k >= 16; k /= 2) {
-            most = fmaxf(most, __shfl_xor(most, k));
-            most_v = fmaxf(most_v, __shfl_xor(most_v, k));
-        }
-        if (threadIdx.x % 64 == 0) {
-            tops[0][threadIdx.x / 64] = most;
-            tops[1][threadIdx.x / 64] = most_v;
-        }
-        __syncthreads();
-        if (threadIdx.x < 2) { // most workgroups find a larger one there
-            const float x = fmaxf(fmaxf(tops[threadIdx.x][0], tops[threadIdx.x][1]), fmaxf(tops[threadIdx.x][2], tops[threadIdx.x][3]));
-            const uint32_t bits = __builtin_bit_cast(uint32_t, x);
-            if (bits > __hip_atomic_load(norms + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-                atomicMax(norms + threadIdx.x, bits);
-        }
-    }
 }
 
-// In half precision ds is rounded to 16 bits times the power of two that brings the bound 2 |d_out| |v| of |d_out . v - D| under 2^15, and p
-// times 2^15 in the sums for d_v: small probabilities and gradients would otherwise vanish. The inverse is applied in 32 bits.
+// In half precision ds is rounded to 16 bits times a power of two, and p times 2^15 in the sums for d_v: small gradients and probabilities would otherwise vanish.
+// The inverse is applied in 32 bits. The power is a lane's own, that is of one row (d_q) or one key (d_k), and follows the largest ds that the lane has met: what other rows
+// and keys hold, and what nobody sees, takes no bits from it. It starts too large and only becomes smaller, by which the lane's sums are then multiplied, as for the
+// running maximum of a softmax; 2^3 of headroom make that rare. (6000 tokens, 16 heads of 128 values trained 0.91 ms, with one power for the whole call 0.90; 3001 tokens of 12 heads 177 us and
+// 180, since that power took the norms of all rows.)
 template <class Type>
-__device__ inline float gradient_scale(const uint32_t* norms)
-{
-    if (Type::wide_range)
-        return 1.f;
-    const float bound = 2.f * sqrtf(__builtin_bit_cast(float, norms[0])) * sqrtf(__builtin_bit_cast(float, norms[1]));
-    if (!(bound > 0.f && bound < INFINITY))
-        return 1.f;
-    int e = 14 - ilogbf(bound);
-    e = e > 60 ? 60 : e < -60 ? -60 : e;
-    return ldexpf(1.f, e);
-}
+struct Growth {
+    float by = Type::wide_range ? 1.f : 0x1p100f;
+    // ds times the power, the lane's sums brought to it. Lanes l and l ^ 32 hold parts of one row's or key's ds.
+    template <int N>
+    __device__ void apply(f32x16& ds, f32x16 (&sums)[N])
+    {
+        if (Type::wide_range)
+            return;
+        float most = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            most = fmaxf(most, fabsf(ds[r]));
+        most = fmaxf(most, other_half(most));
+        if (__any(most * by > 0x1p15f && most < INFINITY)) { // an infinity is in the sums whatever the power is
+            const int e = max(12 - ilogb(most), -100);
+            const float less = most * by > 0x1p15f && most < INFINITY ? __builtin_amdgcn_ldexpf(1.f, e) : by, down = less / by;
+            by = less;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sums[n][r] *= down;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            ds[r] *= by;
+    }
+    static __device__ int ilogb(float x) { return __builtin_amdgcn_frexp_expf(x) - 1; }
+};
 template <class Type>
 constexpr float P_SHIFT = Type::wide_range ? 0.f : 15.f;
 
-// p and ds of 32 x 32 scores: s and dp in, p (times 2^shift) and ds (times `grow`) out. `lse2(r)`, `delta(r)`, `distance(r)`, `seen(r)` of register r.
-// With REST, returns the sum of p (dp - delta) over the lane's registers, times both factors.
+// p and ds of 32 x 32 scores: s and dp in, p and ds (both times 2^shift) out. `lse2(r)`, `delta(r)`, `distance(r)`, `seen(r)` of register r.
+// With REST, returns the sum of p (dp - delta) over the lane's registers, times 2^shift.
 template <int BEND, bool REST, class L, class D, class X, class S>
-__device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, float grow, bool masked, L lse2, D delta, X distance,
+__device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& dp, float slope2, float shift, bool masked, L lse2, D delta, X distance,
                                         S seen)
 {
     f32x16 bent;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-        dp[r] = (dp[r] - delta(r)) * grow;
+        dp[r] -= delta(r);
     float unit = a.scale * LOG2E;
     if (BEND == FAR_CAP) {
         const float in = a.scale / a.cap, back = far_out(a);
@@ -744,8 +734,7 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
 
 template <class Type, int DIM, int BEND>
 __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float* rests, Heads d_out,
-                                                               RowBlock* blocks, uint32_t blocks_per_head, const uint32_t* norms,
-                                                               short* d_q, int64_t out_token, int64_t out_head)
+                                                               RowBlock* blocks, uint32_t blocks_per_head, short* d_q, int64_t out_token, int64_t out_head)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
     constexpr int KT = KEYS_PER_TILE;
@@ -774,7 +763,6 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
         lse2 = b.lse2[row % BLOCK_ROWS];
         delta = b.delta[row % BLOCK_ROWS];
     }
-    const float grow = gradient_scale<Type>(norms);
     const uint32_t kv = head / a.group;
     const char* kb = reinterpret_cast<const char*>(static_cast<const short*>(a.k.data) + kv * a.k.head);
     const char* vb = reinterpret_cast<const char*>(static_cast<const short*>(a.v.data) + kv * a.v.head);
@@ -787,6 +775,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
     for (int e = 0; e < DIM / 32; ++e)
         o[e] = f32x16{};
     float rest = 0.f; // sum of p (dp - D), which would be 0 if D were exact
+    Growth<Type> grow;
 
     auto turn = [&](const short* ks, const short* vs, int key0) {
         if (key0 + KT <= wave_lo || key0 >= wave_hi)
@@ -804,9 +793,10 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
             read_ahead<DIM / 8, DIM / 8, 4, 1>();
             const int key = key0 + 32 * t + 4 * half, i = static_cast<int>(row);
             rest += score_gradients<BEND, true>(
-                a, s, dp, slope2, 0.f, grow, masked, [&](int) { return lse2; }, [&](int) { return delta; },
+                a, s, dp, slope2, 0.f, masked, [&](int) { return lse2; }, [&](int) { return delta; },
                 [&](int r) { return static_cast<float>(i - (key + 8 * (r / 4) + r % 4)); },
                 [&](int r) { const int k = key + 8 * (r / 4) + r % 4; return k >= lo && k < hi; });
+            grow.apply(dp, o);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const s16x8 ds = round8<Type>(dp, u), low = round8<Type>(dp - widen<Type>(ds, u), u);
@@ -842,7 +832,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
     rest += other_half(rest);
     // A share knows only its own part of what D is off by: its d_q is the one of the rounded D, and the kernel that joins them corrects D for the
     // kernel of d_k alone.
-    const float exact = shares > 1 ? delta : delta + rest / grow;
+    const float exact = shares > 1 ? delta : delta + rest;
     float* part = parts + (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens * DIM;
     const uint64_t lost = __ballot(!all_finite(o));
     const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
@@ -885,13 +875,13 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *reinterpret_cast<f32x4*>(part + row * DIM + 32 * e + 8 * g + 4 * half) =
-                        f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]} * (a.scale / grow);
+                        f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]} * (a.scale / grow.by);
         if (half == 0)
-            rests[(static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row] = rest / grow;
+            rests[(static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row] = rest;
     } else if (row < a.tokens) {
         if (half == 0)
             blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = exact;
-        const float back = a.scale / grow;
+        const float back = a.scale / grow.by;
         short* to = d_q + head * out_head + row * out_token;
 #pragma unroll
         for (int e = 0; e < DIM / 32; ++e)
@@ -943,7 +933,7 @@ constexpr int KEYS_PER_GROUP = 128;
 // d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
 template <class Type, int DIM, int BEND>
 __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, const uint32_t* order, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
-                                                                const uint32_t* norms, uint32_t shares, float* parts, short* d_k,
+                                                                uint32_t shares, float* parts, short* d_k,
                                                                 int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
 {
     const HeadTile<DIM> lane_at(threadIdx.x % 64);
@@ -993,7 +983,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
     HeadLoader<RT, DIM, 4> ql, gl;
     ql.begin(a.q, a.dim, wave, lane);
     gl.begin(d_out, a.dim, wave, lane);
-    const float grow = gradient_scale<Type>(norms), grow_k = grow * (Type::wide_range ? 1.f : 0x1p-15f);
+    Growth<Type> grow; // of ds times 2^15, as it comes with p
     f32x16 ok[DIM / 32], ov[DIM / 32];
 #pragma unroll
     for (int e = 0; e < DIM / 32; ++e)
@@ -1053,12 +1043,13 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         const float slope2 = a.slope ? a.slope[head] * LOG2E : 0.f;
         const int row = tile * RT + 4 * half;
         score_gradients<BEND, false>(
-            a, s, dp, slope2, P_SHIFT<Type>, grow_k, masked, [&](int r) { return bs.lse2[4 * half + 8 * (r / 4) + r % 4]; },
+            a, s, dp, slope2, P_SHIFT<Type>, masked, [&](int r) { return bs.lse2[4 * half + 8 * (r / 4) + r % 4]; },
             [&](int r) { return bs.delta[4 * half + 8 * (r / 4) + r % 4]; }, [&](int r) { return static_cast<float>(row + 8 * (r / 4) + r % 4 - key); },
             [&](int r) {
                 const int at = 4 * half + 8 * (r / 4) + r % 4;
                 return key >= bs.lo[at] && key < bs.hi[at];
             });
+        grow.apply(dp, ok);
         if (FIRST)
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -1149,7 +1140,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         }
     }
     if (key < a.tokens && !(redo >> lane % 32 & 1)) {
-        const float back_k = a.scale / grow, back_v = Type::wide_range ? 1.f : 0x1p-15f;
+        const float back_v = Type::wide_range ? 1.f : 0x1p-15f, back_k = a.scale / grow.by * back_v;
         if (shares > 1) {
             float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
 #pragma unroll

@@ -39,3 +39,36 @@ def test_products_of_zero_under_a_small_cap(cap):
     want, size = v[:, 0].double().cumsum(0) / count, v[:, 0].double().abs().cumsum(0) / count
     within(out[:, 0], want, 1.1 * u * (size + want.abs()), "out")
     within(lse[0], count[:, 0].log(), 2e-5 * (1 + count[:, 0].log()), "lse")
+
+
+# ---- half precision ----
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,dim", [(400, 2, 2, 64), (400, 4, 2, 128), (1300, 2, 1, 96)])
+@pytest.mark.parametrize("what", ["padding", "documents", "heads", "rows"])
+def test_large_gradients_elsewhere_take_no_bits_in_half_precision(n, heads, kv_heads, dim, what):
+    """Every gradient is as exact as its own terms allow, whatever finite values stand in padding, in another document, in other heads or in later rows."""
+    g, dtype, u = gen(41), torch.float16, U[torch.float16]
+    q, k, v, d_out = (randn(g, n, h, dim, dtype=dtype) for h in (heads, kv_heads, kv_heads, heads))
+    at = torch.arange(n, device="cuda")
+    ends = torch.tensor([0, n // 3, n - 60], device="cuda")
+    lo, hi = ends[torch.searchsorted(ends, at, right=True) - 1].int(), (at + 1).int()
+    size = torch.full((n, heads, 1), 1e-3, device="cuda")
+    if what == "padding":
+        lo[n - 60:], hi[n - 60:] = 0, 0
+    elif what == "documents":
+        size[:n // 3] = 1e3
+    elif what == "heads":
+        size[:, 0] = 1e3
+    else:
+        size[n // 2::50] = 1e3
+    d_out = (d_out * size).half()
+    if what == "padding":
+        for x in (q, k, v, d_out):
+            x[n - 60:] = torch.where(x[n - 60:] > 0, 6e4, -6e4).half()
+    out, lse = cascade_amd.span_attention(q, k, v, lo, hi)
+    got = cascade_amd.span_attention_backward(d_out, q, k, v, out, lse, lo, hi)
+    want, sums = reference_attention(q, k, v, lo, hi, dim ** -0.5, 0.0, None, d_out, u)
+    for x, name in zip(got, ("d_q", "d_k", "d_v")):
+        # two roundings, and 32-bit sums of what is computed from 32-bit scores: 1e-6 of the terms, whose size `sums` / u bounds; half precision's last step
+        within(x, want[name], 1.1 * (sums[name] + u * want[name].abs()) + 2.0 ** -24, name)
