@@ -190,7 +190,8 @@ void forward(const csa_lm_attention& a, const AttentionWork& w, const csa_lm_hea
     if (order)
         tile_order_kernel<<<1, 1024, 0, s>>>(attention(a), nullptr, w.row_order, nullptr);
     attention_forward_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
-        attention(a), order ? w.row_order : nullptr, w.row_shares, w.row_parts, w.row_stats, static_cast<short*>(out.data), out.token_stride, out.head_stride, lse);
+        ForwardCall{attention(a), order ? w.row_order : nullptr, w.row_shares, w.row_parts, w.row_stats, static_cast<short*>(out.data), out.token_stride,
+                    out.head_stride, lse});
     if (w.row_shares > 1)
         join_rows_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
             w.row_parts, w.row_stats, w.row_shares, static_cast<int64_t>(a.tokens), static_cast<int>(a.head_dim), DIM, static_cast<short*>(out.data),
@@ -210,14 +211,14 @@ void backward(const csa_lm_attention& a, const csa_lm_heads& out, const float* l
     row_blocks_kernel<Type><<<dim3(tiles, a.q_heads), 256, 0, s>>>(at, heads(out), heads(d_out), lse, w.blocks);
     float* rests = reinterpret_cast<float*>(w.row_stats);
     attention_d_q_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, ROWS_PER_GROUP) * a.q_heads * w.row_shares), 256, 0, s>>>(
-        at, order ? w.row_order : nullptr, w.row_shares, w.row_parts, rests, heads(d_out), w.blocks, tiles, static_cast<short*>(d_q.data), d_q.token_stride,
-        d_q.head_stride);
+        QueryCall{at, order ? w.row_order : nullptr, w.row_shares, w.row_parts, rests, heads(d_out), w.blocks, tiles, static_cast<short*>(d_q.data),
+                  d_q.token_stride, d_q.head_stride});
     if (w.row_shares > 1)
         join_d_q_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.q_heads), 256, 0, s>>>(
             w.row_parts, rests, w.row_shares, at.tokens, at.dim, DIM, w.blocks, tiles, static_cast<short*>(d_q.data), d_q.token_stride, d_q.head_stride);
     attention_d_kv_kernel<Type, DIM, BEND><<<static_cast<uint32_t>(parts_of(a.tokens, KEYS_PER_GROUP) * a.kv_heads * w.shares), 256, 0, s>>>(
-        at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride,
-        static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride);
+        KeyCall{at, order ? w.key_order : nullptr, heads(d_out), w.blocks, w.bounds, tiles, w.shares, w.parts, static_cast<short*>(d_k.data), d_k.token_stride,
+                d_k.head_stride, static_cast<short*>(d_v.data), d_v.token_stride, d_v.head_stride});
     if (w.shares > 1)
         join_parts_kernel<Type><<<dim3(static_cast<uint32_t>(parts_of(a.tokens * (a.head_dim / 4), 256)), a.kv_heads, 2), 256, 0, s>>>(
             w.parts, w.shares, at.tokens, at.dim, DIM, static_cast<short*>(d_k.data), d_k.token_stride, d_k.head_stride, static_cast<short*>(d_v.data),

@@ -47,6 +47,29 @@ __device__ inline int again(int x)
     return x;
 }
 
+// The thread and the workgroup, for the first or the second time that a kernel does its work: the second one, which few calls need, makes all it needs by itself and
+// leaves the first one its registers.
+template <bool SECOND>
+__device__ inline int thread_id()
+{
+    return SECOND ? again(threadIdx.x) : threadIdx.x;
+}
+template <bool SECOND>
+__device__ inline uint32_t group_id()
+{
+    return SECOND ? __builtin_amdgcn_readfirstlane(again(blockIdx.x)) : blockIdx.x;
+}
+// A kernel's only argument, with which its argument segment begins, read once more.
+template <class Call>
+__device__ inline Call call_again()
+{
+    auto from = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(from));
+    Call call;
+    __builtin_memcpy(&call, from, sizeof(call));
+    return call;
+}
+
 template <int DIM>
 struct HeadTile {
     static constexpr int PIECES = DIM / 8;
@@ -240,8 +263,9 @@ __device__ inline float far_out(const Attention& a) { return fminf(a.cap / a.sca
 // ---- what a row may not see ----
 //
 // A score that a row may not see becomes a probability of 0, but 0 times an infinity or NaN that stands there is none. What no row of a workgroup sees is
-// not loaded at all (padding behind a text may hold anything); where a sum has become infinite or NaN all the same, it is done again one by one, over what
-// counts and nothing else: documents next to one that has gone wrong stay as they are.
+// not loaded at all (padding behind a text may hold anything). Where a sum has become infinite or NaN all the same, the workgroup goes through its tiles once more, what is
+// not finite in them replaced by zeros, and what sees nothing of that takes its second result: documents next to one that has gone wrong, and rows before a bad one, stay as
+// they are. What does see it keeps the first, infinite or NaN, perhaps in all its values. 4096 tokens, 8 heads of 128 values trained: 0.30 ms, with one infinite row of d_out 0.57, with nothing but NaN 0.89.
 
 template <int N>
 __device__ inline bool all_finite(const f32x16 (&x)[N])
@@ -256,41 +280,52 @@ __device__ inline bool all_finite(const f32x16 (&x)[N])
 }
 
 template <class Type>
-__device__ inline float dot_rows(const short* x, const short* y, int dim)
+__device__ inline bool is_finite(short x) // of a 16-bit pattern
 {
-    float sum = 0.f;
-    for (int d = 0; d < dim; d += 8) {
-        const s16x8 a = *reinterpret_cast<const s16x8*>(x + d), b = *reinterpret_cast<const s16x8*>(y + d);
+    return (x & Type::EXPONENT) != Type::EXPONENT;
+}
+__device__ inline bool is_finite(float x) { return x - x == 0.f; }
+
+// Whether a lane of any of the workgroup's four waves says so. `votes` is used once.
+__device__ inline bool anybody(bool mine, int (&votes)[4])
+{
+    const int some = __any(mine);
+    if (threadIdx.x % 64 == 0)
+        votes[threadIdx.x / 64] = some;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(votes[0] | votes[1] | votes[2] | votes[3]);
+}
+
+// Zeros in place of what is not finite in a tile of 64 keys, by all waves, and whether this lane's row, which sees [lo, hi), sees any of these keys.
+template <class Type, int DIM>
+__device__ inline bool clear_tile(short* tile, uint32_t (&bad)[2], int key0, int lo, int hi)
+{
+    const int me = threadIdx.x;
+    if (me < 2)
+        bad[me] = 0;
+    wait_for_lds();
+    meet();
+    for (int at = me; at < 64 * DIM / 8; at += 256) {
+        s16x8 x = read16(tile + at * 8);
+        bool fine = true;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            sum += to32<Type>(a[i]) * to32<Type>(b[i]);
+            if (!is_finite<Type>(x[i])) {
+                x[i] = 0;
+                fine = false;
+            }
+        if (!fine) {
+            const int key = at / (DIM / 8);
+            *reinterpret_cast<s16x8*>(tile + at * 8) = x;
+            atomicOr(bad + key / 32, 1u << key % 32);
+        }
     }
-    return sum;
+    wait_for_lds();
+    meet();
+    const uint64_t keys = bad[0] | static_cast<uint64_t>(bad[1]) << 32;
+    const int from = max(lo - key0, 0), to = min(hi - key0, 64);
+    return from < to && keys >> from << (64 - (to - from)) != 0;
 }
-
-// The exponent of 2 of one score, and what its gradient is multiplied by.
-__device__ inline float one_score(const Attention& a, float product, float slope2, float distance, float& bent)
-{
-    float z = product * a.scale * LOG2E;
-    bent = 1.f;
-    if (a.cap > CAP_PLAIN) {
-        product = bend_far(product, a.scale / a.cap, far_out(a));
-        z = product * a.scale * LOG2E;
-        bent = 1.f - product * (a.scale / a.cap) * (product * (a.scale / a.cap));
-    } else if (a.cap > 0.f) {
-        const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * near_in(a)));
-        z = a.cap * LOG2E * t;
-        bent = 1.f - t * t;
-    }
-    return z - slope2 * fabsf(distance);
-}
-
-__device__ inline const short* row_of(const Heads& h, uint32_t head, int64_t row)
-{
-    return static_cast<const short*>(h.data) + head * h.head + row * h.token;
-}
-
-__device__ inline float lane_of(float x, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane)); }
 
 constexpr int ROWS_PER_GROUP = 128, KEYS_PER_TILE = 64;
 
@@ -339,16 +374,38 @@ __device__ inline void bend(const Attention& a, f32x16 (&s)[TILES], float& unit,
     }
 }
 
-template <class Type, int DIM, int BEND>
-__global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float2* stats, short* out,
-                                                                   int64_t out_token, int64_t out_head, float* lse)
+struct ForwardCall {
+    Attention a;
+    const uint32_t* order;
+    uint32_t shares;
+    float* parts;
+    float2* stats;
+    short* out;
+    int64_t out_token;
+    int64_t out_head;
+    float* lse;
+};
+
+// The work of a workgroup, and whether the lane's row came out infinite or NaN. SECOND: once more for such rows (`lost`), with zeros in place of what is not finite.
+template <class Type, int DIM, int BEND, bool SECOND>
+__device__ __attribute__((always_inline)) inline bool forward_rows(const ForwardCall& call, short (&k0s)[KEYS_PER_TILE * DIM], short (&v0s)[KEYS_PER_TILE * DIM],
+    short (&k1s)[KEYS_PER_TILE * DIM], short (&v1s)[KEYS_PER_TILE * DIM], uint32_t (&bad)[2], bool lost)
 {
-    const HeadTile<DIM> lane_at(threadIdx.x % 64);
+    const Attention& a = call.a;
+    const uint32_t* const order = call.order;
+    const uint32_t shares = call.shares;
+    float* const parts = call.parts;
+    float2* const stats = call.stats;
+    short* const out = call.out;
+    const int64_t out_token = call.out_token;
+    const int64_t out_head = call.out_head;
+    float* const lse = call.lse;
+    const int thread = thread_id<SECOND>();
+    const HeadTile<DIM> lane_at(thread % 64);
     constexpr int KT = KEYS_PER_TILE;
-    __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
-    const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lane = thread % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(thread / 64);
     uint32_t unit, tile;
-    place_of(blockIdx.x, a.q_heads * shares, gridDim.x / (a.q_heads * shares), order, unit, tile);
+    place_of(group_id<SECOND>(), a.q_heads * shares, gridDim.x / (a.q_heads * shares), order, unit, tile);
     const uint32_t head = unit / shares;
     const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
 
@@ -378,8 +435,9 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
     for (int e = 0; e < DIM / 32; ++e)
         o[e] = f32x16{};
     float top = -3.0e38f, sum = 0.f; // the running maximum may lag behind by 2^8, which spares most rescalings
+    bool hit = false;                // the lane's row sees something that is not finite
 
-    auto turn = [&](const short* ks, const short* vs, int key0) {
+    auto turn = [&](const short* ks, const short* vs, int key0) __attribute__((always_inline)) {
         if (key0 + KT <= wave_lo || key0 >= wave_hi)
             return;
         const HeadTile<DIM> tiles_at = lane_at.afresh();
@@ -449,69 +507,42 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
             meet();
             kl.load(kb, key0 + KT, stop, k1s, wave);
             vl.load(vb, key0 + KT, stop, v1s, wave);
+            if (SECOND)
+                hit |= clear_tile<Type, DIM>(v0s, bad, key0, lo, hi);
             turn(k0s, v0s, key0);
             wait_for_all();
             meet();
             kl.load(kb, key0 + 2 * KT, stop, k0s, wave);
             vl.load(vb, key0 + 2 * KT, stop, v0s, wave);
-            if (key0 + KT < stop)
+            if (key0 + KT < stop) {
+                if (SECOND)
+                    hit |= clear_tile<Type, DIM>(v1s, bad, key0 + KT, lo, hi);
                 turn(k1s, v1s, key0 + KT);
+            }
         }
         wait_for_all();
     }
     sum += other_half(sum);
-    // shares leave their sums as they are, for the kernel that joins them
-    const float share = shares > 1 ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    float* part = parts + (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens * DIM;
-    const uint64_t lost = __ballot(!all_finite(o));
-    const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
-    for (uint32_t left = redo; left; left &= left - 1) {
-        const int r = __builtin_ctz(left);
-        const int64_t i = first + wave * 32 + r;
-        if (i >= a.tokens)
-            continue;
-        const int from = max(start, __builtin_amdgcn_readlane(lo, r)), to = min(stop, __builtin_amdgcn_readlane(hi, r));
-        const float high = lane_of(top, r), factor = lane_of(share, r);
-        float x = 0.f, y = 0.f;
-        for (int j0 = from; j0 < to; j0 += 64) {
-            const int j = j0 + lane, count = min(64, to - j0);
-            float bent, p = 0.f;
-            if (j < to)
-                p = __builtin_amdgcn_exp2f(one_score(a, dot_rows<Type>(row_of(a.q, head, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent) - high) * factor;
-            for (int c = 0; c < count; ++c) {
-                const short* v = row_of(a.v, kv, j0 + c);
-                const float pc = lane_of(p, c);
-                x += lane < a.dim ? pc * to32<Type>(v[lane]) : 0.f;
-                y += lane + 64 < a.dim ? pc * to32<Type>(v[lane + 64]) : 0.f;
-            }
-        }
-        for (int upper = 0; upper < 2; ++upper) {
-            const int d = lane + 64 * upper;
-            if (d >= a.dim)
-                continue;
-            if (shares > 1)
-                part[i * DIM + d] = upper ? y : x;
-            else
-                out[head * out_head + i * out_token + d] = to16<Type>(upper ? y : x);
-        }
-    }
-    if (row < a.tokens && shares > 1) {
-        if (!(redo >> lane % 32 & 1))
+    const bool mine = row < a.tokens && (!SECOND || (lost && !hit));
+    const int64_t place = (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row;
+    if (mine && shares > 1) { // shares leave their sums as they are, for the kernel that joins them
 #pragma unroll
-            for (int e = 0; e < DIM / 32; ++e)
+        for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(part + row * DIM + 32 * e + 8 * g + 4 * half) = f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]};
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(parts + place * DIM + 32 * e + 8 * g + 4 * half) = f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]};
         if (half == 0)
-            stats[(static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row] = make_float2(top, sum);
-    } else if (row < a.tokens) {
+            stats[place] = make_float2(top, sum);
+    } else if (mine) {
+        const bool any = sum > 0.f || sum != sum;
+        const float share = any ? 1.f / sum : 0.f;
         short* to = out + head * out_head + row * out_token;
 #pragma unroll
         for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * e + 8 * g + 4 * half;
-                if (d < a.dim && !(redo >> lane % 32 & 1)) {
+                if (d < a.dim) {
                     s16x4 y;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -520,8 +551,22 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(Attention a, 
                 }
             }
         if (half == 0)
-            lse[head * a.tokens + row] = sum > 0.f || sum != sum ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
+            lse[head * a.tokens + row] = any ? (top + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
     }
+    lost = !all_finite(o);
+    return lost || other_half(lost ? 1.f : 0.f) != 0.f;
+}
+
+template <class Type, int DIM, int BEND>
+__global__ __launch_bounds__(256, 2) void attention_forward_kernel(ForwardCall call)
+{
+    constexpr int KT = KEYS_PER_TILE;
+    __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
+    __shared__ uint32_t bad[2];
+    __shared__ int votes[4];
+    const bool lost = forward_rows<Type, DIM, BEND, false>(call, k0s, v0s, k1s, v1s, bad, false);
+    if (anybody(lost, votes))
+        forward_rows<Type, DIM, BEND, true>(call_again<ForwardCall>(), k0s, v0s, k1s, v1s, bad, lost);
 }
 
 // out and lse of a row from its shares, four values a thread: sums of exponentials of different maxima.
@@ -711,6 +756,8 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
             const bool there = seen(r);
             s[r] = there ? s[r] : -INFINITY;
             dp[r] = there ? dp[r] : 0.f;
+            if (REST && BEND != STRAIGHT)
+                bent[r] = there ? bent[r] : 0.f;
         }
     }
 #pragma unroll
@@ -732,16 +779,42 @@ __device__ inline float score_gradients(const Attention& a, f32x16& s, f32x16& d
     return sum;
 }
 
-template <class Type, int DIM, int BEND>
-__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, const uint32_t* order, uint32_t shares, float* parts, float* rests, Heads d_out,
-                                                               RowBlock* blocks, uint32_t blocks_per_head, short* d_q, int64_t out_token, int64_t out_head)
+struct QueryCall {
+    Attention a;
+    const uint32_t* order;
+    uint32_t shares;
+    float* parts;
+    float* rests;
+    Heads d_out;
+    RowBlock* blocks;
+    uint32_t blocks_per_head;
+    short* d_q;
+    int64_t out_token;
+    int64_t out_head;
+};
+
+// The work of a workgroup, and whether the lane's row came out infinite or NaN. SECOND: once more for such rows (`lost`), with zeros in place of what is not finite.
+template <class Type, int DIM, int BEND, bool SECOND>
+__device__ __attribute__((always_inline)) inline bool d_q_rows(const QueryCall& call, short (&k0s)[KEYS_PER_TILE * DIM], short (&v0s)[KEYS_PER_TILE * DIM],
+    short (&k1s)[KEYS_PER_TILE * DIM], short (&v1s)[KEYS_PER_TILE * DIM], uint32_t (&bad)[2], bool lost)
 {
-    const HeadTile<DIM> lane_at(threadIdx.x % 64);
+    const Attention& a = call.a;
+    const uint32_t* const order = call.order;
+    const uint32_t shares = call.shares;
+    float* const parts = call.parts;
+    float* const rests = call.rests;
+    const Heads& d_out = call.d_out;
+    RowBlock* const blocks = call.blocks;
+    const uint32_t blocks_per_head = call.blocks_per_head;
+    short* const d_q = call.d_q;
+    const int64_t out_token = call.out_token;
+    const int64_t out_head = call.out_head;
+    const int thread = thread_id<SECOND>();
+    const HeadTile<DIM> lane_at(thread % 64);
     constexpr int KT = KEYS_PER_TILE;
-    __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
-    const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lane = thread % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(thread / 64);
     uint32_t unit, tile;
-    place_of(blockIdx.x, a.q_heads * shares, gridDim.x / (a.q_heads * shares), order, unit, tile);
+    place_of(group_id<SECOND>(), a.q_heads * shares, gridDim.x / (a.q_heads * shares), order, unit, tile);
     const uint32_t head = unit / shares;
     const int64_t first = static_cast<int64_t>(tile) * ROWS_PER_GROUP, row = first + wave * 32 + lane % 32;
     int lo, hi, l2, h2;
@@ -761,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
     if (row < a.tokens) {
         const RowBlock& b = blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS];
         lse2 = b.lse2[row % BLOCK_ROWS];
-        delta = b.delta[row % BLOCK_ROWS];
+        delta = b.delta[row % BLOCK_ROWS]; // the second time it is the corrected one, if this kernel corrects it
     }
     const uint32_t kv = head / a.group;
     const char* kb = reinterpret_cast<const char*>(static_cast<const short*>(a.k.data) + kv * a.k.head);
@@ -775,9 +848,10 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
     for (int e = 0; e < DIM / 32; ++e)
         o[e] = f32x16{};
     float rest = 0.f; // sum of p (dp - D), which would be 0 if D were exact
+    bool hit = false; // the lane's row sees something that is not finite
     Growth<Type> grow;
 
-    auto turn = [&](const short* ks, const short* vs, int key0) {
+    auto turn = [&](const short* ks, const short* vs, int key0) __attribute__((always_inline)) {
         if (key0 + KT <= wave_lo || key0 >= wave_hi)
             return;
         const bool masked = key0 < all_lo || key0 + KT > all_hi;
@@ -819,76 +893,44 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
             meet();
             kl.load(kb, key0 + KT, stop, k1s, wave);
             vl.load(vb, key0 + KT, stop, v1s, wave);
+            if (SECOND)
+                hit |= clear_tile<Type, DIM>(k0s, bad, key0, lo, hi);
             turn(k0s, v0s, key0);
             wait_for_all();
             meet();
             kl.load(kb, key0 + 2 * KT, stop, k0s, wave);
             vl.load(vb, key0 + 2 * KT, stop, v0s, wave);
-            if (key0 + KT < stop)
+            if (key0 + KT < stop) {
+                if (SECOND)
+                    hit |= clear_tile<Type, DIM>(k1s, bad, key0 + KT, lo, hi);
                 turn(k1s, v1s, key0 + KT);
+            }
         }
         wait_for_all();
     }
     rest += other_half(rest);
-    // A share knows only its own part of what D is off by: its d_q is the one of the rounded D, and the kernel that joins them corrects D for the
-    // kernel of d_k alone.
-    const float exact = shares > 1 ? delta : delta + rest;
-    float* part = parts + (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens * DIM;
-    const uint64_t lost = __ballot(!all_finite(o));
-    const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
-    for (uint32_t left = redo; left; left &= left - 1) {
-        const int r = __builtin_ctz(left);
-        const int64_t i = first + wave * 32 + r;
-        if (i >= a.tokens)
-            continue;
-        const int from = max(start, __builtin_amdgcn_readlane(lo, r)), to = min(stop, __builtin_amdgcn_readlane(hi, r));
-        const float base = lane_of(lse2, r), mean = lane_of(exact, r);
-        float x = 0.f, y = 0.f;
-        for (int j0 = from; j0 < to; j0 += 64) {
-            const int j = j0 + lane, count = min(64, to - j0);
-            float bent, ds = 0.f;
-            if (j < to) {
-                const float z = one_score(a, dot_rows<Type>(row_of(a.q, head, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent);
-                ds = __builtin_amdgcn_exp2f(z - base) * (dot_rows<Type>(row_of(d_out, head, i), row_of(a.v, kv, j), a.dim) - mean) * bent * a.scale;
-            }
-            for (int c = 0; c < count; ++c) {
-                const short* k = row_of(a.k, kv, j0 + c);
-                const float dc = lane_of(ds, c);
-                x += lane < a.dim ? dc * to32<Type>(k[lane]) : 0.f;
-                y += lane + 64 < a.dim ? dc * to32<Type>(k[lane + 64]) : 0.f;
-            }
-        }
-        for (int upper = 0; upper < 2; ++upper) {
-            const int d = lane + 64 * upper;
-            if (d >= a.dim)
-                continue;
-            if (shares > 1)
-                part[i * DIM + d] = upper ? y : x;
-            else
-                d_q[head * out_head + i * out_token + d] = to16<Type>(upper ? y : x);
-        }
-    }
-    if (row < a.tokens && shares > 1) {
-        if (!(redo >> lane % 32 & 1))
+    const bool mine = row < a.tokens && (!SECOND || (lost && !hit));
+    const float back = a.scale / grow.by;
+    const int64_t place = (static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row;
+    if (mine && shares > 1) { // A share knows only its own part of what D is off by: the kernel that joins them corrects D for the kernel of d_k.
 #pragma unroll
-            for (int e = 0; e < DIM / 32; ++e)
+        for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(part + row * DIM + 32 * e + 8 * g + 4 * half) =
-                        f32x4{o[e][4 * g], o[e][4 * g + 1], o[e][4 * g + 2], o[e][4 * g + 3]} * (a.scale / grow.by);
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<f32x4*>(parts + place * DIM + 32 * e + 8 * k + 4 * half) =
+                    f32x4{o[e][4 * k], o[e][4 * k + 1], o[e][4 * k + 2], o[e][4 * k + 3]} * back;
         if (half == 0)
-            rests[(static_cast<int64_t>(unit % shares) * a.q_heads + head) * a.tokens + row] = rest;
-    } else if (row < a.tokens) {
+            rests[place] = rest;
+    } else if (mine) {
         if (half == 0)
-            blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = exact;
-        const float back = a.scale / grow.by;
+            blocks[static_cast<int64_t>(head) * blocks_per_head + row / BLOCK_ROWS].delta[row % BLOCK_ROWS] = delta + rest;
         short* to = d_q + head * out_head + row * out_token;
 #pragma unroll
         for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int d = 32 * e + 8 * k + 4 * half;
-                if (d < a.dim && !(redo >> lane % 32 & 1)) {
+                if (d < a.dim) {
                     s16x4 y;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -897,6 +939,20 @@ __global__ __launch_bounds__(256, 2) void attention_d_q_kernel(Attention a, cons
                 }
             }
     }
+    lost = !all_finite(o);
+    return lost || other_half(lost ? 1.f : 0.f) != 0.f;
+}
+
+template <class Type, int DIM, int BEND>
+__global__ __launch_bounds__(256, 2) void attention_d_q_kernel(QueryCall call)
+{
+    constexpr int KT = KEYS_PER_TILE;
+    __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
+    __shared__ uint32_t bad[2];
+    __shared__ int votes[4];
+    const bool lost = d_q_rows<Type, DIM, BEND, false>(call, k0s, v0s, k1s, v1s, bad, false);
+    if (anybody(lost, votes))
+        d_q_rows<Type, DIM, BEND, true>(call_again<QueryCall>(), k0s, v0s, k1s, v1s, bad, lost);
 }
 
 // d_q of a row from its shares, four values a thread, and D of the row corrected.
@@ -931,23 +987,52 @@ constexpr int KEYS_PER_GROUP = 128;
 
 // The workgroup's 128 keys by 32 rows a turn, 32 keys a wave. Two waves of a SIMD have 256 registers each: at 128 values a head the sums of d_k and
 // d_v take 128 of them, the wave's keys 32 and the scores 32; the wave's values therefore stay in LDS and are read again every turn.
-template <class Type, int DIM, int BEND>
-__global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, const uint32_t* order, Heads d_out, const RowBlock* blocks, const int2* bounds, uint32_t tiles,
-                                                                uint32_t shares, float* parts, short* d_k,
-                                                                int64_t dk_token, int64_t dk_head, short* d_v, int64_t dv_token, int64_t dv_head)
+struct KeyCall {
+    Attention a;
+    const uint32_t* order;
+    Heads d_out;
+    const RowBlock* blocks;
+    const int2* bounds;
+    uint32_t tiles;
+    uint32_t shares;
+    float* parts;
+    short* d_k;
+    int64_t dk_token;
+    int64_t dk_head;
+    short* d_v;
+    int64_t dv_token;
+    int64_t dv_head;
+};
+
+template <class Type, int DIM, int BEND, bool SECOND>
+__device__ __attribute__((always_inline)) inline bool d_kv_keys(const KeyCall& call, short (&q0s)[BLOCK_ROWS * DIM], short (&g0s)[BLOCK_ROWS * DIM],
+    short (&q1s)[BLOCK_ROWS * DIM], short (&g1s)[BLOCK_ROWS * DIM], short (&vs)[KEYS_PER_GROUP * DIM], RowBlock (&b0s)[2], RowBlock (&b1s)[2], int (&ends)[8],
+    bool lost)
 {
-    const HeadTile<DIM> lane_at(threadIdx.x % 64);
+    const Attention& a = call.a;
+    const uint32_t* const order = call.order;
+    const Heads& d_out = call.d_out;
+    const RowBlock* const blocks = call.blocks;
+    const int2* const bounds = call.bounds;
+    const uint32_t tiles = call.tiles;
+    const uint32_t shares = call.shares;
+    float* const parts = call.parts;
+    short* const d_k = call.d_k;
+    const int64_t dk_token = call.dk_token;
+    const int64_t dk_head = call.dk_head;
+    short* const d_v = call.d_v;
+    const int64_t dv_token = call.dv_token;
+    const int64_t dv_head = call.dv_head;
+    const int thread = thread_id<SECOND>();
+    const HeadTile<DIM> lane_at(thread % 64);
     constexpr int RT = BLOCK_ROWS;
     // A wave goes first while it feeds the matrix unit. Whole calls: 12289 tokens, 16 heads of 128 values 2.98 -> 2.94 ms; 8000 tokens, 16 heads of 96 1.060 -> 1.037;
     // with 64 values it costs: 20000 tokens, 8 heads 2.17 -> 2.28 ms; 3001 tokens, 12 heads 174 -> 181 us. The other two kernels gain nothing by it.
     constexpr bool FIRST = DIM > 64;
-    __shared__ __attribute__((aligned(16))) short q0s[RT * DIM], g0s[RT * DIM], q1s[RT * DIM], g1s[RT * DIM], vs[KEYS_PER_GROUP * DIM];
-    __shared__ __attribute__((aligned(16))) RowBlock b0s[2], b1s[2]; // the second of each is where the load's other half wave puts zeros
-    __shared__ int ends[8];
-    const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lane = thread % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(thread / 64);
     const uint32_t kv_heads = a.q_heads / a.group, units = kv_heads * shares;
     uint32_t unit, which;
-    place_of(blockIdx.x, units, gridDim.x / units, order, unit, which);
+    place_of(group_id<SECOND>(), units, gridDim.x / units, order, unit, which);
     if (!order)
         which = gridDim.x / units - 1 - which; // the first keys, which most rows of a causal text see, first
     const uint32_t kv = unit / shares;
@@ -956,7 +1041,7 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
 
     // The first and the last tile of rows that sees any of these keys.
     int from = NONE, to = -1;
-    for (uint32_t t = threadIdx.x; t < tiles; t += 256) {
+    for (uint32_t t = thread; t < tiles; t += 256) {
         const int2 b = bounds[t];
         if (b.x < last && b.y > first) {
             from = min(from, static_cast<int>(t));
@@ -995,9 +1080,8 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
     const int begin = static_cast<int>(turns * share / shares), mine = static_cast<int>(turns * (share + 1) / shares) - begin;
     const uint32_t first_head = kv * a.group + (count ? begin / count : 0);
     const int first_tile = from + (count ? begin % count : 0);
-    int to_load = mine;
+    int to_load = mine, load_tile = first_tile;
     uint32_t load_head = first_head;
-    int load_tile = first_tile;
     auto load = [&](short* qs, short* gs, RowBlock* bs) {
         const bool there = to_load > 0;
         const int64_t row0 = there ? static_cast<int64_t>(load_tile) * RT : a.tokens; // past the last one: an empty window
@@ -1012,15 +1096,39 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
     };
     uint32_t head = first_head;
     int tile = first_tile;
-    auto turn = [&](short* qs, short* gs, const RowBlock& bs) {
+    bool hit = false; // a row that sees the lane's key is not finite
+    auto turn = [&](short* qs, short* gs, RowBlock& bs) __attribute__((always_inline)) {
         // which of the rows see any of the wave's 32 keys, and which do not see all of them
         const int lo = bs.lo[lane % 32], hi = bs.hi[lane % 32];
-        // Rows that see nothing may hold anything: they become zeros, by all waves, before the tile is used.
-        if (uint32_t empty = static_cast<uint32_t>(__ballot(lo == NONE && tile * RT + lane % 32 < static_cast<int>(a.tokens)))) {
+        // Rows that see nothing may hold anything: they become zeros, by all waves, before the tile is used. The second time so do rows that are not finite.
+        bool out = lo == NONE && tile * RT + lane % 32 < static_cast<int>(a.tokens);
+        if (SECOND) {
+            const int r = lane % 32;
+            bool fine = lo == NONE || (is_finite(bs.lse2[r]) && is_finite(bs.delta[r]));
+            for (int d = 0; d < DIM && lo != NONE; d += 8) {
+                const s16x8 x = read16((half ? gs : qs) + r * DIM + d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    fine &= is_finite<Type>(x[i]);
+            }
+            const uint64_t gone = __ballot(!fine);
+            for (uint32_t rows = static_cast<uint32_t>(gone | gone >> 32); rows; rows &= rows - 1) {
+                const int c = __builtin_ctz(rows);
+                hit |= key >= bs.lo[c] && key < bs.hi[c];
+                out |= c == r;
+            }
+        }
+        if (uint32_t empty = static_cast<uint32_t>(__ballot(out))) {
+            if (SECOND)
+                meet(); // everybody has looked at the rows
             for (; empty; empty &= empty - 1) {
-                const int at = __builtin_ctz(empty) * DIM + static_cast<int>(threadIdx.x % (DIM / 8)) * 8;
-                if (threadIdx.x < DIM / 4)
-                    *reinterpret_cast<s16x8*>((threadIdx.x < DIM / 8 ? qs : gs) + at) = s16x8{};
+                const int r = __builtin_ctz(empty), at = r * DIM + static_cast<int>(thread % (DIM / 8)) * 8;
+                if (thread < DIM / 4)
+                    *reinterpret_cast<s16x8*>((thread < DIM / 8 ? qs : gs) + at) = s16x8{};
+                if (SECOND && thread == 0) {
+                    bs.lse2[r] = INFINITY;
+                    bs.delta[r] = 0.f;
+                }
             }
             wait_for_lds();
             meet();
@@ -1088,77 +1196,25 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
         }
     }
     wait_for_all();
-    const uint64_t lost = __ballot(!all_finite(ok) || !all_finite(ov));
-    const uint32_t redo = static_cast<uint32_t>(lost | lost >> 32);
-    for (uint32_t left = redo; left; left &= left - 1) {
-        const int j = wave_key + __builtin_ctz(left);
-        if (j >= a.tokens)
-            continue;
-        float kx = 0.f, ky = 0.f, vx = 0.f, vy = 0.f;
-        uint32_t h = first_head;
-        int t = first_tile;
-        for (int n = 0; n < mine; ++n) {
-            const float slope2 = a.slope ? a.slope[h] * LOG2E : 0.f;
-            const RowBlock& b = blocks[static_cast<int64_t>(h) * tiles + t];
-            const int r = lane % 32, i = t * RT + r;
-            const bool sees = lane < 32 && b.lo[r] <= j && j < b.hi[r];
-            float bent, p = 0.f, ds = 0.f;
-            if (sees) {
-                const float z = one_score(a, dot_rows<Type>(row_of(a.q, h, i), row_of(a.k, kv, j), a.dim), slope2, static_cast<float>(i - j), bent);
-                p = __builtin_amdgcn_exp2f(z - b.lse2[r]);
-                ds = p * (dot_rows<Type>(row_of(d_out, h, i), row_of(a.v, kv, j), a.dim) - b.delta[r]) * bent * a.scale;
-            }
-            for (uint32_t rows = static_cast<uint32_t>(__ballot(sees)); rows; rows &= rows - 1) {
-                const int c = __builtin_ctz(rows);
-                const short *q = row_of(a.q, h, t * RT + c), *g = row_of(d_out, h, t * RT + c);
-                const float pc = lane_of(p, c), dc = lane_of(ds, c);
-                if (lane < a.dim) {
-                    kx += dc * to32<Type>(q[lane]);
-                    vx += pc * to32<Type>(g[lane]);
-                }
-                if (lane + 64 < a.dim) {
-                    ky += dc * to32<Type>(q[lane + 64]);
-                    vy += pc * to32<Type>(g[lane + 64]);
-                }
-            }
-            h += t == to;
-            t = t < to ? t + 1 : from;
-        }
-        for (int half64 = 0; half64 < 2; ++half64) {
-            const int d = lane + 64 * half64;
-            const float gk = half64 ? ky : kx, gv = half64 ? vy : vx;
-            if (d >= a.dim)
-                continue;
-            if (shares > 1) {
-                float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + j) * DIM + d;
-                part[0] = gk;
-                part[a.tokens * DIM] = gv;
-            } else {
-                d_k[kv * dk_head + static_cast<int64_t>(j) * dk_token + d] = to16<Type>(gk);
-                d_v[kv * dv_head + static_cast<int64_t>(j) * dv_token + d] = to16<Type>(gv);
-            }
-        }
-    }
-    if (key < a.tokens && !(redo >> lane % 32 & 1)) {
-        const float back_v = Type::wide_range ? 1.f : 0x1p-15f, back_k = a.scale / grow.by * back_v;
-        if (shares > 1) {
-            float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
+    const bool writes = key < a.tokens && (!SECOND || (lost && !hit));
+    const float back_v = Type::wide_range ? 1.f : 0x1p-15f, back_k = a.scale / grow.by * back_v;
+    if (writes && shares > 1) {
+        float* part = parts + (static_cast<int64_t>(unit) * 2 * a.tokens + key) * DIM;
 #pragma unroll
-            for (int e = 0; e < DIM / 32; ++e)
+        for (int e = 0; e < DIM / 32; ++e)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    f32x4 y, z;
+            for (int x = 0; x < 4; ++x) {
+                f32x4 y, z;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        y[i] = ok[e][4 * x + i] * back_k;
-                        z[i] = ov[e][4 * x + i] * back_v;
-                    }
-                    const int d = 32 * e + 8 * x + 4 * half;
-                    *reinterpret_cast<f32x4*>(part + d) = y;
-                    *reinterpret_cast<f32x4*>(part + a.tokens * DIM + d) = z;
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = ok[e][4 * x + i] * back_k;
+                    z[i] = ov[e][4 * x + i] * back_v;
                 }
-            return;
-        }
+                const int d = 32 * e + 8 * x + 4 * half;
+                *reinterpret_cast<f32x4*>(part + d) = y;
+                *reinterpret_cast<f32x4*>(part + a.tokens * DIM + d) = z;
+            }
+    } else if (writes) {
         short* kt = d_k + kv * dk_head + static_cast<int64_t>(key) * dk_token;
         short* vt = d_v + kv * dv_head + static_cast<int64_t>(key) * dv_token;
 #pragma unroll
@@ -1178,6 +1234,20 @@ __global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(Attention a, con
                 }
             }
     }
+    lost = !all_finite(ok) || !all_finite(ov);
+    return lost || other_half(lost ? 1.f : 0.f) != 0.f;
+}
+
+template <class Type, int DIM, int BEND>
+__global__ __launch_bounds__(256, 2) void attention_d_kv_kernel(KeyCall call)
+{
+    constexpr int RT = BLOCK_ROWS;
+    __shared__ __attribute__((aligned(16))) short q0s[RT * DIM], g0s[RT * DIM], q1s[RT * DIM], g1s[RT * DIM], vs[KEYS_PER_GROUP * DIM];
+    __shared__ __attribute__((aligned(16))) RowBlock b0s[2], b1s[2]; // the second of each is where the load's other half wave puts zeros
+    __shared__ int ends[8], votes[4];
+    const bool lost = d_kv_keys<Type, DIM, BEND, false>(call, q0s, g0s, q1s, g1s, vs, b0s, b1s, ends, false);
+    if (anybody(lost, votes))
+        d_kv_keys<Type, DIM, BEND, true>(call_again<KeyCall>(), q0s, g0s, q1s, g1s, vs, b0s, b1s, ends, lost);
 }
 
 // The order of tiles by work, most first, for texts whose spans are given: documents differ in length by more than workgroups can make up for by

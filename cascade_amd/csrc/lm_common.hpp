@@ -18,6 +18,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct Bf16 {
     typedef bf16_t value;
     static constexpr bool wide_range = true; // exponents of 32 bits: gradients need no scale
+    static constexpr short EXPONENT = 0x7f80;
     static __device__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c)
     {
         typedef bf16_t v8 __attribute__((ext_vector_type(8)));
@@ -27,6 +28,7 @@ struct Bf16 {
 struct F16 {
     typedef f16_t value;
     static constexpr bool wide_range = false;
+    static constexpr short EXPONENT = 0x7c00;
     static __device__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c)
     {
         typedef f16_t v8 __attribute__((ext_vector_type(8)));

@@ -66,6 +66,9 @@ typedef struct csa_lm_attention {
     csa_lm_heads q, k, v;
 } csa_lm_attention;
 
+/* Infinities and NaN reach the rows that see them and the keys that such rows see, which may become infinite or NaN in all their values, and nothing else:
+ * padding and other documents may hold anything. */
+
 /* out = the softmax over each row's span times v (zeros for rows that see nothing), d_lse[h * tokens + i] = the
  * logarithm of the sum of exponentials of row i's scores (-infinity for rows that see nothing). */
 uint64_t csa_lm_attention_workspace(uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t flags);

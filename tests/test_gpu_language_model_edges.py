@@ -72,3 +72,80 @@ def test_large_gradients_elsewhere_take_no_bits_in_half_precision(n, heads, kv_h
     for x, name in zip(got, ("d_q", "d_k", "d_v")):
         # two roundings, and 32-bit sums of what is computed from 32-bit scores: 1e-6 of the terms, whose size `sums` / u bounds; half precision's last step
         within(x, want[name], 1.1 * (sums[name] + u * want[name].abs()) + 2.0 ** -24, name)
+
+
+# ---- infinities and NaN ----
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "d_out"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("mask,n,heads,kv_heads,dim,dtype", [("window", 700, 2, 1, 64, torch.bfloat16), ("documents", 900, 2, 2, 128, torch.float16),
+                                                             ("causal", 600, 4, 2, 96, torch.bfloat16), ("window", 1700, 1, 1, 128, torch.float16)])
+def test_a_bad_token_reaches_what_sees_it_and_nothing_else(which, value, mask, n, heads, kv_heads, dim, dtype):
+    g = gen(51)
+    x = {"q": randn(g, n, heads, dim, dtype=dtype), "k": randn(g, n, kv_heads, dim, dtype=dtype), "v": randn(g, n, kv_heads, dim, dtype=dtype),
+         "d_out": randn(g, n, heads, dim, dtype=dtype)}
+    lo, hi = spans_for(mask, n, g)
+    at = torch.arange(n, device="cuda")
+    low = torch.zeros_like(at) if lo is None else lo
+    high = at + 1 if hi is None else hi
+    seen = (at >= low[:, None]) & (at < high[:, None])
+
+    def once(how):
+        q, k, v, d_out = (x[name] for name in ("q", "k", "v", "d_out"))
+        out, lse = cascade_amd.span_attention(q, k, v, lo, hi, **how)
+        return out, lse.T[..., None], *cascade_amd.span_attention_backward(d_out, q, k, v, out, lse, lo, hi, **how)
+    for how in ({}, {"cap": 20.0, "slopes": torch.linspace(0.01, 0.1, heads, device="cuda")}, {"cap": 1e3}):
+        clean = once(how)
+        good = x[which].clone()
+        bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+        bad[n // 2], bad[n // 2 + 70] = True, True
+        x[which][bad, 0, 5] = value
+        got = once(how)
+        x[which] = good
+        # rows that are bad or see a bad key, and keys that are bad or that such a row sees
+        rows = bad if which in ("q", "d_out") else (seen & bad).any(1)
+        keys = (seen & rows[:, None]).any(0) | (bad if which in ("k", "v") else torch.zeros_like(bad))
+        for name, a, b in zip(("out", "lse", "d_q", "d_k", "d_v"), got, clean):
+            reached = keys if name in ("d_k", "d_v") else rows if which != "d_out" or name == "d_q" else torch.zeros_like(rows)
+            # the rest is the same but for the moments at which a running maximum was raised, that is two roundings of the type at most, of the largest terms
+            assert torch.isfinite(a[~reached]).all(), name
+            assert ((a - b)[~reached].abs() <= (4 * U[dtype] if name != "lse" else 2e-5) * b.abs().max()).all(), name
+            if math.isnan(value) and (name != "lse" or which != "v") and (name != "d_v" or which != "v"):
+                first = a[:, :1] if name in ("d_k", "d_v") or which in ("q", "d_out") else a
+                assert (~torch.isfinite(first[reached])).any(-1).any(-1).all(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", ["one row of d_out", "one key", "everything"])
+def test_a_step_that_has_overflowed_takes_no_longer_than_a_few(dtype, bad):
+    """By the tiles that are gone through twice it takes up to three times as long as any other; ten times leave room for a busy machine."""
+    g, n = gen(52), 4096
+    q, k, v, d_out = (randn(g, n, h, 128, dtype=dtype) for h in (8, 2, 2, 8))
+
+    def step():
+        out, lse = cascade_amd.span_attention(q, k, v)
+        return (out, *cascade_amd.span_attention_backward(d_out, q, k, v, out, lse))
+
+    def fastest():
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            step()
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    usual = fastest()
+    if bad == "one row of d_out":
+        d_out[n - 5] = math.inf
+    elif bad == "one key":
+        k[3], v[3] = math.nan, math.inf
+    else:
+        for x in (q, k, v, d_out):
+            x.fill_(math.nan)
+    overflowed = fastest()
+    print(f"{bad}: {1000 * usual:.0f} us, {1000 * overflowed:.0f} us")
+    assert not all(torch.isfinite(x).all() for x in step())
+    assert overflowed <= 10 * usual
