@@ -32,6 +32,8 @@ int launched(const char* who)
 
 uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 uint64_t parts_of(uint64_t x, uint64_t size) { return (x + size - 1) / size; }
+// HIP starts fewer than 2^32 threads along an axis. What would need more is refused before the call's first launch.
+bool launchable(uint64_t groups, uint64_t threads) { return groups < (1ull << 32) / threads; }
 bool aligned(const void* p, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 // Hands out the pieces of a workspace, or only adds them up.
@@ -75,7 +77,7 @@ int check_heads(const char* who, const char* what, const csa_lm_heads& h, const 
     return CSA_OK;
 }
 
-int check_attention(const char* who, const csa_lm_attention* a)
+int check_attention(const char* who, const csa_lm_attention* a, bool backward)
 {
     if (!a)
         return fail(CSA_ERR_ARG, "%s: null description", who);
@@ -99,8 +101,7 @@ int check_attention(const char* who, const csa_lm_attention* a)
         if (int rc = check_heads(who, "v", a->v, *a))
             return rc;
     }
-    const uint64_t groups = parts_of(a->tokens, ROWS_PER_GROUP) * a->q_heads;
-    if (groups > 0x7fffffffu || parts_of(a->tokens, BLOCK_ROWS) * a->q_heads > 0x7fffffffu)
+    if (!launchable(parts_of(a->tokens, ROWS_PER_GROUP) * a->q_heads, 256) || (backward && !launchable(parts_of(a->tokens, BLOCK_ROWS), 256)))
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens of %u heads", who, (unsigned long long)a->tokens, a->q_heads);
     return CSA_OK;
 }
@@ -276,6 +277,7 @@ using NarrowHidden = Product<Type, 64, 256, 1, 4, false, true>;
 
 constexpr uint64_t UNITS = 256;               // compute units
 constexpr uint64_t PIECE_BYTES = 256ull << 20; // of P
+constexpr uint64_t PIECE_TILES = 8192;         // of 256 words: 256 rows of P, of half as much again at most, lie within 2^31 bytes
 constexpr uint64_t SHARE_BYTES = 128ull << 20; // of d_hidden's shares beside the first
 
 struct EntropyPlan {
@@ -287,7 +289,8 @@ struct EntropyPlan {
         padded_dim = up(dim, 8);
         const uint64_t tiles256 = parts_of(vocab, 256);
         narrow_logits = tokens * vocab * 2 < up(tiles256 * parts_of(tokens, 256), UNITS) * 65536;
-        const uint64_t fit = PIECE_BYTES / (512 * (tokens ? tokens : 1)), per = fit && fit < tiles256 ? fit : fit ? tiles256 : 1;
+        const uint64_t fit = PIECE_BYTES / (512 * (tokens ? tokens : 1)), most_tiles = tiles256 < PIECE_TILES ? tiles256 : PIECE_TILES;
+        const uint64_t per = fit && fit < most_tiles ? fit : fit ? most_tiles : 1;
         pieces = tiles256 / per;
         if (tiles256 % per * 2 >= per) // a rest of less than half a piece goes with the last one
             ++pieces;
@@ -337,17 +340,33 @@ struct EntropyWork {
     }
 };
 
-int check_entropy(const char* who, int type, const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, const void* target,
+bool walks(const void* p, int64_t stride, uint64_t dim) { return aligned(p, 16) && stride % 8 == 0 && dim % 8 == 0; }
+
+// Whether the operator's launches all hold less than they may. copied: the rows of the larger array that has to be laid out first.
+bool entropy_fits(uint64_t tokens, uint64_t dim, uint64_t vocab, bool backward, uint64_t copied)
+{
+    if (tokens > 1u << 30 || vocab > 1u << 30 || dim >= 1u << 22)
+        return false;
+    const EntropyPlan plan(tokens, dim, vocab);
+    const uint64_t words = backward ? plan.words : vocab, values = tokens * plan.padded_dim;
+    const bool logits = plan.narrow_logits ? launchable(parts_of(words, 128) * parts_of(tokens, 64), 256) : launchable(parts_of(words, 256) * parts_of(tokens, 256), 512);
+    const bool copies = launchable(parts_of((backward && copied < tokens ? tokens : copied) * (plan.padded_dim / 8), 256), 256);
+    if (!backward)
+        return logits && copies && launchable(parts_of(tokens, tokens <= 512 ? 4 : 16), 256);
+    return logits && copies && launchable(parts_of(dim, 256) * parts_of(words, 256), 512) &&
+           launchable(parts_of(tokens, plan.narrow_hidden ? 64 : 256) * parts_of(dim, 256) * plan.shares, 512) &&
+           launchable(parts_of(values / 4, plan.shares > 16 ? 16 : 256), 256) && launchable(parts_of(vocab * dim, 1024), 256);
+}
+
+int check_entropy(const char* who, bool backward, int type, const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, const void* target,
                   uint64_t tokens, uint64_t dim, uint64_t vocab)
 {
     if (type != CSA_LM_BF16 && type != CSA_LM_F16)
         return fail(CSA_ERR_ARG, "%s: type %d is neither CSA_LM_BF16 nor CSA_LM_F16", who, type);
     if (!dim || !vocab)
         return fail(CSA_ERR_ARG, "%s: %llu values a row, %llu words", who, (unsigned long long)dim, (unsigned long long)vocab);
-    if (tokens > 1u << 30 || vocab > 1u << 30 || dim >= 1u << 22)
-        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens, %llu words, %llu values a row", who, (unsigned long long)tokens, (unsigned long long)vocab,
-                    (unsigned long long)dim);
-    if (parts_of(vocab, 256) * parts_of(tokens, 64) > 0x7fffffffu || (tokens > vocab ? tokens : vocab) * up(dim, 8) / 2048 > 0x7fffffffu)
+    const uint64_t hidden_rows = walks(hidden, hidden_stride, dim) ? 0 : tokens, weight_rows = walks(weight, weight_stride, dim) ? 0 : vocab;
+    if (!entropy_fits(tokens, dim, vocab, backward, hidden_rows > weight_rows ? hidden_rows : weight_rows))
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens by %llu words of %llu values in one call", who, (unsigned long long)tokens, (unsigned long long)vocab,
                     (unsigned long long)dim);
     if (!weight || !aligned(weight, 2) || (tokens && (!hidden || !aligned(hidden, 2) || !target)))
@@ -357,8 +376,6 @@ int check_entropy(const char* who, int type, const void* hidden, int64_t hidden_
                     (unsigned long long)dim);
     return CSA_OK;
 }
-
-bool walks(const void* p, int64_t stride, uint64_t dim) { return aligned(p, 16) && stride % 8 == 0 && dim % 8 == 0; }
 
 void lay_out(const void* in, int64_t in_stride, uint64_t rows, uint64_t dim, const int32_t* target, uint64_t vocab, short* out, uint64_t stride, hipStream_t s)
 {
@@ -476,7 +493,7 @@ int csa_lm_spans_u16_dev(const uint16_t* d_text, uint64_t n, uint32_t separator,
 int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream)
 {
     const char* who = "csa_lm_attention_forward_dev";
-    if (int rc = check_attention(who, a))
+    if (int rc = check_attention(who, a, false))
         return rc;
     if (a->tokens == 0)
         return CSA_OK;
@@ -501,7 +518,7 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
                                   csa_lm_heads d_v, void* d_work, uint64_t work_bytes, void* stream)
 {
     const char* who = "csa_lm_attention_backward_dev";
-    if (int rc = check_attention(who, a))
+    if (int rc = check_attention(who, a, true))
         return rc;
     if (a->tokens == 0)
         return CSA_OK;
@@ -524,16 +541,17 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
 
 uint64_t csa_lm_cross_entropy_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t flags)
 {
-    if (!dim || !vocab || tokens > 1u << 30 || vocab > 1u << 30 || dim >= 1u << 22)
+    const bool copies = flags & CSA_LM_COPY_ROWS || dim % 8;
+    if (!dim || !vocab || !entropy_fits(tokens, dim, vocab, flags & CSA_LM_BACKWARD, !copies ? 0 : tokens > vocab ? tokens : vocab))
         return 0;
-    return EntropyWork(nullptr, EntropyPlan(tokens, dim, vocab), tokens, vocab, flags & CSA_LM_BACKWARD, flags & CSA_LM_COPY_ROWS || dim % 8).bytes;
+    return EntropyWork(nullptr, EntropyPlan(tokens, dim, vocab), tokens, vocab, flags & CSA_LM_BACKWARD, copies).bytes;
 }
 
 int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_target,
                                      uint64_t tokens, uint64_t dim, uint64_t vocab, float* d_loss, float* d_lse, void* d_work, uint64_t work_bytes, void* stream)
 {
     const char* who = "csa_lm_cross_entropy_forward_dev";
-    if (int rc = check_entropy(who, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
+    if (int rc = check_entropy(who, false, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
         return rc;
     if (tokens == 0)
         return CSA_OK;
@@ -563,10 +581,10 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
                                       int64_t hidden_grad_stride, void* d_weight_grad, int64_t weight_grad_stride, void* d_work, uint64_t work_bytes, void* stream)
 {
     const char* who = "csa_lm_cross_entropy_backward_dev";
-    if (int rc = check_entropy(who, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
+    if (int rc = check_entropy(who, true, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
         return rc;
-    if (tokens && (!d_lse || !d_loss_grad))
-        return fail(CSA_ERR_ARG, "%s: d_lse or d_loss_grad is null", who);
+    if (tokens && (!d_lse || !d_loss_grad || !aligned(d_lse, 4) || !aligned(d_loss_grad, 4)))
+        return fail(CSA_ERR_ARG, "%s: d_lse or d_loss_grad is null or unaligned", who);
     if ((d_hidden_grad && (!aligned(d_hidden_grad, 2) || hidden_grad_stride < static_cast<int64_t>(dim))) ||
         (d_weight_grad && (!aligned(d_weight_grad, 2) || weight_grad_stride < static_cast<int64_t>(dim))))
         return fail(CSA_ERR_ARG, "%s: a gradient's address is odd or its stride below its rows' length", who);

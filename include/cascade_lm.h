@@ -23,7 +23,7 @@ extern "C" {
 typedef enum csa_lm_type {
     CSA_LM_BF16 = 0,
     CSA_LM_F16 = 1,
-    CSA_LM_F32 = 2 /* gradients to clip only: the matrix units multiply 16-bit values */
+    CSA_LM_F32 = 2 /* gradients to clip only: the matrix units multiply it at a sixteenth of the rate of the other two */
 } csa_lm_type;
 
 /* Flags of the *_workspace functions. */
@@ -57,7 +57,7 @@ typedef struct csa_lm_attention {
     uint32_t q_heads;      /* a multiple of kv_heads: head h of q reads head h / (q_heads / kv_heads) of k and v */
     uint32_t kv_heads;
     uint32_t head_dim;     /* 8 to 128, a multiple of 8 */
-    uint64_t tokens;       /* up to 2^30 */
+    uint64_t tokens;       /* up to 2^30, with fewer than 2^31 rows of q (tokens in 128s times q_heads); fewer than 2^29 for gradients */
     const int32_t* d_lo;   /* row i sees the keys [lo[i], hi[i]), cut to [0, tokens); none where that is empty. NULL: 0 */
     const int32_t* d_hi;   /* NULL: i + 1 */
     const float* d_slope;  /* NULL, or q_heads values: slope[h] * |i - j| is taken off the score of row i and key j */
@@ -86,7 +86,8 @@ int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, c
  * hidden is tokens x dim, weight is vocab x dim, both of `type` (CSA_LM_BF16 or CSA_LM_F16) with their rows *_stride values
  * apart (>= dim, below 2^22). Rows that 16-byte loads cannot walk (an address, a stride or dim that is no multiple of 8 values)
  * are copied to the workspace first, for which it has to be sized with CSA_LM_COPY_ROWS; the rest is read where it lies.
- * tokens, vocab <= 2^30. */
+ * tokens, vocab <= 2^30; 2^39 logits in a forward call (2^37 where tokens or words are few), 2^28 tokens in one, 2^42 values of a weight's
+ * gradient or 2^35 values to copy are too many for its launches: CSA_ERR_TOO_LARGE, and a workspace of 0. Several calls then take some of the tokens each. */
 uint64_t csa_lm_cross_entropy_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t flags);
 int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride,
                                      const int32_t* d_target, uint64_t tokens, uint64_t dim, uint64_t vocab, float* d_loss, float* d_lse,

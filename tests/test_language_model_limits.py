@@ -1,0 +1,43 @@
+"""Sizes that the language-model operators' launches cannot hold are refused before anything is launched. No GPU needed: what is accepted
+here ends at the workspace, which is too small."""
+import ctypes as C
+
+import pytest
+
+from cascade_amd import _native_lm as native
+
+BAD, LARGE = -1, -2
+
+
+def attention(tokens, heads, backward):
+    lib, x = native.load(), 1 << 20  # an address that nothing reads
+    h = native.CsaLmHeads(x, 8 * heads, 8)
+    a = native.CsaLmAttention(0, heads, heads, 8, tokens, None, None, None, 1.0, 0.0, h, h, h)
+    if backward:
+        return lib.csa_lm_attention_backward_dev(C.byref(a), h, x, h, h, h, h, x, 1, None)
+    return lib.csa_lm_attention_forward_dev(C.byref(a), h, x, x, 1, None)
+
+
+def entropy(tokens, dim, vocab, backward):
+    lib, x = native.load(), 1 << 20
+    if backward:
+        return lib.csa_lm_cross_entropy_backward_dev(0, x, dim, x, dim, x, x, x, tokens, dim, vocab, x, dim, x, dim, x, 1, None)
+    return lib.csa_lm_cross_entropy_forward_dev(0, x, dim, x, dim, x, tokens, dim, vocab, x, x, x, 1, None)
+
+
+@pytest.mark.parametrize("tokens,heads,backward,want", [
+    (1 << 24, 128, False, LARGE), (1 << 24, 128, True, LARGE), ((1 << 24) - 128, 128, True, BAD), (1 << 24, 127, True, BAD),
+    (1 << 29, 1, True, LARGE), ((1 << 29) - 32, 1, True, BAD), (1 << 30, 2, False, LARGE), (1 << 15, 65535, True, BAD), (1 << 16, 65535, True, LARGE)])
+def test_attention_over_more_rows_than_a_launch_holds(tokens, heads, backward, want):
+    assert attention(tokens, heads, backward) == want
+
+
+@pytest.mark.parametrize("tokens,dim,vocab,backward,want", [
+    (1 << 23, 64, 65536, False, LARGE), ((1 << 23) - 256, 64, 65536, False, BAD), (1 << 28, 8, 1, False, LARGE), ((1 << 28) - 16, 8, 1, False, BAD),
+    (1 << 23, 64, 65536, True, BAD),  # in pieces of the vocabulary
+    (1 << 30, 8, 300, True, BAD), (1 << 30, 40, 300, True, LARGE), (100, 4096, 1 << 30, False, LARGE), (64, 4096, 1 << 29, False, BAD), (100, 4095, 1 << 30, False, LARGE), (100, 4096, 1 << 23, False, BAD),
+    (100, 4095, 1 << 23, False, LARGE), (100, 4095, 1 << 22, False, BAD), (100, 4096, 1 << 30, True, LARGE), (0, 4096, 1 << 30, True, LARGE)])
+def test_cross_entropy_of_more_than_a_launch_holds(tokens, dim, vocab, backward, want):
+    flags = native.CSA_LM_BACKWARD if backward else 0
+    assert entropy(tokens, dim, vocab, backward) == want
+    assert (native.load().csa_lm_cross_entropy_workspace(tokens, dim, vocab, flags) == 0) == (want == LARGE)
