@@ -284,7 +284,7 @@ struct EntropyPlan {
     uint64_t padded_dim, words, piece_words, pieces; // words: of the largest piece
     uint64_t shares, share_words;
     bool narrow_logits, narrow_hidden;
-    EntropyPlan(uint64_t tokens, uint64_t dim, uint64_t vocab)
+    EntropyPlan(uint64_t tokens, uint64_t dim, uint64_t vocab, bool backward)
     {
         padded_dim = up(dim, 8);
         const uint64_t tiles256 = parts_of(vocab, 256);
@@ -297,13 +297,16 @@ struct EntropyPlan {
         piece_words = per * 256;
         words = pieces * per >= tiles256 ? piece_words : (tiles256 - (pieces - 1) * per) * 256;
 
+        narrow_hidden = tokens <= 128;
+        shares = 1;
+        share_words = words;
+        if (!backward)
+            return;
         // d_hidden has few tiles where there are few tokens: its sum over the words of a piece is then shared out, so that workgroups fill the
         // compute units (two small ones fit one) in whole rounds as well as shares can.
-        narrow_hidden = tokens <= 128;
         const uint64_t tiles = parts_of(tokens, narrow_hidden ? 64 : 256) * parts_of(padded_dim, 256), slots = narrow_hidden ? 2 * UNITS : UNITS;
         const uint64_t room = SHARE_BYTES / (4 * (tokens * padded_dim ? tokens * padded_dim : 1)) + 1, longest = parts_of(words, 4 * SLICE);
         const uint64_t most = room < longest ? room : longest;
-        shares = 1;
         double best = 0;
         for (uint64_t n = 1; n <= most && tiles && n * tiles <= 2 * slots; ++n) {
             const double used = static_cast<double>(n * tiles) / up(n * tiles, slots);
@@ -347,15 +350,15 @@ bool entropy_fits(uint64_t tokens, uint64_t dim, uint64_t vocab, bool backward, 
 {
     if (tokens > 1u << 30 || vocab > 1u << 30 || dim >= 1u << 22)
         return false;
-    const EntropyPlan plan(tokens, dim, vocab);
+    const EntropyPlan plan(tokens, dim, vocab, false); // shares of d_hidden are few workgroups: they need no check
     const uint64_t words = backward ? plan.words : vocab, values = tokens * plan.padded_dim;
     const bool logits = plan.narrow_logits ? launchable(parts_of(words, 128) * parts_of(tokens, 64), 256) : launchable(parts_of(words, 256) * parts_of(tokens, 256), 512);
     const bool copies = launchable(parts_of((backward && copied < tokens ? tokens : copied) * (plan.padded_dim / 8), 256), 256);
     if (!backward)
         return logits && copies && launchable(parts_of(tokens, tokens <= 512 ? 4 : 16), 256);
     return logits && copies && launchable(parts_of(dim, 256) * parts_of(words, 256), 512) &&
-           launchable(parts_of(tokens, plan.narrow_hidden ? 64 : 256) * parts_of(dim, 256) * plan.shares, 512) &&
-           launchable(parts_of(values / 4, plan.shares > 16 ? 16 : 256), 256) && launchable(parts_of(vocab * dim, 1024), 256);
+           launchable(parts_of(tokens, plan.narrow_hidden ? 64 : 256) * parts_of(dim, 256), 512) && launchable(parts_of(values / 4, 256), 256) &&
+           launchable(parts_of(vocab * dim, 1024), 256);
 }
 
 int check_entropy(const char* who, bool backward, int type, const void* hidden, int64_t hidden_stride, const void* weight, int64_t weight_stride, const void* target,
@@ -544,7 +547,7 @@ uint64_t csa_lm_cross_entropy_workspace(uint64_t tokens, uint64_t dim, uint64_t 
     const bool copies = flags & CSA_LM_COPY_ROWS || dim % 8;
     if (!dim || !vocab || !entropy_fits(tokens, dim, vocab, flags & CSA_LM_BACKWARD, !copies ? 0 : tokens > vocab ? tokens : vocab))
         return 0;
-    return EntropyWork(nullptr, EntropyPlan(tokens, dim, vocab), tokens, vocab, flags & CSA_LM_BACKWARD, copies).bytes;
+    return EntropyWork(nullptr, EntropyPlan(tokens, dim, vocab, flags & CSA_LM_BACKWARD), tokens, vocab, flags & CSA_LM_BACKWARD, copies).bytes;
 }
 
 int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_target,
@@ -557,7 +560,7 @@ int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hid
         return CSA_OK;
     if (!d_loss || !d_lse || !aligned(d_loss, 4) || !aligned(d_lse, 4))
         return fail(CSA_ERR_ARG, "%s: d_loss or d_lse is null or unaligned", who);
-    const EntropyPlan plan(tokens, dim, vocab);
+    const EntropyPlan plan(tokens, dim, vocab, false);
     const bool copies = !walks(d_hidden, hidden_stride, dim) || !walks(d_weight, weight_stride, dim);
     const EntropyWork w(d_work, plan, tokens, vocab, false, copies);
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
@@ -588,7 +591,7 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
     if ((d_hidden_grad && (!aligned(d_hidden_grad, 2) || hidden_grad_stride < static_cast<int64_t>(dim))) ||
         (d_weight_grad && (!aligned(d_weight_grad, 2) || weight_grad_stride < static_cast<int64_t>(dim))))
         return fail(CSA_ERR_ARG, "%s: a gradient's address is odd or its stride below its rows' length", who);
-    const EntropyPlan plan(tokens, dim, vocab);
+    const EntropyPlan plan(tokens, dim, vocab, true);
     const EntropyWork w(d_work, plan, tokens, vocab, true, !walks(d_weight, weight_stride, dim));
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
         return rc;
