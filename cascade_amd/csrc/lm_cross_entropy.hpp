@@ -129,13 +129,13 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int6
     }
 }
 
-// The factor of P, range / max |d_loss|, and its inverse.
+// The factor of P, range / max |d_loss|, and its inverse. What is not finite among them has no say: its token is lost whatever the factor is, and takes nothing from the others.
 __global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, const int32_t* target, int64_t tokens, int64_t vocab, float range, float* scale)
 {
     __shared__ float tops[16];
     float top = 0.f;
     for (int64_t n = threadIdx.x; n < tokens; n += 1024)
-        if (target[n] >= 0 && target[n] < vocab)
+        if (target[n] >= 0 && target[n] < vocab && fabsf(d_loss[n]) < INFINITY)
             top = fmaxf(top, fabsf(d_loss[n]));
     for (int d = 32; d; d /= 2)
         top = fmaxf(top, __shfl_xor(top, d));

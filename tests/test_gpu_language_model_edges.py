@@ -149,3 +149,19 @@ def test_a_step_that_has_overflowed_takes_no_longer_than_a_few(dtype, bad):
     print(f"{bad}: {1000 * usual:.0f} us, {1000 * overflowed:.0f} us")
     assert not all(torch.isfinite(x).all() for x in step())
     assert overflowed <= 10 * usual
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_a_token_whose_loss_has_overflowed_takes_no_bits_from_the_others(dtype, value):
+    g, n, dim, vocab = gen(53), 300, 128, 3000
+    hidden, weight = randn(g, n, dim, dtype=dtype), randn(g, vocab, dim, dtype=dtype, scale=2 * dim ** -0.5)
+    target = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    d_loss = torch.full((n,), 3e-3, device="cuda")
+    lse = cascade_amd.linear_cross_entropy(hidden, weight, target)[1]
+    clean = cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse)[0]
+    d_loss[77] = value
+    d_hidden, d_weight = cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse)
+    rest = torch.arange(n, device="cuda") != 77
+    assert torch.equal(d_hidden[rest], clean[rest])
+    assert not torch.isfinite(d_hidden[77]).any() and not torch.isfinite(d_weight).any()
