@@ -6,8 +6,10 @@
 #include "lm_cross_entropy.hpp"
 #include "lm_spans.hpp"
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 
 using namespace lm;
 
@@ -461,6 +463,46 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
     }
 }
 
+// ---- clipping ----
+
+// The first array of the list that is written where another one (or its own `in`, but for the same place) lies: workgroups would read it before or after, as it happens.
+// `count` if there is none, `count + 1` if there is no memory to find out.
+uint32_t first_overlap(const csa_lm_values* list, uint32_t count)
+{
+    struct Span {
+        uintptr_t begin, end;
+        uint32_t index;
+        bool written;
+    };
+    Span few[128];
+    Span* spans = count <= 64 ? few : static_cast<Span*>(malloc(2 * sizeof(Span) * count));
+    if (!spans)
+        return count + 1;
+    uint32_t n = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint64_t bytes = list[i].n * (list[i].type == CSA_LM_F32 ? 4 : 2);
+        const uintptr_t in = reinterpret_cast<uintptr_t>(list[i].in), out = reinterpret_cast<uintptr_t>(list[i].out);
+        if (!bytes)
+            continue;
+        spans[n++] = {out, out + bytes, i, true};
+        if (in != out)
+            spans[n++] = {in, in + bytes, i, false};
+    }
+    std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    uintptr_t written_to = 0, read_to = 0; // where what begins earlier ends
+    uint32_t found = count;
+    for (uint32_t k = 0; k < n && found == count; ++k) {
+        const Span& x = spans[k];
+        if (x.begin < written_to || (x.written && x.begin < read_to))
+            found = x.index;
+        uintptr_t& to = x.written ? written_to : read_to;
+        to = to < x.end ? x.end : to;
+    }
+    if (spans != few)
+        free(spans);
+    return found;
+}
+
 } // namespace
 
 extern "C" {
@@ -636,6 +678,17 @@ int csa_lm_clip_dev(const csa_lm_values* list, uint32_t count, float max_norm, f
         if (v.n > 1ull << 40)
             return fail(CSA_ERR_TOO_LARGE, "%s: array %u has %llu values", who, i, (unsigned long long)v.n);
     }
+    if (const uint32_t which = first_overlap(list, count); which < count)
+        return fail(CSA_ERR_ARG, "%s: array %u lies where another one, or its other address, is written", who, which);
+    else if (which > count)
+        return fail(CSA_ERR_ARG, "%s: no memory to look over %u arrays", who, count);
+    for (uint32_t begin = 0; begin < count; begin += CLIP_TENSORS) {
+        uint64_t chunks = 0;
+        for (uint32_t i = begin; i < count && i < begin + CLIP_TENSORS; ++i)
+            chunks += parts_of(list[i].n, CLIP_CHUNK);
+        if (chunks > 0x7fffffffu)
+            return fail(CSA_ERR_TOO_LARGE, "%s: too many values", who);
+    }
     if (int rc = check_work(who, d_work, work_bytes, csa_lm_clip_workspace(count)))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -658,8 +711,6 @@ int csa_lm_clip_dev(const csa_lm_values* list, uint32_t count, float max_norm, f
                     chunks += parts_of(list[i].n, CLIP_CHUNK);
                 }
             c.first[c.count] = static_cast<uint32_t>(chunks);
-            if (chunks > 0x7fffffffu)
-                return fail(CSA_ERR_TOO_LARGE, "%s: too many values", who);
             const uint32_t groups = static_cast<uint32_t>(chunks < CLIP_GROUPS ? chunks : CLIP_GROUPS);
             if (way == 0 && groups) {
                 squares_kernel<<<groups, 256, 0, s>>>(c, partial + partials);

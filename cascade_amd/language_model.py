@@ -244,9 +244,9 @@ def linear_cross_entropy_backward(d_loss, hidden, weight, target, lse, want_hidd
 
 
 def clip_gradients(grads, max_norm, out=None):
-    """Scales the gradients (a list of dense tensors, float32, bfloat16 or float16, mixed as they come) by min(1, max_norm / norm), where norm is the
-    square root of the sum of all their squares, in place or into `out`, a list of tensors like them. Returns norm, a float32 tensor
-    of no dimensions; where it is not finite the values stay as they are (csa_lm_clip_dev)."""
+    """Scales the gradients (a list of contiguous tensors, at least one, float32, bfloat16 or float16, mixed as they come) by min(1, max_norm / norm), where norm
+    is the square root of the sum of all their squares, in place or into `out`, a list of tensors like them. No tensor may be written twice, or where another one is
+    read. Returns norm, a float32 tensor of no dimensions; where it is not finite the values stay as they are (csa_lm_clip_dev)."""
     import torch
     grads = list(grads)
     out = grads if out is None else list(out)

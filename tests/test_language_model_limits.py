@@ -41,3 +41,35 @@ def test_cross_entropy_of_more_than_a_launch_holds(tokens, dim, vocab, backward,
     flags = native.CSA_LM_BACKWARD if backward else 0
     assert entropy(tokens, dim, vocab, backward) == want
     assert (native.load().csa_lm_cross_entropy_workspace(tokens, dim, vocab, flags) == 0) == (want == LARGE)
+
+
+def clip(*arrays):
+    """Status of a call over (in, out, values, type); one that is accepted ends at the workspace."""
+    lib = native.load()
+    items = (native.CsaLmValues * len(arrays))(*(native.CsaLmValues(*a) for a in arrays))
+    status = lib.csa_lm_clip_dev(items, len(arrays), 1.0, None, None, 0, None)
+    return status, lib.csa_lm_last_error()
+
+
+def test_clipping_refuses_arrays_that_are_written_twice_or_read_elsewhere():
+    x, f32, f16 = 1 << 20, native.CSA_LM_F32, native.CSA_LM_F16
+    for bad in ([(x, x, 10, f32), (x, x, 10, f32)],                            # one tensor twice
+                [(x, x, 10, f32), (x + 36, x + 36, 10, f32)],                  # its last value
+                [(x, x + 4, 10, f32)],                                         # its own place, moved by one
+                [(x, x + 400, 10, f16), (x + 418, x + 800, 10, f16)],          # read where another one is written
+                [(x, x + 800, 10, f32), (x + 400, x + 836, 10, f32)],          # written into one place
+                [(x + 8 * i, x + 8 * i, 2, f32) for i in range(100)] + [(x + 796, x + 796, 1, f32)]):
+        status, message = clip(*bad)
+        assert status == BAD and b"written" in message
+        status, message = clip(*reversed(bad))
+        assert status == BAD and b"written" in message
+    for good in ([(x, x, 10, f32), (x + 40, x + 40, 10, f16)], [(x, x + 400, 10, f32), (x, x + 800, 10, f32)], [(x, x, 10, f32), (x, x, 0, f32)],
+                 [(x + 8 * i, x + 8 * i, 2, f32) for i in range(100)]):
+        status, message = clip(*good)
+        assert status == BAD and b"workspace" in message
+
+
+def test_clipping_refuses_too_many_values_before_any_launch():
+    one = 1 << 40
+    status, message = clip(*((4 * one * i + 16, 4 * one * i + 16, one, native.CSA_LM_F32) for i in range(1, 41)))
+    assert status == LARGE and b"values" in message
