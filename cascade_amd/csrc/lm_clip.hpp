@@ -133,8 +133,8 @@ __global__ __launch_bounds__(256) void clip_kernel(ClipList list, const double* 
     const double norm = sqrt(sum);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0)
         *norm_out = static_cast<float>(norm);
-    // no finite norm, no direction to keep: the values stay, and the norm says so
-    const float factor = norm > max_norm && norm < static_cast<double>(INFINITY) ? static_cast<float>(max_norm / norm) : 1.f;
+    // no finite norm in 32 bits, in which the caller gets it: the values stay, and the norm says so
+    const float factor = norm > max_norm && static_cast<float>(norm) < INFINITY ? static_cast<float>(max_norm / norm) : 1.f;
     const uint32_t chunks = list.first[list.count];
     for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
         const uint32_t c = chunks - 1 - k, t = tensor_of(list, c);

@@ -110,7 +110,7 @@ typedef struct csa_lm_values {
 } csa_lm_values;
 
 /* *d_norm = the square root of the sum of the squares of all values of the `count` arrays of the host list (summed in 64 bits);
- * out = in * min(1, max_norm / norm), rounded to the type. Where the norm is no finite number the values stay as they are.
+ * out = in * min(1, max_norm / norm), rounded to the type. Where the norm is no finite number of 32 bits the values stay as they are.
  * Arrays are aligned to their type's size. No array's out may overlap another's in or out, nor its own in but for the same address: one that is
  * named twice would be scaled twice, or not, and is refused (CSA_ERR_ARG). The list is read before the call returns. */
 uint64_t csa_lm_clip_workspace(uint32_t count);

@@ -165,3 +165,20 @@ def test_a_token_whose_loss_has_overflowed_takes_no_bits_from_the_others(dtype, 
     rest = torch.arange(n, device="cuda") != 77
     assert torch.equal(d_hidden[rest], clean[rest])
     assert not torch.isfinite(d_hidden[77]).any() and not torch.isfinite(d_weight).any()
+
+
+# ---- clipping ----
+
+
+@pytest.mark.parametrize("value,count,finite", [(3e38, 2, False), (3.4e38, 1, True), (1e38, 1000, False), (1e37, 1000, True)])
+def test_values_stay_exactly_where_the_norm_is_not_finite(value, count, finite):
+    """The norm of 32 bits says whether the values were scaled, also where 64 bits hold a larger one."""
+    x = torch.full((count,), value, device="cuda")
+    want = x[0].item() * math.sqrt(count)
+    out = [torch.zeros_like(x)]
+    norm = cascade_amd.clip_gradients([x], 1.0, out=out).item()
+    assert math.isfinite(norm) == finite and (not finite or abs(norm - want) <= 2.0 ** -23 * want)
+    if finite:
+        assert torch.allclose(out[0], torch.full_like(x, count ** -0.5), rtol=1e-5)
+    else:
+        assert torch.equal(out[0], x)
