@@ -258,7 +258,7 @@ def clip_gradients(grads, max_norm, out=None):
     items = []  # csa_lm_values as four 64-bit words each
     for g, o in zip(grads, out):
         if not g.is_contiguous() or g.get_device() != device:
-            raise ValueError("gradients: dense tensors on one GPU")
+            raise ValueError("gradients: contiguous tensors on one GPU")
         if o is not g and (o.dtype != g.dtype or o.shape != g.shape or not o.is_contiguous() or o.get_device() != device):
             raise ValueError("out: tensors like the gradients, one by one")
         items += (g.data_ptr(), o.data_ptr(), g.numel(), _type(g.dtype))
@@ -268,6 +268,7 @@ def clip_gradients(grads, max_norm, out=None):
     size = lib.csa_lm_clip_workspace(len(grads))
     scratch, work = _work(size, norm)
     _enqueue(device, lib.csa_lm_clip_dev, items.buffer_info()[0], len(grads), float(max_norm), norm.data_ptr(), work, size)
+    torch.autograd.graph.increment_version(out)  # they have changed: what autograd has saved of them is stale
     return norm
 
 

@@ -182,3 +182,19 @@ def test_values_stay_exactly_where_the_norm_is_not_finite(value, count, finite):
         assert torch.allclose(out[0], torch.full_like(x, count ** -0.5), rtol=1e-5)
     else:
         assert torch.equal(out[0], x)
+
+
+def test_autograd_notices_that_clipping_has_changed_a_tensor():
+    for in_place in (True, False):
+        g = torch.full((10,), 3.0, device="cuda")
+        scaled = g if in_place else torch.zeros_like(g)
+        x = torch.ones(10, device="cuda", requires_grad=True)
+        y = (x * scaled).sum()  # keeps `scaled` for its gradient
+        before = g._version, scaled._version
+        cascade_amd.clip_gradients([g], 1.0, out=None if in_place else [scaled])
+        assert scaled._version == before[1] + 1 and (in_place or g._version == before[0])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():  # tensors without versions
+        g = torch.full((10,), 3.0, device="cuda")
+        assert cascade_amd.clip_gradients([g], 1.0).item() == pytest.approx(3 * 10 ** 0.5)
