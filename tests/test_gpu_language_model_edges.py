@@ -198,3 +198,69 @@ def test_autograd_notices_that_clipping_has_changed_a_tensor():
     with torch.inference_mode():  # tensors without versions
         g = torch.full((10,), 3.0, device="cuda")
         assert cascade_amd.clip_gradients([g], 1.0).item() == pytest.approx(3 * 10 ** 0.5)
+
+
+# ---- torch.autograd ----
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("wanted", ["qkv", "q", "kv", "v"])
+def test_attend_gives_autograd_the_gradients(dtype, wanted):
+    g, n, u = gen(61), 260, U[dtype]
+    q, k, v = (randn(g, n, h, 64, dtype=dtype) for h in (4, 2, 2))
+    lo, hi = spans_for("documents", n, g)
+    slopes = torch.linspace(0.01, 0.1, 4, device="cuda")
+    for name, x in zip("qkv", (q, k, v)):
+        x.requires_grad_(name in wanted)
+    way = randn(g, 64, dtype=dtype)  # the gradient of the outputs comes expanded, with strides of 0
+    out = cascade_amd.attend(q, k, v, lo, hi, cap=10.0, slopes=slopes)
+    (out * way).sum(dtype=torch.float32).backward()
+    d_out = way.expand(n, 4, 64)
+    want, sums = reference_attention(q.detach(), k.detach(), v.detach(), lo, hi, 0.125, 10.0, slopes, d_out, u)
+    within(out.detach(), want["out"], 1.1 * u * (sums["out"] + want["out"].abs()) + 2.0 ** -24, "out")
+    for name, x in zip("qkv", (q, k, v)):
+        if name not in wanted:
+            assert x.grad is None
+            continue
+        small = 1e-5 * sums["d_" + name].abs().max().item() / u
+        within(x.grad, want["d_" + name], 1.1 * (sums["d_" + name] + u * want["d_" + name].abs()) + small + 2.0 ** -24, name)
+    with torch.no_grad():
+        assert not cascade_amd.attend(q, k, v, lo, hi).requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("wanted", ["both", "hidden", "weight"])
+def test_next_token_loss_gives_autograd_the_gradients(dtype, wanted):
+    g, n, dim, vocab, u = gen(62), 200, 96, 1500, U[dtype]
+    hidden, weight = randn(g, n, dim, dtype=dtype), randn(g, vocab, dim, dtype=dtype, scale=0.2)
+    target = torch.randint(-1, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    target[::7] = -1
+    hidden.requires_grad_(wanted != "weight")
+    weight.requires_grad_(wanted != "hidden")
+    loss = cascade_amd.next_token_loss(hidden, weight, target)
+    (loss.sum() * 3.0).backward()  # an expanded gradient
+    h, w, there = hidden.detach().double(), weight.detach().double(), target >= 0
+    logits = h @ w.T
+    at = target.long().clamp(min=0)[:, None]
+    size = 1 + (h.abs() @ w.abs().T).max(1).values
+    within(loss.detach(), torch.where(there, torch.logsumexp(logits, 1) - logits.gather(1, at)[:, 0], 0.0), 4e-6 * size, "loss")
+    p = torch.softmax(logits, 1).scatter_add_(1, at, torch.full((n, 1), -1.0, dtype=torch.float64, device="cuda")) * there[:, None] * 3.0
+    off = (u + 1e-5) * p.abs()
+    for name, x, want, terms in (("hidden", hidden, p @ w, off @ w.abs()), ("weight", weight, p.T @ h, off.T @ h.abs())):
+        if wanted not in ("both", name):
+            assert x.grad is None
+            continue
+        within(x.grad, want, 1.1 * (terms + u * want.abs()) + 4e-6 * p.abs().max() + 2.0 ** -24, name)
+
+
+def test_gradients_that_are_not_wanted_are_none_and_leave_the_others():
+    g = gen(63)
+    hidden, weight = randn(g, 150, 64, dtype=torch.bfloat16), randn(g, 700, 64, dtype=torch.bfloat16)
+    target = torch.randint(0, 700, (150,), generator=g, device="cuda", dtype=torch.int32)
+    d_loss = torch.rand(150, generator=g, device="cuda")
+    lse = cascade_amd.linear_cross_entropy(hidden, weight, target)[1]
+    both = cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse)
+    one = cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse, want_weight=False)
+    other = cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse, want_hidden=False)
+    assert one[1] is None and other[0] is None and torch.equal(one[0], both[0]) and torch.equal(other[1], both[1])
+    assert cascade_amd.linear_cross_entropy_backward(d_loss, hidden, weight, target, lse, False, False) == (None, None)
