@@ -121,7 +121,8 @@ Attention attention(const csa_lm_attention& a)
 // workgroups of a long document are the last ones to end. A share has KV_TURNS tiles of rows at least, and where it can be, whole heads: workgroups next to
 // each other then read the same rows (12289 tokens, 16 heads of 2: 8 shares 2.91 ms, 11 shares 3.03 ms; 16384 tokens of documents, 16 heads of 4: 4 shares 1.05 ms,
 // 3 shares 1.15 ms, 2 shares 1.36 ms; 3001 tokens, 12 heads of 12: 8 shares 0.26 ms, none 0.34 ms).
-// The sums take 270 MB at most, but for the rounding to whole heads.
+// A workgroup's sums take 128 KB at 128 values a head. Rounded up to a number of shares for each group of keys, KV_GROUPS of them are less than 2 * KV_GROUPS (268 MB), twice as many
+// less than 4 * KV_GROUPS (537 MB: 262016 tokens of 1 head of keys), and whole heads make half as much again of those at most (805 MB).
 constexpr uint64_t KV_GROUPS = 1024, KV_LONG = 512, KV_TURNS = 16;
 
 // The keys that a tile of rows sees are shared out in the same way where there are too few tiles for two workgroups a compute unit; a share has five tiles of

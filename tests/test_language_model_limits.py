@@ -73,3 +73,22 @@ def test_clipping_refuses_too_many_values_before_any_launch():
     one = 1 << 40
     status, message = clip(*((4 * one * i + 16, 4 * one * i + 16, one, native.CSA_LM_F32) for i in range(1, 41)))
     assert status == LARGE and b"values" in message
+
+
+def test_the_sums_of_the_attention_gradients_stay_under_their_bound():
+    """A workgroup has sums of 128 keys by 128 values of d_k and of d_v, in 32 bits: 128 KB. Shares of a call are fewer than 2048 workgroups, 4096 where they are long, and 6144 where
+    whole heads are taken."""
+    lib, largest = native.load(), 0
+    for kv_heads in (1, 2, 3, 4, 8):
+        for group in (1, 2, 3, 4, 5, 7, 8, 16, 71):
+            for tokens in [128 * n - less for n in (1, 100, 511, 513, 682, 1023, 1024, 1025, 1500, 2047, 2048, 2049, 5000) for less in (0, 1, 127)] + [262016]:
+                heads = kv_heads * group
+                size = lib.csa_lm_attention_workspace(tokens, heads, kv_heads, 128, native.CSA_LM_BACKWARD)
+                rows = (tokens + 31) // 32 * (512 * heads + 8)  # row blocks and their bounds
+                forward = lib.csa_lm_attention_workspace(tokens, heads, kv_heads, 128, 0)
+                sums = size - rows - forward
+                assert sums <= 6144 * 131072 + 8192, (tokens, heads, kv_heads)
+                if group == 1:
+                    assert sums <= 4096 * 131072 + 8192
+                largest = max(largest, sums)
+    assert largest > 6100 * 131072  # the bound is reached
