@@ -142,7 +142,7 @@ uint64_t shares_of_rows(uint64_t tokens, uint64_t q_heads)
 int head_width(uint64_t dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
 // Tiles are put in order where spans are given (a causal text is in order the other way round), where not all workgroups run at once anyway
-// (two fit a compute unit), and where one workgroup can rank them.
+// (two or three fit a compute unit), and where one workgroup can rank them.
 bool may_be_ordered(uint64_t tokens, uint64_t q_heads)
 {
     const uint64_t tiles = parts_of(tokens, ROWS_PER_GROUP);

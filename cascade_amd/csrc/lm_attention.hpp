@@ -12,13 +12,13 @@
 //                    mask and distance are a lane's own, with one exchange between the halves of the wave.
 //   d_k and d_v:     a lane holds one key and rows run along the registers; a workgroup owns its keys and walks the rows of all heads that share
 //                    them, or a part of those that is joined with the others' in a fixed order, so nothing is added by atomics and the results do not depend on the order of workgroups. The scores are
-//                    computed twice for that, once here and once for d_q (seven products instead of five).
+//                    computed twice for that, once here and once for d_q, which also takes its score gradients in two halves (eight products instead of five).
 // Tiles of keys or rows come straight from memory into LDS, one tile ahead. The 16-byte pieces of a tile's row stand at
 // places that keep both kinds of reads, sixteen rows' same piece and four rows' neighbouring pieces, in different banks.
 //
-// Measured on 12289 causal tokens, 16 heads of 128 that share 2 (bfloat16): forward 0.60 ms, 1030 TFLOP/s of what is seen; d_q 1.05 ms, 1180; d_k and d_v
-// 1.28 ms, 960. Bound by the matrix units (busy 53 % of the forward kernel's time) and the vector instructions beside them, which the two
-// waves of a SIMD overlap little; LDS is busy 27 %. A large product of the library does 1390.
+// Measured on 12289 causal tokens, 16 heads of 128 that share 2 (bfloat16, averages of six passes, the first of them cold): forward 0.66 ms, 940 TFLOP/s of what is seen;
+// d_q 1.12 ms, 1110; d_k and d_v 1.41 ms, 880; the fastest passes 0.62, 1.08 and 1.31. Bound by the matrix units (busy 57, 68 and 53 % of the three kernels' time) and the vector
+// instructions beside them (52, 58 and 35 %), which the two waves of a SIMD overlap little; LDS is busy 26 to 41 % without conflicts. A large product of the library does 1390.
 #pragma once
 #include "lm_common.hpp"
 
@@ -557,8 +557,10 @@ __device__ __attribute__((always_inline)) inline bool forward_rows(const Forward
     return lost || other_half(lost ? 1.f : 0.f) != 0.f;
 }
 
+// Up to three workgroups a compute unit where heads of 64 values are neither capped nor biased: the second pass would take registers for two (12289 tokens of 16 heads 376 us and 393). Bent ones
+// are shorter with two (8191 capped tokens of 16 heads 259 us and 282); those of 96 fit three as they are, those of 128 two, by their LDS.
 template <class Type, int DIM, int BEND>
-__global__ __launch_bounds__(256, 2) void attention_forward_kernel(ForwardCall call)
+__global__ __launch_bounds__(256, DIM == 64 && BEND == STRAIGHT ? 3 : 2) void attention_forward_kernel(ForwardCall call)
 {
     constexpr int KT = KEYS_PER_TILE;
     __shared__ __attribute__((aligned(16))) short k0s[KT * DIM], v0s[KT * DIM], k1s[KT * DIM], v1s[KT * DIM];
