@@ -9,8 +9,8 @@
 // Places past either matrix's end read as zeros and add nothing.
 //
 // Measured in tiles of 256 x 256 by eight waves (50257 x 8192 x 4096, bfloat16, 32-bit result stored): 1200 TFLOP/s, the library's product 1390, this loop without
-// loads 1530; the matrix units are busy 70 to 74 % of the time (60 for d_hidden, whose rows of 32-bit sums are read and written) at a clock that stands at 1.64 to 1.84 GHz under them. Slices of 32 k in four buffers were 5 %
-// slower, four waves of 128 x 128 each 11 %.
+// loads 1530; the matrix units are busy 70 to 74 % of the time (60 % in the products for d_hidden) at a clock that stands at 1.64 to 1.84 GHz under them. Slices of
+// 32 k in four buffers were 5 % slower, four waves of 128 x 128 each 11 %.
 #pragma once
 #include "lm_common.hpp"
 

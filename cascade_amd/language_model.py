@@ -8,6 +8,8 @@
 
 All take torch tensors on the GPU, enqueue kernels on the current stream of the tensors' device and return without waiting
 (include/cascade_lm.h; there is no CPU form). Scratch memory comes from torch's allocator and belongs to the stream.
+Only attend and next_token_loss are recorded by torch.autograd: the results of the others carry no graph, whatever their inputs want.
+Probabilities and the gradients of scores and logits are rounded to 16 bits on their way into the second products (include/cascade_lm.h has the errors).
 """
 import array
 import ctypes as C
@@ -144,7 +146,8 @@ def span_attention(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
     lo, hi: int32, row i sees the keys [lo[i], hi[i]) (None: 0 and i + 1); a row may see none. scale: of the products
     (None: 1 / sqrt(head_dim)); cap: scores become cap * tanh(score / cap) (0: they stay); slopes: float32 of each head, slopes[h] * |i - j|
     is taken off the score of row i and key j.
-    Returns (out of q's shape, lse float32 (heads, tokens)); rows that see nothing are zeros with lse -inf (csa_lm_attention_forward_dev)."""
+    Returns (out of q's shape, lse float32 (heads, tokens)); rows that see nothing are zeros with lse -inf. What a row may not see may hold anything,
+    infinities and NaN too; what sees those may become infinite or NaN throughout (csa_lm_attention_forward_dev). Without a graph: attend is the one for torch.autograd."""
     import torch
     a, device, keep = _describe(q, k, v, lo, hi, scale, cap, slopes)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -206,7 +209,7 @@ def linear_cross_entropy(hidden, weight, target):
 
     hidden: (tokens, dim), weight: (vocabulary, dim), bfloat16 or float16; target: int32, a token outside [0, vocabulary) has no loss.
     Returns float32 (loss, lse) of each token: lse is the logarithm of the sum of exponentials of its logits
-    (csa_lm_cross_entropy_forward_dev)."""
+    (csa_lm_cross_entropy_forward_dev). Without a graph: next_token_loss is the one for torch.autograd."""
     import torch
     kind = _check_entropy(hidden, weight, target)
     device = _on_gpu(hidden, weight, target)
