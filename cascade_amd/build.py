@@ -10,6 +10,7 @@ Run as `python -m cascade_amd.build`. hipcc cross-compiles for gfx950 without a 
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -42,9 +43,25 @@ def build_hip(extra_flags=()):
     return HIP_LIB
 
 
+LM_SOURCES = ("cascade_lm", "cascade_lm_rows")
+
+
 def build_lm():
+    """The sources of the language-model operators are compiled side by side: those of attention take a minute and a half."""
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    _run([hipcc, *COMMON_FLAGS, "-o", LM_LIB, os.path.join(CSRC, "cascade_lm.hip")])
+    compile_flags = [f for f in COMMON_FLAGS if f != "-shared"]
+    with tempfile.TemporaryDirectory() as scratch:
+        objects, running = [], []
+        for name in LM_SOURCES:
+            objects.append(os.path.join(scratch, name + ".o"))
+            cmd = [hipcc, *compile_flags, "-c", "-o", objects[-1], os.path.join(CSRC, name + ".hip")]
+            print("+", " ".join(cmd), flush=True)
+            running.append((cmd, subprocess.Popen(cmd)))
+        ended = [(cmd, one.wait()) for cmd, one in running]
+        for cmd, status in ended:
+            if status:
+                raise subprocess.CalledProcessError(status, cmd)
+        _run([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-o", LM_LIB, *objects])
     return LM_LIB
 
 

@@ -1,0 +1,361 @@
+// Host side of the language-model operators that go row by row: embeddings and norms. gfx950 only.
+#include "lm_host.hpp"
+
+#include "lm_embed.hpp"
+#include "lm_norm.hpp"
+
+#include <cmath>
+#include <type_traits>
+
+using namespace lm;
+
+namespace {
+
+template <class F>
+void with_values(int type, F f)
+{
+    if (type == CSA_LM_F32)
+        f(float());
+    else if (type == CSA_LM_F16)
+        f(f16_t());
+    else
+        f(bf16_t());
+}
+
+bool is_type(int type) { return type == CSA_LM_BF16 || type == CSA_LM_F16 || type == CSA_LM_F32; }
+uint64_t size_of(int type) { return type == CSA_LM_F32 ? 4 : 2; }
+
+// Rows of an array that is read: null and unaligned addresses, and strides that do not hold a row, are refused.
+int check_rows(const char* who, const char* what, const void* p, int64_t stride, uint64_t dim, int type)
+{
+    if (!p || !aligned(p, size_of(type)))
+        return fail(CSA_ERR_ARG, "%s: %s is null or unaligned", who, what);
+    if (stride < static_cast<int64_t>(dim) || stride >= 1 << 22)
+        return fail(CSA_ERR_ARG, "%s: a stride of %lld values for rows of %llu of %s", who, (long long)stride, (unsigned long long)dim, what);
+    return CSA_OK;
+}
+
+int check_result(const char* who, const char* what, const void* p, int type)
+{
+    return p && aligned(p, size_of(type)) ? CSA_OK : fail(CSA_ERR_ARG, "%s: %s is null or unaligned", who, what);
+}
+
+// ---- embeddings ----
+
+constexpr uint64_t MOST_ROWS = 1ull << 31, MOST_DIM = 1 << 22;
+
+template <class F>
+void with_tokens(uint32_t bytes, F f)
+{
+    if (bytes == 2)
+        f(uint16_t());
+    else
+        f(int32_t());
+}
+
+int check_embed(const char* who, int type, const void* tokens, uint32_t token_bytes, uint64_t n, uint64_t rows, uint64_t dim, float scale)
+{
+    if (!is_type(type))
+        return fail(CSA_ERR_ARG, "%s: type %d", who, type);
+    if (token_bytes != 2 && token_bytes != 4)
+        return fail(CSA_ERR_ARG, "%s: tokens of %u bytes", who, token_bytes);
+    if (!rows || dim < PIECE)
+        return fail(CSA_ERR_ARG, "%s: %llu rows of %llu values; a row has at least 8", who, (unsigned long long)rows, (unsigned long long)dim);
+    if (!std::isfinite(scale))
+        return fail(CSA_ERR_ARG, "%s: scale = %g", who, scale);
+    if (n && (!tokens || !aligned(tokens, token_bytes)))
+        return fail(CSA_ERR_ARG, "%s: tokens are null or unaligned", who);
+    if (n >= 1ull << 31 || rows >= MOST_ROWS || dim >= MOST_DIM || !launchable(parts_of(n * parts_of(dim, PIECE), PIECES_PER_GROUP), 256))
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens, %llu rows of %llu values", who, (unsigned long long)n, (unsigned long long)rows, (unsigned long long)dim);
+    return CSA_OK;
+}
+
+constexpr uint64_t RANKED = 16384; // tokens at most whose places are ranked in one launch
+
+// How a weight's gradient is made.
+struct EmbedPlan {
+    uint64_t lanes, slices, run, runs, groups, rows_each, zero_groups;
+    bool sorted; // by digits
+    int passes, bits;
+    uint64_t segment, segments;
+    EmbedPlan(uint64_t n, uint64_t rows, uint64_t dim)
+    {
+        const uint64_t pieces = parts_of(dim, PIECE);
+        for (lanes = 8; lanes < 64 && lanes < pieces; lanes *= 2) {
+        }
+        slices = parts_of(pieces, lanes);
+        // runs of 8 to 64 entries, so that there are about 4096 waves where the text has as many
+        for (run = 8; run < 64 && parts_of(n, 2 * run) * slices * lanes >= 4096 * 64; run *= 2) {
+        }
+        runs = parts_of(n, run);
+        groups = parts_of(runs * slices, 256 / lanes);
+        rows_each = 32768 / (2 * dim);
+        rows_each = rows_each < 1 ? 1 : rows_each > ZERO_ROWS ? ZERO_ROWS : rows_each;
+        zero_groups = parts_of(rows, rows_each);
+        sorted = n > RANKED;
+        int all = 1; // bits of a word, and of `rows`, which stands for what is none
+        while (rows >> all)
+            ++all;
+        passes = (all + DIGIT_BITS - 1) / DIGIT_BITS;
+        bits = (all + passes - 1) / passes;
+        segment = 256;
+        while (parts_of(n, segment) > MOST_SEGMENTS)
+            segment *= 2;
+        segments = parts_of(n, segment);
+    }
+    bool fits() const { return launchable(groups + zero_groups, 256) && launchable(runs * slices, 256); }
+};
+
+struct EmbedWork {
+    uint32_t *words[2], *places[2], *counts, *totals;
+    float *head, *tail;
+    uint64_t bytes;
+    EmbedWork(void* base, const EmbedPlan& plan, uint64_t n, uint64_t dim)
+    {
+        Carver c{static_cast<char*>(base)};
+        for (int i = 0; i < 2; ++i) {
+            words[i] = c.take<uint32_t>(i == 0 || (plan.sorted && plan.passes > 1) ? n : 0);
+            places[i] = c.take<uint32_t>(i == 0 || (plan.sorted && plan.passes > 1) ? n : 0);
+        }
+        counts = c.take<uint32_t>(plan.sorted ? plan.segments << plan.bits : 0);
+        totals = c.take<uint32_t>(plan.sorted ? 1ull << plan.bits : 0);
+        head = c.take<float>(plan.runs > 1 ? plan.runs * dim : 0);
+        tail = c.take<float>(plan.runs > 1 ? plan.runs * dim : 0);
+        bytes = c.used;
+    }
+};
+
+// The places of the text in the order of their words; which of the two arrays they end up in.
+template <class Token>
+int put_in_order(const Token* tokens, uint64_t n, uint64_t rows, const EmbedPlan& plan, const EmbedWork& w, hipStream_t s)
+{
+    if (!plan.sorted) {
+        rank_places_kernel<<<static_cast<uint32_t>(parts_of(n, 64)), 1024, 0, s>>>(tokens, static_cast<int>(n), static_cast<uint32_t>(rows), w.words[0], w.places[0]);
+        return 0;
+    }
+    const uint32_t digits = 1u << plan.bits, segments = static_cast<uint32_t>(plan.segments), groups = static_cast<uint32_t>(parts_of(plan.segments, 4));
+    int to = plan.passes % 2 ? 0 : 1;
+    for (int pass = 0; pass < plan.passes; ++pass, to ^= 1) {
+        const Entries<Token> e{pass ? nullptr : tokens, w.words[to ^ 1], w.places[to ^ 1], static_cast<int64_t>(n), static_cast<uint32_t>(rows)};
+        count_digits_kernel<<<groups, 256, 0, s>>>(e, static_cast<int64_t>(plan.segment), segments, pass * plan.bits, digits, w.counts);
+        sum_digits_kernel<<<digits, 256, 0, s>>>(w.counts, segments, w.totals);
+        move_digits_kernel<<<groups, 256, 0, s>>>(e, static_cast<int64_t>(plan.segment), segments, pass * plan.bits, digits, w.counts, w.totals, w.words[to], w.places[to]);
+    }
+    return to ^ 1;
+}
+
+template <class T, int LANES>
+void embed_sums(const EmbedPlan& plan, const EmbedSums& e, const T* d_out, T* d_weight, hipStream_t s)
+{
+    embed_sums_kernel<T, LANES><<<static_cast<uint32_t>(plan.groups + plan.zero_groups), 256, 0, s>>>(e, d_out, d_weight);
+    if (plan.runs > 1)
+        embed_join_kernel<T, LANES><<<static_cast<uint32_t>((plan.runs - 1) * plan.slices), 256, 0, s>>>(e, d_weight);
+}
+
+// ---- norms ----
+
+int check_norm(const char* who, int type, int stream_type, uint64_t tokens, uint64_t dim)
+{
+    if (!is_type(type) || (stream_type != type && stream_type != CSA_LM_F32))
+        return fail(CSA_ERR_ARG, "%s: values of type %d beside a residual of type %d", who, type, stream_type);
+    if (dim < PIECE || dim > NORM_DIM)
+        return fail(CSA_ERR_ARG, "%s: rows of %llu values; 8 to %llu are possible", who, (unsigned long long)dim, (unsigned long long)NORM_DIM);
+    if (!launchable(tokens, 256))
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens", who, (unsigned long long)tokens);
+    return CSA_OK;
+}
+
+// f(type, type of the residual, waves a row, pieces a lane) as types
+template <class F>
+void with_norm(int type, int stream_type, uint64_t dim, F f)
+{
+    with_values(type, [&](auto t) {
+        auto sized = [&](auto s) {
+            const auto one = std::integral_constant<int, 1>();
+            const auto four = std::integral_constant<int, 4>();
+            if (dim <= 512)
+                f(t, s, one, one);
+            else if (dim <= 1024)
+                f(t, s, one, std::integral_constant<int, 2>());
+            else if (dim <= 2048)
+                f(t, s, four, one);
+            else if (dim <= 4096)
+                f(t, s, four, std::integral_constant<int, 2>());
+            else if (dim <= 8192)
+                f(t, s, four, four);
+            else
+                f(t, s, four, std::integral_constant<int, 8>());
+        };
+        if (stream_type == CSA_LM_F32)
+            sized(float());
+        else
+            sized(t);
+    });
+}
+
+uint64_t norm_rows(uint64_t dim) { return dim <= 1024 ? 4 : 1; } // of a workgroup at a time
+
+uint64_t norm_groups(uint64_t tokens, uint64_t dim)
+{
+    const uint64_t all = parts_of(tokens, norm_rows(dim));
+    return all < NORM_GROUPS ? all : NORM_GROUPS;
+}
+
+} // namespace
+
+extern "C" {
+
+int csa_lm_embed_forward_dev(int type, const void* d_tokens, uint32_t token_bytes, uint64_t n, const void* d_weight, int64_t weight_stride, uint64_t rows, uint64_t dim,
+                             float scale, void* d_out, void* stream)
+{
+    const char* who = "csa_lm_embed_forward_dev";
+    if (int rc = check_embed(who, type, d_tokens, token_bytes, n, rows, dim, scale))
+        return rc;
+    if (int rc = check_rows(who, "the weight", d_weight, weight_stride, dim, type))
+        return rc;
+    if (n == 0)
+        return CSA_OK;
+    if (int rc = check_result(who, "out", d_out, type))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    with_values(type, [&](auto value) {
+        with_tokens(token_bytes, [&](auto token) {
+            typedef decltype(value) T;
+            typedef decltype(token) Token;
+            embed_kernel<<<static_cast<uint32_t>(parts_of(n * parts_of(dim, PIECE), PIECES_PER_GROUP)), 256, 0, s>>>(
+                static_cast<const Token*>(d_tokens), static_cast<int64_t>(n), static_cast<const T*>(d_weight), weight_stride, static_cast<uint32_t>(rows),
+                static_cast<int>(dim), scale, static_cast<T*>(d_out));
+        });
+    });
+    return launched(who);
+}
+
+uint64_t csa_lm_embed_backward_workspace(uint64_t n, uint64_t rows, uint64_t dim)
+{
+    if (n >= 1ull << 31 || !rows || rows >= MOST_ROWS || dim < PIECE || dim >= MOST_DIM)
+        return 0;
+    const EmbedPlan plan(n, rows, dim);
+    return plan.fits() ? EmbedWork(nullptr, plan, n, dim).bytes : 0;
+}
+
+int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_bytes, uint64_t n, const void* d_out_grad, int64_t out_grad_stride, uint64_t rows, uint64_t dim,
+                              float scale, void* d_weight_grad, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_embed_backward_dev";
+    if (int rc = check_embed(who, type, d_tokens, token_bytes, n, rows, dim, scale))
+        return rc;
+    if (n)
+        if (int rc = check_rows(who, "the gradient of out", d_out_grad, out_grad_stride, dim, type))
+            return rc;
+    if (int rc = check_result(who, "the gradient of the weight", d_weight_grad, type))
+        return rc;
+    const EmbedPlan plan(n, rows, dim);
+    if (!plan.fits())
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens, %llu rows of %llu values", who, (unsigned long long)n, (unsigned long long)rows, (unsigned long long)dim);
+    const EmbedWork w(d_work, plan, n, dim);
+    if (int rc = check_work(who, d_work, work_bytes, w.bytes))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    int in = 0;
+    if (n)
+        with_tokens(token_bytes, [&](auto token) { in = put_in_order(static_cast<const decltype(token)*>(d_tokens), n, rows, plan, w, s); });
+    const EmbedSums e{w.words[in], w.places[in], static_cast<int64_t>(n), static_cast<int64_t>(plan.run), static_cast<int64_t>(plan.runs), out_grad_stride,
+                      static_cast<int64_t>(plan.groups), static_cast<uint32_t>(rows), static_cast<uint32_t>(plan.rows_each), static_cast<int>(dim),
+                      static_cast<int>(plan.slices), scale, w.head, w.tail};
+    with_values(type, [&](auto value) {
+        typedef decltype(value) T;
+        const T* d_out = static_cast<const T*>(d_out_grad);
+        T* d_weight = static_cast<T*>(d_weight_grad);
+        if (plan.lanes == 8)
+            embed_sums<T, 8>(plan, e, d_out, d_weight, s);
+        else if (plan.lanes == 16)
+            embed_sums<T, 16>(plan, e, d_out, d_weight, s);
+        else if (plan.lanes == 32)
+            embed_sums<T, 32>(plan, e, d_out, d_weight, s);
+        else
+            embed_sums<T, 64>(plan, e, d_out, d_weight, s);
+    });
+    return launched(who);
+}
+
+int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const void* d_gain, float eps,
+                            uint64_t tokens, uint64_t dim, void* d_out, void* d_total, float* d_rstd, void* stream)
+{
+    const char* who = "csa_lm_norm_forward_dev";
+    if (int rc = check_norm(who, type, stream_type, tokens, dim))
+        return rc;
+    if (!(eps > 0.f) || !std::isfinite(eps))
+        return fail(CSA_ERR_ARG, "%s: eps = %g is not positive and finite", who, eps);
+    if (!d_residual && stream_type != type)
+        return fail(CSA_ERR_ARG, "%s: without a residual its type is that of x", who);
+    if (d_gain && !aligned(d_gain, size_of(type)))
+        return fail(CSA_ERR_ARG, "%s: the gain is unaligned", who);
+    if (tokens == 0)
+        return CSA_OK;
+    if (int rc = check_rows(who, "x", d_x, x_stride, dim, type))
+        return rc;
+    if (d_residual) {
+        if (int rc = check_rows(who, "the residual", d_residual, residual_stride, dim, stream_type))
+            return rc;
+        if (int rc = check_result(who, "total", d_total, stream_type))
+            return rc;
+    }
+    if (int rc = check_result(who, "out", d_out, type))
+        return rc;
+    if (int rc = check_result(who, "rstd", d_rstd, CSA_LM_F32))
+        return rc;
+    const NormCall c{d_x, d_residual, d_gain, x_stride, residual_stride, static_cast<int64_t>(tokens), static_cast<int>(dim), eps, d_out, d_total, d_rstd};
+    with_norm(type, stream_type, dim, [&](auto t, auto s, auto waves, auto items) {
+        norm_forward_kernel<decltype(t), decltype(s), waves(), items()>
+            <<<static_cast<uint32_t>(parts_of(tokens, norm_rows(dim))), 256, 0, static_cast<hipStream_t>(stream)>>>(c);
+    });
+    return launched(who);
+}
+
+uint64_t csa_lm_norm_backward_workspace(uint64_t tokens, uint64_t dim)
+{
+    return dim < PIECE || dim > NORM_DIM ? 0 : up(norm_groups(tokens, dim) * dim * sizeof(float), 256);
+}
+
+int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, int64_t out_grad_stride, const void* d_total, int64_t total_stride, const float* d_rstd,
+                             const void* d_gain, const void* d_total_grad, int64_t total_grad_stride, uint64_t tokens, uint64_t dim, void* d_x_grad, void* d_residual_grad,
+                             void* d_gain_grad, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_norm_backward_dev";
+    if (int rc = check_norm(who, type, stream_type, tokens, dim))
+        return rc;
+    if ((d_gain && !aligned(d_gain, size_of(type))) || !aligned(d_gain_grad, size_of(type)) || !aligned(d_x_grad, size_of(type)) ||
+        !aligned(d_residual_grad, size_of(stream_type)))
+        return fail(CSA_ERR_ARG, "%s: the gain or a gradient is unaligned", who);
+    if (tokens) {
+        if (int rc = check_rows(who, "the gradient of out", d_out_grad, out_grad_stride, dim, type))
+            return rc;
+        if (int rc = check_rows(who, "total", d_total, total_stride, dim, stream_type))
+            return rc;
+        if (d_total_grad)
+            if (int rc = check_rows(who, "the gradient of total", d_total_grad, total_grad_stride, dim, stream_type))
+                return rc;
+        if (int rc = check_result(who, "rstd", d_rstd, CSA_LM_F32))
+            return rc;
+    }
+    if (d_gain_grad)
+        if (int rc = check_work(who, d_work, work_bytes, csa_lm_norm_backward_workspace(tokens, dim)))
+            return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const uint64_t groups = norm_groups(tokens, dim);
+    float* parts = d_gain_grad ? static_cast<float*>(d_work) : nullptr;
+    const NormGradients c{d_out_grad, d_total, d_gain, d_total_grad, d_rstd, out_grad_stride, total_stride, total_grad_stride, static_cast<int64_t>(tokens),
+                          static_cast<int>(dim), d_x_grad, d_residual_grad, parts};
+    if (groups)
+        with_norm(type, stream_type, dim, [&](auto t, auto r, auto waves, auto items) {
+            norm_backward_kernel<decltype(t), decltype(r), waves(), items()><<<static_cast<uint32_t>(groups), 256, 0, s>>>(c);
+        });
+    if (d_gain_grad)
+        with_values(type, [&](auto t) {
+            norm_gain_kernel<<<static_cast<uint32_t>(parts_of(dim, 16)), 256, 0, s>>>(parts, static_cast<int64_t>(groups), static_cast<int>(dim),
+                                                                                     static_cast<decltype(t)*>(d_gain_grad));
+        });
+    return launched(who);
+}
+
+} // extern "C"

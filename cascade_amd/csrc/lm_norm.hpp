@@ -1,0 +1,205 @@
+// The root-mean-square norm with the addition of the residual in front of it:
+//   total = x + residual, as it is kept;  rstd = (mean of total^2 + eps)^-1/2;  out = total * rstd * gain,
+// and its gradients: with g = d_out * gain and u = total * rstd,
+//   d_total = rstd * (g - u * mean of g u) + what flows into total from elsewhere;  d_gain = sum over rows of d_out * u.
+//
+// Bound by memory: a row is read once and stays in registers, eight values a piece, between the sum over it and the product. A row of up to 1024 values is one
+// wave's, longer ones a workgroup's. Squares are summed in 64 bits, so that no value that the type holds overflows or vanishes.
+// The rows of d_gain are added up by the workgroup that meets them, in registers, and the workgroups' sums by a second kernel in a fixed order.
+#pragma once
+#include "lm_values.hpp"
+
+namespace lm {
+
+constexpr uint64_t NORM_DIM = 16384;    // values of a row that a workgroup's registers hold
+constexpr uint32_t NORM_GROUPS = 512;   // of the backward kernel: sums of d_gain that are added up behind it
+
+struct NormCall {
+    const void *x, *residual, *gain; // gain, residual: or null
+    int64_t x_stride, residual_stride, rows;
+    int dim;
+    double eps;
+    void *out, *total;
+    float* rstd;
+};
+
+// The sum over a row's lanes: a wave's, or all four waves' of the workgroup. lds: two sets of four, taken in turn, so that one barrier a row will do.
+template <int WAVES, class X>
+__device__ inline X row_sum(X x, X* lds)
+{
+    x = wave_sum(x);
+    if (WAVES == 1)
+        return x;
+    if (threadIdx.x % 64 == 0)
+        lds[threadIdx.x / 64] = x;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
+
+// T: of x, gain and out, S: of residual and total. WAVES of a row, ITEMS pieces a lane.
+template <class T, class S, int WAVES, int ITEMS>
+__global__ __launch_bounds__(256) void norm_forward_kernel(NormCall c)
+{
+    constexpr int LANES = WAVES * 64;
+    __shared__ double lds[4];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WAVES) + (WAVES == 1 ? threadIdx.x / 64 : 0);
+    if (row >= c.rows)
+        return;
+    const T* x = static_cast<const T*>(c.x) + row * c.x_stride;
+    Piece at[ITEMS];
+    float t[ITEMS][PIECE];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        at[i] = piece_at((i * LANES + threadIdx.x % LANES) * PIECE, c.dim);
+        load8(x + at[i].d, t[i]);
+    }
+    if (c.residual) {
+        const S* residual = static_cast<const S*>(c.residual) + row * c.residual_stride;
+        S* total = static_cast<S*>(c.total) + row * c.dim;
+        float r[ITEMS][PIECE];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            load8(residual + at[i].d, r[i]);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k)
+                t[i][k] = static_cast<float>(static_cast<S>(t[i][k] + r[i][k])); // the norm is that of the sum as it is kept, which is what the gradients see
+            if (at[i].mine)
+                store8(total + at[i].d, t[i]);
+        }
+    }
+    double sum = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int k = 0; k < PIECE; ++k) {
+            const double y = k < at[i].skip ? 0.f : t[i][k];
+            sum = fma(y, y, sum);
+        }
+    sum = row_sum<WAVES>(sum, lds);
+    const float rstd = static_cast<float>(1.0 / sqrt(sum / c.dim + c.eps));
+    if (threadIdx.x % LANES == 0)
+        c.rstd[row] = rstd;
+    T* out = static_cast<T*>(c.out) + row * c.dim;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        float g[PIECE] = {1, 1, 1, 1, 1, 1, 1, 1};
+        if (c.gain)
+            load8(static_cast<const T*>(c.gain) + at[i].d, g);
+#pragma unroll
+        for (int k = 0; k < PIECE; ++k)
+            t[i][k] = t[i][k] * rstd * g[k];
+        if (at[i].mine)
+            store8(out + at[i].d, t[i]);
+    }
+}
+
+struct NormGradients {
+    const void *d_out, *total, *gain, *d_total; // gain, d_total: or null
+    const float* rstd;
+    int64_t d_out_stride, total_stride, d_total_stride, rows;
+    int dim;
+    void *d_x, *d_residual; // of T and S; or null
+    float* parts;           // a row of dim sums of d_gain for every workgroup; null: not wanted
+};
+
+template <class T, class S, int WAVES, int ITEMS>
+__global__ __launch_bounds__(256) void norm_backward_kernel(NormGradients c)
+{
+    constexpr int LANES = WAVES * 64;
+    __shared__ float lds[2][4];
+    Piece at[ITEMS];
+    float gain[ITEMS][PIECE], sums[ITEMS][PIECE];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        at[i] = piece_at((i * LANES + threadIdx.x % LANES) * PIECE, c.dim);
+#pragma unroll
+        for (int k = 0; k < PIECE; ++k)
+            gain[i][k] = 1, sums[i][k] = 0;
+        if (c.gain)
+            load8(static_cast<const T*>(c.gain) + at[i].d, gain[i]);
+    }
+    int turn = 0;
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * (4 / WAVES) + (WAVES == 1 ? threadIdx.x / 64 : 0), step = static_cast<int64_t>(gridDim.x) * (4 / WAVES);
+    for (int64_t row = begin; row < c.rows; row += step, turn ^= 1) {
+        const T* d_out = static_cast<const T*>(c.d_out) + row * c.d_out_stride;
+        const S* total = static_cast<const S*>(c.total) + row * c.total_stride;
+        const S* d_total = static_cast<const S*>(c.d_total) + row * c.d_total_stride;
+        float g[ITEMS][PIECE], u[ITEMS][PIECE], more[ITEMS][PIECE] = {}, sum = 0;
+        const float rstd = c.rstd[row];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            load8(d_out + at[i].d, g[i]);
+            load8(total + at[i].d, u[i]);
+        }
+        if (c.d_total)
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                load8(d_total + at[i].d, more[i]);
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k) {
+                u[i][k] *= rstd;
+                sums[i][k] += g[i][k] * u[i][k];
+                g[i][k] *= gain[i][k];
+                sum += k < at[i].skip ? 0.f : g[i][k] * u[i][k];
+            }
+        sum = row_sum<WAVES>(sum, lds[turn]) / static_cast<float>(c.dim);
+        T* d_x = static_cast<T*>(c.d_x) + row * c.dim;
+        S* d_residual = static_cast<S*>(c.d_residual) + row * c.dim;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k)
+                g[i][k] = rstd * (g[i][k] - u[i][k] * sum) + more[i][k];
+            if (at[i].mine && c.d_x)
+                store8(d_x + at[i].d, g[i]);
+            if (at[i].mine && c.d_residual)
+                store8(d_residual + at[i].d, g[i]);
+        }
+    }
+    if (!c.parts)
+        return;
+    float* part = c.parts + static_cast<int64_t>(blockIdx.x) * c.dim;
+    if (WAVES == 1) { // the four waves' sums of the same values
+        __shared__ float all[4][ITEMS * 512];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (at[i].mine)
+#pragma unroll
+                for (int k = 0; k < PIECE; ++k)
+                    all[threadIdx.x / 64][at[i].d + k] = sums[i][k];
+        __syncthreads();
+        for (int d = threadIdx.x; d < c.dim; d += 256)
+            part[d] = (all[0][d] + all[1][d]) + (all[2][d] + all[3][d]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (at[i].mine)
+                store8(part + at[i].d, sums[i]);
+    }
+}
+
+// d_gain from the workgroups' sums: 16 values by 16 runs of them a workgroup.
+template <class T>
+__global__ __launch_bounds__(256) void norm_gain_kernel(const float* parts, int64_t count, int dim, T* d_gain)
+{
+    __shared__ float got[16][17];
+    const int x = threadIdx.x % 16, y = threadIdx.x / 16, d = blockIdx.x * 16 + x;
+    float sum = 0;
+    if (d < dim)
+#pragma unroll 8
+        for (int64_t p = y; p < count; p += 16)
+            sum += parts[p * dim + d];
+    got[y][x] = sum;
+    __syncthreads();
+    if (y == 0 && d < dim) {
+        for (int k = 1; k < 16; ++k)
+            sum += got[k][x];
+        d_gain[d] = static_cast<T>(sum);
+    }
+}
+
+} // namespace lm

@@ -1,14 +1,16 @@
 """Operators of a language model over the texts that this package sorts: uint16 tokens, a separator in front of every document.
 
   token_spans                        the keys that each position of a text may see, and the token it has to predict
+  embed_tokens (+ _backward)         the rows of a weight for the tokens of a text, and the gradient of the weight
+  residual_norm (+ _backward)        the addition of a residual and the root-mean-square norm of the sum
   span_attention (+ _backward)       attention of every position over its span of keys
   linear_cross_entropy (+ _backward) the loss of every target over the whole vocabulary, without keeping the logits
   clip_gradients                     the global norm of many gradients, and their clipping
-  attend, next_token_loss            the middle two for torch.autograd
+  embed, add_norm, attend, next_token_loss   the middle ones for torch.autograd
 
 All take torch tensors on the GPU, enqueue kernels on the current stream of the tensors' device and return without waiting
 (include/cascade_lm.h; there is no CPU form). Scratch memory comes from torch's allocator and belongs to the stream.
-Only attend and next_token_loss are recorded by torch.autograd: the results of the others carry no graph, whatever their inputs want.
+Only the latter are recorded by torch.autograd: the results of the others carry no graph, whatever their inputs want.
 Probabilities and the gradients of scores and logits are rounded to 16 bits on their way into the second products (include/cascade_lm.h has the errors).
 """
 import array
@@ -81,6 +83,13 @@ def _address(x):
     return (x.data_ptr() or None) if x is not None else None
 
 
+def _rows(x):
+    """x (rows, dim) with its values side by side, and the distance of its rows."""
+    if not ((x.stride(1) == 1 or x.shape[1] == 1) and (x.shape[0] <= 1 or x.shape[1] <= x.stride(0) < 1 << 22)):
+        x = x.contiguous()
+    return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
 def token_spans(text, separator=SEPARATOR):
     """text: n uint16 tokens (viewed as int16 is fine), one stretch of a corpus. Returns int32 tensors (lo, hi, target) of n values:
     position i may see the keys [lo[i], hi[i]), which begin at the last separator at or before i and end with i itself, and has to
@@ -95,6 +104,108 @@ def token_spans(text, separator=SEPARATOR):
     keep, work = _work(size, text)
     _enqueue(device, lib.csa_lm_spans_u16_dev, _address(text), n, int(separator), _address(lo), _address(hi), _address(target), work, size)
     return lo, hi, target
+
+
+# ---- embeddings ----
+
+
+def _check_tokens(tokens):
+    import torch
+    _check(tokens.dim() == 1 and tokens.is_contiguous() and (tokens.dtype == torch.int32 or (tokens.element_size() == 2 and not tokens.is_floating_point())),
+           "tokens: a dense vector of int32 or 16-bit tokens")
+
+
+def embed_tokens(tokens, weight, scale=1.0):
+    """scale * weight[tokens], rounded once: (n, dim) of weight's type. tokens: n int32, or 16-bit tokens as token_spans takes them (viewed as int16 is fine: they count as
+    unsigned); weight: (rows, dim), float32, bfloat16 or float16, dim at least 8. A token outside [0, rows) gives zeros (csa_lm_embed_forward_dev).
+    Without a graph: embed is the one for torch.autograd."""
+    _check_tokens(tokens)
+    _check(weight.dim() == 2, "weight: (rows, dim)")
+    kind, device = _type(weight.dtype), _on_gpu(tokens, weight)
+    rows, dim = weight.shape
+    weight, stride = _rows(weight)
+    out = weight.new_empty((tokens.numel(), dim))
+    lib = native.load()
+    _enqueue(device, lib.csa_lm_embed_forward_dev, kind, _address(tokens), tokens.element_size(), tokens.numel(), _address(weight), stride, rows, dim, float(scale),
+             _address(out))
+    return out
+
+
+def embed_tokens_backward(d_out, tokens, rows, scale=1.0):
+    """The gradient of the weight, (rows, dim) of d_out's type, for the gradient d_out (n, dim) of embed_tokens' result: the rows of d_out that belong to each word, added up in 32
+    bits in a fixed order, times scale; zeros for words that are not there (csa_lm_embed_backward_dev)."""
+    import torch
+    _check_tokens(tokens)
+    _check(d_out.dim() == 2 and d_out.shape[0] == tokens.numel(), "d_out: (tokens, dim)")
+    kind, device = _type(d_out.dtype), _on_gpu(d_out, tokens)
+    n, dim = d_out.shape
+    d_out, stride = _rows(d_out)
+    d_weight = d_out.new_empty((rows, dim))
+    lib = native.load()
+    size = lib.csa_lm_embed_backward_workspace(n, rows, dim)
+    scratch, work = _work(size, d_out)
+    _enqueue(device, lib.csa_lm_embed_backward_dev, kind, _address(tokens), tokens.element_size(), n, _address(d_out), stride, rows, dim, float(scale),
+             _address(d_weight), work, size)
+    return d_weight
+
+
+# ---- norms ----
+
+
+def _check_norm(x, gain):
+    _check(x.dim() == 2, "rows: (tokens, dim)")
+    _check(gain is None or (gain.dtype == x.dtype and gain.dim() == 1 and gain.numel() == x.shape[1] and gain.is_contiguous()), "gain: a value of x's type for each of a row")
+    return _type(x.dtype)
+
+
+def _check_stream(x, like, what):
+    import torch
+    _check(x.shape == like.shape and x.dtype in (like.dtype, torch.float32), f"{what}: like x, or in float32")
+    return _type(x.dtype)
+
+
+def residual_norm(x, residual=None, gain=None, eps=1e-6):
+    """The root-mean-square norm of x + residual.
+
+    x: (tokens, dim), float32, bfloat16 or float16, dim from 8 to 16384; residual: like x, or a stream of 32 bits beside an x of 16; gain: dim values of x's type (None: ones).
+    Returns (out, total, rstd): total = x + residual in the residual's type (x itself without one), rstd = 1 / sqrt(mean of total^2 + eps) float32 of every token, and out =
+    total * rstd * gain in x's type, from the rounded total (csa_lm_norm_forward_dev). Without a graph: add_norm is the one for torch.autograd."""
+    import torch
+    kind = _check_norm(x, gain)
+    stream = kind if residual is None else _check_stream(residual, x, "residual")
+    device = _on_gpu(x, residual, gain)
+    n, dim = x.shape
+    out, rstd = x.new_empty((n, dim)), x.new_empty(n, dtype=torch.float32)
+    total = x if residual is None else residual.new_empty((n, dim))
+    x, xs = _rows(x)
+    residual, rs = (None, 0) if residual is None else _rows(residual)
+    lib = native.load()
+    _enqueue(device, lib.csa_lm_norm_forward_dev, kind, stream, _address(x), xs, _address(residual), rs, _address(gain), float(eps), n, dim, _address(out),
+             None if residual is None else _address(total), _address(rstd))
+    return out, total, rstd
+
+
+def residual_norm_backward(d_out, total, rstd, gain=None, d_total=None, want_gain=True):
+    """Gradients (d_x, d_residual, d_gain) for the gradients d_out of out and d_total of total (None: total is used nowhere else); total and rstd as residual_norm returned them.
+    d_x is of d_out's type and d_residual of total's: one tensor where these are the same. d_gain is None without a gain, or if it is not wanted (csa_lm_norm_backward_dev)."""
+    import torch
+    kind = _check_norm(d_out, gain)
+    stream = _check_stream(total, d_out, "total")
+    _check(d_total is None or (d_total.shape == total.shape and d_total.dtype == total.dtype), "d_total: like total")
+    device = _on_gpu(d_out, total, rstd, gain, d_total)
+    n, dim = d_out.shape
+    _check(rstd.dim() == 1 and rstd.numel() == n and rstd.dtype == torch.float32 and rstd.is_contiguous(), "rstd: one float32 a token")
+    d_residual = total.new_empty((n, dim))
+    d_x = d_residual if stream == kind else d_out.new_empty((n, dim))
+    d_gain = gain.new_empty(dim) if gain is not None and want_gain else None
+    (d_out, gs), (total, ts) = _rows(d_out), _rows(total)
+    d_total, ds = (None, 0) if d_total is None else _rows(d_total)
+    lib = native.load()
+    size = lib.csa_lm_norm_backward_workspace(n, dim) if d_gain is not None else 0
+    scratch, work = _work(size, d_out)
+    _enqueue(device, lib.csa_lm_norm_backward_dev, kind, stream, _address(d_out), gs, _address(total), ts, _address(rstd), _address(gain), _address(d_total), ds, n, dim,
+             None if stream == kind else _address(d_x), _address(d_residual), _address(d_gain), work, size)
+    return d_x, d_residual, d_gain
 
 
 # ---- attention ----
@@ -179,13 +290,6 @@ def span_attention_backward(d_out, q, k, v, out, lse, lo=None, hi=None, scale=No
 
 
 # ---- cross entropy ----
-
-
-def _rows(x):
-    """x (rows, dim) with its values side by side, and the distance of its rows."""
-    if not ((x.stride(1) == 1 or x.shape[1] == 1) and (x.shape[0] <= 1 or x.shape[1] <= x.stride(0) < 1 << 22)):
-        x = x.contiguous()
-    return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def _entropy_work(lib, hidden, hs, weight, ws, flags):
@@ -278,6 +382,18 @@ def clip_gradients(grads, max_norm, out=None):
 # ---- for torch.autograd ----
 
 
+def embed(tokens, weight, scale=1.0):
+    """embed_tokens, differentiable in weight."""
+    return _functions()[2].apply(tokens, weight, scale)
+
+
+def add_norm(x, residual=None, gain=None, eps=1e-6):
+    """residual_norm's (out, total), differentiable in x, residual and gain. Without a residual total is x."""
+    if residual is None:
+        return _functions()[3].apply(x, None, gain, eps), x
+    return _functions()[3].apply(x, residual, gain, eps)
+
+
 def attend(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
     """span_attention's out, differentiable in q, k and v (slopes are constants: ones that want a gradient are refused)."""
     _check(slopes is None or not slopes.requires_grad, "slopes have no gradient here: detach them")
@@ -293,7 +409,7 @@ _made = None
 
 
 def _functions():
-    """The two torch.autograd functions, made when first asked for: this package imports torch only where it is used."""
+    """The torch.autograd functions, made when first asked for: this package imports torch only where it is used."""
     global _made
     if _made is not None:
         return _made
@@ -329,5 +445,40 @@ def _functions():
             d_hidden, d_weight = linear_cross_entropy_backward(d_loss.contiguous(), hidden, weight, target, lse, want[0], want[1])
             return d_hidden, d_weight, None
 
-    _made = (Attend, NextTokenLoss)
+    class Embed(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, tokens, weight, scale):
+            ctx.save_for_backward(tokens)
+            ctx.how = (weight.shape[0], scale)
+            return embed_tokens(tokens, weight, scale)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, d_out):
+            rows, scale = ctx.how
+            return None, embed_tokens_backward(d_out, *ctx.saved_tensors, rows, scale), None
+
+    class AddNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, residual, gain, eps):
+            out, total, rstd = residual_norm(x, residual, gain, eps)
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(total, rstd, gain)
+            ctx.x_type = x.dtype
+            return out if residual is None else (out, total)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, d_out, d_total=None):
+            total, rstd, gain = ctx.saved_tensors
+            if d_out is None and d_total is None:
+                return None, None, None, None
+            want_x, want_residual, want_gain, _ = ctx.needs_input_grad
+            if d_out is None:  # only total is used
+                d_x, d_residual, d_gain = d_total.to(ctx.x_type), d_total, None
+            else:
+                d_x, d_residual, d_gain = residual_norm_backward(d_out, total, rstd, gain, d_total, want_gain)
+            return d_x if want_x else None, d_residual if want_residual else None, d_gain, None
+
+    _made = (Attend, NextTokenLoss, Embed, AddNorm)
     return _made

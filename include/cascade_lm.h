@@ -29,7 +29,7 @@ extern "C" {
 typedef enum csa_lm_type {
     CSA_LM_BF16 = 0,
     CSA_LM_F16 = 1,
-    CSA_LM_F32 = 2 /* gradients to clip only: the matrix units multiply it at a sixteenth of the rate of the other two */
+    CSA_LM_F32 = 2 /* gradients to clip, embeddings and norms only: the matrix units multiply it at a sixteenth of the rate of the other two */
 } csa_lm_type;
 
 /* Flags of the *_workspace functions. */
@@ -84,6 +84,35 @@ int csa_lm_attention_forward_dev(const csa_lm_attention* a, csa_lm_heads out, fl
  * over the heads of q that share it. A key that no row sees gets zeros. */
 int csa_lm_attention_backward_dev(const csa_lm_attention* a, csa_lm_heads out, const float* d_lse, csa_lm_heads d_out, csa_lm_heads d_q,
                                   csa_lm_heads d_k, csa_lm_heads d_v, void* d_work, uint64_t work_bytes, void* stream);
+
+/* ---- embeddings ---- */
+
+/* out[i] = scale * weight[token[i]], in `type` (any csa_lm_type), zeros where token[i] is no row of the weight, [0, rows). d_tokens: n tokens of token_bytes = 2 (uint16,
+ * a text as it lies) or 4 (int32) bytes. weight: rows x dim, its rows weight_stride values apart (>= dim, below 2^22); out: n x dim, dense. dim >= 8; n, rows < 2^31. */
+int csa_lm_embed_forward_dev(int type, const void* d_tokens, uint32_t token_bytes, uint64_t n, const void* d_weight, int64_t weight_stride, uint64_t rows, uint64_t dim,
+                             float scale, void* d_out, void* stream);
+
+/* weight_grad[v] = scale * the sum over the places i of word v, in a fixed order and in 32 bits, of out_grad[i]; zeros for words that are not there. rows x dim, dense.
+ * Rows of out_grad whose token is no row may hold anything. */
+uint64_t csa_lm_embed_backward_workspace(uint64_t n, uint64_t rows, uint64_t dim);
+int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_bytes, uint64_t n, const void* d_out_grad, int64_t out_grad_stride, uint64_t rows, uint64_t dim,
+                              float scale, void* d_weight_grad, void* d_work, uint64_t work_bytes, void* stream);
+
+/* ---- norm of a residual stream ---- */
+
+/* total = x + residual, rounded to stream_type; rstd[i] = 1 / sqrt(mean of total[i]^2 + eps), of the rounded total, summed in 64 bits; out = total * rstd * gain.
+ * x, gain, out: `type` (any csa_lm_type); residual, total: stream_type, which is `type` or CSA_LM_F32. Rows of x and residual are *_stride values apart (>= dim, below
+ * 2^22), out and total are dense. d_residual NULL: total is x, d_total is not written and stream_type is `type`; d_gain NULL: ones. dim: 8 to 16384, eps > 0, tokens < 2^24. */
+int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const void* d_gain, float eps,
+                            uint64_t tokens, uint64_t dim, void* d_out, void* d_total, float* d_rstd, void* stream);
+
+/* With g = out_grad * gain and u = total * rstd: the gradient of x and residual alike is rstd * (g - u * mean(g u)) + total_grad (stream_type; NULL: none flows into total
+ * from elsewhere), and gain_grad = the sum over tokens of out_grad * u, in a fixed order. x_grad (type), residual_grad (stream_type) and gain_grad (type) are dense; any of them may be
+ * NULL. The workspace is for gain_grad and may be NULL without it. */
+uint64_t csa_lm_norm_backward_workspace(uint64_t tokens, uint64_t dim);
+int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, int64_t out_grad_stride, const void* d_total, int64_t total_stride, const float* d_rstd,
+                             const void* d_gain, const void* d_total_grad, int64_t total_grad_stride, uint64_t tokens, uint64_t dim, void* d_x_grad, void* d_residual_grad,
+                             void* d_gain_grad, void* d_work, uint64_t work_bytes, void* stream);
 
 /* ---- softmax cross entropy over a vocabulary ---- */
 
