@@ -6,9 +6,10 @@ package is the thin host-side mirror of the reference's builder interface for th
 """
 from . import _native, workloads
 from .gpu_saca import GPU_SACA, PartitionSorter, output_cut, pack_keys, partition_ids, sort_partition, sort_partitions, stage_slab
-from .language_model import (add_norm, attend, clip_gradients, embed, embed_tokens, embed_tokens_backward, linear_cross_entropy, linear_cross_entropy_backward,
-                             next_token_loss, residual_norm, residual_norm_backward, span_attention, span_attention_backward, token_spans)
+from .language_model import (add_norm, attend, clip_gradients, distillation_loss, embed, embed_tokens, embed_tokens_backward, linear_cross_entropy,
+                             linear_cross_entropy_backward, linear_distillation, linear_distillation_backward, next_token_loss, residual_norm, residual_norm_backward,
+                             span_attention, span_attention_backward, token_spans)
 
 __all__ = ["GPU_SACA", "PartitionSorter", "output_cut", "pack_keys", "partition_ids", "sort_partition", "sort_partitions", "stage_slab", "workloads", "_native",
-           "add_norm", "attend", "clip_gradients", "embed", "embed_tokens", "embed_tokens_backward", "linear_cross_entropy", "linear_cross_entropy_backward",
-           "next_token_loss", "residual_norm", "residual_norm_backward", "span_attention", "span_attention_backward", "token_spans"]
+           "add_norm", "attend", "clip_gradients", "distillation_loss", "embed", "embed_tokens", "embed_tokens_backward", "linear_cross_entropy",
+           "linear_cross_entropy_backward", "linear_distillation", "linear_distillation_backward", "next_token_loss", "residual_norm", "residual_norm_backward", "span_attention", "span_attention_backward", "token_spans"]

@@ -19,7 +19,7 @@ EXPORTS = (
     "csa_lm_attention_backward_dev", "csa_lm_cross_entropy_workspace", "csa_lm_cross_entropy_forward_dev",
     "csa_lm_cross_entropy_backward_dev", "csa_lm_clip_workspace", "csa_lm_clip_dev", "csa_lm_last_error", "csa_lm_embed_forward_dev",
     "csa_lm_embed_backward_workspace", "csa_lm_embed_backward_dev", "csa_lm_norm_forward_dev", "csa_lm_norm_backward_workspace",
-    "csa_lm_norm_backward_dev",
+    "csa_lm_norm_backward_dev", "csa_lm_distill_workspace", "csa_lm_distill_forward_dev", "csa_lm_distill_backward_dev",
 )
 
 
@@ -83,6 +83,12 @@ def load():
     lib.csa_lm_norm_backward_workspace.argtypes = [u64, u64]
     lib.csa_lm_norm_backward_dev.restype = i32
     lib.csa_lm_norm_backward_dev.argtypes = [i32, i32, vp, i64, vp, i64, vp, vp, vp, i64, u64, u64, vp, vp, vp, vp, u64, vp]
+    lib.csa_lm_distill_workspace.restype = u64
+    lib.csa_lm_distill_workspace.argtypes = [u64, u64, u64, u32, u32]
+    lib.csa_lm_distill_forward_dev.restype = i32
+    lib.csa_lm_distill_forward_dev.argtypes = [i32, vp, i64, vp, i64, vp, vp, u32, f32, u64, u64, u64, vp, vp, vp, u64, vp]
+    lib.csa_lm_distill_backward_dev.restype = i32
+    lib.csa_lm_distill_backward_dev.argtypes = [i32, vp, i64, vp, i64, vp, vp, u32, f32, vp, vp, u64, u64, u64, vp, i64, vp, i64, vp, u64, vp]
     lib.csa_lm_last_error.restype = C.c_char_p
     lib.csa_lm_last_error.argtypes = []
     _lib = lib

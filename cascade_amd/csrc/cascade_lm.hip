@@ -4,6 +4,7 @@
 #include "lm_attention.hpp"
 #include "lm_clip.hpp"
 #include "lm_cross_entropy.hpp"
+#include "lm_distill.hpp"
 #include "lm_spans.hpp"
 
 #include <algorithm>
@@ -336,6 +337,17 @@ int check_entropy(const char* who, bool backward, int type, const void* hidden, 
     return CSA_OK;
 }
 
+int check_entropy_gradients(const char* who, const float* d_lse, const float* d_loss_grad, uint64_t tokens, uint64_t dim, const void* d_hidden_grad, int64_t hidden_grad_stride,
+                            const void* d_weight_grad, int64_t weight_grad_stride)
+{
+    if (tokens && (!d_lse || !d_loss_grad || !aligned(d_lse, 4) || !aligned(d_loss_grad, 4)))
+        return fail(CSA_ERR_ARG, "%s: d_lse or d_loss_grad is null or unaligned", who);
+    if ((d_hidden_grad && (!aligned(d_hidden_grad, 2) || hidden_grad_stride < static_cast<int64_t>(dim))) ||
+        (d_weight_grad && (!aligned(d_weight_grad, 2) || weight_grad_stride < static_cast<int64_t>(dim))))
+        return fail(CSA_ERR_ARG, "%s: a gradient's address is odd or its stride below its rows' length", who);
+    return CSA_OK;
+}
+
 void lay_out(const void* in, int64_t in_stride, uint64_t rows, uint64_t dim, const int32_t* target, uint64_t vocab, short* out, uint64_t stride, hipStream_t s)
 {
     if (const uint64_t threads = rows * (stride / 8))
@@ -363,9 +375,10 @@ void entropy_forward(const EntropyPlan& plan, const EntropyWork& w, const Operan
         join_sums_kernel<16><<<static_cast<uint32_t>(parts_of(hidden.rows, 16)), 256, 0, s>>>(w.part, parts, w.target_logit, target, hidden.rows, weight.rows, loss, lse);
 }
 
-template <class Type>
-void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Operand& hidden, const Operand& weight, const int32_t* target, const float* lse,
-                      const float* d_loss, uint64_t dim, short* d_hidden, int64_t d_hidden_stride, short* d_weight, int64_t d_weight_stride, hipStream_t s)
+// Gradients from the pieces of P, each of which fill(logits, its rows' stride) leaves in w.p; w.scale is there.
+template <class Type, class Fill>
+void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Operand& hidden, const Operand& weight, const int32_t* target, uint64_t dim, short* d_hidden,
+                      int64_t d_hidden_stride, short* d_weight, int64_t d_weight_stride, hipStream_t s, Fill fill)
 {
     typedef WideLogits<Type> WL;
     typedef NarrowLogits<Type> NL;
@@ -375,18 +388,13 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
     typedef NarrowHidden<Type> NH;
     const int64_t tokens = hidden.rows, vocab = weight.rows, d = static_cast<int64_t>(dim), pd = static_cast<int64_t>(plan.padded_dim);
     const bool wide = d_weight && aligned(d_weight, 16) && d_weight_stride % 8 == 0;
-    loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss, target, tokens, vocab, Type::wide_range ? 1.f : 16384.f, w.scale);
     const uint32_t dt = static_cast<uint32_t>(parts_of(dim, WH::BN)), tt = static_cast<uint32_t>(parts_of(tokens, plan.narrow_hidden ? NH::BM : WH::BM));
     for (uint64_t piece = 0; piece < plan.pieces; ++piece) {
         const int64_t first = static_cast<int64_t>(piece * plan.piece_words), words = piece + 1 < plan.pieces ? static_cast<int64_t>(plan.piece_words) : vocab - first;
         const Operand part{static_cast<const short*>(weight.data) + first * weight.stride, weight.stride, words};
         const int64_t ps = static_cast<int64_t>(up(words, 8)); // rows of P
         const uint32_t lt = static_cast<uint32_t>(parts_of(words, plan.narrow_logits ? NL::BM : WL::BM)), nt = static_cast<uint32_t>(parts_of(tokens, plan.narrow_logits ? NL::BN : WL::BN));
-        const Logits l{part, hidden, pd, lt, nt, target, first};
-        if (plan.narrow_logits)
-            logit_gradients_kernel<NL, Type><<<lt * nt, NL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
-        else
-            logit_gradients_kernel<WL, Type><<<lt * nt, WL::THREADS, 0, s>>>(l, lse, d_loss, w.scale, vocab, w.p, ps);
+        fill(Logits{part, hidden, pd, lt, nt, target, first}, ps);
         if (d_weight) {
             const Operand p{w.p, ps, words}, kept{w.kept, pd, d};
             short* to = d_weight + first * d_weight_stride;
@@ -415,6 +423,59 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
         else
             join_shares_kernel<Type, 1><<<static_cast<uint32_t>(parts_of(quads, 256)), 256, 0, s>>>(w.shares, shares, tokens, d, pd, w.scale, d_hidden, d_hidden_stride);
     }
+}
+
+// ---- distillation ----
+
+// Words of a block of the teacher's entries: those of a wave's part of a tile.
+uint64_t block_words(const EntropyPlan& plan) { return plan.narrow_logits ? Lines<NarrowLogits<Bf16>>::LINE : Lines<WideLogits<Bf16>>::LINE; }
+
+struct TeacherWork {
+    int32_t *ids, *counts;
+    float *q, *entropy, *dots;
+    uint16_t* first;
+    uint64_t blocks, bytes;
+    TeacherWork(void* base, uint64_t before, const EntropyPlan& plan, uint64_t tokens, uint64_t vocab, uint64_t kept, bool backward)
+    {
+        Carver c{static_cast<char*>(base), before};
+        blocks = parts_of(vocab, block_words(plan));
+        ids = c.take<int32_t>(tokens * kept);
+        q = c.take<float>(tokens * kept);
+        first = c.take<uint16_t>(tokens * (blocks + 1));
+        counts = c.take<int32_t>(tokens);
+        entropy = c.take<float>(tokens);
+        dots = c.take<float>(backward ? 0 : parts_of(vocab, 256) * 4 * tokens);
+        bytes = c.used;
+    }
+    Teacher teacher(uint64_t kept) const { return {ids, q, first, static_cast<int64_t>(kept), static_cast<int64_t>(blocks)}; }
+};
+
+int check_teacher(const char* who, const int32_t* ids, const float* logits, uint32_t kept, float temperature, uint64_t tokens)
+{
+    if (kept < 1 || kept > MOST_KEPT)
+        return fail(CSA_ERR_ARG, "%s: %u logits a token; 1 to %u are possible", who, kept, MOST_KEPT);
+    if (!(temperature >= 1e-4f) || temperature > 1e4f)
+        return fail(CSA_ERR_ARG, "%s: temperature = %g is not between 1e-4 and 1e4", who, temperature);
+    if (tokens && (!ids || !logits || !aligned(ids, 4) || !aligned(logits, 4)))
+        return fail(CSA_ERR_ARG, "%s: the teacher's ids or logits are null or unaligned", who);
+    if (!launchable(parts_of(tokens, 4), 256))
+        return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens", who, (unsigned long long)tokens);
+    return CSA_OK;
+}
+
+void learn(const EntropyPlan& plan, const TeacherWork& w, const int32_t* ids, const float* logits, uint32_t kept, float temperature, uint64_t tokens, uint64_t vocab, hipStream_t s)
+{
+    const auto launch = [&](auto items) {
+        teacher_kernel<items()><<<static_cast<uint32_t>(parts_of(tokens, 4)), 256, 0, s>>>(
+            ids, logits, static_cast<int64_t>(tokens), static_cast<int>(kept), static_cast<int64_t>(vocab), 1.f / temperature, static_cast<int>(block_words(plan)),
+            static_cast<int64_t>(w.blocks), w.ids, w.q, w.first, w.counts, w.entropy);
+    };
+    if (kept <= 64)
+        launch(std::integral_constant<int, 1>());
+    else if (kept <= 256)
+        launch(std::integral_constant<int, 4>());
+    else
+        launch(std::integral_constant<int, 16>());
 }
 
 // ---- clipping ----
@@ -582,11 +643,8 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
     const char* who = "csa_lm_cross_entropy_backward_dev";
     if (int rc = check_entropy(who, true, type, d_hidden, hidden_stride, d_weight, weight_stride, d_target, tokens, dim, vocab))
         return rc;
-    if (tokens && (!d_lse || !d_loss_grad || !aligned(d_lse, 4) || !aligned(d_loss_grad, 4)))
-        return fail(CSA_ERR_ARG, "%s: d_lse or d_loss_grad is null or unaligned", who);
-    if ((d_hidden_grad && (!aligned(d_hidden_grad, 2) || hidden_grad_stride < static_cast<int64_t>(dim))) ||
-        (d_weight_grad && (!aligned(d_weight_grad, 2) || weight_grad_stride < static_cast<int64_t>(dim))))
-        return fail(CSA_ERR_ARG, "%s: a gradient's address is odd or its stride below its rows' length", who);
+    if (int rc = check_entropy_gradients(who, d_lse, d_loss_grad, tokens, dim, d_hidden_grad, hidden_grad_stride, d_weight_grad, weight_grad_stride))
+        return rc;
     const EntropyPlan plan(tokens, dim, vocab, true);
     const EntropyWork w(d_work, plan, tokens, vocab, true, !walks(d_weight, weight_stride, dim));
     if (int rc = check_work(who, d_work, work_bytes, w.bytes))
@@ -605,8 +663,123 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
         weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
     }
     with_type(type, [&](auto t) {
-        entropy_backward<decltype(t)>(plan, w, hidden, weight, d_target, d_lse, d_loss_grad, dim, static_cast<short*>(d_hidden_grad), hidden_grad_stride,
-                                      static_cast<short*>(d_weight_grad), weight_grad_stride, s);
+        typedef decltype(t) Type;
+        loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss_grad, d_target, hidden.rows, weight.rows, Type::wide_range ? 1.f : 16384.f, 1.f, w.scale);
+        entropy_backward<Type>(plan, w, hidden, weight, d_target, dim, static_cast<short*>(d_hidden_grad), hidden_grad_stride, static_cast<short*>(d_weight_grad),
+                               weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
+                                   typedef WideLogits<Type> W;
+                                   typedef NarrowLogits<Type> N;
+                                   if (plan.narrow_logits)
+                                       logit_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, d_lse, d_loss_grad, w.scale, weight.rows, w.p, ps);
+                                   else
+                                       logit_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, d_lse, d_loss_grad, w.scale, weight.rows, w.p, ps);
+                               });
+    });
+    return launched(who);
+}
+
+uint64_t csa_lm_distill_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t kept, uint32_t flags)
+{
+    const bool copies = flags & CSA_LM_COPY_ROWS || dim % 8, backward = flags & CSA_LM_BACKWARD;
+    if (!dim || !vocab || kept < 1 || kept > MOST_KEPT || !launchable(parts_of(tokens, 4), 256) ||
+        !entropy_fits(tokens, dim, vocab, backward, !copies ? 0 : tokens > vocab ? tokens : vocab))
+        return 0;
+    const EntropyPlan plan(tokens, dim, vocab, backward);
+    return TeacherWork(nullptr, EntropyWork(nullptr, plan, tokens, vocab, backward, copies).bytes, plan, tokens, vocab, kept, backward).bytes;
+}
+
+int csa_lm_distill_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_ids, const float* d_logits,
+                               uint32_t kept, float temperature, uint64_t tokens, uint64_t dim, uint64_t vocab, float* d_loss, float* d_lse, void* d_work, uint64_t work_bytes,
+                               void* stream)
+{
+    const char* who = "csa_lm_distill_forward_dev";
+    if (int rc = check_teacher(who, d_ids, d_logits, kept, temperature, tokens))
+        return rc;
+    if (int rc = check_entropy(who, false, type, d_hidden, hidden_stride, d_weight, weight_stride, d_ids, tokens, dim, vocab))
+        return rc;
+    if (tokens == 0)
+        return CSA_OK;
+    if (!d_loss || !d_lse || !aligned(d_loss, 4) || !aligned(d_lse, 4))
+        return fail(CSA_ERR_ARG, "%s: d_loss or d_lse is null or unaligned", who);
+    const EntropyPlan plan(tokens, dim, vocab, false);
+    const bool copies = !walks(d_hidden, hidden_stride, dim) || !walks(d_weight, weight_stride, dim);
+    const EntropyWork w(d_work, plan, tokens, vocab, false, copies);
+    const TeacherWork tw(d_work, w.bytes, plan, tokens, vocab, kept, false);
+    if (int rc = check_work(who, d_work, work_bytes, tw.bytes))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    Operand hidden{d_hidden, hidden_stride, static_cast<int64_t>(tokens)}, weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
+    if (!walks(d_hidden, hidden_stride, dim)) {
+        lay_out(d_hidden, hidden_stride, tokens, dim, nullptr, vocab, w.hidden, plan.padded_dim, s);
+        hidden = {w.hidden, static_cast<int64_t>(plan.padded_dim), hidden.rows};
+    }
+    if (!walks(d_weight, weight_stride, dim)) {
+        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
+    }
+    learn(plan, tw, d_ids, d_logits, kept, temperature, tokens, vocab, s);
+    with_type(type, [&](auto t) {
+        typedef WideLogits<decltype(t)> W;
+        typedef NarrowLogits<decltype(t)> N;
+        const uint32_t mt = static_cast<uint32_t>(parts_of(vocab, plan.narrow_logits ? N::BM : W::BM)), nt = static_cast<uint32_t>(parts_of(tokens, plan.narrow_logits ? N::BN : W::BN));
+        const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), mt, nt, nullptr, 0};
+        const float rate = 1.f / temperature;
+        if (plan.narrow_logits)
+            distill_sums_kernel<N><<<mt * nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, w.part, tw.dots);
+        else
+            distill_sums_kernel<W><<<mt * nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, w.part, tw.dots);
+        const int64_t parts = mt * static_cast<int64_t>(plan.narrow_logits ? N::WM : W::WM);
+        if (tokens <= 512) // as many lanes a token as in the cross entropy
+            join_distill_kernel<4><<<static_cast<uint32_t>(parts_of(tokens, 4)), 256, 0, s>>>(w.part, tw.dots, parts, tw.counts, tw.entropy, hidden.rows, d_loss, d_lse);
+        else
+            join_distill_kernel<16><<<static_cast<uint32_t>(parts_of(tokens, 16)), 256, 0, s>>>(w.part, tw.dots, parts, tw.counts, tw.entropy, hidden.rows, d_loss, d_lse);
+    });
+    return launched(who);
+}
+
+int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_ids, const float* d_logits,
+                                uint32_t kept, float temperature, const float* d_lse, const float* d_loss_grad, uint64_t tokens, uint64_t dim, uint64_t vocab,
+                                void* d_hidden_grad, int64_t hidden_grad_stride, void* d_weight_grad, int64_t weight_grad_stride, void* d_work, uint64_t work_bytes, void* stream)
+{
+    const char* who = "csa_lm_distill_backward_dev";
+    if (int rc = check_teacher(who, d_ids, d_logits, kept, temperature, tokens))
+        return rc;
+    if (int rc = check_entropy(who, true, type, d_hidden, hidden_stride, d_weight, weight_stride, d_ids, tokens, dim, vocab))
+        return rc;
+    if (int rc = check_entropy_gradients(who, d_lse, d_loss_grad, tokens, dim, d_hidden_grad, hidden_grad_stride, d_weight_grad, weight_grad_stride))
+        return rc;
+    const EntropyPlan plan(tokens, dim, vocab, true);
+    const EntropyWork w(d_work, plan, tokens, vocab, true, !walks(d_weight, weight_stride, dim));
+    const TeacherWork tw(d_work, w.bytes, plan, tokens, vocab, kept, true);
+    if (int rc = check_work(who, d_work, work_bytes, tw.bytes))
+        return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (tokens == 0) { // the sum over no tokens
+        if (d_weight_grad)
+            zero_rows_kernel<<<static_cast<uint32_t>(parts_of(vocab * dim, 1024)), 256, 0, s>>>(static_cast<short*>(d_weight_grad), weight_grad_stride, vocab, dim);
+        return launched(who);
+    }
+    learn(plan, tw, d_ids, d_logits, kept, temperature, tokens, vocab, s);
+    Operand weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
+    lay_out(d_hidden, hidden_stride, tokens, dim, tw.counts, vocab, w.kept, plan.padded_dim, s);
+    const Operand hidden{w.kept, static_cast<int64_t>(plan.padded_dim), static_cast<int64_t>(tokens)};
+    if (!walks(d_weight, weight_stride, dim)) {
+        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
+    }
+    with_type(type, [&](auto t) {
+        typedef decltype(t) Type;
+        const float rate = 1.f / temperature;
+        loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss_grad, tw.counts, hidden.rows, weight.rows, Type::wide_range ? 1.f : 16384.f, rate, w.scale);
+        entropy_backward<Type>(plan, w, hidden, weight, tw.counts, dim, static_cast<short*>(d_hidden_grad), hidden_grad_stride, static_cast<short*>(d_weight_grad),
+                               weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
+                                   typedef WideLogits<Type> W;
+                                   typedef NarrowLogits<Type> N;
+                                   if (plan.narrow_logits)
+                                       distill_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps);
+                                   else
+                                       distill_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps);
+                               });
     });
     return launched(who);
 }

@@ -81,6 +81,15 @@ __device__ inline float other_half(float x)
     return __builtin_bit_cast(float, threadIdx.x & 32 ? r[0] : r[1]);
 }
 
+// The sum over the lanes of a wave, in all of them.
+template <class X>
+__device__ inline X wave_sum(X x)
+{
+    for (int d = 32; d; d /= 2)
+        x += __shfl_xor(x, d);
+    return x;
+}
+
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 

@@ -87,6 +87,14 @@ __global__ __launch_bounds__(P::THREADS) void logit_sums_kernel(Logits l, float2
     }
 }
 
+// (maximum, sum of exponentials over it)
+__device__ inline void add_exponentials(float2& sum, float2 v)
+{
+    const float high = fmaxf(sum.x, v.x);
+    sum.y = sum.y * __builtin_amdgcn_exp2f((sum.x - high) * LOG2E) + v.y * __builtin_amdgcn_exp2f((v.x - high) * LOG2E);
+    sum.x = high;
+}
+
 // lse and loss from the waves' maxima and sums: TOKENS tokens by 256 / TOKENS runs of them a workgroup.
 template <int TOKENS>
 __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int64_t parts, const float* target_logit, const int32_t* target,
@@ -96,11 +104,6 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int6
     __shared__ float2 got[RUNS][TOKENS + 1];
     const int x = threadIdx.x % TOKENS, y = threadIdx.x / TOKENS;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * TOKENS + x;
-    auto add = [](float2& sum, float2 v) { // (maximum, sum of exponentials over it)
-        const float high = fmaxf(sum.x, v.x);
-        sum.y = sum.y * __builtin_amdgcn_exp2f((sum.x - high) * LOG2E) + v.y * __builtin_amdgcn_exp2f((v.x - high) * LOG2E);
-        sum.x = high;
-    };
     const float2 none = make_float2(-3.0e38f, 0.f);
     float2 sum = none;
     if (n < tokens)
@@ -111,13 +114,13 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int6
                 v[k] = p + k * RUNS < parts ? part[(p + k * RUNS) * tokens + n] : none;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                add(sum, v[k]);
+                add_exponentials(sum, v[k]);
         }
     got[y][x] = sum;
     for (int far = RUNS / 2; far; far /= 2) {
         __syncthreads();
         if (y < far) {
-            add(sum, got[y + far][x]);
+            add_exponentials(sum, got[y + far][x]);
             got[y][x] = sum;
         }
     }
@@ -129,8 +132,8 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int6
     }
 }
 
-// The factor of P, range / max |d_loss|, and its inverse. What is not finite among them has no say: its token is lost whatever the factor is, and takes nothing from the others.
-__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, const int32_t* target, int64_t tokens, int64_t vocab, float range, float* scale)
+// The factor of P, range / max |d_loss|, and what the products of P are scaled back with: its inverse times `rate`, the logits' own. What is not finite among them has no say: its token is lost whatever the factor is, and takes nothing from the others.
+__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, const int32_t* target, int64_t tokens, int64_t vocab, float range, float rate, float* scale)
 {
     __shared__ float tops[16];
     float top = 0.f;
@@ -147,7 +150,7 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, c
             top = fmaxf(top, tops[w]);
         const bool fine = top > 1e-30f && top < 1e30f; // both factors are ordinary numbers
         scale[0] = fine ? range / top : 1.f;
-        scale[1] = fine ? top / range : 1.f;
+        scale[1] = (fine ? top / range : 1.f) * rate;
     }
 }
 

@@ -45,13 +45,4 @@ __device__ inline void store8(T* p, const float (&x)[PIECE])
     *reinterpret_cast<Eight<T>*>(p) = raw;
 }
 
-// The sum over the lanes of a wave, in all of them.
-template <class X>
-__device__ inline X wave_sum(X x)
-{
-    for (int d = 32; d; d /= 2)
-        x += __shfl_xor(x, d);
-    return x;
-}
-
 } // namespace lm

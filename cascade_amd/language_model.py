@@ -5,8 +5,9 @@
   residual_norm (+ _backward)        the addition of a residual and the root-mean-square norm of the sum
   span_attention (+ _backward)       attention of every position over its span of keys
   linear_cross_entropy (+ _backward) the loss of every target over the whole vocabulary, without keeping the logits
+  linear_distillation (+ _backward)  the divergence of that softmax from a teacher's over the logits that it kept
   clip_gradients                     the global norm of many gradients, and their clipping
-  embed, add_norm, attend, next_token_loss   the middle ones for torch.autograd
+  embed, add_norm, attend, next_token_loss, distillation_loss   the middle ones for torch.autograd
 
 All take torch tensors on the GPU, enqueue kernels on the current stream of the tensors' device and return without waiting
 (include/cascade_lm.h; there is no CPU form). Scratch memory comes from torch's allocator and belongs to the stream.
@@ -292,20 +293,27 @@ def span_attention_backward(d_out, q, k, v, out, lse, lo=None, hi=None, scale=No
 # ---- cross entropy ----
 
 
-def _entropy_work(lib, hidden, hs, weight, ws, flags):
+def _entropy_work(lib, hidden, hs, weight, ws, flags, kept=None):
+    """The workspace of the cross entropy, or of the distillation from `kept` logits a token."""
     if hidden.data_ptr() % 16 or weight.data_ptr() % 16 or hs % 8 or ws % 8:
         flags |= native.CSA_LM_COPY_ROWS
-    size = lib.csa_lm_cross_entropy_workspace(hidden.shape[0], hidden.shape[1], weight.shape[0], flags)
+    n, dim, vocab = *hidden.shape, weight.shape[0]
+    size = lib.csa_lm_cross_entropy_workspace(n, dim, vocab, flags) if kept is None else lib.csa_lm_distill_workspace(n, dim, vocab, kept, flags)
     return (size, *_work(size, hidden))
+
+
+def _check_linear(hidden, weight):
+    _check(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1], "hidden: (tokens, dim), weight: (vocabulary, dim)")
+    _check(hidden.dtype == weight.dtype, "hidden and weight have to be of one type")
+    _check(weight.numel() > 0, "weight has to hold something")
+    return _matrix_type(hidden.dtype)
 
 
 def _check_entropy(hidden, weight, target):
     import torch
-    _check(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1], "hidden: (tokens, dim), weight: (vocabulary, dim)")
-    _check(hidden.dtype == weight.dtype, "hidden and weight have to be of one type")
-    _check(weight.numel() > 0, "weight has to hold something")
+    kind = _check_linear(hidden, weight)
     _check(target.dim() == 1 and target.numel() == hidden.shape[0] and target.dtype == torch.int32 and target.is_contiguous(), "target: one int32 a token")
-    return _matrix_type(hidden.dtype)
+    return kind
 
 
 def linear_cross_entropy(hidden, weight, target):
@@ -344,6 +352,60 @@ def linear_cross_entropy_backward(d_loss, hidden, weight, target, lse, want_hidd
     size, scratch, work = _entropy_work(lib, hidden, hs, weight, ws, native.CSA_LM_BACKWARD)
     _enqueue(device, lib.csa_lm_cross_entropy_backward_dev, kind, _address(hidden), hs, weight.data_ptr(), ws, _address(target), _address(lse), _address(d_loss), n,
              dim, weight.shape[0], _address(d_hidden), dim, _address(d_weight), dim, work, size)
+    return d_hidden, d_weight
+
+
+# ---- distillation ----
+
+
+def _check_teacher(hidden, ids, logits):
+    """The number of logits kept of a token, and the logits in 32 bits."""
+    import torch
+    _check(ids.dim() == 2 and ids.shape[0] == hidden.shape[0] and ids.dtype == torch.int32 and ids.is_contiguous(), "ids: int32 (tokens, kept)")
+    _check(logits.shape == ids.shape and logits.is_contiguous(), "logits: as many as ids")
+    _type(logits.dtype)
+    return ids.shape[1], logits.float()
+
+
+def linear_distillation(hidden, weight, ids, logits, temperature=1.0):
+    """The divergence of softmax(hidden @ weight.T / temperature) from a teacher's softmax over the logits that it kept of every token, without keeping the student's logits.
+
+    hidden: (tokens, dim), weight: (vocabulary, dim), bfloat16 or float16; ids: int32 (tokens, kept), words in any order; logits: the teacher's, as many, float32, bfloat16 or
+    float16. An id outside [0, vocabulary) or a logit of -infinity is no entry; a token without entries has no loss. With q the softmax of a token's logits / temperature over its entries
+    and z its own, the loss is the sum of q (ln q - ln softmax(z)): what an entire teacher would leave out is not counted. (A loss that is to weigh like a cross entropy is taken
+    times temperature squared.) Returns float32 (loss, lse) of each token: lse is the logarithm of the sum of exponentials of z (csa_lm_distill_forward_dev). Without a
+    graph: distillation_loss is the one for torch.autograd."""
+    import torch
+    kind = _check_linear(hidden, weight)
+    kept, logits = _check_teacher(hidden, ids, logits)
+    device = _on_gpu(hidden, weight, ids, logits)
+    n, dim = hidden.shape
+    loss, lse = hidden.new_empty(n, dtype=torch.float32), hidden.new_empty(n, dtype=torch.float32)
+    lib = native.load()
+    (hidden, hs), (weight, ws) = _rows(hidden), _rows(weight)
+    size, scratch, work = _entropy_work(lib, hidden, hs, weight, ws, 0, kept)
+    _enqueue(device, lib.csa_lm_distill_forward_dev, kind, _address(hidden), hs, weight.data_ptr(), ws, _address(ids), _address(logits), kept, float(temperature), n, dim,
+             weight.shape[0], _address(loss), _address(lse), work, size)
+    return loss, lse
+
+
+def linear_distillation_backward(d_loss, hidden, weight, ids, logits, lse, temperature=1.0, want_hidden=True, want_weight=True):
+    """Gradients (d_hidden, d_weight), of hidden's type, for the gradient d_loss (float32, one a token) of the losses; lse as linear_distillation returned it
+    (csa_lm_distill_backward_dev). A gradient that is not wanted is None; the teacher's logits have none."""
+    import torch
+    kind = _check_linear(hidden, weight)
+    kept, logits = _check_teacher(hidden, ids, logits)
+    device = _on_gpu(hidden, weight, ids, logits, d_loss, lse)
+    n, dim = hidden.shape
+    for x in (d_loss, lse):
+        _check(x.dim() == 1 and x.numel() == n and x.dtype == torch.float32 and x.is_contiguous(), "d_loss, lse: one float32 a token")
+    d_hidden = hidden.new_empty((n, dim)) if want_hidden else None
+    d_weight = weight.new_empty(weight.shape) if want_weight else None
+    lib = native.load()
+    (hidden, hs), (weight, ws) = _rows(hidden), _rows(weight)
+    size, scratch, work = _entropy_work(lib, hidden, hs, weight, ws, native.CSA_LM_BACKWARD, kept)
+    _enqueue(device, lib.csa_lm_distill_backward_dev, kind, _address(hidden), hs, weight.data_ptr(), ws, _address(ids), _address(logits), kept, float(temperature),
+             _address(lse), _address(d_loss), n, dim, weight.shape[0], _address(d_hidden), dim, _address(d_weight), dim, work, size)
     return d_hidden, d_weight
 
 
@@ -403,6 +465,12 @@ def attend(q, k, v, lo=None, hi=None, scale=None, cap=0.0, slopes=None):
 def next_token_loss(hidden, weight, target):
     """linear_cross_entropy's loss of every token, differentiable in hidden and weight."""
     return _functions()[1].apply(hidden, weight, target)
+
+
+def distillation_loss(hidden, weight, ids, logits, temperature=1.0):
+    """linear_distillation's loss of every token, differentiable in hidden and weight (the teacher is a constant: logits that want a gradient are refused)."""
+    _check(not logits.requires_grad, "the teacher's logits have no gradient here: detach them")
+    return _functions()[4].apply(hidden, weight, ids, logits, temperature)
 
 
 _made = None
@@ -480,5 +548,20 @@ def _functions():
                 d_x, d_residual, d_gain = residual_norm_backward(d_out, total, rstd, gain, d_total, want_gain)
             return d_x if want_x else None, d_residual if want_residual else None, d_gain, None
 
-    _made = (Attend, NextTokenLoss, Embed, AddNorm)
+    class Distillation(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, hidden, weight, ids, logits, temperature):
+            loss, lse = linear_distillation(hidden, weight, ids, logits, temperature)
+            ctx.save_for_backward(hidden, weight, ids, logits, lse)
+            ctx.temperature = temperature
+            return loss
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, d_loss):
+            want = ctx.needs_input_grad
+            d_hidden, d_weight = linear_distillation_backward(d_loss.contiguous(), *ctx.saved_tensors, ctx.temperature, want[0], want[1])
+            return d_hidden, d_weight, None, None, None
+
+    _made = (Attend, NextTokenLoss, Embed, AddNorm, Distillation)
     return _made
