@@ -74,7 +74,7 @@ def load():
     lib.csa_lm_embed_forward_dev.restype = i32
     lib.csa_lm_embed_forward_dev.argtypes = [i32, vp, u32, u64, vp, i64, u64, u64, f32, vp, vp]
     lib.csa_lm_embed_backward_workspace.restype = u64
-    lib.csa_lm_embed_backward_workspace.argtypes = [u64, u64, u64]
+    lib.csa_lm_embed_backward_workspace.argtypes = [i32, u64, u64, u64]
     lib.csa_lm_embed_backward_dev.restype = i32
     lib.csa_lm_embed_backward_dev.argtypes = [i32, vp, u32, u64, vp, i64, u64, u64, f32, vp, vp, u64, vp]
     lib.csa_lm_norm_forward_dev.restype = i32

@@ -40,6 +40,9 @@ int check_result(const char* who, const char* what, const void* p, int type)
     return p && aligned(p, size_of(type)) ? CSA_OK : fail(CSA_ERR_ARG, "%s: %s is null or unaligned", who, what);
 }
 
+// Results of more bytes go past the caches, the last of which holds 256 MB: nobody would find them there.
+constexpr uint64_t CACHED = 128ull << 20;
+
 // ---- embeddings ----
 
 constexpr uint64_t MOST_ROWS = 1ull << 31, MOST_DIM = 1 << 22;
@@ -53,57 +56,66 @@ void with_tokens(uint32_t bytes, F f)
         f(int32_t());
 }
 
+uint64_t pieces_of(int type, uint64_t dim) { return parts_of(dim, 16 / size_of(type)); }
+// Up to FEW pieces a lane takes one of them, beyond four, whose loads are under way together.
+constexpr uint64_t FEW = 1ull << 23;
+int embed_turns(int type, uint64_t n, uint64_t dim) { return n * pieces_of(type, dim) <= FEW ? 1 : 4; }
+uint64_t embed_groups(int type, uint64_t n, uint64_t dim) { return parts_of(n * pieces_of(type, dim), 256 * embed_turns(type, n, dim)); }
+
 int check_embed(const char* who, int type, const void* tokens, uint32_t token_bytes, uint64_t n, uint64_t rows, uint64_t dim, float scale)
 {
     if (!is_type(type))
         return fail(CSA_ERR_ARG, "%s: type %d", who, type);
     if (token_bytes != 2 && token_bytes != 4)
         return fail(CSA_ERR_ARG, "%s: tokens of %u bytes", who, token_bytes);
-    if (!rows || dim < PIECE)
+    if (!rows || dim < LEAST_DIM)
         return fail(CSA_ERR_ARG, "%s: %llu rows of %llu values; a row has at least 8", who, (unsigned long long)rows, (unsigned long long)dim);
     if (!std::isfinite(scale))
         return fail(CSA_ERR_ARG, "%s: scale = %g", who, scale);
     if (n && (!tokens || !aligned(tokens, token_bytes)))
         return fail(CSA_ERR_ARG, "%s: tokens are null or unaligned", who);
-    if (n >= 1ull << 31 || rows >= MOST_ROWS || dim >= MOST_DIM || !launchable(parts_of(n * parts_of(dim, PIECE), PIECES_PER_GROUP), 256))
+    if (n >= 1ull << 31 || rows >= MOST_ROWS || dim >= MOST_DIM || !launchable(embed_groups(type, n, dim), 256))
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens, %llu rows of %llu values", who, (unsigned long long)n, (unsigned long long)rows, (unsigned long long)dim);
     return CSA_OK;
 }
 
-constexpr uint64_t RANKED = 16384; // tokens at most whose places are ranked in one launch
+constexpr uint64_t RANKED = 8192; // tokens at most whose places are ranked in one launch
 
 // How a weight's gradient is made.
 struct EmbedPlan {
-    uint64_t lanes, slices, run, runs, groups, rows_each, zero_groups;
-    bool sorted; // by digits
+    uint64_t lanes, slices, run, block, blocks, groups, rows_each, zero_groups;
+    bool sorted;     // by digits
+    bool zero_first; // all of the gradient, beside the ordering's first kernel; otherwise the rows of words that are not there, beside the sums
     int passes, bits;
     uint64_t segment, segments;
-    EmbedPlan(uint64_t n, uint64_t rows, uint64_t dim)
+    EmbedPlan(int type, uint64_t n, uint64_t rows, uint64_t dim)
     {
-        const uint64_t pieces = parts_of(dim, PIECE);
+        const uint64_t pieces = pieces_of(type, dim);
         for (lanes = 8; lanes < 64 && lanes < pieces; lanes *= 2) {
         }
         slices = parts_of(pieces, lanes);
-        // runs of 8 to 64 entries, so that there are about 4096 waves where the text has as many
-        for (run = 8; run < 64 && parts_of(n, 2 * run) * slices * lanes >= 4096 * 64; run *= 2) {
+        // runs of 8 to 64 entries, so that there are about 2048 waves where the text has as many
+        for (run = 8; run < 64 && parts_of(n, 2 * run) * slices * lanes >= 2048 * 64; run *= 2) {
         }
-        runs = parts_of(n, run);
-        groups = parts_of(runs * slices, 256 / lanes);
-        rows_each = 32768 / (2 * dim);
+        block = run * (256 / lanes);
+        blocks = parts_of(n, block);
+        groups = blocks * slices;
+        rows_each = 16384 / dim;
         rows_each = rows_each < 1 ? 1 : rows_each > ZERO_ROWS ? ZERO_ROWS : rows_each;
-        zero_groups = parts_of(rows, rows_each);
         sorted = n > RANKED;
+        zero_first = n && (!sorted || rows >= 2 * n); // at most half of the rows are written twice
+        zero_groups = zero_first ? parts_of(rows * dim * size_of(type), ZERO_BYTES) : parts_of(rows, rows_each);
         int all = 1; // bits of a word, and of `rows`, which stands for what is none
         while (rows >> all)
             ++all;
         passes = (all + DIGIT_BITS - 1) / DIGIT_BITS;
         bits = (all + passes - 1) / passes;
-        segment = 256;
+        segment = TURN;
         while (parts_of(n, segment) > MOST_SEGMENTS)
-            segment *= 2;
+            segment += TURN;
         segments = parts_of(n, segment);
     }
-    bool fits() const { return launchable(groups + zero_groups, 256) && launchable(runs * slices, 256); }
+    bool fits() const { return launchable(groups + zero_groups, 256) && launchable(zero_groups + RANKED, 1024); }
 };
 
 struct EmbedWork {
@@ -119,27 +131,40 @@ struct EmbedWork {
         }
         counts = c.take<uint32_t>(plan.sorted ? plan.segments << plan.bits : 0);
         totals = c.take<uint32_t>(plan.sorted ? 1ull << plan.bits : 0);
-        head = c.take<float>(plan.runs > 1 ? plan.runs * dim : 0);
-        tail = c.take<float>(plan.runs > 1 ? plan.runs * dim : 0);
+        head = c.take<float>(plan.blocks > 1 ? plan.blocks * dim : 0);
+        tail = c.take<float>(plan.blocks > 1 ? plan.blocks * dim : 0);
         bytes = c.used;
     }
 };
 
-// The places of the text in the order of their words; which of the two arrays they end up in.
+// The places of the text in the order of their words, and zeros in d_weight where the plan says so; which of the two arrays they end up in.
 template <class Token>
-int put_in_order(const Token* tokens, uint64_t n, uint64_t rows, const EmbedPlan& plan, const EmbedWork& w, hipStream_t s)
+int put_in_order(const Token* tokens, uint64_t n, uint64_t rows, const EmbedPlan& plan, const EmbedWork& w, void* d_weight, uint64_t bytes, hipStream_t s)
 {
+    const uint32_t zero_groups = plan.zero_first ? static_cast<uint32_t>(plan.zero_groups) : 0;
     if (!plan.sorted) {
-        rank_places_kernel<<<static_cast<uint32_t>(parts_of(n, 64)), 1024, 0, s>>>(tokens, static_cast<int>(n), static_cast<uint32_t>(rows), w.words[0], w.places[0]);
+        const uint32_t groups = static_cast<uint32_t>(parts_of(n, RANKED_EACH));
+        const auto launch = [&](auto registers) {
+            rank_places_kernel<Token, registers()><<<groups + zero_groups, 1024, 0, s>>>(tokens, static_cast<int>(n), static_cast<uint32_t>(rows), w.words[0], w.places[0],
+                                                                                         Zeros{static_cast<char*>(d_weight), static_cast<int64_t>(bytes), groups});
+        };
+        if (n <= 1024)
+            launch(std::integral_constant<int, 1>());
+        else if (n <= 2048)
+            launch(std::integral_constant<int, 2>());
+        else
+            launch(std::integral_constant<int, RANKED / 1024>());
         return 0;
     }
-    const uint32_t digits = 1u << plan.bits, segments = static_cast<uint32_t>(plan.segments), groups = static_cast<uint32_t>(parts_of(plan.segments, 4));
+    const uint32_t digits = 1u << plan.bits, segments = static_cast<uint32_t>(plan.segments);
+    const int64_t segment = static_cast<int64_t>(plan.segment);
     int to = plan.passes % 2 ? 0 : 1;
     for (int pass = 0; pass < plan.passes; ++pass, to ^= 1) {
         const Entries<Token> e{pass ? nullptr : tokens, w.words[to ^ 1], w.places[to ^ 1], static_cast<int64_t>(n), static_cast<uint32_t>(rows)};
-        count_digits_kernel<<<groups, 256, 0, s>>>(e, static_cast<int64_t>(plan.segment), segments, pass * plan.bits, digits, w.counts);
+        const Zeros zeros{static_cast<char*>(d_weight), static_cast<int64_t>(bytes), segments};
+        count_digits_kernel<<<segments + (pass ? 0 : zero_groups), 256, 0, s>>>(e, segment, segments, pass * plan.bits, digits, w.counts, zeros);
         sum_digits_kernel<<<digits, 256, 0, s>>>(w.counts, segments, w.totals);
-        move_digits_kernel<<<groups, 256, 0, s>>>(e, static_cast<int64_t>(plan.segment), segments, pass * plan.bits, digits, w.counts, w.totals, w.words[to], w.places[to]);
+        move_digits_kernel<<<segments, 256, 0, s>>>(e, segment, segments, pass * plan.bits, digits, w.counts, w.totals, w.words[to], w.places[to]);
     }
     return to ^ 1;
 }
@@ -147,9 +172,9 @@ int put_in_order(const Token* tokens, uint64_t n, uint64_t rows, const EmbedPlan
 template <class T, int LANES>
 void embed_sums(const EmbedPlan& plan, const EmbedSums& e, const T* d_out, T* d_weight, hipStream_t s)
 {
-    embed_sums_kernel<T, LANES><<<static_cast<uint32_t>(plan.groups + plan.zero_groups), 256, 0, s>>>(e, d_out, d_weight);
-    if (plan.runs > 1)
-        embed_join_kernel<T, LANES><<<static_cast<uint32_t>((plan.runs - 1) * plan.slices), 256, 0, s>>>(e, d_weight);
+    embed_sums_kernel<T, LANES><<<static_cast<uint32_t>(plan.groups + (plan.zero_first ? 0 : plan.zero_groups)), 256, 0, s>>>(e, d_out, d_weight);
+    if (plan.blocks > 1)
+        embed_join_kernel<T, LANES><<<static_cast<uint32_t>((plan.blocks - 1) * plan.slices), 256, 0, s>>>(e, d_weight);
 }
 
 // ---- norms ----
@@ -158,9 +183,9 @@ int check_norm(const char* who, int type, int stream_type, uint64_t tokens, uint
 {
     if (!is_type(type) || (stream_type != type && stream_type != CSA_LM_F32))
         return fail(CSA_ERR_ARG, "%s: values of type %d beside a residual of type %d", who, type, stream_type);
-    if (dim < PIECE || dim > NORM_DIM)
+    if (dim < LEAST_DIM || dim > NORM_DIM)
         return fail(CSA_ERR_ARG, "%s: rows of %llu values; 8 to %llu are possible", who, (unsigned long long)dim, (unsigned long long)NORM_DIM);
-    if (!launchable(tokens, 256))
+    if (!launchable(tokens, 1024))
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens", who, (unsigned long long)tokens);
     return CSA_OK;
 }
@@ -171,20 +196,25 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
 {
     with_values(type, [&](auto t) {
         auto sized = [&](auto s) {
-            const auto one = std::integral_constant<int, 1>();
-            const auto four = std::integral_constant<int, 4>();
-            if (dim <= 512)
-                f(t, s, one, one);
-            else if (dim <= 1024)
-                f(t, s, one, std::integral_constant<int, 2>());
-            else if (dim <= 2048)
-                f(t, s, four, one);
-            else if (dim <= 4096)
-                f(t, s, four, std::integral_constant<int, 2>());
-            else if (dim <= 8192)
-                f(t, s, four, four);
-            else
-                f(t, s, four, std::integral_constant<int, 8>());
+            typedef std::integral_constant<int, 1> One;
+            typedef std::integral_constant<int, 2> Two;
+            typedef std::integral_constant<int, 4> Four;
+            typedef std::integral_constant<int, 16> Sixteen;
+            constexpr uint64_t V = PIECE<decltype(s)>;
+            if (dim <= 64 * V)
+                f(t, s, One(), One());
+            else if (dim <= 128 * V)
+                f(t, s, One(), Two());
+            else if (dim <= 256 * V)
+                f(t, s, Four(), One());
+            else if (dim <= 512 * V)
+                f(t, s, Four(), Two());
+            else if (dim <= 1024 * V)
+                f(t, s, Sixteen(), One());
+            else if (V == 8 || dim <= 2048 * V)
+                f(t, s, Sixteen(), Two());
+            else if constexpr (V == 4)
+                f(t, s, Sixteen(), Four());
         };
         if (stream_type == CSA_LM_F32)
             sized(float());
@@ -193,13 +223,10 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
     });
 }
 
-uint64_t norm_rows(uint64_t dim) { return dim <= 1024 ? 4 : 1; } // of a workgroup at a time
+uint64_t norm_rows(int waves) { return waves == 1 ? 4 : 1; } // of a workgroup at a time
 
-uint64_t norm_groups(uint64_t tokens, uint64_t dim)
-{
-    const uint64_t all = parts_of(tokens, norm_rows(dim));
-    return all < NORM_GROUPS ? all : NORM_GROUPS;
-}
+// Workgroups of the backward kernel, at most.
+uint64_t norm_groups(uint64_t tokens) { return tokens < NORM_GROUPS ? tokens : NORM_GROUPS; }
 
 } // namespace
 
@@ -222,19 +249,27 @@ int csa_lm_embed_forward_dev(int type, const void* d_tokens, uint32_t token_byte
         with_tokens(token_bytes, [&](auto token) {
             typedef decltype(value) T;
             typedef decltype(token) Token;
-            embed_kernel<<<static_cast<uint32_t>(parts_of(n * parts_of(dim, PIECE), PIECES_PER_GROUP)), 256, 0, s>>>(
-                static_cast<const Token*>(d_tokens), static_cast<int64_t>(n), static_cast<const T*>(d_weight), weight_stride, static_cast<uint32_t>(rows),
-                static_cast<int>(dim), scale, static_cast<T*>(d_out));
+            const auto launch = [&](auto turns, auto past) {
+                embed_kernel<T, Token, turns(), past()><<<static_cast<uint32_t>(embed_groups(type, n, dim)), 256, 0, s>>>(
+                    static_cast<const Token*>(d_tokens), static_cast<int64_t>(n), static_cast<const T*>(d_weight), weight_stride, static_cast<uint32_t>(rows),
+                    static_cast<int>(dim), scale, static_cast<T*>(d_out));
+            };
+            if (embed_turns(type, n, dim) == 1)
+                launch(std::integral_constant<int, 1>(), std::false_type());
+            else if (n * dim * sizeof(T) <= CACHED)
+                launch(std::integral_constant<int, 4>(), std::false_type());
+            else
+                launch(std::integral_constant<int, 4>(), std::true_type());
         });
     });
     return launched(who);
 }
 
-uint64_t csa_lm_embed_backward_workspace(uint64_t n, uint64_t rows, uint64_t dim)
+uint64_t csa_lm_embed_backward_workspace(int type, uint64_t n, uint64_t rows, uint64_t dim)
 {
-    if (n >= 1ull << 31 || !rows || rows >= MOST_ROWS || dim < PIECE || dim >= MOST_DIM)
+    if (!is_type(type) || n >= 1ull << 31 || !rows || rows >= MOST_ROWS || dim < LEAST_DIM || dim >= MOST_DIM)
         return 0;
-    const EmbedPlan plan(n, rows, dim);
+    const EmbedPlan plan(type, n, rows, dim);
     return plan.fits() ? EmbedWork(nullptr, plan, n, dim).bytes : 0;
 }
 
@@ -249,7 +284,7 @@ int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_byt
             return rc;
     if (int rc = check_result(who, "the gradient of the weight", d_weight_grad, type))
         return rc;
-    const EmbedPlan plan(n, rows, dim);
+    const EmbedPlan plan(type, n, rows, dim);
     if (!plan.fits())
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens, %llu rows of %llu values", who, (unsigned long long)n, (unsigned long long)rows, (unsigned long long)dim);
     const EmbedWork w(d_work, plan, n, dim);
@@ -258,8 +293,10 @@ int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_byt
     const hipStream_t s = static_cast<hipStream_t>(stream);
     int in = 0;
     if (n)
-        with_tokens(token_bytes, [&](auto token) { in = put_in_order(static_cast<const decltype(token)*>(d_tokens), n, rows, plan, w, s); });
-    const EmbedSums e{w.words[in], w.places[in], static_cast<int64_t>(n), static_cast<int64_t>(plan.run), static_cast<int64_t>(plan.runs), out_grad_stride,
+        with_tokens(token_bytes, [&](auto token) {
+            in = put_in_order(static_cast<const decltype(token)*>(d_tokens), n, rows, plan, w, d_weight_grad, rows * dim * size_of(type), s);
+        });
+    const EmbedSums e{w.words[in], w.places[in], static_cast<int64_t>(n), static_cast<int64_t>(plan.run), static_cast<int64_t>(plan.block), static_cast<int64_t>(plan.blocks), out_grad_stride,
                       static_cast<int64_t>(plan.groups), static_cast<uint32_t>(rows), static_cast<uint32_t>(plan.rows_each), static_cast<int>(dim),
                       static_cast<int>(plan.slices), scale, w.head, w.tail};
     with_values(type, [&](auto value) {
@@ -307,14 +344,14 @@ int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t 
     const NormCall c{d_x, d_residual, d_gain, x_stride, residual_stride, static_cast<int64_t>(tokens), static_cast<int>(dim), eps, d_out, d_total, d_rstd};
     with_norm(type, stream_type, dim, [&](auto t, auto s, auto waves, auto items) {
         norm_forward_kernel<decltype(t), decltype(s), waves(), items()>
-            <<<static_cast<uint32_t>(parts_of(tokens, norm_rows(dim))), 256, 0, static_cast<hipStream_t>(stream)>>>(c);
+            <<<static_cast<uint32_t>(parts_of(tokens, norm_rows(waves()))), NORM_THREADS<waves()>, 0, static_cast<hipStream_t>(stream)>>>(c);
     });
     return launched(who);
 }
 
 uint64_t csa_lm_norm_backward_workspace(uint64_t tokens, uint64_t dim)
 {
-    return dim < PIECE || dim > NORM_DIM ? 0 : up(norm_groups(tokens, dim) * dim * sizeof(float), 256);
+    return dim < LEAST_DIM || dim > NORM_DIM ? 0 : up(norm_groups(tokens) * dim * sizeof(float), 256);
 }
 
 int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, int64_t out_grad_stride, const void* d_total, int64_t total_stride, const float* d_rstd,
@@ -342,13 +379,14 @@ int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, 
         if (int rc = check_work(who, d_work, work_bytes, csa_lm_norm_backward_workspace(tokens, dim)))
             return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint64_t groups = norm_groups(tokens, dim);
+    uint64_t groups = 0;
     float* parts = d_gain_grad ? static_cast<float*>(d_work) : nullptr;
     const NormGradients c{d_out_grad, d_total, d_gain, d_total_grad, d_rstd, out_grad_stride, total_stride, total_grad_stride, static_cast<int64_t>(tokens),
                           static_cast<int>(dim), d_x_grad, d_residual_grad, parts};
-    if (groups)
+    if (tokens)
         with_norm(type, stream_type, dim, [&](auto t, auto r, auto waves, auto items) {
-            norm_backward_kernel<decltype(t), decltype(r), waves(), items()><<<static_cast<uint32_t>(groups), 256, 0, s>>>(c);
+            groups = norm_groups(parts_of(tokens, norm_rows(waves())));
+            norm_backward_kernel<decltype(t), decltype(r), waves(), items()><<<static_cast<uint32_t>(groups), NORM_THREADS<waves()>, 0, s>>>(c);
         });
     if (d_gain_grad)
         with_values(type, [&](auto t) {

@@ -3,7 +3,7 @@
 // and its gradients: with g = d_out * gain and u = total * rstd,
 //   d_total = rstd * (g - u * mean of g u) + what flows into total from elsewhere;  d_gain = sum over rows of d_out * u.
 //
-// Bound by memory: a row is read once and stays in registers, eight values a piece, between the sum over it and the product. A row of up to 1024 values is one
+// Bound by memory: a row is read once and stays in registers, in pieces, between the sum over it and the product. A row of up to 1024 values is one
 // wave's, longer ones a workgroup's. Squares are summed in 64 bits, so that no value that the type holds overflows or vanishes.
 // The rows of d_gain are added up by the workgroup that meets them, in registers, and the workgroups' sums by a second kernel in a fixed order.
 #pragma once
@@ -23,7 +23,11 @@ struct NormCall {
     float* rstd;
 };
 
-// The sum over a row's lanes: a wave's, or all four waves' of the workgroup. lds: two sets of four, taken in turn, so that one barrier a row will do.
+// Rows go to workgroups of four waves, a wave or all four a row, or of sixteen.
+template <int WAVES>
+constexpr int NORM_THREADS = WAVES == 16 ? 1024 : 256;
+
+// The sum over a row's lanes. lds: of a place for each wave, not that of the sum before.
 template <int WAVES, class X>
 __device__ inline X row_sum(X x, X* lds)
 {
@@ -33,47 +37,52 @@ __device__ inline X row_sum(X x, X* lds)
     if (threadIdx.x % 64 == 0)
         lds[threadIdx.x / 64] = x;
     __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    x = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+        x += lds[w];
+    return x;
 }
 
 // T: of x, gain and out, S: of residual and total. WAVES of a row, ITEMS pieces a lane.
 template <class T, class S, int WAVES, int ITEMS>
-__global__ __launch_bounds__(256) void norm_forward_kernel(NormCall c)
+__global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_forward_kernel(NormCall c)
 {
+    constexpr int V = PIECE<S>;
     constexpr int LANES = WAVES * 64;
-    __shared__ double lds[4];
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WAVES) + (WAVES == 1 ? threadIdx.x / 64 : 0);
+    __shared__ double lds[WAVES];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (WAVES == 1 ? 4 : 1) + (WAVES == 1 ? threadIdx.x / 64 : 0);
     if (row >= c.rows)
         return;
     const T* x = static_cast<const T*>(c.x) + row * c.x_stride;
     Piece at[ITEMS];
-    float t[ITEMS][PIECE];
+    float t[ITEMS][V];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        at[i] = piece_at((i * LANES + threadIdx.x % LANES) * PIECE, c.dim);
-        load8(x + at[i].d, t[i]);
+        at[i] = piece_at<V>((i * LANES + threadIdx.x % LANES) * V, c.dim);
+        load(x + at[i].d, t[i]);
     }
     if (c.residual) {
         const S* residual = static_cast<const S*>(c.residual) + row * c.residual_stride;
         S* total = static_cast<S*>(c.total) + row * c.dim;
-        float r[ITEMS][PIECE];
+        float r[ITEMS][V];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
-            load8(residual + at[i].d, r[i]);
+            load(residual + at[i].d, r[i]);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-            for (int k = 0; k < PIECE; ++k)
+            for (int k = 0; k < V; ++k)
                 t[i][k] = static_cast<float>(static_cast<S>(t[i][k] + r[i][k])); // the norm is that of the sum as it is kept, which is what the gradients see
             if (at[i].mine)
-                store8(total + at[i].d, t[i]);
+                store(total + at[i].d, t[i]);
         }
     }
     double sum = 0;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int k = 0; k < PIECE; ++k) {
+        for (int k = 0; k < V; ++k) {
             const double y = k < at[i].skip ? 0.f : t[i][k];
             sum = fma(y, y, sum);
         }
@@ -84,14 +93,17 @@ __global__ __launch_bounds__(256) void norm_forward_kernel(NormCall c)
     T* out = static_cast<T*>(c.out) + row * c.dim;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        float g[PIECE] = {1, 1, 1, 1, 1, 1, 1, 1};
-        if (c.gain)
-            load8(static_cast<const T*>(c.gain) + at[i].d, g);
+        float g[V];
 #pragma unroll
-        for (int k = 0; k < PIECE; ++k)
+        for (int k = 0; k < V; ++k)
+            g[k] = 1;
+        if (c.gain)
+            load(static_cast<const T*>(c.gain) + at[i].d, g);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
             t[i][k] = t[i][k] * rstd * g[k];
         if (at[i].mine)
-            store8(out + at[i].d, t[i]);
+            store(out + at[i].d, t[i]);
     }
 }
 
@@ -105,42 +117,43 @@ struct NormGradients {
 };
 
 template <class T, class S, int WAVES, int ITEMS>
-__global__ __launch_bounds__(256) void norm_backward_kernel(NormGradients c)
+__global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_backward_kernel(NormGradients c)
 {
+    constexpr int V = PIECE<S>;
     constexpr int LANES = WAVES * 64;
-    __shared__ float lds[2][4];
+    __shared__ float lds[2][WAVES];
     Piece at[ITEMS];
-    float gain[ITEMS][PIECE], sums[ITEMS][PIECE];
+    float gain[ITEMS][V], sums[ITEMS][V];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        at[i] = piece_at((i * LANES + threadIdx.x % LANES) * PIECE, c.dim);
+        at[i] = piece_at<V>((i * LANES + threadIdx.x % LANES) * V, c.dim);
 #pragma unroll
-        for (int k = 0; k < PIECE; ++k)
+        for (int k = 0; k < V; ++k)
             gain[i][k] = 1, sums[i][k] = 0;
         if (c.gain)
-            load8(static_cast<const T*>(c.gain) + at[i].d, gain[i]);
+            load(static_cast<const T*>(c.gain) + at[i].d, gain[i]);
     }
     int turn = 0;
-    const int64_t begin = static_cast<int64_t>(blockIdx.x) * (4 / WAVES) + (WAVES == 1 ? threadIdx.x / 64 : 0), step = static_cast<int64_t>(gridDim.x) * (4 / WAVES);
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * (WAVES == 1 ? 4 : 1) + (WAVES == 1 ? threadIdx.x / 64 : 0), step = static_cast<int64_t>(gridDim.x) * (WAVES == 1 ? 4 : 1);
     for (int64_t row = begin; row < c.rows; row += step, turn ^= 1) {
         const T* d_out = static_cast<const T*>(c.d_out) + row * c.d_out_stride;
         const S* total = static_cast<const S*>(c.total) + row * c.total_stride;
         const S* d_total = static_cast<const S*>(c.d_total) + row * c.d_total_stride;
-        float g[ITEMS][PIECE], u[ITEMS][PIECE], more[ITEMS][PIECE] = {}, sum = 0;
+        float g[ITEMS][V], u[ITEMS][V], more[ITEMS][V] = {}, sum = 0;
         const float rstd = c.rstd[row];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            load8(d_out + at[i].d, g[i]);
-            load8(total + at[i].d, u[i]);
+            load(d_out + at[i].d, g[i]);
+            load(total + at[i].d, u[i]);
         }
         if (c.d_total)
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
-                load8(d_total + at[i].d, more[i]);
+                load(d_total + at[i].d, more[i]);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int k = 0; k < PIECE; ++k) {
+            for (int k = 0; k < V; ++k) {
                 u[i][k] *= rstd;
                 sums[i][k] += g[i][k] * u[i][k];
                 g[i][k] *= gain[i][k];
@@ -152,24 +165,24 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormGradients c)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-            for (int k = 0; k < PIECE; ++k)
+            for (int k = 0; k < V; ++k)
                 g[i][k] = rstd * (g[i][k] - u[i][k] * sum) + more[i][k];
             if (at[i].mine && c.d_x)
-                store8(d_x + at[i].d, g[i]);
+                store(d_x + at[i].d, g[i]);
             if (at[i].mine && c.d_residual)
-                store8(d_residual + at[i].d, g[i]);
+                store(d_residual + at[i].d, g[i]);
         }
     }
     if (!c.parts)
         return;
     float* part = c.parts + static_cast<int64_t>(blockIdx.x) * c.dim;
     if (WAVES == 1) { // the four waves' sums of the same values
-        __shared__ float all[4][ITEMS * 512];
+        __shared__ float all[4][ITEMS * 64 * V];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (at[i].mine)
 #pragma unroll
-                for (int k = 0; k < PIECE; ++k)
+                for (int k = 0; k < V; ++k)
                     all[threadIdx.x / 64][at[i].d + k] = sums[i][k];
         __syncthreads();
         for (int d = threadIdx.x; d < c.dim; d += 256)
@@ -178,7 +191,7 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(NormGradients c)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (at[i].mine)
-                store8(part + at[i].d, sums[i]);
+                store(part + at[i].d, sums[i]);
     }
 }
 

@@ -1,12 +1,15 @@
-// Eight values at a time of rows of 16-bit or 32-bit floating point that may begin anywhere and have any length from eight on. Sixteen bytes that begin at no
-// multiple of sixteen are one access all the same; a row's last piece, where it is not whole, is moved back over the piece before it. What two pieces
-// hold both is computed and stored twice, with the same result, and left out of sums once.
+// Rows of 16-bit or 32-bit floating point, which may begin anywhere and have any length from eight on, in pieces of V values: sixteen bytes, or eight where a
+// 16-bit row goes with one of 32. What begins at no multiple of its size is one access all the same; a row's last piece, where it is not whole, is moved back over the piece
+// before it. What two pieces hold both is computed and stored twice, with the same result, and left out of sums once.
 #pragma once
 #include "lm_common.hpp"
 
 namespace lm {
 
-constexpr int PIECE = 8;
+constexpr int LEAST_DIM = 8;
+
+template <class T>
+constexpr int PIECE = 16 / sizeof(T);
 
 struct Piece {
     int d;     // its first value
@@ -14,35 +17,42 @@ struct Piece {
     bool mine; // the row has such a piece
 };
 
-// The piece that begins at `first`, a multiple of eight, of a row of dim >= 8 values. It is always there to be read.
+// The piece that begins at `first`, a multiple of V, of a row of dim values. It is always there to be read.
+template <int V>
 __device__ inline Piece piece_at(int first, int dim)
 {
-    const int d = first < dim - PIECE ? first : dim - PIECE;
-    return {d, first < dim ? first - d : PIECE, first < dim};
+    const int d = first < dim - V ? first : dim - V;
+    return {d, first < dim ? first - d : V, first < dim};
 }
 
-template <class T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-    T x[PIECE];
+template <class T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Several {
+    T x[V];
 };
 
-template <class T>
-__device__ inline void load8(const T* p, float (&x)[PIECE])
+template <class T, int V>
+__device__ inline void load(const T* p, float (&x)[V])
 {
-    const Eight<T> raw = *reinterpret_cast<const Eight<T>*>(p);
+    const Several<T, V> raw = *reinterpret_cast<const Several<T, V>*>(p);
 #pragma unroll
-    for (int k = 0; k < PIECE; ++k)
+    for (int k = 0; k < V; ++k)
         x[k] = static_cast<float>(raw.x[k]);
 }
 
-template <class T>
-__device__ inline void store8(T* p, const float (&x)[PIECE])
+// PAST: past the caches, for results that are larger than those.
+template <bool PAST = false, class T, int V>
+__device__ inline void store(T* p, const float (&x)[V])
 {
-    Eight<T> raw;
+    Several<T, V> raw;
 #pragma unroll
-    for (int k = 0; k < PIECE; ++k)
+    for (int k = 0; k < V; ++k)
         raw.x[k] = static_cast<T>(x[k]);
-    *reinterpret_cast<Eight<T>*>(p) = raw;
+    if constexpr (PAST) {
+        typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) * V / 4), aligned(sizeof(T))));
+        __builtin_nontemporal_store(__builtin_bit_cast(words, raw), reinterpret_cast<words*>(p));
+    } else {
+        *reinterpret_cast<Several<T, V>*>(p) = raw;
+    }
 }
 
 } // namespace lm

@@ -143,7 +143,7 @@ def embed_tokens_backward(d_out, tokens, rows, scale=1.0):
     d_out, stride = _rows(d_out)
     d_weight = d_out.new_empty((rows, dim))
     lib = native.load()
-    size = lib.csa_lm_embed_backward_workspace(n, rows, dim)
+    size = lib.csa_lm_embed_backward_workspace(kind, n, rows, dim)
     scratch, work = _work(size, d_out)
     _enqueue(device, lib.csa_lm_embed_backward_dev, kind, _address(tokens), tokens.element_size(), n, _address(d_out), stride, rows, dim, float(scale),
              _address(d_weight), work, size)

@@ -94,7 +94,7 @@ int csa_lm_embed_forward_dev(int type, const void* d_tokens, uint32_t token_byte
 
 /* weight_grad[v] = scale * the sum over the places i of word v, in a fixed order and in 32 bits, of out_grad[i]; zeros for words that are not there. rows x dim, dense.
  * Rows of out_grad whose token is no row may hold anything. */
-uint64_t csa_lm_embed_backward_workspace(uint64_t n, uint64_t rows, uint64_t dim);
+uint64_t csa_lm_embed_backward_workspace(int type, uint64_t n, uint64_t rows, uint64_t dim);
 int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_bytes, uint64_t n, const void* d_out_grad, int64_t out_grad_stride, uint64_t rows, uint64_t dim,
                               float scale, void* d_weight_grad, void* d_work, uint64_t work_bytes, void* stream);
 
@@ -102,7 +102,7 @@ int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_byt
 
 /* total = x + residual, rounded to stream_type; rstd[i] = 1 / sqrt(mean of total[i]^2 + eps), of the rounded total, summed in 64 bits; out = total * rstd * gain.
  * x, gain, out: `type` (any csa_lm_type); residual, total: stream_type, which is `type` or CSA_LM_F32. Rows of x and residual are *_stride values apart (>= dim, below
- * 2^22), out and total are dense. d_residual NULL: total is x, d_total is not written and stream_type is `type`; d_gain NULL: ones. dim: 8 to 16384, eps > 0, tokens < 2^24. */
+ * 2^22), out and total are dense. d_residual NULL: total is x, d_total is not written and stream_type is `type`; d_gain NULL: ones. dim: 8 to 16384, eps > 0, tokens < 2^22. */
 int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const void* d_gain, float eps,
                             uint64_t tokens, uint64_t dim, void* d_out, void* d_total, float* d_rstd, void* stream);
 
