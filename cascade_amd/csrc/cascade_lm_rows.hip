@@ -190,7 +190,7 @@ int check_norm(const char* who, int type, int stream_type, uint64_t tokens, uint
     return CSA_OK;
 }
 
-// f(type, type of the residual, waves a row, pieces a lane) as types
+// f(type, type of the residual, waves a row, pieces a lane) as types: pieces are of sixteen bytes of the residual, and a row has more than half as many as fit (lm_norm.hpp counts on it)
 template <class F>
 void with_norm(int type, int stream_type, uint64_t dim, F f)
 {
@@ -225,8 +225,13 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
 
 uint64_t norm_rows(int waves) { return waves == 1 ? 4 : 1; } // of a workgroup at a time
 
-// Workgroups of the backward kernel, at most.
-uint64_t norm_groups(uint64_t tokens) { return tokens < NORM_GROUPS ? tokens : NORM_GROUPS; }
+// Workgroups of the backward kernel, each with sums of d_gain of its own: as many as fit the compute units at once, or half as many where the sums would otherwise cost more than is
+// won (30000 rows of 100 values: 768 32 us, 512 34 us; 8192 of 4096: 512 95 us, 768 99 us; 2500 of 12000: 256 98 us, 512 105 us).
+uint64_t norm_groups(uint64_t tokens, int waves, int items, uint64_t stream_size)
+{
+    const uint64_t all = parts_of(tokens, norm_rows(waves)), most = waves == 16 && (items > 1 || stream_size < 4) ? 256 : waves < 16 && items == 1 ? NORM_GROUPS : 512;
+    return all < most ? all : most;
+}
 
 } // namespace
 
@@ -341,7 +346,8 @@ int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t 
         return rc;
     if (int rc = check_result(who, "rstd", d_rstd, CSA_LM_F32))
         return rc;
-    const NormCall c{d_x, d_residual, d_gain, x_stride, residual_stride, static_cast<int64_t>(tokens), static_cast<int>(dim), eps, d_out, d_total, d_rstd};
+    const NormCall c{d_x, d_residual, d_gain, x_stride, residual_stride, static_cast<int64_t>(tokens), static_cast<int>(dim), eps, d_out, d_total, d_rstd,
+                     tokens * dim * (size_of(type) + (d_residual ? size_of(stream_type) : 0)) > CACHED};
     with_norm(type, stream_type, dim, [&](auto t, auto s, auto waves, auto items) {
         norm_forward_kernel<decltype(t), decltype(s), waves(), items()>
             <<<static_cast<uint32_t>(parts_of(tokens, norm_rows(waves()))), NORM_THREADS<waves()>, 0, static_cast<hipStream_t>(stream)>>>(c);
@@ -351,7 +357,7 @@ int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t 
 
 uint64_t csa_lm_norm_backward_workspace(uint64_t tokens, uint64_t dim)
 {
-    return dim < LEAST_DIM || dim > NORM_DIM ? 0 : up(norm_groups(tokens) * dim * sizeof(float), 256);
+    return dim < LEAST_DIM || dim > NORM_DIM ? 0 : up((tokens < NORM_GROUPS ? tokens : NORM_GROUPS) * dim * sizeof(float), 256);
 }
 
 int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, int64_t out_grad_stride, const void* d_total, int64_t total_stride, const float* d_rstd,
@@ -382,10 +388,11 @@ int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, 
     uint64_t groups = 0;
     float* parts = d_gain_grad ? static_cast<float*>(d_work) : nullptr;
     const NormGradients c{d_out_grad, d_total, d_gain, d_total_grad, d_rstd, out_grad_stride, total_stride, total_grad_stride, static_cast<int64_t>(tokens),
-                          static_cast<int>(dim), d_x_grad, d_residual_grad, parts};
+                          static_cast<int>(dim), d_x_grad, d_residual_grad,
+                          tokens * dim * ((d_x_grad ? size_of(type) : 0) + (d_residual_grad ? size_of(stream_type) : 0)) > CACHED, parts};
     if (tokens)
         with_norm(type, stream_type, dim, [&](auto t, auto r, auto waves, auto items) {
-            groups = norm_groups(parts_of(tokens, norm_rows(waves())));
+            groups = norm_groups(tokens, waves(), items(), size_of(stream_type));
             norm_backward_kernel<decltype(t), decltype(r), waves(), items()><<<static_cast<uint32_t>(groups), NORM_THREADS<waves()>, 0, s>>>(c);
         });
     if (d_gain_grad)

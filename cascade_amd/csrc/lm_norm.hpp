@@ -12,7 +12,7 @@
 namespace lm {
 
 constexpr uint64_t NORM_DIM = 16384;    // values of a row that a workgroup's registers hold
-constexpr uint32_t NORM_GROUPS = 512;   // of the backward kernel: sums of d_gain that are added up behind it
+constexpr uint32_t NORM_GROUPS = 768;   // of the backward kernel at most: sums of d_gain that are added up behind it
 
 struct NormCall {
     const void *x, *residual, *gain; // gain, residual: or null
@@ -21,6 +21,7 @@ struct NormCall {
     double eps;
     void *out, *total;
     float* rstd;
+    bool past; // results go past the caches
 };
 
 // Rows go to workgroups of four waves, a wave or all four a row, or of sixteen.
@@ -44,6 +45,23 @@ __device__ inline X row_sum(X x, X* lds)
     return x;
 }
 
+// A lane's i-th piece. A row that has ITEMS pieces a lane is longer than half as many: the first half of them is whole.
+template <int V, int LANES, int ITEMS>
+__device__ inline Piece piece_of_row(int i, int dim)
+{
+    const int first = (i * LANES + threadIdx.x % LANES) * V;
+    return i < ITEMS / 2 ? Piece{first, 0, true} : piece_at<V>(first, dim);
+}
+
+template <class T, int V>
+__device__ inline void store_result(bool past, T* p, const float (&x)[V])
+{
+    if (past)
+        store<true>(p, x);
+    else
+        store(p, x);
+}
+
 // T: of x, gain and out, S: of residual and total. WAVES of a row, ITEMS pieces a lane.
 template <class T, class S, int WAVES, int ITEMS>
 __global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_forward_kernel(NormCall c)
@@ -59,7 +77,7 @@ __global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_forward_kernel(NormC
     float t[ITEMS][V];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        at[i] = piece_at<V>((i * LANES + threadIdx.x % LANES) * V, c.dim);
+        at[i] = piece_of_row<V, LANES, ITEMS>(i, c.dim);
         load(x + at[i].d, t[i]);
     }
     if (c.residual) {
@@ -75,7 +93,7 @@ __global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_forward_kernel(NormC
             for (int k = 0; k < V; ++k)
                 t[i][k] = static_cast<float>(static_cast<S>(t[i][k] + r[i][k])); // the norm is that of the sum as it is kept, which is what the gradients see
             if (at[i].mine)
-                store(total + at[i].d, t[i]);
+                store_result(c.past, total + at[i].d, t[i]);
         }
     }
     double sum = 0;
@@ -103,7 +121,7 @@ __global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_forward_kernel(NormC
         for (int k = 0; k < V; ++k)
             t[i][k] = t[i][k] * rstd * g[k];
         if (at[i].mine)
-            store(out + at[i].d, t[i]);
+            store_result(c.past, out + at[i].d, t[i]);
     }
 }
 
@@ -113,64 +131,94 @@ struct NormGradients {
     int64_t d_out_stride, total_stride, d_total_stride, rows;
     int dim;
     void *d_x, *d_residual; // of T and S; or null
+    bool past;              // these go past the caches
     float* parts;           // a row of dim sums of d_gain for every workgroup; null: not wanted
 };
 
+// A row's values stay as they lie in memory until they are used, before the sum over the row and after it. (The next row on its way while one is worked on took more registers than it gave:
+// 8192 values 84 -> 85 us, 12000 138 -> 188.)
 template <class T, class S, int WAVES, int ITEMS>
 __global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_backward_kernel(NormGradients c)
 {
-    constexpr int V = PIECE<S>;
-    constexpr int LANES = WAVES * 64;
+    constexpr int V = PIECE<S>, LANES = WAVES * 64;
     __shared__ float lds[2][WAVES];
     Piece at[ITEMS];
-    float gain[ITEMS][V], sums[ITEMS][V];
+    Raw<T, V> gain[ITEMS];
+    float sums[ITEMS][V];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        at[i] = piece_at<V>((i * LANES + threadIdx.x % LANES) * V, c.dim);
+        at[i] = piece_of_row<V, LANES, ITEMS>(i, c.dim);
 #pragma unroll
         for (int k = 0; k < V; ++k)
-            gain[i][k] = 1, sums[i][k] = 0;
+            sums[i][k] = 0;
         if (c.gain)
-            load(static_cast<const T*>(c.gain) + at[i].d, gain[i]);
+            gain[i] = load_raw<T, V>(static_cast<const T*>(c.gain) + at[i].d);
     }
-    int turn = 0;
-    const int64_t begin = static_cast<int64_t>(blockIdx.x) * (WAVES == 1 ? 4 : 1) + (WAVES == 1 ? threadIdx.x / 64 : 0), step = static_cast<int64_t>(gridDim.x) * (WAVES == 1 ? 4 : 1);
-    for (int64_t row = begin; row < c.rows; row += step, turn ^= 1) {
-        const T* d_out = static_cast<const T*>(c.d_out) + row * c.d_out_stride;
-        const S* total = static_cast<const S*>(c.total) + row * c.total_stride;
-        const S* d_total = static_cast<const S*>(c.d_total) + row * c.d_total_stride;
-        float g[ITEMS][V], u[ITEMS][V], more[ITEMS][V] = {}, sum = 0;
-        const float rstd = c.rstd[row];
+    struct Row {
+        Raw<T, V> d_out[ITEMS];
+        Raw<S, V> total[ITEMS], d_total[ITEMS];
+        float rstd;
+    } now;
+    auto load_row = [&](Row& to, int64_t row) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            load(d_out + at[i].d, g[i]);
-            load(total + at[i].d, u[i]);
+            to.d_out[i] = load_raw<T, V>(static_cast<const T*>(c.d_out) + row * c.d_out_stride + at[i].d);
+            to.total[i] = load_raw<S, V>(static_cast<const S*>(c.total) + row * c.total_stride + at[i].d);
         }
         if (c.d_total)
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
-                load(d_total + at[i].d, more[i]);
+                to.d_total[i] = load_raw<S, V>(static_cast<const S*>(c.d_total) + row * c.d_total_stride + at[i].d);
+        to.rstd = c.rstd[row];
+    };
+    // g and u of a piece
+    auto unpacked = [&](const Row& row, int i, float (&d_out)[V], float (&g)[V], float (&u)[V]) {
+        unpack<T, V>(row.d_out[i], d_out);
+        unpack<S, V>(row.total[i], u);
+        float a[V];
+        if (c.gain)
+            unpack<T, V>(gain[i], a);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+        for (int k = 0; k < V; ++k) {
+            u[k] *= row.rstd;
+            g[k] = c.gain ? d_out[k] * a[k] : d_out[k];
+        }
+    };
+    int turn = 0;
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * (WAVES == 1 ? 4 : 1) + (WAVES == 1 ? threadIdx.x / 64 : 0), step = static_cast<int64_t>(gridDim.x) * (WAVES == 1 ? 4 : 1);
+    for (int64_t row = begin; row < c.rows; row += step, turn ^= 1) {
+        load_row(now, row);
+        float sum = 0, d_out[V], g[V], u[V];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            unpacked(now, i, d_out, g, u);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                u[i][k] *= rstd;
-                sums[i][k] += g[i][k] * u[i][k];
-                g[i][k] *= gain[i][k];
-                sum += k < at[i].skip ? 0.f : g[i][k] * u[i][k];
+                sums[i][k] += d_out[k] * u[k];
+                sum += k < at[i].skip ? 0.f : g[k] * u[k];
             }
+        }
         sum = row_sum<WAVES>(sum, lds[turn]) / static_cast<float>(c.dim);
         T* d_x = static_cast<T*>(c.d_x) + row * c.dim;
         S* d_residual = static_cast<S*>(c.d_residual) + row * c.dim;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
+            asm volatile("" : "+v"(now.d_out[i]), "+v"(now.total[i])); // unpacked anew: kept, they would take twice the registers over the sum
+            unpacked(now, i, d_out, g, u);
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                g[i][k] = rstd * (g[i][k] - u[i][k] * sum) + more[i][k];
+                g[k] = now.rstd * (g[k] - u[k] * sum);
+            if (c.d_total) {
+                float more[V];
+                unpack<S, V>(now.d_total[i], more);
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    g[k] += more[k];
+            }
             if (at[i].mine && c.d_x)
-                store(d_x + at[i].d, g[i]);
+                store_result(c.past, d_x + at[i].d, g);
             if (at[i].mine && c.d_residual)
-                store(d_residual + at[i].d, g[i]);
+                store_result(c.past, d_residual + at[i].d, g);
         }
     }
     if (!c.parts)

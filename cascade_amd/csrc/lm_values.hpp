@@ -30,13 +30,29 @@ struct __attribute__((packed, aligned(sizeof(T)))) Several {
     T x[V];
 };
 
+// V values as they lie in memory.
+template <class T, int V>
+using Raw = uint32_t __attribute__((ext_vector_type(sizeof(T) * V / 4)));
+
+template <class T, int V>
+__device__ inline Raw<T, V> load_raw(const T* p)
+{
+    return __builtin_bit_cast(Raw<T, V>, *reinterpret_cast<const Several<T, V>*>(p));
+}
+
+template <class T, int V>
+__device__ inline void unpack(Raw<T, V> raw, float (&x)[V])
+{
+    const Several<T, V> y = __builtin_bit_cast(Several<T, V>, raw);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        x[k] = static_cast<float>(y.x[k]);
+}
+
 template <class T, int V>
 __device__ inline void load(const T* p, float (&x)[V])
 {
-    const Several<T, V> raw = *reinterpret_cast<const Several<T, V>*>(p);
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-        x[k] = static_cast<float>(raw.x[k]);
+    unpack<T, V>(load_raw<T, V>(p), x);
 }
 
 // PAST: past the caches, for results that are larger than those.
@@ -48,8 +64,8 @@ __device__ inline void store(T* p, const float (&x)[V])
     for (int k = 0; k < V; ++k)
         raw.x[k] = static_cast<T>(x[k]);
     if constexpr (PAST) {
-        typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) * V / 4), aligned(sizeof(T))));
-        __builtin_nontemporal_store(__builtin_bit_cast(words, raw), reinterpret_cast<words*>(p));
+        typedef uint32_t anywhere __attribute__((ext_vector_type(sizeof(T) * V / 4), aligned(sizeof(T))));
+        __builtin_nontemporal_store(__builtin_bit_cast(anywhere, raw), reinterpret_cast<anywhere*>(p));
     } else {
         *reinterpret_cast<Several<T, V>*>(p) = raw;
     }
