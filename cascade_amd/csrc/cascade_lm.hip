@@ -472,6 +472,8 @@ void learn(const EntropyPlan& plan, const TeacherWork& w, const int32_t* ids, co
     };
     if (kept <= 64)
         launch(std::integral_constant<int, 1>());
+    else if (kept <= 128)
+        launch(std::integral_constant<int, 2>());
     else if (kept <= 256)
         launch(std::integral_constant<int, 4>());
     else

@@ -137,9 +137,20 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, c
 {
     __shared__ float tops[16];
     float top = 0.f;
-    for (int64_t n = threadIdx.x; n < tokens; n += 1024)
-        if (target[n] >= 0 && target[n] < vocab && fabsf(d_loss[n]) < INFINITY)
-            top = fmaxf(top, fabsf(d_loss[n]));
+    for (int64_t n0 = threadIdx.x; n0 < tokens; n0 += 8 * 1024) { // eight loads on their way at a time
+        int32_t goal[8];
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t n = n0 + k * 1024 < tokens ? n0 + k * 1024 : n0;
+            goal[k] = target[n];
+            x[k] = fabsf(d_loss[n]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (goal[k] >= 0 && goal[k] < vocab && x[k] < INFINITY)
+                top = fmaxf(top, x[k]);
+    }
     for (int d = 32; d; d /= 2)
         top = fmaxf(top, __shfl_xor(top, d));
     if (threadIdx.x % 64 == 0)

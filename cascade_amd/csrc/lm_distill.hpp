@@ -181,15 +181,19 @@ __global__ __launch_bounds__(P::THREADS) void distill_sums_kernel(Logits l, Teac
                 dot += teacher.q[n * teacher.kept + e] * Words::word(lines, lane % 32, static_cast<int>(teacher.ids[n * teacher.kept + e] - mw));
             dot += other_half(dot);
         }
+        if (rows < Words::LINE) // words past the end, in a few tiles only
+#pragma unroll
+            for (int i = 0; i < P::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * i + 8 * (r / 4) + r % 4 >= left)
+                        sums[i][j][r] = -INFINITY;
         float top = -3.0e38f;
 #pragma unroll
         for (int i = 0; i < P::TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                if (32 * i + 8 * (r / 4) + r % 4 >= left) // words past the end
-                    sums[i][j][r] = -INFINITY;
+            for (int r = 0; r < 16; ++r)
                 top = fmaxf(top, sums[i][j][r]);
-            }
         const float steps = rate * LOG2E;
         float sum = 0.f;
 #pragma unroll
