@@ -458,26 +458,30 @@ int check_teacher(const char* who, const int32_t* ids, const float* logits, uint
         return fail(CSA_ERR_ARG, "%s: temperature = %g is not between 1e-4 and 1e4", who, temperature);
     if (tokens && (!ids || !logits || !aligned(ids, 4) || !aligned(logits, 4)))
         return fail(CSA_ERR_ARG, "%s: the teacher's ids or logits are null or unaligned", who);
-    if (!launchable(parts_of(tokens, 4), 256))
+    if (!launchable(tokens, 256))
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens", who, (unsigned long long)tokens);
     return CSA_OK;
 }
 
 void learn(const EntropyPlan& plan, const TeacherWork& w, const int32_t* ids, const float* logits, uint32_t kept, float temperature, uint64_t tokens, uint64_t vocab, hipStream_t s)
 {
-    const auto launch = [&](auto items) {
-        teacher_kernel<items()><<<static_cast<uint32_t>(parts_of(tokens, 4)), 256, 0, s>>>(
+    const auto launch = [&](auto waves, auto items) {
+        teacher_kernel<waves(), items()><<<static_cast<uint32_t>(parts_of(tokens, 4 / waves())), 256, 0, s>>>(
             ids, logits, static_cast<int64_t>(tokens), static_cast<int>(kept), static_cast<int64_t>(vocab), 1.f / temperature, static_cast<int>(block_words(plan)),
             static_cast<int64_t>(w.blocks), w.ids, w.q, w.first, w.counts, w.entropy);
     };
-    if (kept <= 64)
-        launch(std::integral_constant<int, 1>());
-    else if (kept <= 128)
-        launch(std::integral_constant<int, 2>());
+    // few tokens leave compute units without work: four waves for each, which share out the blocks
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    typedef std::integral_constant<int, 4> Four;
+    if (kept <= 64 && tokens > 1024)
+        launch(One(), One());
+    else if (kept <= 128 && tokens > 1024)
+        launch(One(), Two());
     else if (kept <= 256)
-        launch(std::integral_constant<int, 4>());
+        launch(Four(), One());
     else
-        launch(std::integral_constant<int, 16>());
+        launch(Four(), Four());
 }
 
 // ---- clipping ----
@@ -683,7 +687,7 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
 uint64_t csa_lm_distill_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t kept, uint32_t flags)
 {
     const bool copies = flags & CSA_LM_COPY_ROWS || dim % 8, backward = flags & CSA_LM_BACKWARD;
-    if (!dim || !vocab || kept < 1 || kept > MOST_KEPT || !launchable(parts_of(tokens, 4), 256) ||
+    if (!dim || !vocab || kept < 1 || kept > MOST_KEPT || !launchable(tokens, 256) ||
         !entropy_fits(tokens, dim, vocab, backward, !copies ? 0 : tokens > vocab ? tokens : vocab))
         return 0;
     const EntropyPlan plan(tokens, dim, vocab, backward);

@@ -141,7 +141,7 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
  * logit is -infinity, is none, whatever else it holds; a token without entries has no loss. With q = the softmax over a token's entries of logits / temperature, and z[n][v] = sum_d hidden[n][d]
  * weight[v][d] / temperature, which are never kept,
  *   d_lse[n] = ln sum_v exp(z[n][v]);   d_loss[n] = sum over its entries of q (ln q - z[n][id]) + d_lse[n], 0 without entries.
- * A word that is listed twice counts with both. Arguments, copies and limits are those of the cross entropy, with fewer than 2^26 tokens; temperature: 1e-4 to 1e4. */
+ * A word that is listed twice counts with both. Arguments, copies and limits are those of the cross entropy, with fewer than 2^24 tokens; temperature: 1e-4 to 1e4. */
 uint64_t csa_lm_distill_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab, uint32_t kept, uint32_t flags);
 int csa_lm_distill_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_ids, const float* d_logits,
                                uint32_t kept, float temperature, uint64_t tokens, uint64_t dim, uint64_t vocab, float* d_loss, float* d_lse, void* d_work, uint64_t work_bytes,

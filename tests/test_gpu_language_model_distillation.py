@@ -121,6 +121,7 @@ def test_distillation_over_the_corpus_vocabulary():
 def test_distillation_in_pieces_of_the_vocabulary():
     """More than one piece of the vocabulary, and shares of d_hidden, in both tile widths."""
     check_distillation(6000, 64, 50257, 16, torch.bfloat16, seed=5)
+    check_distillation(1500, 64, 3000, 100, torch.float16, seed=6)
 
 
 def test_distillation_of_uneven_weights():
