@@ -4,9 +4,10 @@ The corpus is the benchmark's token text (uint16, 0xFFFF in front of every docum
 sorted on the GPU; neighbours in the suffix array that begin with the same tokens are repeated passages, and a position
 whose passage also stands earlier in the corpus is left out of the loss. The training step then packs a stretch of the corpus as it
 lies, without padding: spans keep attention inside documents, the loss runs over the whole vocabulary without keeping its logits, and the
-gradients are clipped by their global norm.
+gradients are clipped by their global norm. With --student, a smaller model then learns from the trained one: from the largest logits that the
+teacher has for every token, in place of the tokens that follow.
 
-    python examples/train_on_documents.py [--tokens 200000] [--steps 20] [--length 4096]
+    python examples/train_on_documents.py [--tokens 200000] [--steps 20] [--length 4096] [--student 10]
 """
 import argparse
 import os
@@ -61,23 +62,41 @@ class Model(torch.nn.Module):
         # the further away a key is, the less it counts: a different rate for each head, in place of positions
         self.register_buffer("slopes", torch.exp2(-8.0 * torch.arange(1, heads + 1) / heads))
 
-    @staticmethod
-    def norm(x):
-        return (x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + 1e-6)).to(x.dtype)
+    def hidden(self, tokens, lo, hi):
+        """What the vocabulary's weight is multiplied with, of every token. Each norm takes the addition in front of it along."""
+        y, x = cascade_amd.add_norm(cascade_amd.embed(tokens, self.embedding))
+        for qkv, out, up, down in zip(self.qkv, self.out, self.up, self.down):
+            q, k, v = (y @ qkv.T).view(-1, self.heads + 2 * self.kv_heads, self.head_dim).split([self.heads, self.kv_heads, self.kv_heads], 1)
+            y, x = cascade_amd.add_norm(cascade_amd.attend(q, k, v, lo, hi, slopes=self.slopes).flatten(1) @ out.T, x)
+            y, x = cascade_amd.add_norm(torch.nn.functional.silu(y @ up.T) @ down.T, x)
+        return y
 
     def forward(self, tokens, lo, hi, target):
         """The loss of every token's target."""
-        x = self.embedding[tokens]
-        for qkv, out, up, down in zip(self.qkv, self.out, self.up, self.down):
-            y = (self.norm(x) @ qkv.T).view(-1, self.heads + 2 * self.kv_heads, self.head_dim)
-            q, k, v = y.split([self.heads, self.kv_heads, self.kv_heads], 1)
-            x = x + cascade_amd.attend(q, k, v, lo, hi, slopes=self.slopes).flatten(1) @ out.T
-            x = x + torch.nn.functional.silu(self.norm(x) @ up.T) @ down.T
-        return cascade_amd.next_token_loss(self.norm(x), self.words, target)
+        return cascade_amd.next_token_loss(self.hidden(tokens, lo, hi), self.words, target)
 
 
-def train(tokens=200000, steps=20, length=4096, passage=32, rate=0.5, max_norm=1.0, seed=0, say=print):
-    """Losses of the steps, and how much of the corpus was left out as repeated."""
+def stretch(text, step, length):
+    """A step's part of the corpus: where it begins, its tokens (a separator is the word behind the others), spans and targets."""
+    begin = step * length % max(1, text.numel() - length + 1)
+    part = text[begin:begin + length]
+    words = part.int() & 0xFFFF
+    return begin, torch.where(words == SEPARATOR, VOCAB, words), *cascade_amd.token_spans(part, separator=SEPARATOR)
+
+
+def descend(weights, max_norm, rate):
+    """A step down the clipped gradients, and their norm."""
+    weights = [w for w in weights if w.grad is not None]
+    norm = cascade_amd.clip_gradients([w.grad for w in weights], max_norm)
+    with torch.no_grad():
+        for w in weights:
+            w.sub_(w.grad, alpha=rate)
+            w.grad = None
+    return norm
+
+
+def train(tokens=200000, steps=20, length=4096, passage=32, rate=0.5, max_norm=1.0, seed=0, say=print, keep=None):
+    """Losses of the steps, and how much of the corpus was left out as repeated. keep: a list that gets the text, what repeats in it, and the model."""
     torch.manual_seed(seed)
     text = torch.from_numpy(workloads.generate(3, tokens).view("int16")).cuda()
     seen_before = repeated(text, passage)
@@ -87,22 +106,45 @@ def train(tokens=200000, steps=20, length=4096, passage=32, rate=0.5, max_norm=1
     weights = list(model.parameters())
     losses = []
     for step in range(steps):
-        begin = step * length % max(1, tokens - length + 1)
-        part = text[begin:begin + length]
-        lo, hi, target = cascade_amd.token_spans(part, separator=SEPARATOR)
+        begin, words, lo, hi, target = stretch(text, step, length)
         counts = (target >= 0) & ~seen_before[begin:begin + length]
-        words = part.int() & 0xFFFF
-        loss = model(torch.where(words == SEPARATOR, VOCAB, words).long(), lo, hi, torch.where(counts, target, -1))
+        loss = model(words, lo, hi, torch.where(counts, target, -1))
         loss = loss.sum() / counts.sum().clamp(min=1)
         loss.backward()
-        norm = cascade_amd.clip_gradients([w.grad for w in weights], max_norm)
-        with torch.no_grad():
-            for w in weights:
-                w.sub_(w.grad, alpha=rate)
-                w.grad = None
+        norm = descend(weights, max_norm, rate)
         losses.append(loss.item())
         say(f"step {step}: loss {losses[-1]:.4f}, gradient norm {norm.item():.3f}")
+    if keep is not None:
+        keep += [text, seen_before, model]
     return losses, share
+
+
+def top_logits(model, words, lo, hi, kept, at_once=1024):
+    """(ids, logits) of the `kept` largest logits that the model has for every token, some tokens at a time: all of them are never there."""
+    with torch.no_grad():
+        hidden = model.hidden(words, lo, hi)
+        parts = [(part @ model.words.T).float().topk(kept, 1) for part in hidden.split(at_once)]
+    return torch.cat([p.indices for p in parts]).int(), torch.cat([p.values for p in parts])
+
+
+def distil(text, seen_before, teacher, steps=10, length=4096, kept=32, temperature=1.0, rate=0.5, max_norm=1.0, seed=1, say=print):
+    """A smaller model learns from a teacher's top logits: how far it is from them at every step. Repeated passages have none."""
+    torch.manual_seed(seed)
+    student = Model(dim=128, heads=2, kv_heads=1, blocks=1).cuda()
+    weights = list(student.parameters())
+    losses = []
+    for step in range(steps):
+        begin, words, lo, hi, target = stretch(text, step, length)
+        counts = (target >= 0) & ~seen_before[begin:begin + length]
+        ids, logits = top_logits(teacher, words, lo, hi, kept)
+        ids = torch.where(counts[:, None], ids, -1)
+        loss = cascade_amd.distillation_loss(student.hidden(words, lo, hi), student.words, ids, logits, temperature)
+        loss = loss.sum() / counts.sum().clamp(min=1)
+        loss.backward()
+        norm = descend(weights, max_norm, rate)
+        losses.append(loss.item())
+        say(f"student's step {step}: divergence {losses[-1]:.4f}, gradient norm {norm.item():.3f}")
+    return losses, student
 
 
 if __name__ == "__main__":
@@ -110,5 +152,9 @@ if __name__ == "__main__":
     ap.add_argument("--tokens", type=int, default=200000)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--length", type=int, default=4096)
+    ap.add_argument("--student", type=int, default=0, help="steps that a smaller model learns from the trained one")
     a = ap.parse_args()
-    train(a.tokens, a.steps, a.length)
+    kept = []
+    train(a.tokens, a.steps, a.length, keep=kept)
+    if a.student:
+        distil(*kept, steps=a.student, length=a.length)
