@@ -375,6 +375,16 @@ void entropy_forward(const EntropyPlan& plan, const EntropyWork& w, const Operan
         join_sums_kernel<16><<<static_cast<uint32_t>(parts_of(hidden.rows, 16)), 256, 0, s>>>(w.part, parts, w.target_logit, target, hidden.rows, weight.rows, loss, lse);
 }
 
+template <class Type>
+void join_shares(const float* parts, uint64_t shares, int64_t tokens, int64_t dim, int64_t stride, const float* scale, short* d_hidden, int64_t d_hidden_stride, hipStream_t s)
+{
+    const uint64_t quads = static_cast<uint64_t>(tokens * stride / 4);
+    if (shares > 16) // many shares of few values: sixteen lanes add up those of four
+        join_shares_kernel<Type, 16><<<static_cast<uint32_t>(parts_of(quads, 16)), 256, 0, s>>>(parts, static_cast<uint32_t>(shares), tokens, dim, stride, scale, d_hidden, d_hidden_stride);
+    else
+        join_shares_kernel<Type, 1><<<static_cast<uint32_t>(parts_of(quads, 256)), 256, 0, s>>>(parts, static_cast<uint32_t>(shares), tokens, dim, stride, scale, d_hidden, d_hidden_stride);
+}
+
 // Gradients from the pieces of P, each of which fill(logits, its rows' stride) leaves in w.p; w.scale is there.
 template <class Type, class Fill>
 void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Operand& hidden, const Operand& weight, const int32_t* target, uint64_t dim, short* d_hidden,
@@ -415,14 +425,8 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
                 hidden_gradients_kernel<WH><<<groups, WH::THREADS, 0, s>>>(p, across, words, plan.share_words, tt, dt, w.shares, pd, piece > 0);
         }
     }
-    if (d_hidden) {
-        const uint64_t quads = static_cast<uint64_t>(tokens * pd / 4);
-        const uint32_t shares = static_cast<uint32_t>(plan.shares);
-        if (shares > 16) // many shares of few values: sixteen lanes add up those of four
-            join_shares_kernel<Type, 16><<<static_cast<uint32_t>(parts_of(quads, 16)), 256, 0, s>>>(w.shares, shares, tokens, d, pd, w.scale, d_hidden, d_hidden_stride);
-        else
-            join_shares_kernel<Type, 1><<<static_cast<uint32_t>(parts_of(quads, 256)), 256, 0, s>>>(w.shares, shares, tokens, d, pd, w.scale, d_hidden, d_hidden_stride);
-    }
+    if (d_hidden)
+        join_shares<Type>(w.shares, plan.shares, tokens, d, pd, w.scale, d_hidden, d_hidden_stride, s);
 }
 
 // ---- distillation ----
@@ -430,12 +434,31 @@ void entropy_backward(const EntropyPlan& plan, const EntropyWork& w, const Opera
 // Words of a block of the teacher's entries: those of a wave's part of a tile.
 uint64_t block_words(const EntropyPlan& plan) { return plan.narrow_logits ? Lines<NarrowLogits<Bf16>>::LINE : Lines<WideLogits<Bf16>>::LINE; }
 
+// Products of few tokens have kernels of their own, up to a vocabulary of one piece.
+bool few_tokens(const EntropyPlan& plan, uint64_t tokens) { return tokens <= FEW_TOKENS && plan.pieces == 1; }
+
+// Shares of d_hidden there: a workgroup a compute unit, of at least a slice for each of its waves.
+struct FewPlan {
+    uint64_t parts, shares, share_words, chunks, chunk_words;
+    FewPlan(uint64_t dim, uint64_t vocab)
+    {
+        parts = parts_of(dim, FEW_DIMS);
+        const uint64_t want = UNITS / parts, most = parts_of(vocab, 4 * SLICE);
+        share_words = up(parts_of(vocab, want < 1 ? 1 : want < most ? want : most), SLICE);
+        shares = parts_of(vocab, share_words);
+        // and of d_weight: eight waves a compute unit, in 32s of words
+        chunk_words = up(parts_of(vocab * parts, 8 * UNITS), 32);
+        chunks = parts_of(vocab, chunk_words);
+    }
+};
+
 struct TeacherWork {
     int32_t *ids, *counts;
-    float *q, *entropy, *dots;
+    float *q, *entropy, *dots, *shares;
     uint16_t* first;
+    short* by_words; // of few tokens
     uint64_t blocks, bytes;
-    TeacherWork(void* base, uint64_t before, const EntropyPlan& plan, uint64_t tokens, uint64_t vocab, uint64_t kept, bool backward)
+    TeacherWork(void* base, uint64_t before, const EntropyPlan& plan, uint64_t tokens, uint64_t dim, uint64_t vocab, uint64_t kept, bool backward)
     {
         Carver c{static_cast<char*>(base), before};
         blocks = parts_of(vocab, block_words(plan));
@@ -445,6 +468,9 @@ struct TeacherWork {
         counts = c.take<int32_t>(tokens);
         entropy = c.take<float>(tokens);
         dots = c.take<float>(backward ? 0 : parts_of(vocab, 256) * 4 * tokens);
+        const bool few = backward && few_tokens(plan, tokens);
+        by_words = c.take<short>(few ? vocab * FEW_TOKENS : 0);
+        shares = c.take<float>(few ? FewPlan(dim, vocab).shares * tokens * plan.padded_dim : 0);
         bytes = c.used;
     }
     Teacher teacher(uint64_t kept) const { return {ids, q, first, static_cast<int64_t>(kept), static_cast<int64_t>(blocks)}; }
@@ -691,7 +717,7 @@ uint64_t csa_lm_distill_workspace(uint64_t tokens, uint64_t dim, uint64_t vocab,
         !entropy_fits(tokens, dim, vocab, backward, !copies ? 0 : tokens > vocab ? tokens : vocab))
         return 0;
     const EntropyPlan plan(tokens, dim, vocab, backward);
-    return TeacherWork(nullptr, EntropyWork(nullptr, plan, tokens, vocab, backward, copies).bytes, plan, tokens, vocab, kept, backward).bytes;
+    return TeacherWork(nullptr, EntropyWork(nullptr, plan, tokens, vocab, backward, copies).bytes, plan, tokens, dim, vocab, kept, backward).bytes;
 }
 
 int csa_lm_distill_forward_dev(int type, const void* d_hidden, int64_t hidden_stride, const void* d_weight, int64_t weight_stride, const int32_t* d_ids, const float* d_logits,
@@ -710,7 +736,7 @@ int csa_lm_distill_forward_dev(int type, const void* d_hidden, int64_t hidden_st
     const EntropyPlan plan(tokens, dim, vocab, false);
     const bool copies = !walks(d_hidden, hidden_stride, dim) || !walks(d_weight, weight_stride, dim);
     const EntropyWork w(d_work, plan, tokens, vocab, false, copies);
-    const TeacherWork tw(d_work, w.bytes, plan, tokens, vocab, kept, false);
+    const TeacherWork tw(d_work, w.bytes, plan, tokens, dim, vocab, kept, false);
     if (int rc = check_work(who, d_work, work_bytes, tw.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -756,7 +782,7 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
         return rc;
     const EntropyPlan plan(tokens, dim, vocab, true);
     const EntropyWork w(d_work, plan, tokens, vocab, true, !walks(d_weight, weight_stride, dim));
-    const TeacherWork tw(d_work, w.bytes, plan, tokens, vocab, kept, true);
+    const TeacherWork tw(d_work, w.bytes, plan, tokens, dim, vocab, kept, true);
     if (int rc = check_work(who, d_work, work_bytes, tw.bytes))
         return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -777,15 +803,32 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
         typedef decltype(t) Type;
         const float rate = 1.f / temperature;
         loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss_grad, tw.counts, hidden.rows, weight.rows, Type::wide_range ? 1.f : 16384.f, rate, w.scale);
-        entropy_backward<Type>(plan, w, hidden, weight, tw.counts, dim, static_cast<short*>(d_hidden_grad), hidden_grad_stride, static_cast<short*>(d_weight_grad),
-                               weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
-                                   typedef WideLogits<Type> W;
-                                   typedef NarrowLogits<Type> N;
-                                   if (plan.narrow_logits)
-                                       distill_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps);
-                                   else
-                                       distill_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps);
-                               });
+        typedef WideLogits<Type> W;
+        typedef NarrowLogits<Type> N;
+        short *d_hidden_to = static_cast<short*>(d_hidden_grad), *d_weight_to = static_cast<short*>(d_weight_grad);
+        if (few_tokens(plan, tokens)) {
+            const FewPlan few(dim, vocab);
+            const int64_t stride = static_cast<int64_t>(up(vocab, SLICE)), d = static_cast<int64_t>(dim), words = weight.rows;
+            const uint32_t parts = static_cast<uint32_t>(few.parts), chunks = static_cast<uint32_t>(few.chunks);
+            const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), static_cast<uint32_t>(parts_of(vocab, N::BM)), 1, tw.counts, 0};
+            distill_gradients_kernel<N, Type><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride, d_weight_to ? tw.by_words : nullptr);
+            if (d_weight_to)
+                few_weight_gradients_kernel<Type><<<static_cast<uint32_t>(parts_of(few.parts * few.chunks, 4)), 256, 0, s>>>(
+                    Operand{w.kept, hidden.stride, d}, tw.by_words, static_cast<int>(tokens), words, static_cast<int64_t>(few.chunk_words), parts, chunks, w.scale, d_weight_to,
+                    weight_grad_stride, aligned(d_weight_to, 16) && weight_grad_stride % 8 == 0);
+            if (d_hidden_to) {
+                few_hidden_gradients_kernel<Type><<<parts * static_cast<uint32_t>(few.shares), 256, 0, s>>>(
+                    w.p, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
+                join_shares<Type>(tw.shares, few.shares, hidden.rows, d, hidden.stride, w.scale, d_hidden_to, hidden_grad_stride, s);
+            }
+            return;
+        }
+        entropy_backward<Type>(plan, w, hidden, weight, tw.counts, dim, d_hidden_to, hidden_grad_stride, d_weight_to, weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
+            if (plan.narrow_logits)
+                distill_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr);
+            else
+                distill_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr);
+        });
     });
     return launched(who);
 }

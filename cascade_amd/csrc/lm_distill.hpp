@@ -7,7 +7,7 @@
 // tile that is done lays its logits, or their exponentials, into LDS in 32 bits, a line of words for each token, and the token's lanes pick theirs there, or take q off
 // before anything is rounded: p - q, which a student that has learnt leaves small, keeps all its bits.
 #pragma once
-#include "lm_cross_entropy.hpp"
+#include "lm_few_tokens.hpp"
 
 namespace lm {
 
@@ -283,9 +283,10 @@ __global__ __launch_bounds__(256) void join_distill_kernel(const float2* part, c
 }
 
 // P[n][v] = d_loss[n] (exp(z - lse[n]) - q) relative to the largest |d_loss|, as logit_gradients_kernel leaves it; 1 / T is in what the products are scaled back with.
+// by_words: where there are few tokens, P in the other order, too (lm_few_tokens.hpp); or null.
 template <class P, class Type>
 __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l, Teacher teacher, float rate, const float* lse, const float* d_loss, const float* scale,
-                                                                       short* out, int64_t stride)
+                                                                       short* out, int64_t stride, short* by_words)
 {
     LM_TILE_BUFFERS(P);
     typedef Lines<P> Words;
@@ -315,6 +316,14 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
                     Words::word(lines, lane, static_cast<int>(teacher.ids[n * teacher.kept + e] - word0)) -= teacher.q[n * teacher.kept + e] * factor;
         }
         wait_for_lds();
+        if (by_words)
+            for (int k = 0; k < Words::PIECES; k += 2) { // four words a lane
+                const int piece = k + lane / 32;
+                const f32x4 y = *reinterpret_cast<const f32x4*>(Words::piece(lines, lane % 32, piece));
+                for (int r = 0; r < 4; ++r)
+                    if (mw + 4 * piece + r < l.weight.rows)
+                        by_words[(mw + 4 * piece + r) * FEW_TOKENS + n] = to16<Type>(y[r]);
+            }
 #pragma unroll
         for (int c = 0; c < 32; c += 64 / EIGHTS) {
             const int token = c + lane / EIGHTS;
@@ -338,11 +347,11 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
         }
         wait_for_lds();
     }
-    // k of the products to come runs along these rows, to a multiple of 8
-    const int64_t tail = l.weight.rows + threadIdx.x % 8;
-    if (mi == l.mt - 1 && tail < stride)
-        for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8)
-            out[n * stride + tail] = 0;
+    // k of the products to come runs along these rows, to a multiple of 8, or of 64
+    if (mi == l.mt - 1)
+        for (int64_t tail = l.weight.rows + threadIdx.x % 8; tail < stride; tail += 8)
+            for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8)
+                out[n * stride + tail] = 0;
 }
 
 } // namespace lm

@@ -107,6 +107,14 @@ def test_distillation_layouts(dim, layout):
     check_distillation(70, dim, 333, 10, torch.bfloat16, layout=layout, seed=dim)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65])  # up to 64, whose products have kernels of their own
+def test_distillation_of_few_tokens(n, dtype):
+    for dim, vocab in ((8, 33), (120, 63), (128, 64), (136, 65), (264, 1000), (512, 16384 + 7)):
+        check_distillation(n, dim, vocab, 5, dtype, seed=n + dim)
+    check_distillation(n, 4100, 300, 5, dtype, layout="odd", seed=n)
+
+
 @pytest.mark.parametrize("temperature", [0.05, 0.5, 1.0, 3.0, 20.0, 1000.0])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_distillation_temperatures(temperature, dtype):
