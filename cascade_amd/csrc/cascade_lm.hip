@@ -817,8 +817,14 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
                     Operand{w.kept, hidden.stride, d}, tw.by_words, static_cast<int>(tokens), words, static_cast<int64_t>(few.chunk_words), parts, chunks, w.scale, d_weight_to,
                     weight_grad_stride, aligned(d_weight_to, 16) && weight_grad_stride % 8 == 0);
             if (d_hidden_to) {
-                few_hidden_gradients_kernel<Type><<<parts * static_cast<uint32_t>(few.shares), 256, 0, s>>>(
-                    w.p, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
+                const auto launch = [&](auto rows) {
+                    few_hidden_gradients_kernel<Type, rows()><<<parts * static_cast<uint32_t>(few.shares), 256, 0, s>>>(
+                        w.p, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
+                };
+                if (tokens <= 32)
+                    launch(std::integral_constant<int, 1>());
+                else
+                    launch(std::integral_constant<int, 2>());
                 join_shares<Type>(tw.shares, few.shares, hidden.rows, d, hidden.stride, w.scale, d_hidden_to, hidden_grad_stride, s);
             }
             return;

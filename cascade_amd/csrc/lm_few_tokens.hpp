@@ -2,7 +2,9 @@
 // vocabulary's rows, the other by reading them, and take no barriers on the way: a wave walks words on its own, its next ones on their way while it multiplies.
 //
 // P comes in both orders: along the words (tokens x words, zeros behind the last word up to a multiple of 64) and along the tokens (words x 64, zeros for tokens that there are not).
-// 61 tokens of 512 values, 50257 words: d_weight 13 us and d_hidden 15 (by the tiles of lm_product.hpp: 21 and 18, and twice as many shares to add up).
+// d_weight of 61 tokens of 512 values and 50257 words takes 14 us, of 40 of 2560 50 us, 5.1 TB/s (by the tiles of lm_product.hpp 21 and 77: one workgroup a compute unit, which waits for its
+// loads, multiplies and stores one after the other). d_hidden reads the weight behind what has just been written: 18 and 86 us, as by tiles, but 6 us instead of 34 over 3000
+// words, whose tiles are too few.
 #pragma once
 #include "lm_cross_entropy.hpp"
 
@@ -102,92 +104,75 @@ __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hi
     }
 }
 
-// One share of d_hidden: FEW_DIMS values of all tokens, over the words [share, share + words_each); the four waves take slices of 64 words in turn, and add up what they
-// have at the end.
-template <class Type>
-__global__ __launch_bounds__(256) void few_hidden_gradients_kernel(const short* p, int64_t p_stride, Operand weight, int tokens, int64_t words, int64_t words_each, uint32_t parts,
-                                                                   float* out, int64_t stride)
+// One share of d_hidden: FEW_DIMS values of 32 ROWS tokens, over words_each words; the four waves take 64 words in turn (a line of P), and add up what they have at the end. A wave loads
+// words as they lie, four neighbouring values a lane, 16 words at a time and DEPTH times as many on their way, and turns blocks of eight words by four
+// values in its registers: the k-th product of a step has the k-th of every lane's values.
+template <class Type, int ROWS>
+__global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const short* p, int64_t p_stride, Operand weight, int tokens, int64_t words, int64_t words_each, uint32_t parts,
+                                                                      float* out, int64_t stride)
 {
-    typedef Loader<FEW_DIMS, true, 1> Words;
-    constexpr int TILES = FEW_DIMS / 32, STEPS = SLICE / 16, ROWS = FEW_TOKENS / 32;
-    __shared__ __attribute__((aligned(16))) short b0[4][FEW_DIMS * SLICE], b1[4][FEW_DIMS * SLICE];
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    constexpr int DEPTH = 4, STEP = 16, VALUES = 4;
+    __shared__ f32x4 all[4][ROWS * 16 * 64];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t share = blockIdx.x / parts;
     const int64_t d0 = static_cast<int64_t>(blockIdx.x % parts) * FEW_DIMS, begin = share * words_each, end = begin + words_each < words ? begin + words_each : words;
-    Reader<FEW_DIMS, true, TILES> read;
-    read.begin(0, lane);
-    f32x16 sums[ROWS][TILES] = {};
-    struct Entries {
-        s16x8 x[STEPS][ROWS];
-    } now, next;
-    // a slice of the weight on its way to LDS, and of P to registers
-    auto load = [&](short* buffer, Entries& e, int64_t k0) {
-        if (k0 >= end)
-            return;
-        Words w;
-        w.begin(weight, d0, k0, end, 0, lane);
-        w.load(buffer, k0, 0);
+    const int64_t line = weight.stride * 2;
+    const int64_t d = d0 + VALUES * (lane % 32);
+    const bool there = d < stride; // of the row's values, up to a multiple of eight
+    const uint32_t offset = there ? static_cast<uint32_t>(8 * half * line + VALUES * (lane % 32) * 2) : OUTSIDE;
+    f32x16 sums[ROWS][VALUES] = {};
+    struct Step {
+        u32x2 w[8];
+        s16x8 p[ROWS];
+    } steps[DEPTH];
+    auto load = [&](Step& s, int64_t k0) { // behind the end: zeros, by an empty window, and any P
+        const int64_t left = end - k0, bytes = (left < STEP ? left : STEP) * line - d0 * 2;
+        const buffer_t rows = window(static_cast<const char*>(weight.data) + k0 * line + d0 * 2, left > 0 ? static_cast<uint32_t>(bytes) : 0);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
+        for (int i = 0; i < 8; ++i)
+            s.w[i] = __builtin_amdgcn_raw_buffer_load_b64(rows, static_cast<int>(offset + (there ? i * static_cast<uint32_t>(line) : 0)), 0, 0);
+        const int64_t k = left > 0 ? k0 : begin;
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                const int token = 32 * i + lane % 32;
-                e.x[s][i] = read16(p + (token < tokens ? token : tokens - 1) * p_stride + k0 + s * 16 + half * 8); // rows of tokens that there are not are not stored
-            }
-    };
-    auto multiply = [&](const short* buffer, const Entries& e, int64_t k0) {
-        if (k0 >= end)
-            return;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            s16x8 w[TILES];
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-                w[t] = read.read(buffer, t, s);
-#pragma unroll
-            for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-                for (int t = 0; t < TILES; ++t)
-                    sums[i][t] = Type::mfma32(e.x[s][i], w[t], sums[i][t]);
+        for (int i = 0; i < ROWS; ++i) {
+            const int token = 32 * i + lane % 32;
+            s.p[i] = read16(p + (token < tokens ? token : tokens - 1) * p_stride + k + 8 * half); // rows of tokens that there are not are not stored
         }
     };
-    constexpr int64_t TURN = 4 * SLICE; // of all waves
+    auto multiply = [&](const Step& s) {
+#pragma unroll
+        for (int k = 0; k < VALUES; ++k) {
+            u32x4 turned;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                turned[i] = __builtin_amdgcn_perm(s.w[2 * i + 1][k / 2], s.w[2 * i][k / 2], k % 2 ? 0x07060302 : 0x05040100);
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+                sums[i][k] = Type::mfma32(s.p[i], __builtin_bit_cast(s16x8, turned), sums[i][k]);
+        }
+    };
+    static_assert(DEPTH * STEP == SLICE, "a turn's words of a wave");
     const int64_t first = begin + wave * SLICE;
-    load(b0[wave], now, first);
-    settle();
-    for (int64_t k0 = first; k0 < end; k0 += 2 * TURN) { // two slices a turn, one from each buffer
-        load(b1[wave], next, k0 + TURN);
-        multiply(b0[wave], now, k0);
-        settle();
-        load(b0[wave], now, k0 + 2 * TURN);
-        multiply(b1[wave], next, k0 + TURN);
-        settle();
-    }
-    __syncthreads(); // no load is in flight
-    // all sums in LDS, a wave's 32 KB after the other; then two tiles a wave
-    constexpr int EACH = ROWS * TILES * 16 * 64;
-    float* lines[4] = {reinterpret_cast<float*>(b0), reinterpret_cast<float*>(b0) + EACH, reinterpret_cast<float*>(b1), reinterpret_cast<float*>(b1) + EACH};
-    static_assert(2 * EACH * sizeof(float) <= sizeof(b0), "two waves' sums fit a buffer");
-    float* own = wave < 2 ? lines[0] + wave * EACH : lines[2] + (wave - 2) * EACH;
+#pragma unroll
+    for (int s = 0; s < DEPTH; ++s)
+        load(steps[s], first + s * STEP);
+    for (int64_t k0 = first; k0 < end; k0 += 4 * SLICE)
+#pragma unroll
+        for (int s = 0; s < DEPTH; ++s) {
+            if (k0 + s * STEP < end)
+                multiply(steps[s]);
+            load(steps[s], k0 + 4 * SLICE + s * STEP);
+        }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                own[((i * TILES + t) * 16 + r) * 64 + lane] = sums[i][t][r];
+        for (int r = 0; r < 16; ++r)
+            all[wave][(i * 16 + r) * 64 + lane] = f32x4{sums[i][0][r], sums[i][1][r], sums[i][2][r], sums[i][3][r]};
     __syncthreads();
-    constexpr int TILES_EACH = ROWS * TILES / 4;
-    for (int k = 0; k < TILES_EACH; ++k) {
-        const int tile = wave * TILES_EACH + k, i = tile / TILES, t = tile % TILES;
-        const int64_t d = d0 + 32 * t + lane % 32;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int at = (tile * 16 + r) * 64 + lane, token = 32 * i + 8 * (r / 4) + 4 * half + r % 4;
-            const float sum = (lines[0][at] + lines[1][at]) + (lines[2][at] + lines[3][at]);
-            if (token < tokens && d < weight.rows)
-                out[(static_cast<int64_t>(share) * tokens + token) * stride + d] = sum;
-        }
+    for (int k = 0; k < ROWS * 4; ++k) { // a quarter of the rows a wave
+        const int row = wave * ROWS * 4 + k, i = row / 16, r = row % 16, token = 32 * i + 8 * (r / 4) + 4 * half + r % 4, at = row * 64 + lane;
+        if (token < tokens && there)
+            *reinterpret_cast<f32x4*>(out + (static_cast<int64_t>(share) * tokens + token) * stride + d) = (all[0][at] + all[1][at]) + (all[2][at] + all[3][at]);
     }
 }
 
