@@ -185,7 +185,7 @@ int check_norm(const char* who, int type, int stream_type, uint64_t tokens, uint
         return fail(CSA_ERR_ARG, "%s: values of type %d beside a residual of type %d", who, type, stream_type);
     if (dim < LEAST_DIM || dim > NORM_DIM)
         return fail(CSA_ERR_ARG, "%s: rows of %llu values; 8 to %llu are possible", who, (unsigned long long)dim, (unsigned long long)NORM_DIM);
-    if (!launchable(tokens, 1024))
+    if (!launchable(tokens, dim <= 2048 ? 256 : 1024)) // of a row, at most
         return fail(CSA_ERR_TOO_LARGE, "%s: %llu tokens", who, (unsigned long long)tokens);
     return CSA_OK;
 }

@@ -194,7 +194,7 @@ __global__ __launch_bounds__(NORM_THREADS<WAVES>) void norm_backward_kernel(Norm
             unpacked(now, i, d_out, g, u);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                sums[i][k] += d_out[k] * u[k];
+                sums[i][k] += d_out[k] == 0.f ? 0.f : d_out[k] * u[k]; // what no gradient reaches (padding) may hold anything
                 sum += k < at[i].skip ? 0.f : g[k] * u[k];
             }
         }

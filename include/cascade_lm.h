@@ -102,12 +102,13 @@ int csa_lm_embed_backward_dev(int type, const void* d_tokens, uint32_t token_byt
 
 /* total = x + residual, rounded to stream_type; rstd[i] = 1 / sqrt(mean of total[i]^2 + eps), of the rounded total, summed in 64 bits; out = total * rstd * gain.
  * x, gain, out: `type` (any csa_lm_type); residual, total: stream_type, which is `type` or CSA_LM_F32. Rows of x and residual are *_stride values apart (>= dim, below
- * 2^22), out and total are dense. d_residual NULL: total is x, d_total is not written and stream_type is `type`; d_gain NULL: ones. dim: 8 to 16384, eps > 0, tokens < 2^22. */
+ * 2^22), out and total are dense. d_residual NULL: total is x, d_total is not written and stream_type is `type`; d_gain NULL: ones. dim: 8 to 16384, eps > 0, fewer than 2^24
+ * tokens, 2^22 of rows of more than 2048 values. */
 int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const void* d_gain, float eps,
                             uint64_t tokens, uint64_t dim, void* d_out, void* d_total, float* d_rstd, void* stream);
 
 /* With g = out_grad * gain and u = total * rstd: the gradient of x and residual alike is rstd * (g - u * mean(g u)) + total_grad (stream_type; NULL: none flows into total
- * from elsewhere), and gain_grad = the sum over tokens of out_grad * u, in a fixed order. x_grad (type), residual_grad (stream_type) and gain_grad (type) are dense; any of them may be
+ * from elsewhere), and gain_grad = the sum over tokens of out_grad * u, in a fixed order, to which rows whose out_grad is zero add nothing, whatever they hold. x_grad (type), residual_grad (stream_type) and gain_grad (type) are dense; any of them may be
  * NULL. The workspace is for gain_grad and may be NULL without it. */
 uint64_t csa_lm_norm_backward_workspace(uint64_t tokens, uint64_t dim);
 int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, int64_t out_grad_stride, const void* d_total, int64_t total_stride, const float* d_rstd,

@@ -190,6 +190,24 @@ def test_logits_of_16_bits(kind):
 
 
 @pytest.mark.parametrize("n", [50, 600])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_bad_weight_of_a_token_reaches_its_own_gradient_only(n, value):
+    """In d_hidden; every word's gradient is a sum over all tokens."""
+    g = gen(17)
+    hidden, weight = randn(g, n, 64, dtype=torch.float16), randn(g, 900, 64, dtype=torch.float16, scale=0.2)
+    ids, logits = teacher(g, n, 9, 900, ignored=0.0)
+    ids[5] = torch.arange(9)
+    d_loss = torch.rand(n, generator=g, device="cuda")
+    lse = cascade_amd.linear_distillation(hidden, weight, ids, logits)[1]
+    d_loss[5] = 0.5 * d_loss.max()  # not the largest one, by which all are held
+    clean = cascade_amd.linear_distillation_backward(d_loss, hidden, weight, ids, logits, lse, want_weight=False)[0]
+    d_loss[5] = value
+    got = cascade_amd.linear_distillation_backward(d_loss, hidden, weight, ids, logits, lse, want_weight=False)[0]
+    rest = torch.arange(n, device="cuda") != 5
+    assert torch.equal(got[rest], clean[rest]) and not torch.isfinite(got[5]).any()
+
+
+@pytest.mark.parametrize("n", [50, 600])
 def test_tokens_without_entries_may_hold_anything(n):
     g = gen(11)
     hidden, weight = randn(g, n, 64, dtype=torch.bfloat16), randn(g, 500, 64, dtype=torch.bfloat16)
@@ -267,6 +285,19 @@ def test_autograd_of_distillation():
     assert torch.equal(torch.autograd.grad(loss.sum(), weight)[0], want[1])
     with pytest.raises(ValueError, match="teacher"):
         cascade_amd.distillation_loss(hidden, weight, ids, logits.requires_grad_())
+
+
+@pytest.mark.parametrize("n", [1, 40, 64, 65, 400])
+def test_a_gradient_that_is_not_wanted_changes_nothing(n):
+    g = gen(16)
+    hidden, weight = randn(g, n, 72, dtype=torch.bfloat16), randn(g, 700, 72, dtype=torch.bfloat16, scale=0.2)
+    ids, logits = teacher(g, n, 6, 700)
+    d_loss = torch.rand(n, generator=g, device="cuda")
+    how = (d_loss, hidden, weight, ids, logits, cascade_amd.linear_distillation(hidden, weight, ids, logits)[1])
+    both = cascade_amd.linear_distillation_backward(*how)
+    first = cascade_amd.linear_distillation_backward(*how, want_weight=False)
+    second = cascade_amd.linear_distillation_backward(*how, want_hidden=False)
+    assert torch.equal(first[0], both[0]) and first[1] is None and second[0] is None and torch.equal(second[1], both[1])
 
 
 @pytest.mark.parametrize("n,vocab", [(40, 3000), (1100, 2000)])

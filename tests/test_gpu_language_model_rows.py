@@ -114,6 +114,57 @@ def test_embed_of_a_very_long_text():
     got = cascade_amd.embed_tokens_backward(d_out, tokens, 50)
     counts = torch.bincount(words_of(tokens, 50) + 1, minlength=51)[1:].double()[:, None]
     within(got, counts.expand(50, 2048), 2.0 ** -8 * counts.expand(50, 2048), "counts")
+    del d_out
+    weight = randn(gen(3), 50, 2048, dtype=torch.bfloat16)
+    out, word = cascade_amd.embed_tokens(tokens, weight), words_of(tokens, 50)
+    for part in (slice(0, 5000), slice(n - 5000, n)):
+        assert torch.equal(out[part], torch.where(word[part, None] >= 0, weight[word[part].clamp(min=0)], 0.0))
+
+
+def test_norm_of_a_very_long_text():
+    """Offsets past 2^32 bytes, and results that go past the caches."""
+    n, dim = 300000, 4096
+    g = gen(4)
+    few = randn(g, 1000, dim, dtype=torch.bfloat16)
+    x = few.repeat(n // 1000, 1)  # 2.5 GB
+    out, total, rstd = cascade_amd.residual_norm(x, x)
+    want = cascade_amd.residual_norm(few, few)
+    for a, b in zip((out, total, rstd), want):
+        assert torch.equal(a.view(n // 1000, *b.shape), b.expand(n // 1000, *b.shape))
+    gain = torch.ones(dim, dtype=torch.bfloat16, device="cuda")
+    d_x, _, d_gain = cascade_amd.residual_norm_backward(x, total, rstd, gain, total)
+    d_few, _, d_few_gain = cascade_amd.residual_norm_backward(few, want[1], want[2], gain, want[1])
+    assert torch.equal(d_x.view(n // 1000, 1000, dim), d_few.expand(n // 1000, 1000, dim))
+    # sums of the same 1000 rows, 300 times: off by the rounding of both results, and by 32-bit sums of 300000 terms over 512 workgroups, joined by 16 runs
+    terms = (few.double() * want[1].double() * want[2].double()[:, None]).abs().sum(0)
+    assert ((d_gain.double() - 300 * d_few_gain.double()).abs() <= 300 * (2.1 * 2.0 ** -8 * d_few_gain.double().abs() + E * (300000 / 512 + 60) * terms)).all()
+
+
+def test_tokens_of_any_16_bit_type_and_place():
+    g = gen(5)
+    tokens = torch.randint(0, 60000, (901,), generator=g, device="cuda")
+    weight = randn(g, 60000, 24, dtype=torch.float16)
+    want = cascade_amd.embed_tokens(tokens[1:].int(), weight)
+    short = torch.where(tokens >= 1 << 15, tokens - (1 << 16), tokens).to(torch.int16)
+    assert torch.equal(cascade_amd.embed_tokens(short[1:], weight), want) and torch.equal(cascade_amd.embed_tokens(short.view(torch.uint16)[1:], weight), want)
+    d_out = randn(g, 900, 24, dtype=torch.float16)
+    grads = [cascade_amd.embed_tokens_backward(d_out, t, 60000) for t in (tokens[1:].int(), short[1:], short.view(torch.uint16)[1:])]
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+def test_two_calls_at_once_share_nothing():
+    g = gen(6)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    inputs = [(text(20000, 3000, "zipf", g), randn(g, 20000, 64, dtype=torch.bfloat16)) for _ in range(2)]
+    want = [cascade_amd.embed_tokens_backward(d, t, 3000) for t, d in inputs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, (t, d) in zip(streams, inputs):
+            with torch.cuda.stream(s):
+                got.append(cascade_amd.embed_tokens_backward(d, t, 3000))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i % 2]) for i, a in enumerate(got))
 
 
 def test_embed_of_nothing():
@@ -268,6 +319,20 @@ def test_a_bad_token_stays_in_its_row(value, dim):
     for a, b in zip((*got, *cascade_amd.residual_norm_backward(d_out, got[1], got[2])[:2]), (*clean, *grads[:2])):
         assert torch.equal(a[rest], b[rest])
     assert got[0][4].isnan().any()
+
+
+@pytest.mark.parametrize("dim", [70, 700, 1030, 9000])
+def test_padding_without_gradient_takes_nothing_from_the_gain(dim):
+    g = gen(18)
+    x, r, d_out = (randn(g, 30, dim, dtype=torch.bfloat16) for _ in range(3))
+    gain = (1 + randn(g, dim, scale=0.2)).bfloat16()
+    d_out[20:] = 0
+    _, total, rstd = cascade_amd.residual_norm(x, r, gain)
+    want = cascade_amd.residual_norm_backward(d_out, total, rstd, gain)
+    x[20:25], r[25:] = math.nan, math.inf
+    _, total, rstd = cascade_amd.residual_norm(x, r, gain)
+    got = cascade_amd.residual_norm_backward(d_out, total, rstd, gain)
+    assert torch.equal(got[2], want[2]) and torch.equal(got[0][:20], want[0][:20])
 
 
 # ---- gradients by torch.autograd, and against differences ----

@@ -92,7 +92,10 @@ def test_norm_gradient_arguments(change):
 
 
 def test_norm_of_more_than_a_launch_holds():
-    assert norm(tokens=1 << 22) == norm_backward(tokens=1 << 22) == LARGE
+    assert norm(tokens=1 << 24) == norm_backward(tokens=1 << 24) == LARGE
+    assert norm(tokens=1 << 22, dim=2049, xs=2049, rs=2049) == norm_backward(tokens=1 << 22, dim=2049, gs=2049, ts=2049, ds=2049) == LARGE
+    for fine in (dict(tokens=(1 << 24) - 1), dict(tokens=(1 << 22) - 1, dim=2049, gs=2049, ts=2049, ds=2049)):
+        assert norm_backward(**fine) == BAD and b"workspace" in native.load().csa_lm_last_error()
     size = native.load().csa_lm_norm_backward_workspace
     assert size(5, 7) == size(5, 16385) == 0
     assert size(1, 64) == 256 and all(size(1 << 20, dim) <= 4096 * 4 * dim + 256 for dim in (8, 1024, 16384))
