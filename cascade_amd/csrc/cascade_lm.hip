@@ -456,7 +456,7 @@ struct TeacherWork {
     int32_t *ids, *counts;
     float *q, *entropy, *dots, *shares;
     uint16_t* first;
-    short* by_words; // of few tokens
+    short *low, *by_words; // of few tokens
     uint64_t blocks, bytes;
     TeacherWork(void* base, uint64_t before, const EntropyPlan& plan, uint64_t tokens, uint64_t dim, uint64_t vocab, uint64_t kept, bool backward)
     {
@@ -469,6 +469,7 @@ struct TeacherWork {
         entropy = c.take<float>(tokens);
         dots = c.take<float>(backward ? 0 : parts_of(vocab, 256) * 4 * tokens);
         const bool few = backward && few_tokens(plan, tokens);
+        low = few && tokens <= TWICE_TOKENS ? c.take<short>(tokens * up(vocab, SLICE)) : nullptr;
         by_words = c.take<short>(few ? vocab * FEW_TOKENS : 0);
         shares = c.take<float>(few ? FewPlan(dim, vocab).shares * tokens * plan.padded_dim : 0);
         bytes = c.used;
@@ -811,17 +812,25 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
             const int64_t stride = static_cast<int64_t>(up(vocab, SLICE)), d = static_cast<int64_t>(dim), words = weight.rows;
             const uint32_t parts = static_cast<uint32_t>(few.parts), chunks = static_cast<uint32_t>(few.chunks);
             const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), static_cast<uint32_t>(parts_of(vocab, N::BM)), 1, tw.counts, 0};
-            distill_gradients_kernel<N, Type><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride, d_weight_to ? tw.by_words : nullptr);
-            if (d_weight_to)
-                few_weight_gradients_kernel<Type><<<static_cast<uint32_t>(parts_of(few.parts * few.chunks, 4)), 256, 0, s>>>(
-                    Operand{w.kept, hidden.stride, d}, tw.by_words, static_cast<int>(tokens), words, static_cast<int64_t>(few.chunk_words), parts, chunks, w.scale, d_weight_to,
-                    weight_grad_stride, aligned(d_weight_to, 16) && weight_grad_stride % 8 == 0);
+            distill_gradients_kernel<N, Type><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride, tw.low, d_weight_to ? tw.by_words : nullptr);
+            const bool twice = tokens <= TWICE_TOKENS;
+            if (d_weight_to) {
+                const auto launch = [&](auto most) {
+                    few_weight_gradients_kernel<Type, most()><<<static_cast<uint32_t>(parts_of(few.parts * few.chunks, 4)), 256, 0, s>>>(
+                        Operand{w.kept, hidden.stride, d}, tw.by_words, static_cast<int>(tokens), words, static_cast<int64_t>(few.chunk_words), parts, chunks, w.scale, d_weight_to,
+                        weight_grad_stride, aligned(d_weight_to, 16) && weight_grad_stride % 8 == 0);
+                };
+                if (twice)
+                    launch(std::integral_constant<int, TWICE_TOKENS>());
+                else
+                    launch(std::integral_constant<int, FEW_TOKENS>());
+            }
             if (d_hidden_to) {
                 const auto launch = [&](auto rows) {
                     few_hidden_gradients_kernel<Type, rows()><<<parts * static_cast<uint32_t>(few.shares), 256, 0, s>>>(
-                        w.p, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
+                        w.p, tw.low, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
                 };
-                if (tokens <= 32)
+                if (twice)
                     launch(std::integral_constant<int, 1>());
                 else
                     launch(std::integral_constant<int, 2>());
@@ -831,9 +840,9 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
         }
         entropy_backward<Type>(plan, w, hidden, weight, tw.counts, dim, d_hidden_to, hidden_grad_stride, d_weight_to, weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
             if (plan.narrow_logits)
-                distill_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr);
+                distill_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr, nullptr);
             else
-                distill_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr);
+                distill_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr, nullptr);
         });
     });
     return launched(who);

@@ -283,10 +283,10 @@ __global__ __launch_bounds__(256) void join_distill_kernel(const float2* part, c
 }
 
 // P[n][v] = d_loss[n] (exp(z - lse[n]) - q) relative to the largest |d_loss|, as logit_gradients_kernel leaves it; 1 / T is in what the products are scaled back with.
-// by_words: where there are few tokens, P in the other order, too (lm_few_tokens.hpp); or null.
+// by_words: where there are few tokens, P in the other order, too, and low, what the rounding leaves of it, where there are so few that both numbers have a place there (lm_few_tokens.hpp); or null.
 template <class P, class Type>
 __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l, Teacher teacher, float rate, const float* lse, const float* d_loss, const float* scale,
-                                                                       short* out, int64_t stride, short* by_words)
+                                                                       short* out, int64_t stride, short* low, short* by_words)
 {
     LM_TILE_BUFFERS(P);
     typedef Lines<P> Words;
@@ -316,33 +316,44 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
                     Words::word(lines, lane, static_cast<int>(teacher.ids[n * teacher.kept + e] - word0)) -= teacher.q[n * teacher.kept + e] * factor;
         }
         wait_for_lds();
-        if (by_words)
+        if (by_words && (!low || n < TWICE_TOKENS))
             for (int k = 0; k < Words::PIECES; k += 2) { // four words a lane
                 const int piece = k + lane / 32;
                 const f32x4 y = *reinterpret_cast<const f32x4*>(Words::piece(lines, lane % 32, piece));
                 for (int r = 0; r < 4; ++r)
-                    if (mw + 4 * piece + r < l.weight.rows)
-                        by_words[(mw + 4 * piece + r) * FEW_TOKENS + n] = to16<Type>(y[r]);
+                    if (mw + 4 * piece + r < l.weight.rows) {
+                        short* to = by_words + (mw + 4 * piece + r) * FEW_TOKENS + n;
+                        const short rounded = to16<Type>(y[r]);
+                        to[0] = rounded;
+                        if (low)
+                            to[TWICE_TOKENS] = to16<Type>(y[r] - to32<Type>(rounded));
+                    }
             }
 #pragma unroll
         for (int c = 0; c < 32; c += 64 / EIGHTS) {
             const int token = c + lane / EIGHTS;
-            const f32x4 low = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight)), high = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight + 1));
-            s16x8 y;
+            const f32x4 front = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight)), back = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight + 1));
+            s16x8 y, rest;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                y[r] = to16<Type>(low[r]);
-                y[4 + r] = to16<Type>(high[r]);
+            for (int r = 0; r < 8; ++r) {
+                const float x = r < 4 ? front[r] : back[r - 4];
+                y[r] = to16<Type>(x);
+                rest[r] = to16<Type>(x - to32<Type>(y[r]));
             }
             if (first + token >= tokens || m >= l.weight.rows)
                 continue;
-            short* to = out + (first + token) * stride + m;
+            const int64_t to = (first + token) * stride + m;
             if (m + 8 <= l.weight.rows) {
-                *reinterpret_cast<s16x8*>(to) = y;
+                *reinterpret_cast<s16x8*>(out + to) = y;
+                if (low)
+                    *reinterpret_cast<s16x8*>(low + to) = rest;
             } else {
                 for (int r = 0; r < 8; ++r)
-                    if (m + r < l.weight.rows)
-                        to[r] = y[r];
+                    if (m + r < l.weight.rows) {
+                        out[to + r] = y[r];
+                        if (low)
+                            low[to + r] = rest[r];
+                    }
             }
         }
         wait_for_lds();
@@ -351,7 +362,11 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
     if (mi == l.mt - 1)
         for (int64_t tail = l.weight.rows + threadIdx.x % 8; tail < stride; tail += 8)
             for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8)
+            {
                 out[n * stride + tail] = 0;
+                if (low)
+                    low[n * stride + tail] = 0;
+            }
 }
 
 } // namespace lm

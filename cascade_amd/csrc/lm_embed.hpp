@@ -82,7 +82,7 @@ __device__ inline void write_zeros(const Zeros& z)
 constexpr int RANKED_EACH = 32; // places a workgroup
 
 // RANKED_EACH places a workgroup, all compared with all REGISTERS * 1024 >= n places of the text, which lie in the registers of its 16 waves: a comparison and a count of its lanes for
-// each place and 64 others. 8192 places: 13 us alone, nothing beside the zeros of 50257 rows of 4096 values.
+// each place and 64 others. 8192 places: 10 us alone, 58 us with the zeros of 50257 rows of 4096 values (7.1 TB/s).
 template <class Token, int REGISTERS>
 __global__ __launch_bounds__(1024) void rank_places_kernel(const Token* tokens, int n, uint32_t rows, uint32_t* words, uint32_t* places, Zeros zeros)
 {

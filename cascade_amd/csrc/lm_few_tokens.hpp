@@ -2,6 +2,9 @@
 // vocabulary's rows, the other by reading them, and take no barriers on the way: a wave walks words on its own, its next ones on their way while it multiplies.
 //
 // P comes in both orders: along the words (tokens x words, zeros behind the last word up to a multiple of 64) and along the tokens (words x 64, zeros for tokens that there are not).
+// Up to 32 tokens it is the sum of two numbers of 16 bits, what the rounding leaves being the second one, in rows of its own and behind the first 32 of a word: the few entries that weigh
+// most, a token's likeliest words, would otherwise leave errors of up to 1.6 times those of the results' own rounding, where more tokens even them out (1.4 times). It takes the places of the
+// tokens that are not there, and no time; for 33 to 64 it would be 14 %.
 // d_weight of 61 tokens of 512 values and 50257 words takes 14 us, of 40 of 2560 50 us, 5.1 TB/s (by the tiles of lm_product.hpp 21 and 77: one workgroup a compute unit, which waits for its
 // loads, multiplies and stores one after the other). d_hidden reads the weight behind what has just been written: 18 and 86 us, as by tiles, but 6 us instead of 34 over 3000
 // words, whose tiles are too few.
@@ -10,7 +13,8 @@
 
 namespace lm {
 
-constexpr int FEW_TOKENS = 64, FEW_DIMS = 128; // of a wave
+constexpr int FEW_TOKENS = 64, TWICE_TOKENS = 32; // at most; and where P has two numbers
+constexpr int FEW_DIMS = 128;                     // of a wave
 
 // All of the wave's loads and LDS accesses are done; the compiler moves none across.
 __device__ inline void settle()
@@ -22,12 +26,12 @@ __device__ inline void settle()
 
 // d_weight: a wave has FEW_DIMS values of all tokens in registers and walks `words_each` words, 32 at a time: products of values and words, which it turns in LDS
 // and stores as lines of a word.
-template <class Type>
+template <class Type, int TOKENS>
 __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hidden, const short* p_words, int tokens, int64_t words, int64_t words_each, uint32_t parts, uint32_t chunks,
                                                                    const float* scale, short* out, int64_t stride, bool wide)
 {
     typedef Loader<FEW_DIMS, true, 1> Values;
-    constexpr int TILES = FEW_DIMS / 32, STEPS = FEW_TOKENS / 16, PIECES = FEW_DIMS / 8;
+    constexpr int TILES = FEW_DIMS / 32, STEPS = FEW_TOKENS / 16, KINDS = TOKENS / 16, PIECES = FEW_DIMS / 8;
     __shared__ __attribute__((aligned(16))) short all[4][FEW_DIMS * SLICE];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t id = blockIdx.x * 4 + wave;
@@ -35,7 +39,7 @@ __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hi
         return;
     short* mine = all[wave];
     const int64_t d0 = static_cast<int64_t>(id % parts) * FEW_DIMS, begin = static_cast<int64_t>(id / parts) * words_each, end = begin + words_each < words ? begin + words_each : words;
-    s16x8 values[STEPS][TILES];
+    s16x8 values[KINDS][TILES]; // with two numbers of P the tokens come twice
     {
         Values load;
         load.begin(hidden, d0, 0, tokens, 0, lane);
@@ -44,7 +48,7 @@ __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hi
         read.begin(0, lane);
         settle();
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
+        for (int s = 0; s < KINDS; ++s)
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
                 values[s][t] = read.read(mine, t, s);
@@ -66,10 +70,9 @@ __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hi
         f32x16 sums[TILES] = {};
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
-            if (s * 16 < tokens)
 #pragma unroll
-                for (int t = 0; t < TILES; ++t)
-                    sums[t] = Type::mfma32(values[s][t], now[s], sums[t]);
+            for (int t = 0; t < TILES; ++t)
+                sums[t] = Type::mfma32(values[s % KINDS][t], now[s], sums[t]);
         const int column = lane % 32; // a line holds a word's values; its pieces stand at places piece ^ word
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -108,7 +111,7 @@ __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hi
 // words as they lie, four neighbouring values a lane, 16 words at a time and DEPTH times as many on their way, and turns blocks of eight words by four
 // values in its registers: the k-th product of a step has the k-th of every lane's values.
 template <class Type, int ROWS>
-__global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const short* p, int64_t p_stride, Operand weight, int tokens, int64_t words, int64_t words_each, uint32_t parts,
+__global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const short* p, const short* p_low, int64_t p_stride, Operand weight, int tokens, int64_t words, int64_t words_each, uint32_t parts,
                                                                       float* out, int64_t stride)
 {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const shor
     f32x16 sums[ROWS][VALUES] = {};
     struct Step {
         u32x2 w[8];
-        s16x8 p[ROWS];
+        s16x8 p[2]; // of the first and the last 32 tokens, or both numbers of 32
     } steps[DEPTH];
     auto load = [&](Step& s, int64_t k0) { // behind the end: zeros, by an empty window, and any P
         const int64_t left = end - k0, bytes = (left < STEP ? left : STEP) * line - d0 * 2;
@@ -134,9 +137,10 @@ __global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const shor
             s.w[i] = __builtin_amdgcn_raw_buffer_load_b64(rows, static_cast<int>(offset + (there ? i * static_cast<uint32_t>(line) : 0)), 0, 0);
         const int64_t k = left > 0 ? k0 : begin;
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            const int token = 32 * i + lane % 32;
-            s.p[i] = read16(p + (token < tokens ? token : tokens - 1) * p_stride + k + 8 * half); // rows of tokens that there are not are not stored
+        for (int i = 0; i < 2; ++i) {
+            const int token = (ROWS == 2 ? 32 * i : 0) + lane % 32;
+            const int64_t at = (token < tokens ? token : tokens - 1) * p_stride + k + 8 * half; // rows of tokens that there are not are not stored
+            s.p[i] = read16((ROWS == 1 && i ? p_low : p) + at);
         }
     };
     auto multiply = [&](const Step& s) {
@@ -147,8 +151,8 @@ __global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const shor
             for (int i = 0; i < 4; ++i)
                 turned[i] = __builtin_amdgcn_perm(s.w[2 * i + 1][k / 2], s.w[2 * i][k / 2], k % 2 ? 0x07060302 : 0x05040100);
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i)
-                sums[i][k] = Type::mfma32(s.p[i], __builtin_bit_cast(s16x8, turned), sums[i][k]);
+            for (int i = 0; i < 2; ++i)
+                sums[i % ROWS][k] = Type::mfma32(s.p[i], __builtin_bit_cast(s16x8, turned), sums[i % ROWS][k]);
         }
     };
     static_assert(DEPTH * STEP == SLICE, "a turn's words of a wave");

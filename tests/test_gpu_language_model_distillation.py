@@ -121,6 +121,25 @@ def test_distillation_temperatures(temperature, dtype):
     check_distillation(200, 128, 1000, 20, dtype, temperature=temperature, seed=4)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 5, 32])
+def test_gradients_of_few_tokens_are_rounded_once(n, dtype):
+    """Up to 32 tokens the gradients of the logits have twice the bits, that is errors of u^2: what is left is the rounding of the results, which those of the formula have, too, and sums of 32
+    bits, below a twentieth of it. (The average of a rounding off by up to u of a value, evenly, is u / sqrt(3), not u / sqrt(12), as was first written here.)"""
+    g = gen(n)
+    dim, vocab = 200, 4000
+    hidden, weight = randn(g, n, dim, dtype=dtype), randn(g, vocab, dim, dtype=dtype, scale=2 * dim ** -0.5)
+    ids, logits = teacher(g, n, 10, vocab, ignored=0.0)
+    ids[:, 0], logits[:, 0] = 3, 9.0  # no token without entries
+    d_loss = torch.full((n,), 1.00390625 - 2.0 ** -10, device="cuda")
+    lse = cascade_amd.linear_distillation(hidden, weight, ids, logits, 2.0)[1]
+    got = cascade_amd.linear_distillation_backward(d_loss, hidden, weight, ids, logits, lse, 2.0)
+    _, _, p, q, _ = reference(hidden, weight, ids, logits, 2.0)
+    d_z = (p - q) * d_loss.double()[:, None] / 2.0
+    for a, b in zip(got, (d_z @ weight.double(), d_z.T @ hidden.double())):
+        assert (a.double() - b).norm() <= 1.05 * (b.to(dtype).double() - b).norm()
+
+
 def test_distillation_over_the_corpus_vocabulary():
     check_distillation(600, 256, 50257, 50, torch.bfloat16, seed=3)
     check_distillation(40, 256, 65535, 100, torch.float16, seed=4)
