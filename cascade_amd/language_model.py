@@ -23,14 +23,23 @@ from . import _native_lm as native
 SEPARATOR = 0xFFFF
 
 
-_kinds = None  # the library's number of every dtype; made when first asked for: this package imports torch only where it is used
+# What the calls need of torch, looked up when the first tensor comes: this package imports torch only where it is used, and looking it up in every call costs a small one
+# 0.5 us of 8.
+_kinds = None  # the library's number of every dtype
+_float32 = _int32 = _raw_stream = _current_device = None
+
+
+def _look_up():
+    global _kinds, _float32, _int32, _raw_stream, _current_device
+    import torch
+    _float32, _int32 = torch.float32, torch.int32
+    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice  # a stream's address, without the object around it
+    _kinds = {torch.bfloat16: native.CSA_LM_BF16, torch.float16: native.CSA_LM_F16, torch.float32: native.CSA_LM_F32}
 
 
 def _type(dtype):
-    global _kinds
     if _kinds is None:
-        import torch
-        _kinds = {torch.bfloat16: native.CSA_LM_BF16, torch.float16: native.CSA_LM_F16, torch.float32: native.CSA_LM_F32}
+        _look_up()
     kind = _kinds.get(dtype)
     if kind is None:
         raise TypeError(f"{dtype} is none of bfloat16, float16 and float32")
@@ -60,15 +69,18 @@ def _on_gpu(*tensors):
 
 
 def _enqueue(device, call, *args):
-    """call(*args, stream) with the device's current stream, and the device made current for the launches. (The stream's address without
-    the object that torch.cuda.current_stream makes around it: 0.1 us instead of 1.2, of the 11 that a small call takes.)"""
-    import torch
-    stream = torch._C._cuda_getCurrentRawStream(device) or None
-    if device == torch.cuda.current_device():
-        native.check(call(*args, stream))
+    """call(*args, stream) with the device's current stream, and the device made current for the launches."""
+    if _kinds is None:
+        _look_up()
+    stream = _raw_stream(device) or None
+    if device == _current_device():
+        status = call(*args, stream)
     else:
+        import torch
         with torch.cuda.device(device):
-            native.check(call(*args, stream))
+            status = call(*args, stream)
+    if status:
+        native.check(status)
 
 
 def _work(size, like):
@@ -111,32 +123,34 @@ def token_spans(text, separator=SEPARATOR):
 
 
 def _check_tokens(tokens):
-    import torch
-    _check(tokens.dim() == 1 and tokens.is_contiguous() and (tokens.dtype == torch.int32 or (tokens.element_size() == 2 and not tokens.is_floating_point())),
+    """The bytes of a token."""
+    if _kinds is None:
+        _look_up()
+    size = tokens.element_size()
+    _check(tokens.dim() == 1 and tokens.is_contiguous() and (tokens.dtype == _int32 or (size == 2 and not tokens.is_floating_point())),
            "tokens: a dense vector of int32 or 16-bit tokens")
+    return size
 
 
 def embed_tokens(tokens, weight, scale=1.0):
     """scale * weight[tokens], rounded once: (n, dim) of weight's type. tokens: n int32, or 16-bit tokens as token_spans takes them (viewed as int16 is fine: they count as
     unsigned); weight: (rows, dim), float32, bfloat16 or float16, dim at least 8. A token outside [0, rows) gives zeros (csa_lm_embed_forward_dev).
     Without a graph: embed is the one for torch.autograd."""
-    _check_tokens(tokens)
+    size = _check_tokens(tokens)
     _check(weight.dim() == 2, "weight: (rows, dim)")
     kind, device = _type(weight.dtype), _on_gpu(tokens, weight)
-    rows, dim = weight.shape
+    n, (rows, dim) = tokens.numel(), weight.shape
     weight, stride = _rows(weight)
-    out = weight.new_empty((tokens.numel(), dim))
+    out = weight.new_empty((n, dim))
     lib = native.load()
-    _enqueue(device, lib.csa_lm_embed_forward_dev, kind, _address(tokens), tokens.element_size(), tokens.numel(), _address(weight), stride, rows, dim, float(scale),
-             _address(out))
+    _enqueue(device, lib.csa_lm_embed_forward_dev, kind, _address(tokens), size, n, _address(weight), stride, rows, dim, float(scale), _address(out))
     return out
 
 
 def embed_tokens_backward(d_out, tokens, rows, scale=1.0):
     """The gradient of the weight, (rows, dim) of d_out's type, for the gradient d_out (n, dim) of embed_tokens' result: the rows of d_out that belong to each word, added up in 32
     bits in a fixed order, times scale; zeros for words that are not there (csa_lm_embed_backward_dev)."""
-    import torch
-    _check_tokens(tokens)
+    token_size = _check_tokens(tokens)
     _check(d_out.dim() == 2 and d_out.shape[0] == tokens.numel(), "d_out: (tokens, dim)")
     kind, device = _type(d_out.dtype), _on_gpu(d_out, tokens)
     n, dim = d_out.shape
@@ -145,7 +159,7 @@ def embed_tokens_backward(d_out, tokens, rows, scale=1.0):
     lib = native.load()
     size = lib.csa_lm_embed_backward_workspace(kind, n, rows, dim)
     scratch, work = _work(size, d_out)
-    _enqueue(device, lib.csa_lm_embed_backward_dev, kind, _address(tokens), tokens.element_size(), n, _address(d_out), stride, rows, dim, float(scale),
+    _enqueue(device, lib.csa_lm_embed_backward_dev, kind, _address(tokens), token_size, n, _address(d_out), stride, rows, dim, float(scale),
              _address(d_weight), work, size)
     return d_weight
 
@@ -154,14 +168,15 @@ def embed_tokens_backward(d_out, tokens, rows, scale=1.0):
 
 
 def _check_norm(x, gain):
+    """The type, and the numbers of rows and of their values."""
     _check(x.dim() == 2, "rows: (tokens, dim)")
-    _check(gain is None or (gain.dtype == x.dtype and gain.dim() == 1 and gain.numel() == x.shape[1] and gain.is_contiguous()), "gain: a value of x's type for each of a row")
-    return _type(x.dtype)
+    dtype, (n, dim) = x.dtype, x.shape
+    _check(gain is None or (gain.dtype == dtype and gain.dim() == 1 and gain.numel() == dim and gain.is_contiguous()), "gain: a value of x's type for each of a row")
+    return _type(dtype), n, dim
 
 
-def _check_stream(x, like, what):
-    import torch
-    _check(x.shape == like.shape and x.dtype in (like.dtype, torch.float32), f"{what}: like x, or in float32")
+def _check_stream(x, like, message):
+    _check(x.shape == like.shape and (x.dtype == like.dtype or x.dtype == _float32), message)
     return _type(x.dtype)
 
 
@@ -171,12 +186,10 @@ def residual_norm(x, residual=None, gain=None, eps=1e-6):
     x: (tokens, dim), float32, bfloat16 or float16, dim from 8 to 16384; residual: like x, or a stream of 32 bits beside an x of 16; gain: dim values of x's type (None: ones).
     Returns (out, total, rstd): total = x + residual in the residual's type (x itself without one), rstd = 1 / sqrt(mean of total^2 + eps) float32 of every token, and out =
     total * rstd * gain in x's type, from the rounded total (csa_lm_norm_forward_dev). Without a graph: add_norm is the one for torch.autograd."""
-    import torch
-    kind = _check_norm(x, gain)
-    stream = kind if residual is None else _check_stream(residual, x, "residual")
+    kind, n, dim = _check_norm(x, gain)
+    stream = kind if residual is None else _check_stream(residual, x, "residual: like x, or in float32")
     device = _on_gpu(x, residual, gain)
-    n, dim = x.shape
-    out, rstd = x.new_empty((n, dim)), x.new_empty(n, dtype=torch.float32)
+    out, rstd = x.new_empty((n, dim)), x.new_empty(n, dtype=_float32)
     total = x if residual is None else residual.new_empty((n, dim))
     x, xs = _rows(x)
     residual, rs = (None, 0) if residual is None else _rows(residual)
@@ -189,13 +202,11 @@ def residual_norm(x, residual=None, gain=None, eps=1e-6):
 def residual_norm_backward(d_out, total, rstd, gain=None, d_total=None, want_gain=True):
     """Gradients (d_x, d_residual, d_gain) for the gradients d_out of out and d_total of total (None: total is used nowhere else); total and rstd as residual_norm returned them.
     d_x is of d_out's type and d_residual of total's: one tensor where these are the same. d_gain is None without a gain, or if it is not wanted (csa_lm_norm_backward_dev)."""
-    import torch
-    kind = _check_norm(d_out, gain)
-    stream = _check_stream(total, d_out, "total")
+    kind, n, dim = _check_norm(d_out, gain)
+    stream = _check_stream(total, d_out, "total: like d_out, or in float32")
     _check(d_total is None or (d_total.shape == total.shape and d_total.dtype == total.dtype), "d_total: like total")
     device = _on_gpu(d_out, total, rstd, gain, d_total)
-    n, dim = d_out.shape
-    _check(rstd.dim() == 1 and rstd.numel() == n and rstd.dtype == torch.float32 and rstd.is_contiguous(), "rstd: one float32 a token")
+    _check(rstd.dim() == 1 and rstd.numel() == n and rstd.dtype == _float32 and rstd.is_contiguous(), "rstd: one float32 a token")
     d_residual = total.new_empty((n, dim))
     d_x = d_residual if stream == kind else d_out.new_empty((n, dim))
     d_gain = gain.new_empty(dim) if gain is not None and want_gain else None
