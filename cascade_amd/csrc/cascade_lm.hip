@@ -348,11 +348,20 @@ int check_entropy_gradients(const char* who, const float* d_lse, const float* d_
     return CSA_OK;
 }
 
-void lay_out(const void* in, int64_t in_stride, uint64_t rows, uint64_t dim, const int32_t* target, uint64_t vocab, short* out, uint64_t stride, hipStream_t s)
+void lay_out(const void* in, int64_t in_stride, uint64_t rows, uint64_t dim, short* out, uint64_t stride, hipStream_t s)
 {
     if (const uint64_t threads = rows * (stride / 8))
-        lay_out_rows_kernel<<<static_cast<uint32_t>(parts_of(threads, 256)), 256, 0, s>>>(static_cast<const short*>(in), in_stride, rows, dim, target, vocab, out, stride,
+        lay_out_rows_kernel<<<static_cast<uint32_t>(parts_of(threads, 256)), 256, 0, s>>>(static_cast<const short*>(in), in_stride, rows, dim, out, stride,
                                                                                           walks(in, in_stride, dim));
+}
+
+// The rows of hidden that have a target, and the factors of the losses' gradients; rate: of the logits.
+void begin_gradients(int type, const void* hidden, int64_t hidden_stride, uint64_t tokens, uint64_t dim, const int32_t* target, uint64_t vocab, const float* d_loss, float rate,
+                     const EntropyPlan& plan, const EntropyWork& w, hipStream_t s)
+{
+    const LossScale scale{d_loss, type == CSA_LM_BF16 ? 1.f : 16384.f, rate, w.scale}; // P of half precision reaches 16384
+    scale_and_lay_out_kernel<<<1 + static_cast<uint32_t>(parts_of(tokens * (plan.padded_dim / 8), 1024)), 1024, 0, s>>>(
+        scale, static_cast<const short*>(hidden), hidden_stride, tokens, dim, target, vocab, w.kept, plan.padded_dim, walks(hidden, hidden_stride, dim));
 }
 
 template <class Type>
@@ -658,11 +667,11 @@ int csa_lm_cross_entropy_forward_dev(int type, const void* d_hidden, int64_t hid
     const hipStream_t s = static_cast<hipStream_t>(stream);
     Operand hidden{d_hidden, hidden_stride, static_cast<int64_t>(tokens)}, weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
     if (!walks(d_hidden, hidden_stride, dim)) {
-        lay_out(d_hidden, hidden_stride, tokens, dim, nullptr, vocab, w.hidden, plan.padded_dim, s);
+        lay_out(d_hidden, hidden_stride, tokens, dim, w.hidden, plan.padded_dim, s);
         hidden = {w.hidden, static_cast<int64_t>(plan.padded_dim), hidden.rows};
     }
     if (!walks(d_weight, weight_stride, dim)) {
-        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        lay_out(d_weight, weight_stride, vocab, dim, w.weight, plan.padded_dim, s);
         weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
     }
     with_type(type, [&](auto t) { entropy_forward<decltype(t)>(plan, w, hidden, weight, d_target, d_loss, d_lse, s); });
@@ -689,15 +698,14 @@ int csa_lm_cross_entropy_backward_dev(int type, const void* d_hidden, int64_t hi
         return launched(who);
     }
     Operand weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
-    lay_out(d_hidden, hidden_stride, tokens, dim, d_target, vocab, w.kept, plan.padded_dim, s);
+    begin_gradients(type, d_hidden, hidden_stride, tokens, dim, d_target, vocab, d_loss_grad, 1.f, plan, w, s);
     const Operand hidden{w.kept, static_cast<int64_t>(plan.padded_dim), static_cast<int64_t>(tokens)};
     if (!walks(d_weight, weight_stride, dim)) {
-        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        lay_out(d_weight, weight_stride, vocab, dim, w.weight, plan.padded_dim, s);
         weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
     }
     with_type(type, [&](auto t) {
         typedef decltype(t) Type;
-        loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss_grad, d_target, hidden.rows, weight.rows, Type::wide_range ? 1.f : 16384.f, 1.f, w.scale);
         entropy_backward<Type>(plan, w, hidden, weight, d_target, dim, static_cast<short*>(d_hidden_grad), hidden_grad_stride, static_cast<short*>(d_weight_grad),
                                weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
                                    typedef WideLogits<Type> W;
@@ -743,11 +751,11 @@ int csa_lm_distill_forward_dev(int type, const void* d_hidden, int64_t hidden_st
     const hipStream_t s = static_cast<hipStream_t>(stream);
     Operand hidden{d_hidden, hidden_stride, static_cast<int64_t>(tokens)}, weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
     if (!walks(d_hidden, hidden_stride, dim)) {
-        lay_out(d_hidden, hidden_stride, tokens, dim, nullptr, vocab, w.hidden, plan.padded_dim, s);
+        lay_out(d_hidden, hidden_stride, tokens, dim, w.hidden, plan.padded_dim, s);
         hidden = {w.hidden, static_cast<int64_t>(plan.padded_dim), hidden.rows};
     }
     if (!walks(d_weight, weight_stride, dim)) {
-        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        lay_out(d_weight, weight_stride, vocab, dim, w.weight, plan.padded_dim, s);
         weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
     }
     learn(plan, tw, d_ids, d_logits, kept, temperature, tokens, vocab, s);
@@ -794,16 +802,15 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
     }
     learn(plan, tw, d_ids, d_logits, kept, temperature, tokens, vocab, s);
     Operand weight{d_weight, weight_stride, static_cast<int64_t>(vocab)};
-    lay_out(d_hidden, hidden_stride, tokens, dim, tw.counts, vocab, w.kept, plan.padded_dim, s);
+    const float rate = 1.f / temperature;
+    begin_gradients(type, d_hidden, hidden_stride, tokens, dim, tw.counts, vocab, d_loss_grad, rate, plan, w, s);
     const Operand hidden{w.kept, static_cast<int64_t>(plan.padded_dim), static_cast<int64_t>(tokens)};
     if (!walks(d_weight, weight_stride, dim)) {
-        lay_out(d_weight, weight_stride, vocab, dim, nullptr, vocab, w.weight, plan.padded_dim, s);
+        lay_out(d_weight, weight_stride, vocab, dim, w.weight, plan.padded_dim, s);
         weight = {w.weight, static_cast<int64_t>(plan.padded_dim), weight.rows};
     }
     with_type(type, [&](auto t) {
         typedef decltype(t) Type;
-        const float rate = 1.f / temperature;
-        loss_scale_kernel<<<1, 1024, 0, s>>>(d_loss_grad, tw.counts, hidden.rows, weight.rows, Type::wide_range ? 1.f : 16384.f, rate, w.scale);
         typedef WideLogits<Type> W;
         typedef NarrowLogits<Type> N;
         short *d_hidden_to = static_cast<short*>(d_hidden_grad), *d_weight_to = static_cast<short*>(d_weight_grad);

@@ -132,39 +132,6 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float2* part, int6
     }
 }
 
-// The factor of P, range / max |d_loss|, and what the products of P are scaled back with: its inverse times `rate`, the logits' own. What is not finite among them has no say: its token is lost whatever the factor is, and takes nothing from the others.
-__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* d_loss, const int32_t* target, int64_t tokens, int64_t vocab, float range, float rate, float* scale)
-{
-    __shared__ float tops[16];
-    float top = 0.f;
-    for (int64_t n0 = threadIdx.x; n0 < tokens; n0 += 8 * 1024) { // eight loads on their way at a time
-        int32_t goal[8];
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int64_t n = n0 + k * 1024 < tokens ? n0 + k * 1024 : n0;
-            goal[k] = target[n];
-            x[k] = fabsf(d_loss[n]);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (goal[k] >= 0 && goal[k] < vocab && x[k] < INFINITY)
-                top = fmaxf(top, x[k]);
-    }
-    for (int d = 32; d; d /= 2)
-        top = fmaxf(top, __shfl_xor(top, d));
-    if (threadIdx.x % 64 == 0)
-        tops[threadIdx.x / 64] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w)
-            top = fmaxf(top, tops[w]);
-        const bool fine = top > 1e-30f && top < 1e30f; // both factors are ordinary numbers
-        scale[0] = fine ? range / top : 1.f;
-        scale[1] = (fine ? top / range : 1.f) * rate;
-    }
-}
-
 template <class P, class Type>
 __global__ __launch_bounds__(P::THREADS) void logit_gradients_kernel(Logits l, const float* lse, const float* d_loss, const float* scale, int64_t vocab,
                                                                      short* out, int64_t stride)
@@ -284,12 +251,12 @@ __global__ __launch_bounds__(256) void join_shares_kernel(const float* shares, u
             out[n * out_stride + d + i] = to16<Type>(sum[i] * back);
 }
 
-// Rows in a layout that 16-byte loads can walk: padded to 8 values with zeros; with targets, rows without one are zeros (their
+// A row's piece of eight in a layout that 16-byte loads can walk: padded to 8 values with zeros; with targets, rows without one are zeros (their
 // values may be anything, and 0 times infinity is no 0).
-__global__ __launch_bounds__(256) void lay_out_rows_kernel(const short* in, int64_t in_stride, int64_t rows, int64_t dim, const int32_t* target, int64_t vocab,
-                                                           short* out, int64_t stride, bool whole)
+__device__ inline void lay_out_piece(int64_t at, const short* in, int64_t in_stride, int64_t rows, int64_t dim, const int32_t* target, int64_t vocab, short* out, int64_t stride,
+                                     bool whole)
 {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, pieces = stride / 8;
+    const int64_t pieces = stride / 8;
     if (at >= rows * pieces)
         return;
     const int64_t row = at / pieces, d = at % pieces * 8;
@@ -302,6 +269,56 @@ __global__ __launch_bounds__(256) void lay_out_rows_kernel(const short* in, int6
             v[i] = d + i < dim ? in[row * in_stride + d + i] : static_cast<short>(0);
     }
     *reinterpret_cast<s16x8*>(out + row * stride + d) = v;
+}
+
+__global__ __launch_bounds__(256) void lay_out_rows_kernel(const short* in, int64_t in_stride, int64_t rows, int64_t dim, short* out, int64_t stride, bool whole)
+{
+    lay_out_piece(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, in, in_stride, rows, dim, nullptr, 0, out, stride, whole);
+}
+
+// The factor of P, range / max |d_loss|, and what the products of P are scaled back with: its inverse times `rate`, the logits' own. What is not finite among them has no say: its token is lost whatever the factor is, and takes nothing from the others.
+struct LossScale {
+    const float* d_loss;
+    float range, rate;
+    float* scale; // two
+};
+
+// What the gradients begin with: the first workgroup finds the factor, the others lay out the rows of hidden.
+__global__ __launch_bounds__(1024) void scale_and_lay_out_kernel(LossScale l, const short* in, int64_t in_stride, int64_t rows, int64_t dim, const int32_t* target, int64_t vocab,
+                                                                short* out, int64_t stride, bool whole)
+{
+    if (blockIdx.x) {
+        lay_out_piece(static_cast<int64_t>(blockIdx.x - 1) * 1024 + threadIdx.x, in, in_stride, rows, dim, target, vocab, out, stride, whole);
+        return;
+    }
+    __shared__ float tops[16];
+    float top = 0.f;
+    for (int64_t n0 = threadIdx.x; n0 < rows; n0 += 8 * 1024) { // eight loads on their way at a time
+        int32_t goal[8];
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t n = n0 + k * 1024 < rows ? n0 + k * 1024 : n0;
+            goal[k] = target[n];
+            x[k] = fabsf(l.d_loss[n]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (goal[k] >= 0 && goal[k] < vocab && x[k] < INFINITY)
+                top = fmaxf(top, x[k]);
+    }
+    for (int d = 32; d; d /= 2)
+        top = fmaxf(top, __shfl_xor(top, d));
+    if (threadIdx.x % 64 == 0)
+        tops[threadIdx.x / 64] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w)
+            top = fmaxf(top, tops[w]);
+        const bool fine = top > 1e-30f && top < 1e30f; // both factors are ordinary numbers
+        l.scale[0] = fine ? l.range / top : 1.f;
+        l.scale[1] = (fine ? top / l.range : 1.f) * l.rate;
+    }
 }
 
 __global__ __launch_bounds__(256) void zero_rows_kernel(short* out, int64_t stride, int64_t rows, int64_t dim)
