@@ -819,7 +819,8 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
             const int64_t stride = static_cast<int64_t>(up(vocab, SLICE)), d = static_cast<int64_t>(dim), words = weight.rows;
             const uint32_t parts = static_cast<uint32_t>(few.parts), chunks = static_cast<uint32_t>(few.chunks);
             const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), static_cast<uint32_t>(parts_of(vocab, N::BM)), 1, tw.counts, 0};
-            distill_gradients_kernel<N, Type><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride, tw.low, d_weight_to ? tw.by_words : nullptr);
+            distill_gradients_kernel<N, Type, true><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride,
+                                                                                FewGradients{d_weight_to ? tw.by_words : nullptr, tw.low});
             const bool twice = tokens <= TWICE_TOKENS;
             if (d_weight_to) {
                 const auto launch = [&](auto most) {
@@ -847,9 +848,9 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
         }
         entropy_backward<Type>(plan, w, hidden, weight, tw.counts, dim, d_hidden_to, hidden_grad_stride, d_weight_to, weight_grad_stride, s, [&](const Logits& l, int64_t ps) {
             if (plan.narrow_logits)
-                distill_gradients_kernel<N, Type><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr, nullptr);
+                distill_gradients_kernel<N, Type, false><<<l.mt * l.nt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, {});
             else
-                distill_gradients_kernel<W, Type><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, nullptr, nullptr);
+                distill_gradients_kernel<W, Type, false><<<l.mt * l.nt, W::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, ps, {});
         });
     });
     return launched(who);

@@ -282,11 +282,16 @@ __global__ __launch_bounds__(256) void join_distill_kernel(const float2* part, c
     }
 }
 
+// Where there are few tokens (lm_few_tokens.hpp): P in the other order, too, and what its rounding leaves, where there are so few that both numbers have a place there; or null.
+struct FewGradients {
+    short *by_words, *low;
+};
+
 // P[n][v] = d_loss[n] (exp(z - lse[n]) - q) relative to the largest |d_loss|, as logit_gradients_kernel leaves it; 1 / T is in what the products are scaled back with.
-// by_words: where there are few tokens, P in the other order, too, and low, what the rounding leaves of it, where there are so few that both numbers have a place there (lm_few_tokens.hpp); or null.
-template <class P, class Type>
+// FEW: of few tokens.
+template <class P, class Type, bool FEW>
 __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l, Teacher teacher, float rate, const float* lse, const float* d_loss, const float* scale,
-                                                                       short* out, int64_t stride, short* low, short* by_words)
+                                                                       short* out, int64_t stride, FewGradients few)
 {
     LM_TILE_BUFFERS(P);
     typedef Lines<P> Words;
@@ -316,16 +321,16 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
                     Words::word(lines, lane, static_cast<int>(teacher.ids[n * teacher.kept + e] - word0)) -= teacher.q[n * teacher.kept + e] * factor;
         }
         wait_for_lds();
-        if (by_words && (!low || n < TWICE_TOKENS))
+        if (FEW && few.by_words && (!few.low || n < TWICE_TOKENS))
             for (int k = 0; k < Words::PIECES; k += 2) { // four words a lane
                 const int piece = k + lane / 32;
                 const f32x4 y = *reinterpret_cast<const f32x4*>(Words::piece(lines, lane % 32, piece));
                 for (int r = 0; r < 4; ++r)
                     if (mw + 4 * piece + r < l.weight.rows) {
-                        short* to = by_words + (mw + 4 * piece + r) * FEW_TOKENS + n;
+                        short* to = few.by_words + (mw + 4 * piece + r) * FEW_TOKENS + n;
                         const short rounded = to16<Type>(y[r]);
                         to[0] = rounded;
-                        if (low)
+                        if (few.low)
                             to[TWICE_TOKENS] = to16<Type>(y[r] - to32<Type>(rounded));
                     }
             }
@@ -333,26 +338,27 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
         for (int c = 0; c < 32; c += 64 / EIGHTS) {
             const int token = c + lane / EIGHTS;
             const f32x4 front = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight)), back = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight + 1));
-            s16x8 y, rest;
+            s16x8 y, rest = {};
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 const float x = r < 4 ? front[r] : back[r - 4];
                 y[r] = to16<Type>(x);
-                rest[r] = to16<Type>(x - to32<Type>(y[r]));
+                if (FEW)
+                    rest[r] = to16<Type>(x - to32<Type>(y[r]));
             }
             if (first + token >= tokens || m >= l.weight.rows)
                 continue;
             const int64_t to = (first + token) * stride + m;
             if (m + 8 <= l.weight.rows) {
                 *reinterpret_cast<s16x8*>(out + to) = y;
-                if (low)
-                    *reinterpret_cast<s16x8*>(low + to) = rest;
+                if (FEW && few.low)
+                    *reinterpret_cast<s16x8*>(few.low + to) = rest;
             } else {
                 for (int r = 0; r < 8; ++r)
                     if (m + r < l.weight.rows) {
                         out[to + r] = y[r];
-                        if (low)
-                            low[to + r] = rest[r];
+                        if (FEW && few.low)
+                            few.low[to + r] = rest[r];
                     }
             }
         }
@@ -361,11 +367,10 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
     // k of the products to come runs along these rows, to a multiple of 8, or of 64
     if (mi == l.mt - 1)
         for (int64_t tail = l.weight.rows + threadIdx.x % 8; tail < stride; tail += 8)
-            for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8)
-            {
+            for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8) {
                 out[n * stride + tail] = 0;
-                if (low)
-                    low[n * stride + tail] = 0;
+                if (FEW && few.low)
+                    few.low[n * stride + tail] = 0;
             }
 }
 
