@@ -6,8 +6,8 @@
 // the tokens that are not there, and no time. (With one, its rounding and the results' own add up to 1.4 times the latter where entries are many; the few of a short text, a token's
 // likeliest words, spread about that: 18 tokens came to 1.6. From 33 on, where 120 draws lay between 1.2 and 1.5, a second number takes 14 %: 83 us -> 94 for the 61 tokens below.)
 // d_weight of 61 tokens of 512 values and 50257 words takes 14 us, of 40 of 2560 50 us, 5.1 TB/s (by the tiles of lm_product.hpp 21 and 77: one workgroup a compute unit, which waits for its
-// loads, multiplies and stores one after the other). d_hidden reads the weight behind what has just been written: 18 and 86 us, as by tiles, but 6 us instead of 34 over 3000
-// words, whose tiles are too few.
+// loads, multiplies and stores one after the other). d_hidden reads the weight behind what has just been written: 15 and 86 us, by tiles 18 and 86, and 6 us instead of 34
+// over 3000 words, whose tiles are too few.
 #pragma once
 #include "lm_cross_entropy.hpp"
 
@@ -34,7 +34,8 @@ __global__ __launch_bounds__(256, 2) void few_weight_gradients_kernel(Operand hi
     constexpr int TILES = FEW_DIMS / 32, STEPS = FEW_TOKENS / 16, KINDS = TOKENS / 16, PIECES = FEW_DIMS / 8;
     __shared__ __attribute__((aligned(16))) short all[4][FEW_DIMS * SLICE];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t id = blockIdx.x * 4 + wave;
+    // lines of memory that two waves share are written by one XCD (61 tokens of 968 values 155 -> 151 us trained; where there are none it takes 1 % more of 4096 values)
+    const uint32_t id = (stride % 64 ? by_xcd(blockIdx.x, gridDim.x) : blockIdx.x) * 4 + wave;
     if (id >= parts * chunks) // whole waves, which meet nobody
         return;
     short* mine = all[wave];
@@ -118,8 +119,8 @@ __global__ __launch_bounds__(256, 1) void few_hidden_gradients_kernel(const shor
     constexpr int DEPTH = 4, STEP = 16, VALUES = 4;
     __shared__ f32x4 all[4][ROWS * 16 * 64];
     const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t share = blockIdx.x / parts;
-    const int64_t d0 = static_cast<int64_t>(blockIdx.x % parts) * FEW_DIMS, begin = share * words_each, end = begin + words_each < words ? begin + words_each : words;
+    const uint32_t id = by_xcd(blockIdx.x, gridDim.x), share = id / parts; // the parts that read the same of P: by way of one L2 (61 tokens of 512 values trained 82 -> 80 us, of 1000 138 -> 126)
+    const int64_t d0 = static_cast<int64_t>(id % parts) * FEW_DIMS, begin = share * words_each, end = begin + words_each < words ? begin + words_each : words;
     const int64_t line = weight.stride * 2;
     const int64_t d = d0 + VALUES * (lane % 32);
     const bool there = d < stride; // of the row's values, up to a multiple of eight
