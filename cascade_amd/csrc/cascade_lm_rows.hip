@@ -190,7 +190,10 @@ int check_norm(const char* who, int type, int stream_type, uint64_t tokens, uint
     return CSA_OK;
 }
 
-// f(type, type of the residual, waves a row, pieces a lane) as types: pieces are of sixteen bytes of the residual, and a row has more than half as many as fit (lm_norm.hpp counts on it)
+// f(type, type of the residual, waves a row, pieces a lane) as types: pieces are of sixteen bytes of the residual, and a row has more than half as many as fit (lm_norm.hpp counts on
+// it). Lanes without a piece wait with the others, so counts in between pay: three a lane instead of lanes of four times as many waves (bfloat16, trained: 27272 rows of 1100 values
+// 115 -> 88 us, 5859 of 5120 109 -> 89; float32, 2500 of 12000 222 -> 191), but for a wave's rows of float32 (42857 of 700 values 178 -> 192). Four a lane of four waves: 3662 rows of 8192
+// bfloat16 values 95 us by sixteen waves, 92 by four.
 template <class F>
 void with_norm(int type, int stream_type, uint64_t dim, F f)
 {
@@ -198,6 +201,7 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
         auto sized = [&](auto s) {
             typedef std::integral_constant<int, 1> One;
             typedef std::integral_constant<int, 2> Two;
+            typedef std::integral_constant<int, 3> Three;
             typedef std::integral_constant<int, 4> Four;
             typedef std::integral_constant<int, 16> Sixteen;
             constexpr uint64_t V = PIECE<decltype(s)>;
@@ -205,16 +209,24 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
                 f(t, s, One(), One());
             else if (dim <= 128 * V)
                 f(t, s, One(), Two());
+            else if (sizeof(t) == 2 && dim <= 192 * V)
+                f(t, s, One(), Three());
             else if (dim <= 256 * V)
                 f(t, s, Four(), One());
             else if (dim <= 512 * V)
                 f(t, s, Four(), Two());
+            else if (dim <= 768 * V)
+                f(t, s, Four(), Three());
             else if (dim <= 1024 * V)
-                f(t, s, Sixteen(), One());
+                f(t, s, Four(), Four());
             else if (V == 8 || dim <= 2048 * V)
                 f(t, s, Sixteen(), Two());
-            else if constexpr (V == 4)
-                f(t, s, Sixteen(), Four());
+            else if constexpr (V == 4) {
+                if (dim <= 3 * 1024 * V)
+                    f(t, s, Sixteen(), Three());
+                else
+                    f(t, s, Sixteen(), Four());
+            }
         };
         if (stream_type == CSA_LM_F32)
             sized(float());
@@ -226,10 +238,11 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
 uint64_t norm_rows(int waves) { return waves == 1 ? 4 : 1; } // of a workgroup at a time
 
 // Workgroups of the backward kernel, each with sums of d_gain of its own: as many as fit the compute units at once, or half as many where the sums would otherwise cost more than is
-// won (30000 rows of 100 values: 768 32 us, 512 34 us; 8192 of 4096: 512 95 us, 768 99 us; 2500 of 12000: 256 98 us, 512 105 us).
-uint64_t norm_groups(uint64_t tokens, int waves, int items, uint64_t stream_size)
+// won (30000 rows of 100 values: 768 32 us, 512 34 us; 8192 of 4096: 512 95 us, 768 99 us; 5859 of 5120: 512 89 us, 768 100 us; 3662 of 8192: 512 92 us, 256 108 us; 2500 of 12000:
+// 256 98 us, 512 105 us).
+uint64_t norm_groups(uint64_t tokens, int waves, int items)
 {
-    const uint64_t all = parts_of(tokens, norm_rows(waves)), most = waves == 16 && (items > 1 || stream_size < 4) ? 256 : waves < 16 && items == 1 ? NORM_GROUPS : 512;
+    const uint64_t all = parts_of(tokens, norm_rows(waves)), most = waves == 16 ? 256 : items == 1 ? NORM_GROUPS : 512;
     return all < most ? all : most;
 }
 
@@ -392,7 +405,7 @@ int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, 
                           tokens * dim * ((d_x_grad ? size_of(type) : 0) + (d_residual_grad ? size_of(stream_type) : 0)) > CACHED, parts};
     if (tokens)
         with_norm(type, stream_type, dim, [&](auto t, auto r, auto waves, auto items) {
-            groups = norm_groups(tokens, waves(), items(), size_of(stream_type));
+            groups = norm_groups(tokens, waves(), items());
             norm_backward_kernel<decltype(t), decltype(r), waves(), items()><<<static_cast<uint32_t>(groups), NORM_THREADS<waves()>, 0, s>>>(c);
         });
     if (d_gain_grad)

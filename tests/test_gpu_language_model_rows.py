@@ -262,8 +262,8 @@ KINDS = [(torch.bfloat16, None), (torch.float16, None), (torch.float32, None), (
 
 
 @pytest.mark.parametrize("dtype,stream", KINDS)
-@pytest.mark.parametrize("dim", [8, 9, 12, 15, 16, 64, 100, 505, 511, 512, 513, 520, 765, 1023, 1024, 1025, 1536, 2047, 2048, 2049, 2880, 4095, 4096, 4097, 5120, 8191, 8192,
-                                 8193, 12000, 16383, 16384])
+@pytest.mark.parametrize("dim", [8, 9, 12, 15, 16, 64, 100, 505, 511, 512, 513, 520, 765, 768, 769, 1023, 1024, 1025, 1536, 1537, 2047, 2048, 2049, 2880, 4095, 4096, 4097, 5120, 6144, 6145, 8191, 8192,
+                                 8193, 12000, 12288, 12289, 16383, 16384])
 def test_norm_row_lengths(dim, dtype, stream):
     check_norm(5, dim, dtype, stream, seed=dim)
 
