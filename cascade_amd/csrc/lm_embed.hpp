@@ -5,7 +5,7 @@
 // Backward: places are put in the order of their words first, so that a row of d_weight is the sum of neighbouring entries, without atomics and in a fixed
 // order. A short text is ranked in one launch: place i goes to where it has as many entries before it as there are pairs (word, place) below its own, all pairs
 // compared. A longer one takes a stable sort by digits of up to 9 bits, three launches each: workgroups count the digits of their segments, the counts of a digit are summed over the
-// segments, and the workgroups move their segments, with ballots that tell a lane how many lanes before it hold its digit.
+// segments (few are by those who move them), and the workgroups move their segments, with ballots that tell a lane how many lanes before it hold its digit.
 // The order is cut into runs of entries, whatever words they hold, so that frequent words are shared out: a team of lanes adds up a run's rows in 32 bits and stores
 // the words that lie inside it. Of words that reach over a run's ends the teams of a workgroup join their sums in LDS, in the order of the runs, and what reaches over the ends of the
 // workgroup's block of runs is left as a partial sum, which a second kernel joins in the order of the blocks.
@@ -206,8 +206,8 @@ __global__ __launch_bounds__(256) void sum_digits_kernel(uint32_t* counts, uint3
 }
 
 // A workgroup a segment, a turn at a time: each of its waves has a quarter of the turn, ranks its entries among those of their digit in that quarter and counts them, and
-// begins behind the counts of the waves before it.
-template <class Token>
+// begins behind the counts of the waves before it. SUMMED: counts and totals are sums over the segments; otherwise the workgroup adds up all counts itself.
+template <class Token, bool SUMMED>
 __global__ __launch_bounds__(256) void move_digits_kernel(Entries<Token> e, int64_t segment, uint32_t segments, int shift, uint32_t digits, const uint32_t* counts,
                                                           const uint32_t* totals, uint32_t* words, uint32_t* places)
 {
@@ -222,8 +222,19 @@ __global__ __launch_bounds__(256) void move_digits_kernel(Entries<Token> e, int6
 #pragma unroll
         for (int k = 0; k < EACH; ++k) { // neighbouring digits a lane
             const uint32_t d = threadIdx.x * EACH + k;
-            x[k] = d < digits ? totals[d] : 0;
-            before[k] = d < digits ? counts[d * static_cast<uint64_t>(segments) + blockIdx.x] : 0;
+            const uint32_t* mine = counts + d * static_cast<uint64_t>(segments);
+            x[k] = before[k] = 0;
+            if (SUMMED && d < digits) {
+                x[k] = totals[d];
+                before[k] = mine[blockIdx.x];
+            } else if (d < digits) {
+#pragma unroll 8
+                for (uint32_t s = 0; s < segments; ++s) {
+                    const uint32_t count = mine[s];
+                    before[k] += s < blockIdx.x ? count : 0;
+                    x[k] += count;
+                }
+            }
             sum += x[k];
         }
         uint32_t to = sums_to(sum);
