@@ -446,6 +446,9 @@ uint64_t block_words(const EntropyPlan& plan) { return plan.narrow_logits ? Line
 // Products of few tokens have kernels of their own, up to a vocabulary of one piece.
 bool few_tokens(const EntropyPlan& plan, uint64_t tokens) { return tokens <= FEW_TOKENS && plan.pieces == 1; }
 
+// Tokens that a word's line of P has room for, twice.
+int few_width(uint64_t tokens) { return tokens <= FEW_TOKENS / 2 ? FEW_TOKENS / 2 : FEW_TOKENS; }
+
 // Shares of d_hidden there: a workgroup a compute unit, of at least a slice for each of its waves.
 struct FewPlan {
     uint64_t parts, shares, share_words, chunks, chunk_words;
@@ -466,6 +469,7 @@ struct TeacherWork {
     float *q, *entropy, *dots, *shares;
     uint16_t* first;
     short *low, *by_words; // of few tokens
+    uint32_t* heavy; // blocks of 64 words whose P needs both numbers
     uint64_t blocks, bytes;
     TeacherWork(void* base, uint64_t before, const EntropyPlan& plan, uint64_t tokens, uint64_t dim, uint64_t vocab, uint64_t kept, bool backward)
     {
@@ -478,8 +482,9 @@ struct TeacherWork {
         entropy = c.take<float>(tokens);
         dots = c.take<float>(backward ? 0 : parts_of(vocab, 256) * 4 * tokens);
         const bool few = backward && few_tokens(plan, tokens);
-        low = few && tokens <= TWICE_TOKENS ? c.take<short>(tokens * up(vocab, SLICE)) : nullptr;
-        by_words = c.take<short>(few ? vocab * FEW_TOKENS : 0);
+        low = c.take<short>(few ? tokens * up(vocab, SLICE) : 0);
+        by_words = c.take<short>(few ? vocab * 2 * few_width(tokens) : 0);
+        heavy = c.take<uint32_t>(few ? parts_of(vocab, SLICE) : 0);
         shares = c.take<float>(few ? FewPlan(dim, vocab).shares * tokens * plan.padded_dim : 0);
         bytes = c.used;
     }
@@ -820,25 +825,26 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
             const uint32_t parts = static_cast<uint32_t>(few.parts), chunks = static_cast<uint32_t>(few.chunks);
             const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), static_cast<uint32_t>(parts_of(vocab, N::BM)), 1, tw.counts, 0};
             distill_gradients_kernel<N, Type, true><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride,
-                                                                                FewGradients{d_weight_to ? tw.by_words : nullptr, tw.low});
-            const bool twice = tokens <= TWICE_TOKENS;
+                                                                                FewGradients{d_weight_to ? tw.by_words : nullptr, tw.low, few_width(tokens),
+                                                                                             reinterpret_cast<uint16_t*>(tw.heavy), (Type::wide_range ? 1.f : 16384.f) / 8});
+            const bool half = few_width(tokens) < FEW_TOKENS;
             if (d_weight_to) {
                 const auto launch = [&](auto most) {
                     few_weight_gradients_kernel<Type, most()><<<static_cast<uint32_t>(parts_of(few.parts * few.chunks, 4)), 256, 0, s>>>(
-                        Operand{w.kept, hidden.stride, d}, tw.by_words, static_cast<int>(tokens), words, static_cast<int64_t>(few.chunk_words), parts, chunks, w.scale, d_weight_to,
+                        Operand{w.kept, hidden.stride, d}, tw.by_words, tw.heavy, static_cast<int>(tokens), words, static_cast<int64_t>(few.chunk_words), parts, chunks, w.scale, d_weight_to,
                         weight_grad_stride, aligned(d_weight_to, 16) && weight_grad_stride % 8 == 0);
                 };
-                if (twice)
-                    launch(std::integral_constant<int, TWICE_TOKENS>());
+                if (half)
+                    launch(std::integral_constant<int, FEW_TOKENS / 2>());
                 else
                     launch(std::integral_constant<int, FEW_TOKENS>());
             }
             if (d_hidden_to) {
                 const auto launch = [&](auto rows) {
                     few_hidden_gradients_kernel<Type, rows()><<<parts * static_cast<uint32_t>(few.shares), 256, 0, s>>>(
-                        w.p, tw.low, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
+                        w.p, tw.low, tw.heavy, stride, Operand{weight.data, weight.stride, d}, static_cast<int>(tokens), words, static_cast<int64_t>(few.share_words), parts, tw.shares, hidden.stride);
                 };
-                if (twice)
+                if (half)
                     launch(std::integral_constant<int, 1>());
                 else
                     launch(std::integral_constant<int, 2>());

@@ -282,9 +282,12 @@ __global__ __launch_bounds__(256) void join_distill_kernel(const float2* part, c
     }
 }
 
-// Where there are few tokens (lm_few_tokens.hpp): P in the other order, too, and what its rounding leaves, where there are so few that both numbers have a place there; or null.
+// What few tokens take beside P (lm_few_tokens.hpp).
 struct FewGradients {
-    short *by_words, *low;
+    short *by_words, *low; // P and what its rounding leaves in the other order, in rows of `width` tokens each, or null; what the rounding leaves in P's order
+    int width;
+    uint16_t* heavy; // two a block of 64 words, for 32 tokens each: whether an entry there is larger than `least`
+    float least;     // an eighth of the largest one that may be
 };
 
 // P[n][v] = d_loss[n] (exp(z - lse[n]) - q) relative to the largest |d_loss|, as logit_gradients_kernel leaves it; 1 / T is in what the products are scaled back with.
@@ -307,6 +310,7 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
     constexpr int EIGHTS = Words::LINE / 8;
     const int eight = lane % EIGHTS;
     const int64_t m = mw + eight * 8;
+    static_assert(!FEW || Words::LINE == SLICE, "a line of P is a wave's");
 #pragma unroll
     for (int j = 0; j < P::TN; ++j) {
         const int64_t first = n0 + P::wave_n() + 32 * j, n = first + lane % 32;
@@ -321,19 +325,19 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
                     Words::word(lines, lane, static_cast<int>(teacher.ids[n * teacher.kept + e] - word0)) -= teacher.q[n * teacher.kept + e] * factor;
         }
         wait_for_lds();
-        if (FEW && few.by_words && (!few.low || n < TWICE_TOKENS))
+        if (FEW && few.by_words && n < few.width)
             for (int k = 0; k < Words::PIECES; k += 2) { // four words a lane
                 const int piece = k + lane / 32;
                 const f32x4 y = *reinterpret_cast<const f32x4*>(Words::piece(lines, lane % 32, piece));
                 for (int r = 0; r < 4; ++r)
                     if (mw + 4 * piece + r < l.weight.rows) {
-                        short* to = few.by_words + (mw + 4 * piece + r) * FEW_TOKENS + n;
+                        short* to = few.by_words + (mw + 4 * piece + r) * (2 * few.width) + n;
                         const short rounded = to16<Type>(y[r]);
                         to[0] = rounded;
-                        if (few.low)
-                            to[TWICE_TOKENS] = to16<Type>(y[r] - to32<Type>(rounded));
+                        to[few.width] = to16<Type>(y[r] - to32<Type>(rounded));
                     }
             }
+        bool heavy = false;
 #pragma unroll
         for (int c = 0; c < 32; c += 64 / EIGHTS) {
             const int token = c + lane / EIGHTS;
@@ -343,24 +347,31 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
             for (int r = 0; r < 8; ++r) {
                 const float x = r < 4 ? front[r] : back[r - 4];
                 y[r] = to16<Type>(x);
-                if (FEW)
+                if (FEW) {
                     rest[r] = to16<Type>(x - to32<Type>(y[r]));
+                    heavy |= fabsf(x) > few.least && fabsf(x) <= 8 * few.least; // infinite weights change nothing for other tokens
+                }
             }
             if (first + token >= tokens || m >= l.weight.rows)
                 continue;
             const int64_t to = (first + token) * stride + m;
             if (m + 8 <= l.weight.rows) {
                 *reinterpret_cast<s16x8*>(out + to) = y;
-                if (FEW && few.low)
+                if (FEW)
                     *reinterpret_cast<s16x8*>(few.low + to) = rest;
             } else {
                 for (int r = 0; r < 8; ++r)
                     if (m + r < l.weight.rows) {
                         out[to + r] = y[r];
-                        if (FEW && few.low)
+                        if (FEW)
                             few.low[to + r] = rest[r];
                     }
             }
+        }
+        if (FEW) {
+            const bool some = __any(heavy);
+            if (lane == 0 && mw < l.weight.rows)
+                few.heavy[mw / SLICE * 2 + first / 32] = some;
         }
         wait_for_lds();
     }
@@ -369,7 +380,7 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
         for (int64_t tail = l.weight.rows + threadIdx.x % 8; tail < stride; tail += 8)
             for (int64_t n = n0 + threadIdx.x / 8; n < n0 + P::BN && n < tokens; n += P::THREADS / 8) {
                 out[n * stride + tail] = 0;
-                if (FEW && few.low)
+                if (FEW)
                     few.low[n * stride + tail] = 0;
             }
 }

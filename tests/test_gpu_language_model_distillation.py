@@ -140,6 +140,26 @@ def test_gradients_of_few_tokens_are_rounded_once(n, dtype):
         assert (a.double() - b).norm() <= 1.05 * (b.to(dtype).double() - b).norm()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [33, 50, 64])
+def test_heavy_gradients_of_33_to_64_tokens_are_rounded_once(n, dtype):
+    """There the gradients of the logits have twice the bits in blocks of 64 words with an entry above an eighth of the largest weight. What is below that may be rounded twice: off by up to u of
+    each product that it is part of; the rest as above."""
+    g = gen(n)
+    dim, vocab = 200, 4000
+    hidden, weight = randn(g, n, dim, dtype=dtype), randn(g, vocab, dim, dtype=dtype, scale=2 * dim ** -0.5)
+    ids, logits = teacher(g, n, 10, vocab, ignored=0.0)
+    ids[:, 0], logits[:, 0] = torch.randint(0, vocab, (n,), generator=g, device="cuda").int() // 9 * 9, 9.0  # (not relative to the other logits, as was first written here: what stands beside ids that are none is NaN, in the oracle as well)
+    d_loss = torch.full((n,), 1.00390625 - 2.0 ** -10, device="cuda")
+    lse = cascade_amd.linear_distillation(hidden, weight, ids, logits, 1.5)[1]
+    got = cascade_amd.linear_distillation_backward(d_loss, hidden, weight, ids, logits, lse, 1.5)
+    _, _, p, q, _ = reference(hidden, weight, ids, logits, 1.5)
+    d_z, u = (p - q) * d_loss.double()[:, None] / 1.5, torch.finfo(dtype).eps / 2
+    light = torch.where((p - q).abs() <= 1 / 8, d_z, 0).abs()
+    for a, b, more in zip(got, (d_z @ weight.double(), d_z.T @ hidden.double()), (light @ weight.double().abs(), light.T @ hidden.double().abs())):
+        assert (a.double() - b).norm() <= 1.05 * (b.to(dtype).double() - b).norm() + u * more.norm()
+
+
 def test_distillation_over_the_corpus_vocabulary():
     check_distillation(600, 256, 50257, 50, torch.bfloat16, seed=3)
     check_distillation(40, 256, 65535, 100, torch.float16, seed=4)
