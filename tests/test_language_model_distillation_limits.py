@@ -59,13 +59,13 @@ def test_more_than_a_launch_holds(tokens, dim, vocab):
 
 def test_workspaces_hold_the_entries_and_no_logits():
     """Beside the cross entropy's: ids and q, the first entry of each block of at least 64 words in 16 bits, a few numbers of every token, and forwards a number for
-    each part of the vocabulary that a wave sums. Up to 64 tokens, backwards, also 64 values of 16 bits for every word and a sum of d_hidden for every workgroup of 128 values, one a compute unit, and up to 32 what the
-    rounding leaves of the gradients of the logits."""
+    each part of the vocabulary that a wave sums. Up to 64 tokens, backwards, also twice 32 or 64 values of 16 bits for every word, what the rounding leaves of the gradients of the logits,
+    a number for each block of 64 words, and a sum of d_hidden for every workgroup of 128 values, one a compute unit."""
     lib = native.load()
     for tokens in (1, 32, 33, 61, 64, 65, 4099, 8192):
         for kept in (1, 64, 1024):
             for flags in (0, native.CSA_LM_BACKWARD):
                 more = lib.csa_lm_distill_workspace(tokens, 1024, 50257, kept, flags) - lib.csa_lm_cross_entropy_workspace(tokens, 1024, 50257, flags)
-                few = 50304 * 2 * tokens * (tokens <= 32) + 50257 * 128 + 256 * 128 * 4 * tokens if flags and tokens <= 64 else 0
+                few = 50304 * 2 * tokens + 50257 * (128 if tokens <= 32 else 256) + 786 * 4 + 256 * 128 * 4 * tokens if flags and tokens <= 64 else 0
                 assert tokens * kept * 8 <= more <= tokens * (kept * 8 + 2 * 787 + 8 + (0 if flags else 4 * 788)) + few + 8 * 256
     assert lib.csa_lm_distill_workspace(5, 64, 300, 0, 0) == lib.csa_lm_distill_workspace(5, 64, 300, 1025, 0) == 0
