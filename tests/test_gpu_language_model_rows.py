@@ -104,6 +104,22 @@ def test_embed_of_long_texts(n, rows, bits):
         check_embed(text(n, rows, spread, gen(n), bits), rows, 24, torch.float16 if bits == 16 else torch.float32, seed=n)
 
 
+@pytest.mark.parametrize("n", [100, 5000, 8192, 8193, 70001, 262144 + 5])
+@pytest.mark.parametrize("dim", [24, 56, 120, 250, 600])  # teams of 8, 16, 32 and 64 lanes, one slice of a row and several
+@pytest.mark.parametrize("spread", ["zipf", "even", "one"])
+def test_embed_gradients_of_whole_numbers_are_exact(spread, dim, n):
+    """Small whole numbers add up without rounding in 32 bits, whatever the order: every sum has to be that of 64-bit integers. A lost, doubled or swapped row changes it."""
+    g = gen(n + dim)
+    rows = 3000
+    tokens = text(n, rows, spread, g)
+    d_out = torch.randint(-8, 9, (n, dim), generator=g, device="cuda")  # 8 n < 2^24
+    word = words_of(tokens, rows)
+    want = torch.zeros(rows, dim, dtype=torch.int64, device="cuda").index_add_(0, word[word >= 0], d_out[word >= 0])
+    for dtype in TYPES:
+        got = cascade_amd.embed_tokens_backward(d_out.to(dtype), tokens, rows)
+        assert torch.equal(got, want.float().to(dtype))  # rounded to the type once
+
+
 def test_embed_of_a_very_long_text():
     """More tokens than there are segments of the smallest size, and offsets past 2^32 bytes in d_out."""
     n, rows = 4300000, 70001
