@@ -160,6 +160,47 @@ def test_heavy_gradients_of_33_to_64_tokens_are_rounded_once(n, dtype):
         assert (a.double() - b).norm() <= 1.05 * (b.to(dtype).double() - b).norm() + u * more.norm()
 
 
+def check_rows_of_33_to_64_tokens(n, d_loss, dtype):
+    """Both gradients row by row, where each token has one word, in a block of 64 words of its own, that it finds unlikely: an entry of -d_loss nearly, and small ones. A row is off by the rounding of
+    the result, by a twentieth of that for sums of 32 bits, and by what a single rounding makes of its small entries: u of each, one sign as likely as the other, so that their squares add up (to a
+    tenth more: the rows that they are multiplied with are nearly at right angles), and in half precision half a step of 2^-24 of the largest weight over 2^14. That is up to 1.13 times the rounding in
+    d_hidden. With an entry of -d_loss that is rounded once as well it is 2, which is shown on the formula's values."""
+    g = gen(n)
+    dim, blocks = 200, 70
+    hidden, weight = randn(g, n, dim, dtype=dtype), randn(g, 64 * blocks, dim, dtype=dtype, scale=dim ** -0.5)
+    h, w = hidden.double(), weight.double()
+    at = torch.arange(n, device="cuda")
+    block = torch.randperm(blocks, generator=g, device="cuda")[:n]
+    words = (h @ w.T).view(n, blocks, 64)[at, block].argmin(1) + 64 * block
+    ids, logits = words[:, None].int(), torch.zeros(n, 1, device="cuda")
+    lse = cascade_amd.linear_distillation(hidden, weight, ids, logits)[1]
+    got = cascade_amd.linear_distillation_backward(d_loss, hidden, weight, ids, logits, lse)
+    _, _, p, q, _ = reference(hidden, weight, ids, logits, 1.0)
+    d_z, u, top, full = (p - q) * d_loss.double()[:, None], U[dtype], d_loss.max().double(), 16384.0 if dtype == torch.float16 else 1.0
+    off = (u * torch.where((p - q).abs() > 1 / 8, 0.0, d_z)) ** 2 + (top * 2.0 ** -25 / full if dtype == torch.float16 else 0.0) ** 2
+    once = (d_z * (full / top)).to(dtype).double() * (top / full)
+    for name, a, want, more, worse in (("d_hidden", got[0], d_z @ w, off @ w.square(), once @ w),
+                                       ("d_weight", got[1][words], (d_z.T @ h)[words], (off.T @ h.square())[words], (once.T @ h)[words])):
+        bound = 1.05 * (want.to(dtype).double() - want).norm(dim=1) + 1.1 * more.sum(1).sqrt()
+        # all rows but those whose weight happens to need few bits
+        assert ((worse.to(dtype).double() - want).norm(dim=1) > bound).sum() >= n - 5, name
+        ratio = (a.double() - want).norm(dim=1) / bound
+        assert (ratio <= 1).all(), f"{name}: {int((ratio > 1).sum())} of {n} rows are off by up to {ratio.max().item():.2f} of the bound"
+
+
+def weights_that_need_bits(n, far, dtype):
+    """One token's weight is 2, by which all are held; the others lie three quarters of the way to where rounding changes sides, over powers of two from 1 to 2^-far."""
+    w = (1 + 0.75 * U[dtype]) * torch.exp2(-(torch.arange(n, device="cuda") % (far + 1)).float())
+    w[0] = 2.0
+    return w
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [33, 50, 64])
+def test_rows_of_33_to_64_tokens_of_even_weights(n, dtype):
+    check_rows_of_33_to_64_tokens(n, weights_that_need_bits(n, 0, dtype), dtype)
+
+
 def test_distillation_over_the_corpus_vocabulary():
     check_distillation(600, 256, 50257, 50, torch.bfloat16, seed=3)
     check_distillation(40, 256, 65535, 100, torch.float16, seed=4)
