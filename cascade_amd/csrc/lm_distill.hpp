@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void teacher_kernel(const int32_t* ids, const 
     for (int i = 0; i < ITEMS; ++i) {
         const int k = i * LANES + lane;
         const int32_t id = k < kept ? ids[n * kept + k] : -1;
-        told[i] = id >= 0 && id < vocab ? logits[n * kept + k] * rate : -INFINITY;
+        told[i] = id >= 0 && id < vocab ? logits[n * kept + k] : -INFINITY;
         word[i] = told[i] == -INFINITY ? NONE : static_cast<uint32_t>(id); // nothing is told: no entry
         here += word[i] != NONE;
         top = fmaxf(top, told[i]);
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void teacher_kernel(const int32_t* ids, const 
     float sum = 0, part = 0;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        told[i] -= top;
+        told[i] = (told[i] - top) * rate; // in this order nothing finite becomes infinite but what has no weight
         sum += word[i] != NONE ? expf(told[i]) : 0.f;
     }
     sum = over_lanes(sum, sum_of);
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(256) void teacher_kernel(const int32_t* ids, const 
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const float q = expf(told[i]) / sum;
-        part += word[i] != NONE ? q * (told[i] - all) : 0.f;
+        part += word[i] != NONE && told[i] != -INFINITY ? q * (told[i] - all) : 0.f;
         told[i] = q;
     }
     part = over_lanes(part, sum_of);

@@ -201,6 +201,37 @@ def test_rows_of_33_to_64_tokens_of_even_weights(n, dtype):
     check_rows_of_33_to_64_tokens(n, weights_that_need_bits(n, 0, dtype), dtype)
 
 
+@pytest.mark.parametrize("n", [40, 90, 1100])  # four waves a token, and one
+@pytest.mark.parametrize("kept", [5, 100, 300])
+@pytest.mark.parametrize("temperature", [0.25, 1.0, 3.0])
+def test_only_minus_infinity_is_no_entry(temperature, kept, n):
+    """Finite logits are entries, however low or high, and a softmax is that of the logits less their largest one: less 1000 is nothing at these temperatures."""
+    g = gen(n + kept)
+    dim, vocab = 64, 500
+    lowest, highest = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
+    ids = torch.randint(0, vocab, (n, kept), generator=g, device="cuda", dtype=torch.int32)
+    logits = randn(g, n, kept, scale=3.0)
+    logits[0] = lowest
+    logits[1] = highest
+    logits[2, 1:] = lowest
+    logits[3, :2] = lowest
+    logits[3, 2:] = -math.inf
+    logits[4, 1:] = lowest
+    logits[4, 0] = highest
+    logits[5] = -math.inf
+    logits[6, 1:] = -2e38
+    logits[6, 0] = lowest
+    logits[7] += 1e30
+    told = logits - logits.amax(1, keepdim=True)  # -infinity less itself is NaN: token 5 stays without entries
+    told = torch.where(torch.isnan(told), -math.inf, torch.where(torch.isinf(logits), -math.inf, told.clamp(min=-1000.0)))
+    hidden, weight, _, _, loss, lse, grads = check_distillation(n, dim, vocab, kept, torch.bfloat16, temperature, told=(ids, told), weights=torch.ones(n, device="cuda"), seed=n)
+    got = cascade_amd.linear_distillation(hidden, weight, ids, logits, temperature)
+    assert torch.equal(got[0], loss) and torch.equal(got[1], lse)
+    found = cascade_amd.linear_distillation_backward(torch.ones(n, device="cuda"), hidden, weight, ids, logits, lse, temperature)
+    assert all(torch.equal(a, b) for a, b in zip(found, grads))
+    assert loss[0] > 0 and loss[5] == 0
+
+
 def test_distillation_over_the_corpus_vocabulary():
     check_distillation(600, 256, 50257, 50, torch.bfloat16, seed=3)
     check_distillation(40, 256, 65535, 100, torch.float16, seed=4)
