@@ -826,7 +826,7 @@ int csa_lm_distill_backward_dev(int type, const void* d_hidden, int64_t hidden_s
             const Logits l{weight, hidden, static_cast<int64_t>(plan.padded_dim), static_cast<uint32_t>(parts_of(vocab, N::BM)), 1, tw.counts, 0};
             distill_gradients_kernel<N, Type, true><<<l.mt, N::THREADS, 0, s>>>(l, tw.teacher(kept), rate, d_lse, d_loss_grad, w.scale, w.p, stride,
                                                                                 FewGradients{d_weight_to ? tw.by_words : nullptr, tw.low, few_width(tokens),
-                                                                                             reinterpret_cast<uint16_t*>(tw.heavy), (Type::wide_range ? 1.f : 16384.f) / 8});
+                                                                                             reinterpret_cast<uint16_t*>(tw.heavy)});
             const bool half = few_width(tokens) < FEW_TOKENS;
             if (d_weight_to) {
                 const auto launch = [&](auto most) {

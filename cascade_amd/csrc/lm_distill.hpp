@@ -286,8 +286,7 @@ __global__ __launch_bounds__(256) void join_distill_kernel(const float2* part, c
 struct FewGradients {
     short *by_words, *low; // P and what its rounding leaves in the other order, in rows of `width` tokens each, or null; what the rounding leaves in P's order
     int width;
-    uint16_t* heavy; // two a block of 64 words, for 32 tokens each: whether an entry there is larger than `least`
-    float least;     // an eighth of the largest one that may be
+    uint16_t* heavy; // two a block of 64 words, for 32 tokens each: whether an entry there is larger than an eighth of its token's weight
 };
 
 // P[n][v] = d_loss[n] (exp(z - lse[n]) - q) relative to the largest |d_loss|, as logit_gradients_kernel leaves it; 1 / T is in what the products are scaled back with.
@@ -341,6 +340,7 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
 #pragma unroll
         for (int c = 0; c < 32; c += 64 / EIGHTS) {
             const int token = c + lane / EIGHTS;
+            const float least = FEW ? fabsf(__shfl(factor, token)) * 0.125f : 0.f;
             const f32x4 front = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight)), back = *reinterpret_cast<const f32x4*>(Words::piece(lines, token, 2 * eight + 1));
             s16x8 y, rest = {};
 #pragma unroll
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(P::THREADS) void distill_gradients_kernel(Logits l,
                 y[r] = to16<Type>(x);
                 if (FEW) {
                     rest[r] = to16<Type>(x - to32<Type>(y[r]));
-                    heavy |= fabsf(x) > few.least && fabsf(x) <= 8 * few.least; // infinite weights change nothing for other tokens
+                    heavy |= fabsf(x) > least; // never of infinite weights, which change nothing for other tokens
                 }
             }
             if (first + token >= tokens || m >= l.weight.rows)

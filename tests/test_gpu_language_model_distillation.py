@@ -201,6 +201,14 @@ def test_rows_of_33_to_64_tokens_of_even_weights(n, dtype):
     check_rows_of_33_to_64_tokens(n, weights_that_need_bits(n, 0, dtype), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [33, 50, 64])
+@pytest.mark.parametrize("far", [3, 8])
+def test_rows_of_33_to_64_tokens_of_uneven_weights(far, n, dtype):
+    """How exact a token's gradient is does not depend on how much the others weigh."""
+    check_rows_of_33_to_64_tokens(n, weights_that_need_bits(n, far, dtype), dtype)
+
+
 @pytest.mark.parametrize("n", [40, 90, 1100])  # four waves a token, and one
 @pytest.mark.parametrize("kept", [5, 100, 300])
 @pytest.mark.parametrize("temperature", [0.25, 1.0, 3.0])
