@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256) void embed_sums_kernel(EmbedSums e, const T* d
     }
     enum { HEAD = 1, THROUGH = 2, TAIL = 4 }; // the run's first word comes from the run before, and goes on behind this one; its last word begins in it and goes on
     constexpr int TEAMS = 256 / LANES, AHEAD = 8;
-    __shared__ float heads[TEAMS][V][LANES], tails[TEAMS][V][LANES];
+    __shared__ float heads[TEAMS][V][LANES];
     __shared__ int reach[TEAMS];
     const int64_t block = blockIdx.x / e.slices;
     const int team = threadIdx.x / LANES, x = threadIdx.x % LANES;
@@ -364,11 +364,13 @@ __global__ __launch_bounds__(256) void embed_sums_kernel(EmbedSums e, const T* d
         auto close = [&](bool goes_on) { // the sum of `word` is complete as far as this run goes
             if (word >= e.rows)
                 return;
-            if (continued || goes_on) {
-                reaches |= continued ? HEAD | (goes_on ? THROUGH : 0) : TAIL;
+            if (continued) {
+                reaches |= HEAD | (goes_on ? THROUGH : 0);
 #pragma unroll
                 for (int k = 0; k < V; ++k)
-                    (continued ? heads : tails)[team][k][x] = sum[k];
+                    heads[team][k][x] = sum[k];
+            } else if (goes_on) { // the last word: `sum` stays as it is, and goes on below
+                reaches |= TAIL;
             } else if (at.mine) {
 #pragma unroll
                 for (int k = 0; k < V; ++k)
