@@ -212,12 +212,13 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
             typedef std::integral_constant<int, 4> Four;
             typedef std::integral_constant<int, 16> Sixteen;
             constexpr uint64_t V = PIECE<decltype(s)>;
+            if constexpr (sizeof(t) == 2)
+                if (dim > 128 * V && dim <= 192 * V)
+                    return f(t, s, One(), Three());
             if (dim <= 64 * V)
                 f(t, s, One(), One());
             else if (dim <= 128 * V)
                 f(t, s, One(), Two());
-            else if (sizeof(t) == 2 && dim <= 192 * V)
-                f(t, s, One(), Three());
             else if (dim <= 256 * V)
                 f(t, s, Four(), One());
             else if (dim <= 512 * V)
