@@ -4,6 +4,7 @@
 #include "lm_embed.hpp"
 #include "lm_norm.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -244,6 +245,7 @@ void with_norm(int type, int stream_type, uint64_t dim, F f)
 }
 
 uint64_t norm_rows(int waves) { return waves == 1 ? 4 : 1; } // of a workgroup at a time
+uint64_t norm_sums(uint64_t tokens) { return tokens < NORM_GROUPS ? tokens : NORM_GROUPS; } // rows of d_gain's sums that the workspace holds
 
 // Workgroups of the backward kernel, each with sums of d_gain of its own: as many as fit the compute units at once, or half as many where the sums would otherwise cost more than is
 // won (30000 rows of 100 values: 768 32 us, 512 34 us; 8192 of 4096: 512 95 us, 768 99 us; 5859 of 5120: 512 89 us, 768 100 us; 3662 of 8192: 512 92 us, 256 108 us; 2500 of 12000:
@@ -251,7 +253,7 @@ uint64_t norm_rows(int waves) { return waves == 1 ? 4 : 1; } // of a workgroup a
 uint64_t norm_groups(uint64_t tokens, int waves, int items)
 {
     const uint64_t all = parts_of(tokens, norm_rows(waves)), most = waves == 16 ? 256 : items == 1 ? NORM_GROUPS : 512;
-    return all < most ? all : most;
+    return std::min({all, most, norm_sums(tokens)});
 }
 
 } // namespace
@@ -378,7 +380,7 @@ int csa_lm_norm_forward_dev(int type, int stream_type, const void* d_x, int64_t 
 
 uint64_t csa_lm_norm_backward_workspace(uint64_t tokens, uint64_t dim)
 {
-    return dim < LEAST_DIM || dim > NORM_DIM ? 0 : up((tokens < NORM_GROUPS ? tokens : NORM_GROUPS) * dim * sizeof(float), 256);
+    return dim < LEAST_DIM || dim > NORM_DIM ? 0 : up(norm_sums(tokens) * dim * sizeof(float), 256);
 }
 
 int csa_lm_norm_backward_dev(int type, int stream_type, const void* d_out_grad, int64_t out_grad_stride, const void* d_total, int64_t total_stride, const float* d_rstd,

@@ -99,3 +99,15 @@ def test_norm_of_more_than_a_launch_holds():
     size = native.load().csa_lm_norm_backward_workspace
     assert size(5, 7) == size(5, 16385) == 0
     assert size(1, 64) == 256 and all(size(1 << 20, dim) <= 4096 * 4 * dim + 256 for dim in (8, 1024, 16384))
+
+
+def test_norm_workspaces_hold_a_row_of_sums_for_every_workgroup():
+    """Of as many workgroups as there are tokens, 768 at most: no row less, which a workgroup would write past the end, and none more."""
+    size = native.load().csa_lm_norm_backward_workspace
+    for tokens in (0, 1, 2, 255, 256, 257, 511, 512, 513, 767, 768, 769, 1 << 20, (1 << 24) - 1):
+        for dim in (8, 9, 63, 64, 1000, 4096, 16383, 16384):
+            assert size(tokens, dim) == -(-min(tokens, 768) * dim * 4 // 256) * 256
+            if tokens:
+                need = size(tokens, dim)
+                strides = dict(gs=dim, ts=dim, ds=dim, dim=dim, tokens=min(tokens, (1 << 22) - 1))
+                assert norm_backward(size=need - 1, **strides) == BAD and str(need).encode() in native.load().csa_lm_last_error()
