@@ -4,8 +4,8 @@
 // Forward: bound by memory, a row read and a row written a token.
 // Backward: places are put in the order of their words first, so that a row of d_weight is the sum of neighbouring entries, without atomics and in a fixed
 // order. A short text is ranked in one launch: place i goes to where it has as many entries before it as there are pairs (word, place) below its own, all pairs
-// compared. A longer one takes a stable sort by digits of up to 9 bits, three launches each: workgroups count the digits of their segments, the counts of a digit are summed over the
-// segments (few are by those who move them), and the workgroups move their segments, with ballots that tell a lane how many lanes before it hold its digit.
+// compared. A longer one takes a stable sort by digits of up to 9 bits, two launches each, or three where there are many segments: workgroups count the digits of their segments, the counts of a digit
+// are summed over the segments (few are by those who move them), and the workgroups move their segments, with ballots that tell a lane how many lanes before it hold its digit.
 // The order is cut into runs of entries, whatever words they hold, so that frequent words are shared out: a team of lanes adds up a run's rows in 32 bits and stores
 // the words that lie inside it. Of words that reach over a run's ends the teams of a workgroup join their sums in LDS, in the order of the runs, and what reaches over the ends of the
 // workgroup's block of runs is left as a partial sum, which a second kernel joins in the order of the blocks.

@@ -5,8 +5,9 @@
 // not). It is the sum of two numbers of 16 bits, what the rounding leaves being the second one, in rows of its own and behind the first ones of a word. With one number its rounding and the
 // results' own add up to 1.4 times the latter where entries are many, but a short text's errors are those of a few entries, its tokens' likeliest words, and spread about that: up to 1.6 times.
 // For up to 32 tokens the second number takes the places of tokens that are not there, and no time. For 33 to 64 it is read and multiplied where it matters, in blocks of 64 words that
-// hold an entry above an eighth of its token's weight: errors of 1.00 to 1.16 times, where those entries make most of the sums, for 7 % of the time (61 tokens of 512 values trained 80 -> 85 us,
-// 40 of 2560 260 -> 265); in all blocks it would be 12 and 9 %.
+// hold an entry above an eighth of its token's weight: errors of 1.00 to 1.18 times, where those entries make most of the sums, for 7 % of the time (61 tokens of 512 values trained 80 -> 85 us,
+// 40 of 2560 260 -> 265); in all blocks it would be 12 and 9 %. An entry is held against its own token's weight, since a row of d_hidden is as large as that: 64 tokens of 512 values whose weights differ
+// by up to 2^10 take 86 us, 83 if only entries above an eighth of the largest weight counted, which left the rows of the others with errors of about twice the rounding.
 // d_weight of 61 tokens of 512 values and 50257 words takes 16 us, of 40 of 2560 58 us, of 3 of 4096 73 us, 5.6 TB/s (by the tiles of lm_product.hpp, with one number, 21, 77 and 118: one
 // workgroup a compute unit, which waits for its loads, multiplies and stores one after the other). d_hidden reads the weight behind what has just been written: 18 and 86 us, by tiles the
 // same, but 6 us instead of 34 over 3000 words, whose tiles are too few.
