@@ -26,7 +26,7 @@ extern "C" {
  * relative to, is made of the rounded out and corrected for d_k. Against results that are rounded nowhere else, errors over short documents grow from 1.7e-3 to 1.9e-3 (out) and 2.4e-3
  * (gradients) in CSA_LM_BF16, from 2.1e-4 to 2.9e-4 in CSA_LM_F16, relative to the norm; those of the cross entropy's gradients stay at the result's rounding, those of distillation
  * grow from 1.7e-3 to 2.3e-3 and from 2.1e-4 to 2.9e-4 (up to 3.9e-3 and 4.9e-4 where a teacher weighs the words of all tokens alike), and stay at the result's rounding for up to 32
- * tokens (of 33 to 64, as far as entries above an eighth of their token's weight go: up to 1.18 times it). Few entries make most of a short text's gradients, so that errors spread: of 65 to some
+ * tokens (of 33 to 64, as far as entries above an eighth of their token's weight go: up to 1.18 times it where these make most of the sums). Few entries make most of a short text's gradients, so that errors spread: of 65 to some
  * hundred tokens up to 1.5 times the result's rounding, up to 1.7 where the tokens' weights differ by up to 2^10. Embeddings and norms round once, at the end. */
 
 typedef enum csa_lm_type {
